@@ -100,3 +100,25 @@ def fwd_bf16_static_scratch(Q, K, V, O, softmax_lse, batch, seqlen_q, seqlen_k, 
          softmax_lse or None, seqused_k or None, batch, seqlen_q, seqlen_k, num_heads_q, num_heads_kv, head_dim,
          *map(C.addressof, strides),
          softmax_scale, kv_splits, kv_static_rows, 1 if pdl else 0, stream)
+
+
+# ------------------------------------------------------------------ paged FP8 cache (no counterpart in the reference)
+def paged_workspace_bytes(tokens, batch, max_new, num_heads_q, num_heads_kv, head_dim) -> int:
+    """Bytes of ``paged_fwd_fp8``'s workspace for at most these figures, on the current device.  Zero it once."""
+    n = C.c_longlong(0)
+    call("frt_b200_paged_attention_workspace_bytes", tokens, batch, max_new, num_heads_q, num_heads_kv, head_dim, C.addressof(n))
+    return n.value
+
+
+def paged_fwd_fp8(Q, O, softmax_lse, k_cache, v_cache, k_scale, v_scale, block_table, table_stride, cu_seqlens, seq_lens, tokens,
+                  batch, max_new, num_blocks, block_size, num_heads_q, num_heads_kv, head_dim, softmax_scale, workspace,
+                  workspace_bytes, stream=0, *, softcap=0.0, window=0, causal=True, q_stride=0, o_stride=0):
+    """Attention of packed new tokens over the cache of ``flash_rt_kernels.paged_kv_append_fp8``: one token per sequence, a few, or
+    a chunk of a prompt.  ``Q``, ``O`` (tokens, hq * head_dim) bf16 (strides in elements, 0: packed), ``softmax_lse`` (hq, tokens)
+    fp32 or 0; ``max_new``: new tokens of the longest sequence, or more.  ``window`` > 0: a token sees the last ``window``
+    positions up to its own; ``causal=False``: all of its sequence.  ``softcap`` > 0: softcap * tanh(score / softcap)."""
+    width = num_heads_q * head_dim
+    call("frt_b200_paged_attention_fp8", Q, q_stride or width, O, o_stride or width, softmax_lse or None, k_cache, v_cache, k_scale,
+         v_scale, block_table, table_stride, cu_seqlens or None, seq_lens, tokens, batch, max_new, num_blocks, block_size,
+         num_heads_q, num_heads_kv, head_dim, float(softmax_scale), float(softcap), window, workspace, workspace_bytes,
+         0 if causal else 2, stream)

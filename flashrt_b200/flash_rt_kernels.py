@@ -139,6 +139,24 @@ def qkv_split_rope_devpos(qkv, rope_weights, Q, K, V, devpos, seq, q_dim, k_dim,
          _f(pdl), stream)
 
 
+# ------------------------------------------------------------------ paged FP8 key/value cache (no counterpart in the reference)
+def paged_kv_append_fp8(qkv, rope, Q, k_cache, v_cache, k_scale, v_scale, block_table, table_stride, cu_seqlens, seq_lens, tokens,
+                        batch, num_blocks, block_size, num_heads_q, num_heads_kv, head_dim, rope_rows, stream=0, *, qkv_stride=0,
+                        halves=False):
+    """New tokens of a packed QKV projection into a paged E4M3 cache with one scale per (block, head); keys and queries rotated.
+
+    ``qkv`` (tokens, (hq + 2 hkv) * head_dim) bf16 (``qkv_stride`` elements between rows, 0: packed), ``rope`` (rope_rows,
+    head_dim) fp32 with [cos0, sin0, ...] of every position (0: no rotation), ``Q`` (tokens, hq * head_dim) bf16 (0: not written),
+    ``k_cache`` / ``v_cache`` (num_blocks, hkv, block_size, head_dim), ``k_scale`` / ``v_scale`` (num_blocks, hkv) fp32,
+    ``block_table`` (batch, table_stride) int32, ``cu_seqlens`` (batch + 1) int32 (0: one token per sequence), ``seq_lens``
+    (batch) int32 with the new tokens included.  ``halves``: pairs (i, i + head_dim / 2) instead of neighbours.
+    The scale of a block grows with its largest value and the codes that it holds are rounded again; see the header."""
+    width = (num_heads_q + 2 * num_heads_kv) * head_dim
+    call("frt_b200_paged_kv_append_fp8", qkv, qkv_stride or width, rope or None, rope_rows, Q or None, k_cache, v_cache, k_scale,
+         v_scale, block_table, table_stride, cu_seqlens or None, seq_lens, tokens, batch, num_blocks, block_size, num_heads_q,
+         num_heads_kv, head_dim, 2 if halves else 0, stream)
+
+
 # ------------------------------------------------------------------ classifier-free guidance (csrc/bindings.cpp:1133-1141)
 def cfg_combine_into_residual(residual, v_cond, v_uncond, beta, n, stream=0, *, pdl=False, f32=False):
     """residual += v_uncond + beta * (v_cond - v_uncond).  ``f32=True`` (not in the reference): fp32 arrays."""

@@ -507,6 +507,51 @@ int frt_b200_expert_loop_schedule(int G, int cta, int gl, int phase, int att_uni
  * issuer, 3 worker, 4 grid barrier); synchronises the device. */
 int frt_b200_expert_loop_status(int reset);
 
+/* ---------------------------------------------------------------- paged E4M3 key/value cache: append, attention
+ * A cache of blocks ("pages") for causal decoding of ragged batches; no counterpart in the reference, whose attention reads dense
+ * 16-bit caches (qkv_split_rope_devpos, csrc/kernels/rope.cu:215-277; csrc/attention/fa2_wrapper.cu).
+ *   k_cache, v_cache (num_blocks, num_heads_kv, block_size, head_dim) E4M3 codes; k_scale, v_scale (num_blocks, num_heads_kv) fp32,
+ *   a stored value is code * scale.  head_dim 64, 128 or 256; block_size 16, 32, 64 or 128.
+ *   block_table (batch, table_stride) int32: block of tokens [j * block_size, (j + 1) * block_size) of a sequence.
+ *   The new tokens of all sequences are packed behind one another: cu_seqlens (batch + 1) int32, from 0 up (NULL: one token per
+ *   sequence, tokens == batch); seq_lens (batch) int32: tokens of a sequence in all, the new ones included, so that new token i
+ *   of n has position seq_lens - n + i.  Tables and lengths are device arrays that are read when the launch runs: one captured
+ *   graph serves every step.  Rows behind the last sequence are neither read nor written.
+ *
+ * Append: Q <- rotated queries, K and V of the packed row into the cache.  qkv (tokens, (hq + 2 hkv) * head_dim) bf16, rows
+ *   qkv_stride elements apart; rope (rope_rows, head_dim) fp32, row = position, [cos0, sin0, cos1, sin1, ...], NULL: no rotation;
+ *   Q (tokens, hq * head_dim) bf16 or NULL.  Per block, head and tensor, over the new tokens of this call:
+ *     s = max(s_old if the block holds earlier tokens, max |finite y| / 448, 1e-12);  code = e4m3(clamp(y * (1 / s), +-448));
+ *     codes that the block holds already, if s has grown: e4m3(c * (s_old / s)).  y: the rotated key in fp32, the value.
+ *   Infinite values are clamped, NaN becomes -448 (as in frt_b200_quantize_fp8_static).  A block that is written belongs to one
+ *   sequence; what a block holds behind its sequence's tokens is left as it was.  Left out, neither rotated nor stored: tokens
+ *   with a negative position (seq_lens 0: an idle slot) or one without a table row.  Keys and values whose page is no block of the
+ *   pool (a negative entry), or lies outside the table, are not stored.
+ *   flags bit 1: pairs are (i, i + head_dim / 2) instead of (2 i, 2 i + 1). */
+int frt_b200_paged_kv_append_fp8(const void* qkv, long long qkv_stride, const float* rope, int rope_rows, void* Q,
+                                 void* k_cache, void* v_cache, float* k_scale, float* v_scale, const int* block_table,
+                                 int table_stride, const int* cu_seqlens, const int* seq_lens, int tokens, int batch,
+                                 int num_blocks, int block_size, int num_heads_q, int num_heads_kv, int head_dim, int flags,
+                                 void* stream);
+/* Attention of the new tokens over that cache (no counterpart in the reference): O = softmax(cap(softmax_scale Q K^T)) V, query
+ *   head hh on key/value head hh / (hq / hkv).  Q, O (tokens, hq * head_dim) bf16, rows q_stride / o_stride elements apart;
+ *   lse (hq, tokens) fp32 or NULL.  A token sees the positions up to its own, with window > 0 the last `window` of them, with
+ *   flags bit 1 (no window then) all seq_lens.  softcap > 0: scores become softcap * tanh(s / softcap).  Keys whose page is no
+ *   block of the pool are absent.  A row that sees no key is zero, its lse -infinity.  Codes and scales are finite, scales
+ *   positive, as the append leaves them; nothing is read behind a sequence's end or in front of its window.
+ *   max_new: new tokens of the longest sequence, or more; a choice of the kernel, whose results agree to rounding.
+ *   workspace: frt_b200_paged_attention_workspace_bytes bytes for the same figures, 16-byte aligned, zeroed once; every launch
+ *   leaves it ready for the next, of any shape that it is large enough for.  Launches that share one must not overlap. */
+int frt_b200_paged_attention_fp8(const void* Q, long long q_stride, void* O, long long o_stride, float* lse,
+                                 const void* k_cache, const void* v_cache, const float* k_scale, const float* v_scale,
+                                 const int* block_table, int table_stride, const int* cu_seqlens, const int* seq_lens, int tokens,
+                                 int batch, int max_new, int num_blocks, int block_size, int num_heads_q, int num_heads_kv,
+                                 int head_dim, float softmax_scale, float softcap, int window, void* workspace,
+                                 long long workspace_bytes, int flags, void* stream);
+/* no counterpart in the reference: bytes of that workspace (on the current device) */
+int frt_b200_paged_attention_workspace_bytes(int tokens, int batch, int max_new, int num_heads_q, int num_heads_kv, int head_dim,
+                                             long long* out_bytes);
+
 /* number of SMs of the current device (grid sizing) */
 int frt_b200_device_sm_count(void);
 
