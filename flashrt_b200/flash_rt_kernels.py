@@ -255,6 +255,12 @@ def quantize_fp8_device(input, output, d_scale, n, stream=0):  # noqa: A002
     call("frt_b200_quantize_fp8_device", input, output, d_scale, n, stream)
 
 
+def quantize_int8_rows(input, output, row_scale, rows, dim, stream=0, *, in_stride=0):  # noqa: A002
+    """(rows, dim) bf16 -> int8 with one fp32 scale per row, max |x| / 127 (no counterpart in the reference).  ``in_stride``:
+    elements between rows, 0: packed.  The activations of :meth:`GemmRunner.int8_nt`."""
+    call("frt_b200_quantize_int8_rows", input, in_stride or dim, output, row_scale, rows, dim, 0, stream)
+
+
 def fp8_accumulate_scale_max(src_scale, dst_scale, stream=0):
     call("frt_b200_fp8_accumulate_scale_max", src_scale, dst_scale, stream)
 
@@ -298,6 +304,11 @@ class GemmRunner:
         """``fp8_nt_dev`` that may split K through the caller's workspace (M > 256; the form is chosen by size)."""
         call("frt_b200_gemm_fp8_nt_splitk", A, B, D, M, N, K, d_scale_a, d_scale_b, bias, workspace, workspace_bytes, counters,
              _f(pdl), stream)
+
+    def int8_nt(self, A, B, D, M, N, K, token_scale, channel_scale, stream=0, *, bias=0, pdl=False):
+        """D(M,N) bf16 = (A(M,K) . B(N,K)^T) * token_scale[m] * channel_scale[n] + bias[n] of int8 matrices, exact integer sums
+        (no counterpart in the reference).  K % 16 == 0; any M and N."""
+        call("frt_b200_gemm_int8_nt", A, B, D, M, N, K, token_scale, channel_scale, bias or None, _f(pdl), stream)
 
     # -- the decoder's projections with the norm kernel between them folded in ------------------------------
     def fp8_nt_dev_gate_residual(self, A, B, M, N, K, d_scale_a, d_scale_b, residual, gate, stats_out, stream=0, *,

@@ -552,6 +552,20 @@ int frt_b200_paged_attention_fp8(const void* Q, long long q_stride, void* O, lon
 int frt_b200_paged_attention_workspace_bytes(int tokens, int batch, int max_new, int num_heads_q, int num_heads_kv, int head_dim,
                                              long long* out_bytes);
 
+/* ---------------------------------------------------------------- 8-bit integer products with a scale per token and channel
+ * No counterpart in the reference (its 8-bit products have one scale per tensor: csrc/gemm/gemm_runner.cu:67-76).
+ * Rows of activations to 8-bit integers: s = max(max |finite x| / 127, 1e-12), q = clamp(rint(x * (1 / s)), +-127); infinities are
+ *   clamped, NaN becomes 0.  in (rows, dim) bf16, rows in_stride elements apart; out (rows, dim) int8; row_scale (rows) fp32.
+ *   dim % 16 == 0, in_stride % 8 == 0, in and out 16-byte aligned. */
+int frt_b200_quantize_int8_rows(const void* in_bf16, long long in_stride, void* out_s8, float* row_scale, int rows, int dim,
+                                int flags, void* stream);
+/* D(M,N) bf16 = (sum_k A[m][k] W[n][k]) * token_scale[m] * channel_scale[n] + bias[n] (no counterpart in the reference): A (M, K) and
+ *   W (N, K) int8, K contiguous, 16-byte aligned; token_scale (M), channel_scale (N) fp32; bias (N) bf16 or NULL.  The sums are
+ *   32-bit integers and exact: K % 16 == 0, K < 131072; any M, any N.  flags bit 0: the weights are settled and may be read
+ *   before the kernel in front has ended.  A wait that gave up shows in frt_b200_gemm_status. */
+int frt_b200_gemm_int8_nt(const void* A, const void* W, void* D, int M, int N, int K, const float* token_scale,
+                          const float* channel_scale, const void* bias, int flags, void* stream);
+
 /* number of SMs of the current device (grid sizing) */
 int frt_b200_device_sm_count(void);
 
