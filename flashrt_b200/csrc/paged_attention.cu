@@ -12,21 +12,28 @@
 // the row's largest lose bits).
 //
 // What bounds it: a decode step reads every key and value once and does 4 x group flops per byte, so memory does, and the kernel is
-// built to keep loads in flight: no shared memory and no barrier on the way of keys and values.  A warp takes KT keys at a time with
-// 16-byte loads straight into registers, whose layout IS the operand of mma.sync m16n8k16: keys are the M rows of K . Q^T and
-// dimensions the M rows of V^T . P^T, so a group of up to eight query rows fills the N side and no tensor work is wasted; which
-// dimension a k index stands for is free, hence a lane's 16 contiguous bytes serve four k steps.  The pairs of keys that V^T wants
-// side by side come from one byte permutation, which unpacking 8-bit codes costs anyway; the conversion itself is the hardware's
-// e4m3x2 -> f16x2 (measured 86 values per clock and SM with its surroundings, where 25 arrive from memory; shifts and masks gave 43).
-// P^T comes from the scores by movmatrix.  The next tile's keys are requested as soon as this one's are converted, its values likewise.
+// built to keep copies in flight.  Every warp works alone: it owns a ring of slots (KT keys and their values, 8 KB each) that it fills
+// itself by TMA, two or three tiles ahead and across the items of its work, so neither the join of an item's warps nor the set-up of
+// the next one lets the memory wait.  (The form before loaded into registers, one tile ahead: 64 sequences of 1500 .. 6000 tokens, 32
+// heads on 8 of 128: 142 us, memory 42 % busy, every second cycle of a warp spent on a load.)
+// Codes go from shared memory to the tensor cores as fp16: keys are the M rows of K . Q^T and dimensions the M rows of V^T . P^T
+// (mma.sync m16n8k16), so a group of up to eight query rows fills the N side and no tensor work is wasted.  Which dimension a k index
+// stands for is free, hence a lane's 16 contiguous bytes serve four k steps; the pairs of keys that V^T wants side by side come from
+// one byte permutation.  The conversion itself is the hardware's e4m3x2 -> f16x2 (measured 86 values per clock and SM with its
+// surroundings, where 25 arrive from memory; shifts and masks gave 43).  P^T comes from the scores by movmatrix.  TMA's swizzle, and an
+// order of keys and dimensions over the lanes that sets neighbouring groups four rows or chunks apart, keep the reads free of bank
+// conflicts (heads of 64: the values' reads meet twice).
 //
 // Split: the work is one line of (sequence, head, row tile, key tile) units, cut evenly over the CTAs whatever the lengths are.  A CTA
 // whose range ends inside an item leaves fp32 partials in the workspace; the CTA that arrives last at the item adds them in
 // order, so results do not depend on the order of arrival.  No host knowledge of lengths: a captured graph serves every step.
 #include "common.cuh"
+#include "tc05.cuh"
 #include "flashrt_b200.h"
 
 #include <cuda_fp16.h>
+
+#include <type_traits>
 
 namespace frt {
 
@@ -43,6 +50,8 @@ struct PagedAttnParams {
     int table_stride, tokens, batch, num_blocks, block_size, block_shift, hq, hkv, group;
     float scale, cap;
     int window, causal;
+    int pool_rows;               // rows of a cache seen as a matrix of head_dim columns
+    int* status;
     unsigned* counters;
     float2* part_ml;             // [cta][2][rows] (m, l)
     float* part_o;               // [cta][2][rows][D]
@@ -51,15 +60,20 @@ struct PagedAttnParams {
 template <int D, int NT>
 struct PagedCfg {
     static constexpr int ROWS = 8 * NT;
-    static constexpr int ST = D == 256 ? 1 : 2;       // 16-key steps of a warp's tile
-    static constexpr int KT = 16 * ST;
+    static constexpr int KT = 4096 / D;               // keys of a warp's tile: 4 KB of keys, 4 KB of values
+    static constexpr int ST = KT / 16;                // 16-key steps
     static constexpr int NW = 8;
     static constexpr int THREADS = 32 * NW;
-    static constexpr int CTAS = D == 256 || NT == 2 ? 1 : 2;      // per SM (registers)
+    static constexpr int SLOT_BYTES = 2 * KT * D;
+    static constexpr int SLOTS = NT == 1 && D <= 128 ? 3 : 2;
+    static constexpr int RING_BYTES = NW * SLOTS * SLOT_BYTES;
+    static constexpr int WRITERS = NT == 1 && D != 128 ? NW : NW / 2;      // warps whose accumulators are in shared memory at once
     static constexpr int PITCH = D + 4;               // floats of an accumulator row in shared memory
     static constexpr int Q_BYTES = NT * (D / 16) * 32 * 8;
-    static constexpr int ACC_BYTES = NW * ROWS * PITCH * 4;
-    static constexpr int SMEM_BYTES = Q_BYTES + ACC_BYTES;
+    static constexpr int ACC_BYTES = WRITERS * ROWS * PITCH * 4;
+    static constexpr int SMEM_BYTES = 1024 + RING_BYTES + Q_BYTES + ACC_BYTES;
+    static constexpr bool Q_REGS = NT == 1;           // query fragments stay in registers
+    static_assert(SMEM_BYTES <= 232448 - 6 * 1024, "dynamic and static shared memory of a CTA");
 };
 
 // One sequence's share of the work line.
@@ -109,16 +123,25 @@ __device__ __forceinline__ void mma_f16_16816(float (&c)[4], const uint32_t (&a)
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-// cache bytes: coherent (the append in front may still run when this kernel starts), not kept in L1, in program order
-template <int WORDS>
-__device__ __forceinline__ void ld_codes(const uint8_t* p, uint32_t* w) {
-    if constexpr (WORDS == 2)
-        asm volatile("ld.global.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "l"(p));
-    else
-#pragma unroll
-        for (int i = 0; i < WORDS; i += 4)
-            asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
-                         : "=r"(w[i]), "=r"(w[i + 1]), "=r"(w[i + 2]), "=r"(w[i + 3]) : "l"(p + 4 * i));
+__device__ __forceinline__ uint4 ld_shared_v4(uint32_t a) {
+    uint4 r;
+    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "r"(a) : "memory");
+    return r;
+}
+__device__ __forceinline__ uint2 ld_shared_v2(uint32_t a) {
+    uint2 r;
+    asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(r.x), "=r"(r.y) : "r"(a) : "memory");
+    return r;
+}
+__device__ __forceinline__ float ld_shared_f(uint32_t a) {
+    float r;
+    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(r) : "r"(a) : "memory");
+    return r;
+}
+// 4 bytes to shared memory (zero if !there); the thread's arrival at `bar` follows its copies
+__device__ __forceinline__ void copy_scale(uint32_t dst, const float* src, bool there, uint32_t bar) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(there ? 4 : 0) : "memory");
+    asm volatile("cp.async.mbarrier.arrive.noinc.shared.b64 [%0];" ::"r"(bar) : "memory");
 }
 
 // tanh through the hardware's exp2 and reciprocal: 2^-22 absolute, where tanh.approx has 2^-11
@@ -128,22 +151,68 @@ __device__ __forceinline__ float soft_cap(float s, float cap, float inv_cap2) {
     return cap * (1.0f - 2.0f * r);
 }
 
+// A stretch of the work line inside one item: what a warp has to know to copy its tiles, and where the item's rows are.
+struct PagedSegment {
+    int b, item;                 // sequence; (head, row tile) inside it
+    long long first, end;        // line positions: of the item, behind the stretch
+    int items, h, row0, rows, tiles;
+    int len, n, start;
+    int key_lo, key_hi;          // keys that any row sees
+    int tile_lo, tile_hi;        // tiles of the stretch with such keys
+};
+// the stretch that begins at line position `at` < w1; b, item, first are set
+template <int KT, int ROWS>
+__device__ __forceinline__ void paged_segment(const PagedAttnParams& p, PagedSegment& g, long long at, long long w1) {
+    PagedSeq s = paged_seq<KT, ROWS>(p, g.b);
+    while (g.item >= s.row_tiles * p.hkv && g.b + 1 < p.batch) {             // through with the sequence, or one without new tokens
+        ++g.b;
+        g.item = 0;
+        s = paged_seq<KT, ROWS>(p, g.b);
+    }
+    g.items = s.row_tiles * p.hkv;
+    g.h = g.item / s.row_tiles;
+    g.row0 = (g.item - g.h * s.row_tiles) * ROWS;
+    g.rows = min(ROWS, s.n * p.group - g.row0);
+    g.tiles = s.tiles;
+    g.len = s.len;
+    g.n = s.n;
+    g.start = s.start;
+    g.end = min(g.first + s.tiles, w1);
+    const int p0 = s.len - s.n + g.row0 / p.group, p1 = s.len - s.n + (g.row0 + g.rows - 1) / p.group;
+    g.key_lo = p.window > 0 ? max(0, p0 - p.window + 1) : 0;
+    g.key_hi = p.causal ? min(s.len, p1 + 1) : s.len;
+    g.tile_lo = max(s.t0 + (int)(at - g.first), g.key_lo / KT);
+    g.tile_hi = min(s.t0 + (int)(g.end - g.first), g.key_hi > 0 ? (g.key_hi + KT - 1) / KT : 0);
+}
+
 template <int D, int NT>
-__global__ void __launch_bounds__(256, (PagedCfg<D, NT>::CTAS))
-paged_attention_kernel(PagedAttnParams p) {
+__global__ void __launch_bounds__(256, 1)
+paged_attention_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, PagedAttnParams p) {
     using Cfg = PagedCfg<D, NT>;
-    constexpr int ST = Cfg::ST, KT = Cfg::KT, NW = Cfg::NW, ROWS = Cfg::ROWS, SEGS = D / 64, VW = D / 32, MT = D / 16;
+    constexpr int ST = Cfg::ST, KT = Cfg::KT, NW = Cfg::NW, ROWS = Cfg::ROWS, SEGS = D / 64, MT = D / 16, SLOTS = Cfg::SLOTS;
     constexpr float LOG2E = 1.4426950408889634f;
-    extern __shared__ __align__(16) uint8_t smem[];
-    uint2* q_s = reinterpret_cast<uint2*>(smem);                             // [nt][k step][lane]
-    float* acc_s = reinterpret_cast<float*>(smem + Cfg::Q_BYTES);            // [warp][row][PITCH]
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+    uint2* q_s = reinterpret_cast<uint2*>(smem + Cfg::RING_BYTES);           // [nt][k step][lane]
+    float* acc_s = reinterpret_cast<float*>(smem + Cfg::RING_BYTES + Cfg::Q_BYTES);       // [warp][row][PITCH]
     __shared__ float2 ml_s[NW][ROWS];
     __shared__ float rf_s[ROWS];
+    __shared__ float scale_s[NW][SLOTS][ST][2];
+    __shared__ uint64_t full_s[NW][SLOTS];
     __shared__ long long scan_s[256];
     __shared__ long long warp_s[8];
     __shared__ unsigned last_s;
+    __shared__ volatile int abort_s;
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
+    if (lane < SLOTS) tc::mbar_init(&full_s[warp][lane], 1 + 2 * ST);        // the copies' bytes, one arrival per scale
+    if (tid == 0) {
+        tc::tma_prefetch_desc(&tmK);
+        tc::tma_prefetch_desc(&tmV);
+    }
+    tc::mbar_fence_init();
+    const uint64_t deadline = tc::global_timer_ns() + FRT_KERNEL_DEADLINE_NS;
+    if (tid == 0) abort_s = 0;
     pdl_launch_dependents();
     pdl_wait();
 
@@ -172,34 +241,90 @@ paged_attention_kernel(PagedAttnParams p) {
     const int cta = blockIdx.x;
     if (cta >= grid || total == 0) return;
     const long long w0 = total * cta / grid, w1 = total * (cta + 1) / grid;
-    int b, item;                                                             // sequence; (head, row tile) inside it
-    long long at = w0, first;                                                // first: line position of the item
+    PagedSegment cur;
     {
         int lo = 0, hi = 256;
         while (hi - lo > 1) {
             const int mid = (lo + hi) >> 1;
             if (scan_s[mid] <= w0) lo = mid; else hi = mid;
         }
-        b = lo * per;
-        first = scan_s[lo];
+        cur.b = lo * per;
+        cur.first = scan_s[lo];
         for (;;) {                                                           // ends before the chunk does: w0 lies in it
-            const long long u = paged_units<KT, ROWS>(p, b);
-            if (w0 < first + u || b + 1 >= p.batch) break;
-            first += u;
-            ++b;
+            const long long u = paged_units<KT, ROWS>(p, cur.b);
+            if (w0 < cur.first + u || cur.b + 1 >= p.batch) break;
+            cur.first += u;
+            ++cur.b;
         }
-        const PagedSeq s = paged_seq<KT, ROWS>(p, b);
-        item = (int)((w0 - first) / s.tiles);
-        first += (long long)item * s.tiles;
+        cur.item = (int)((w0 - cur.first) / paged_seq<KT, ROWS>(p, cur.b).tiles);
+        cur.first += (long long)cur.item * paged_seq<KT, ROWS>(p, cur.b).tiles;
     }
+    paged_segment<KT, ROWS>(p, cur, w0, w1);
 
-    while (at < w1) {
-        const PagedSeq s = paged_seq<KT, ROWS>(p, b);
-        const int items = s.row_tiles * p.hkv;
-        if (item >= items) { ++b; item = 0; continue; }                      // a sequence without new tokens has no items
-        const int h = item / s.row_tiles, row0 = (item - h * s.row_tiles) * ROWS;
-        const long long end = min(first + s.tiles, w1);
-        const int rows = min(ROWS, s.n * p.group - row0);
+    // ---------------- this warp's copies: `nx` runs ahead of the computation by the slots of the ring
+    const uint32_t ring = tc::smem_u32(smem) + (uint32_t)warp * (SLOTS * Cfg::SLOT_BYTES);
+    const uint32_t full_a = tc::smem_u32(&full_s[warp][0]), scale_a = tc::smem_u32(&scale_s[warp][0][0][0]);
+    PagedSegment nx = cur;
+    int nx_tile = cur.tile_lo + warp, nx_page = -1, nx_slot = 0;
+    // to the next tile there is for this warp; lanes 2 st, 2 st + 1 ask for the page of its st-th 16 keys
+    auto seek = [&] {
+        while (nx_tile >= nx.tile_hi) {
+            if (nx.end >= w1) { nx_tile = 0x7fffffff; return; }
+            const long long at = nx.end;
+            nx.first = at;                                                   // a stretch that does not end the work ends its item
+            ++nx.item;
+            paged_segment<KT, ROWS>(p, nx, at, w1);
+            nx_tile = nx.tile_lo + warp;
+        }
+        const int k0 = nx_tile * KT + (lane >> 1) * 16, box = min(KT, p.block_size), head = k0 & ~(box - 1);
+        nx_page = -1;                                                        // a box without keys of the item is not looked at
+        if (lane < 2 * ST && head < nx.key_hi && head + box > nx.key_lo)
+            nx_page = p.table[(size_t)nx.b * p.table_stride + (head >> p.block_shift)];
+        if (nx_page >= p.num_blocks) nx_page = -1;
+    };
+    auto copy = [&] {
+        if (nx_tile == 0x7fffffff) return;
+        const uint32_t bar = full_a + 8 * nx_slot, dst = ring + nx_slot * Cfg::SLOT_BYTES;
+        if (lane < 2 * ST) {
+            const float* src = lane & 1 ? p.v_scale : p.k_scale;
+            copy_scale(scale_a + (nx_slot * ST * 2 + lane) * 4, src + (size_t)max(nx_page, 0) * p.hkv + nx.h, nx_page >= 0, bar);
+        }
+        if (lane == 0) tc::mbar_arrive_expect_tx(bar, Cfg::SLOT_BYTES);
+        // one box per block (or per tile inside one): lane 2 st of its first 16 keys issues it; rows beyond the pool arrive as zeros
+        const int box = min(KT, p.block_size), st = lane >> 1;
+        if (lane < 2 * ST && (st * 16) % box == 0) {
+            const int k0 = nx_tile * KT + st * 16;
+            const int row = nx_page >= 0 ? (nx_page * p.hkv + nx.h) * p.block_size + (k0 & (p.block_size - 1)) : p.pool_rows;
+            const CUtensorMap* map = lane & 1 ? &tmV : &tmK;
+            constexpr int INNER = D < 128 ? D : 128;
+            const uint32_t to = dst + (lane & 1) * (KT * D) + st * 16 * INNER;
+#pragma unroll
+            for (int x = 0; x < D; x += INNER) tc::tma_load_2d(to + x * KT, map, bar, x, row);
+        }
+        if (++nx_slot == SLOTS) nx_slot = 0;
+        nx_tile += NW;
+    };
+    for (int i = 0; i < SLOTS; ++i) {
+        seek();
+        copy();
+    }
+    seek();
+    int slot = 0;
+    uint32_t phase = 0;
+
+    // where this lane's operands are in a slot (see the top: groups of lanes four rows or chunks apart)
+    const int krow = D == 64 ? g : (g >> 1) | ((g & 1) << 2), dchunk = krow;
+    const uint32_t k_off = D == 64 ? g * 64 + ((c ^ ((g >> 1) & 3)) << 4) : krow * 128 + ((c ^ krow) << 4);
+    const uint32_t v_off = KT * D + (D == 64 ? 2 * c * 64 + (((g >> 1) ^ c) << 4) + (g & 1) * 8 : c * 128 + ((dchunk ^ c) << 4));
+    constexpr int STEP = D == 64 ? 64 : 128;                                 // bytes from row to row
+
+    for (long long at = w0; at < w1;) {
+        if (at != w0) {
+            cur.first = at;
+            ++cur.item;
+            paged_segment<KT, ROWS>(p, cur, at, w1);
+        }
+        const int rows = cur.rows, row0 = cur.row0, h = cur.h;
 
         // queries -> fp16 operand fragments, at most 1 in magnitude: one warp per row
         __syncthreads();                                                     // the item before is through with shared memory
@@ -209,7 +334,7 @@ paged_attention_kernel(PagedAttnParams p) {
             float top = 0.0f;
             if (r < rows) {
                 const int i = (row0 + r) / p.group, hh = h * p.group + (row0 + r) % p.group;
-                const uint32_t* src = reinterpret_cast<const uint32_t*>(p.q + (size_t)(s.start + i) * p.q_stride + (size_t)hh * D + lane * PL);
+                const uint32_t* src = reinterpret_cast<const uint32_t*>(p.q + (size_t)(cur.start + i) * p.q_stride + (size_t)hh * D + lane * PL);
 #pragma unroll
                 for (int j = 0; j < PL / 2; ++j) unpack_bf16x2(src[j], x[2 * j], x[2 * j + 1]);
             } else {
@@ -236,27 +361,24 @@ paged_attention_kernel(PagedAttnParams p) {
         // this lane's rows: 2c, 2c + 1 of every n tile
         float rf[NT][2];
         int row_hi[NT][2], row_lo[NT][2];
-        int all_hi = 0x7fffffff, all_lo = 0;                                 // keys that every row sees
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
                 const int r = nt * 8 + 2 * c + x;
                 rf[nt][x] = rf_s[r] * p.scale * (p.cap > 0.0f ? 1.0f : LOG2E);
-                const int pos = s.len - s.n + (row0 + min(r, rows - 1)) / p.group;
-                row_hi[nt][x] = p.causal ? min(pos + 1, s.len) : s.len;
+                const int pos = cur.len - cur.n + (row0 + min(r, rows - 1)) / p.group;
+                row_hi[nt][x] = p.causal ? min(pos + 1, cur.len) : cur.len;
                 row_lo[nt][x] = p.window > 0 ? max(0, pos - p.window + 1) : 0;
             }
-        {
-            const int p0 = s.len - s.n + row0 / p.group, p1 = s.len - s.n + (row0 + rows - 1) / p.group;
-            all_hi = p.causal ? min(p0 + 1, s.len) : s.len;
-            all_lo = p.window > 0 ? max(0, p1 - p.window + 1) : 0;
+        const int p0 = cur.len - cur.n + row0 / p.group, p1 = cur.len - cur.n + (row0 + rows - 1) / p.group;
+        const int all_hi = p.causal ? min(p0 + 1, cur.len) : cur.len;        // keys that every row sees
+        const int all_lo = p.window > 0 ? max(0, p1 - p.window + 1) : 0;
+        uint2 q_r[Cfg::Q_REGS ? MT : 1];
+        if constexpr (Cfg::Q_REGS) {
+#pragma unroll
+            for (int j = 0; j < MT; ++j) q_r[j] = q_s[j * 32 + lane];
         }
-        const int key_lo = p.window > 0 ? max(0, s.len - s.n + row0 / p.group - p.window + 1) : 0;
-        const int key_hi = p.causal ? min(s.len, s.len - s.n + (row0 + rows - 1) / p.group + 1) : s.len;   // any row's keys
-        // tiles of this CTA's share, without those that no row sees
-        const int tile_lo = max(s.t0 + (int)(at - first), key_lo / KT);
-        const int tile_hi = min(s.t0 + (int)(end - first), key_hi > 0 ? (key_hi + KT - 1) / KT : 0);
 
         float m[NT][2], l[NT][2], acc[NT][MT][4];
 #pragma unroll
@@ -268,84 +390,14 @@ paged_attention_kernel(PagedAttnParams p) {
 #pragma unroll
                 for (int x = 0; x < 4; ++x) acc[nt][j][x] = 0.0f;
         }
-        uint32_t kw[ST][2][SEGS][4], vw[ST][4][VW];
-        // pages and scales of a tile; a page that holds no key of the item, or is no block of the pool, reads as absent
-        int page_n[ST];
-        float ks_n[ST], vs_n[ST];
-        const int* table = p.table + (size_t)b * p.table_stride;
-        auto load_meta = [&](int tile) {
-#pragma unroll
-            for (int st = 0; st < ST; ++st) {
-                const int k0 = tile * KT + st * 16;
-                int page = -1;
-                if (tile < tile_hi && k0 < key_hi && k0 + 16 > key_lo) page = table[k0 >> p.block_shift];
-                if (page >= p.num_blocks) page = -1;
-                page_n[st] = page;
-                ks_n[st] = vs_n[st] = 1.0f;
-                if (page >= 0) {
-                    ks_n[st] = p.k_scale[(size_t)page * p.hkv + h];
-                    vs_n[st] = fmaxf(p.v_scale[(size_t)page * p.hkv + h], 1e-30f);
-                }
-            }
-        };
-        auto block_base = [&](int page, int k0) {
-            return (((size_t)max(page, 0) * p.hkv + h) * p.block_size + (k0 & (p.block_size - 1))) * D;
-        };
-        auto load_k = [&](int tile) {
-#pragma unroll
-            for (int st = 0; st < ST; ++st) {
-                const int k0 = tile * KT + st * 16;
-                const uint8_t* base = p.k + block_base(page_n[st], k0) + c * 16;
-#pragma unroll
-                for (int x = 0; x < 2; ++x) {
-                    const int r = g + 8 * x;
-                    if (page_n[st] >= 0 && k0 + r < key_hi) {
-#pragma unroll
-                        for (int sg = 0; sg < SEGS; ++sg) ld_codes<4>(base + r * D + sg * 64, kw[st][x][sg]);
-                    } else {
-#pragma unroll
-                        for (int sg = 0; sg < SEGS; ++sg)
-#pragma unroll
-                            for (int y = 0; y < 4; ++y) kw[st][x][sg][y] = 0;
-                    }
-                }
-            }
-        };
-        auto load_v = [&](int tile) {
-#pragma unroll
-            for (int st = 0; st < ST; ++st) {
-                const int k0 = tile * KT + st * 16;
-                const uint8_t* base = p.v + block_base(page_n[st], k0) + g * (D / 8);
-#pragma unroll
-                for (int x = 0; x < 4; ++x) {
-                    const int r = 2 * c + (x & 1) + 8 * (x >> 1);
-                    // what lies outside the item's keys may be anything, and 0 x NaN is NaN: it is not read
-                    if (page_n[st] >= 0 && k0 + r < key_hi && k0 + r >= key_lo) ld_codes<VW>(base + r * D, vw[st][x]);
-                    else {
-#pragma unroll
-                        for (int y = 0; y < VW; ++y) vw[st][x][y] = 0;
-                    }
-                }
-            }
-        };
 
-        int tile = tile_lo + warp;
-        load_meta(tile);
-        if (tile < tile_hi) {
-            load_k(tile);
-            load_v(tile);
-        }
-        while (tile < tile_hi) {
-            const int next = tile + NW;
-            float ks[ST], vs[ST];
-            bool there[ST];
-#pragma unroll
-            for (int st = 0; st < ST; ++st) {
-                ks[st] = ks_n[st];
-                vs[st] = vs_n[st];
-                there[st] = page_n[st] >= 0;
+        for (int tile = cur.tile_lo + warp; tile < cur.tile_hi; tile += NW) {
+            const uint32_t base = ring + slot * Cfg::SLOT_BYTES;
+            if (!tc::mbar_wait_until(full_a + 8 * slot, phase, deadline, &abort_s)) {
+                if (!abort_s && lane == 0) atomicCAS(p.status, 0, 1 | (blockIdx.x << 8));
+                abort_s = 1;
             }
-            load_meta(next);
+            __syncwarp();
             // ---- scores: [key][row]
             float sc[ST][NT][4];
 #pragma unroll
@@ -355,50 +407,75 @@ paged_attention_kernel(PagedAttnParams p) {
 #pragma unroll
                     for (int x = 0; x < 4; ++x) sc[st][nt][x] = 0.0f;
 #pragma unroll
-            for (int sg = 0; sg < SEGS; ++sg)
+            for (int sg = 0; sg < SEGS; ++sg) {
+                uint32_t kw[ST][2][4];
+                const uint32_t kb = base + (sg >> 1) * (KT * 128) + (sg & 1 ? k_off ^ 64 : k_off);
+#pragma unroll
+                for (int st = 0; st < ST; ++st)
+#pragma unroll
+                    for (int x = 0; x < 2; ++x) {
+                        const uint4 w = ld_shared_v4(kb + (st * 16 + x * 8) * STEP);
+                        kw[st][x][0] = w.x; kw[st][x][1] = w.y; kw[st][x][2] = w.z; kw[st][x][3] = w.w;
+                    }
 #pragma unroll
                 for (int y = 0; y < 4; ++y) {
                     uint2 qf[NT];
 #pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) qf[nt] = q_s[(nt * MT + sg * 4 + y) * 32 + lane];
+                    for (int nt = 0; nt < NT; ++nt) qf[nt] = Cfg::Q_REGS ? q_r[sg * 4 + y] : q_s[(nt * MT + sg * 4 + y) * 32 + lane];
 #pragma unroll
                     for (int st = 0; st < ST; ++st) {
                         uint32_t a[4];
-                        e4m3x4_to_f16(kw[st][0][sg][y], a[0], a[2]);
-                        e4m3x4_to_f16(kw[st][1][sg][y], a[1], a[3]);
+                        e4m3x4_to_f16(kw[st][0][y], a[0], a[2]);
+                        e4m3x4_to_f16(kw[st][1][y], a[1], a[3]);
 #pragma unroll
                         for (int nt = 0; nt < NT; ++nt) mma_f16_16816(sc[st][nt], a, qf[nt].x, qf[nt].y);
                     }
                 }
-            if (next < tile_hi) load_k(next);
+            }
             // ---- base-2 logits with the values' scale, mask, running maximum
             const int key0 = tile * KT;
             bool open = key0 >= all_lo && key0 + KT <= all_hi;
+            float ks[ST], lv[ST], inv_vs[ST], top[NT][2];
 #pragma unroll
-            for (int st = 0; st < ST; ++st) open = open && there[st];
-            float top[NT][2], inv_vs[ST];
+            for (int st = 0; st < ST; ++st) {
+                ks[st] = ld_shared_f(scale_a + ((slot * ST + st) * 2) * 4);
+                const float vs = ld_shared_f(scale_a + ((slot * ST + st) * 2 + 1) * 4);
+                open = open && vs != 0.0f;                                   // zero: an absent page
+                lv[st] = __log2f(fmaxf(vs, 1e-30f));
+                inv_vs[st] = vs != 0.0f ? __frcp_rn(fmaxf(vs, 1e-30f)) : 0.0f;
+            }
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) top[nt][0] = top[nt][1] = -INFINITY;
 #pragma unroll
-            for (int st = 0; st < ST; ++st) {
-                const float lv = __log2f(vs[st]);
-                inv_vs[st] = __frcp_rn(vs[st]);
+            for (int st = 0; st < ST; ++st)
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                     for (int x = 0; x < 4; ++x) {
                         const float f = rf[nt][x & 1] * ks[st];
                         float u;
-                        if (p.cap > 0.0f) u = fmaf(soft_cap(sc[st][nt][x] * f, p.cap, 2.0f * LOG2E / p.cap), LOG2E, lv);
-                        else u = fmaf(sc[st][nt][x], f, lv);
-                        if (!open) {
-                            const int key = key0 + st * 16 + g + 8 * (x >> 1);
-                            if (!there[st] || key >= row_hi[nt][x & 1] || key < row_lo[nt][x & 1]) u = -INFINITY;
-                        }
+                        if (p.cap > 0.0f) u = fmaf(soft_cap(sc[st][nt][x] * f, p.cap, 2.0f * LOG2E / p.cap), LOG2E, lv[st]);
+                        else u = fmaf(sc[st][nt][x], f, lv[st]);
                         sc[st][nt][x] = u;
-                        top[nt][x & 1] = fmaxf(top[nt][x & 1], u);
                     }
+            if (!open) {
+#pragma unroll
+                for (int st = 0; st < ST; ++st)
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                        for (int x = 0; x < 4; ++x) {
+                            const int key = key0 + st * 16 + krow + 8 * (x >> 1);
+                            if (inv_vs[st] == 0.0f || key >= row_hi[nt][x & 1] || key < row_lo[nt][x & 1]) sc[st][nt][x] = -INFINITY;
+                        }
             }
+#pragma unroll
+            for (int st = 0; st < ST; ++st)
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) top[nt][x & 1] = fmaxf(top[nt][x & 1], sc[st][nt][x]);
+            bool grown = false;
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -407,50 +484,89 @@ paged_attention_kernel(PagedAttnParams p) {
                     t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 4));
                     t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 8));
                     t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 16));
-                    const float mn = fmaxf(m[nt][x], t), safe = mn == -INFINITY ? 0.0f : mn;
-                    const float down = ex2(m[nt][x] - safe);
-                    m[nt][x] = mn;
-                    l[nt][x] *= down;
-#pragma unroll
-                    for (int j = 0; j < MT; ++j) {
-                        acc[nt][j][x] *= down;
-                        acc[nt][j][2 + x] *= down;
-                    }
-                    top[nt][x] = 15.0f - safe;
+                    top[nt][x] = fmaxf(m[nt][x], t);
+                    grown = grown || top[nt][x] > m[nt][x];
                 }
+            if (__any_sync(0xffffffffu, grown)) {
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int x = 0; x < 2; ++x) {
+                        const float down = ex2(m[nt][x] - (top[nt][x] == -INFINITY ? 0.0f : top[nt][x]));
+                        m[nt][x] = top[nt][x];
+                        l[nt][x] *= down;
+#pragma unroll
+                        for (int j = 0; j < MT; ++j) {
+                            acc[nt][j][x] *= down;
+                            acc[nt][j][2 + x] *= down;
+                        }
+                    }
+            }
             // ---- weights -> P^T fragments
             uint32_t pf[ST][NT][2];
 #pragma unroll
-            for (int st = 0; st < ST; ++st)
+            for (int nt = 0; nt < NT; ++nt) {
+                float ref[2];
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt) {
+                for (int x = 0; x < 2; ++x) ref[x] = 15.0f - (m[nt][x] == -INFINITY ? 0.0f : m[nt][x]);
+#pragma unroll
+                for (int st = 0; st < ST; ++st) {
                     float w[4];
 #pragma unroll
                     for (int x = 0; x < 4; ++x) {
-                        w[x] = ex2(sc[st][nt][x] + top[nt][x & 1]);
+                        w[x] = ex2(sc[st][nt][x] + ref[x & 1]);
                         l[nt][x & 1] = fmaf(w[x], inv_vs[st], l[nt][x & 1]);
                     }
                     pf[st][nt][0] = transpose_8x8(pack_f16x2(w[0], w[1]));
                     pf[st][nt][1] = transpose_8x8(pack_f16x2(w[2], w[3]));
                 }
+            }
             // ---- values: [dimension][row]
 #pragma unroll
-            for (int i = 0; i < VW; ++i)
+            for (int st = 0; st < ST; ++st) {
 #pragma unroll
-                for (int st = 0; st < ST; ++st) {
-                    uint32_t a[4], e[4];
-                    e4m3x4_to_f16(__byte_perm(vw[st][0][i], vw[st][1][i], 0x5140), a[0], a[1]);
-                    e4m3x4_to_f16(__byte_perm(vw[st][2][i], vw[st][3][i], 0x5140), a[2], a[3]);
-                    e4m3x4_to_f16(__byte_perm(vw[st][0][i], vw[st][1][i], 0x7362), e[0], e[1]);
-                    e4m3x4_to_f16(__byte_perm(vw[st][2][i], vw[st][3][i], 0x7362), e[2], e[3]);
+                for (int half = 0; half < (D == 256 ? 2 : 1); ++half) {
+                    constexpr int W = D == 64 ? 2 : 4;                       // words of a lane and key
+                    uint32_t vw[4][W];
 #pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) {
-                        mma_f16_16816(acc[nt][2 * i], a, pf[st][nt][0], pf[st][nt][1]);
-                        mma_f16_16816(acc[nt][2 * i + 1], e, pf[st][nt][0], pf[st][nt][1]);
+                    for (int x = 0; x < 4; ++x) {                            // k indices 2c, 2c + 1, 2c + 8, 2c + 9
+                        if constexpr (D == 64) {
+                            const uint2 w = ld_shared_v2(base + v_off + (st * 16 + (x & 1) + 8 * (x >> 1)) * 64);
+                            vw[x][0] = w.x; vw[x][1] = w.y;
+                        } else {
+                            const uint4 w = ld_shared_v4(base + (x & 1 ? (v_off ^ 64) + 512 : v_off) + (st * 16 + 8 * (x >> 1)) * 128 +
+                                                         half * (KT * 128));
+                            vw[x][0] = w.x; vw[x][1] = w.y; vw[x][2] = w.z; vw[x][3] = w.w;
+                        }
+                        if (!open) {
+                            // what lies outside the item's keys may be anything, and 0 x NaN is NaN
+                            const int key = key0 + st * 16 + (D == 64 ? 2 * c + (x & 1) : c + 4 * (x & 1)) + 8 * (x >> 1);
+                            if (key >= cur.key_hi || key < cur.key_lo) {
+#pragma unroll
+                                for (int y = 0; y < W; ++y) vw[x][y] = 0;
+                            }
+                        }
+                    }
+#pragma unroll
+                    for (int y = 0; y < W; ++y) {
+                        const int j = 2 * (half * 4 + y);
+                        uint32_t a[4], e[4];
+                        e4m3x4_to_f16(__byte_perm(vw[0][y], vw[1][y], 0x5140), a[0], a[1]);
+                        e4m3x4_to_f16(__byte_perm(vw[2][y], vw[3][y], 0x5140), a[2], a[3]);
+                        e4m3x4_to_f16(__byte_perm(vw[0][y], vw[1][y], 0x7362), e[0], e[1]);
+                        e4m3x4_to_f16(__byte_perm(vw[2][y], vw[3][y], 0x7362), e[2], e[3]);
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt) {
+                            mma_f16_16816(acc[nt][j], a, pf[st][nt][0], pf[st][nt][1]);
+                            mma_f16_16816(acc[nt][j + 1], e, pf[st][nt][0], pf[st][nt][1]);
+                        }
                     }
                 }
-            if (next < tile_hi) load_v(next);
-            tile = next;
+            }
+            __syncwarp();                                                    // the slot is read: the next tile may land there
+            copy();
+            seek();
+            if (++slot == SLOTS) { slot = 0; phase ^= 1; }
         }
 
         // ---------------- the warps' results
@@ -462,16 +578,53 @@ paged_attention_kernel(PagedAttnParams p) {
                 t += __shfl_xor_sync(0xffffffffu, t, 4);
                 t += __shfl_xor_sync(0xffffffffu, t, 8);
                 t += __shfl_xor_sync(0xffffffffu, t, 16);
-                const int r = nt * 8 + 2 * c + x;
-                if (g == 0) ml_s[warp][r] = make_float2(m[nt][x], t);
-                float* dst = acc_s + ((size_t)warp * ROWS + r) * Cfg::PITCH + g * (D / 8);
-#pragma unroll
-                for (int j = 0; j < MT; j += 2)
-                    *reinterpret_cast<float4*>(dst + 2 * j) =
-                        make_float4(acc[nt][j][x], acc[nt][j][2 + x], acc[nt][j + 1][x], acc[nt][j + 1][2 + x]);
+                if (g == 0) ml_s[warp][nt * 8 + 2 * c + x] = make_float2(m[nt][x], t);
             }
-        __syncthreads();
-        const bool split = !(at == first && end == first + s.tiles);
+        // this lane's row and dimensions 4 i .. 4 i + 3 of its piece in an accumulator
+        auto place = [&](int w, int nt, int x, int i) {
+            const int d = D == 64 ? g * 8 + 4 * i : (i >> 2) * 128 + dchunk * 16 + 4 * (i & 3);
+            return reinterpret_cast<float4*>(acc_s + ((size_t)w * ROWS + nt * 8 + 2 * c + x) * Cfg::PITCH + d);
+        };
+        auto put = [&](int w) {
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int x = 0; x < 2; ++x)
+#pragma unroll
+                    for (int i = 0; i < MT / 2; ++i)
+                        *place(w, nt, x, i) = make_float4(acc[nt][2 * i][x], acc[nt][2 * i][2 + x], acc[nt][2 * i + 1][x], acc[nt][2 * i + 1][2 + x]);
+        };
+        if constexpr (Cfg::WRITERS == NW) {
+            put(warp);
+            __syncthreads();
+        } else {
+            // the upper half's accumulators first, each into the registers of a warp of the lower half
+            if (warp >= NW / 2) put(warp - NW / 2);
+            __syncthreads();
+            if (warp < NW / 2) {
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int x = 0; x < 2; ++x) {
+                        const int r = nt * 8 + 2 * c + x;
+                        const float2 a = ml_s[warp][r], b = ml_s[warp + NW / 2][r];
+                        const float mm = fmaxf(a.x, b.x), safe = mm == -INFINITY ? 0.0f : mm, fa = ex2(a.x - safe), fb = ex2(b.x - safe);
+#pragma unroll
+                        for (int i = 0; i < MT / 2; ++i) {
+                            const float4 o = *place(warp, nt, x, i);
+                            acc[nt][2 * i][x] = acc[nt][2 * i][x] * fa + o.x * fb;
+                            acc[nt][2 * i][2 + x] = acc[nt][2 * i][2 + x] * fa + o.y * fb;
+                            acc[nt][2 * i + 1][x] = acc[nt][2 * i + 1][x] * fa + o.z * fb;
+                            acc[nt][2 * i + 1][2 + x] = acc[nt][2 * i + 1][2 + x] * fa + o.w * fb;
+                        }
+                        __syncwarp();
+                        if (g == 0) ml_s[warp][r] = make_float2(mm, a.y * fa + b.y * fb);
+                    }
+                put(warp);
+            }
+            __syncthreads();
+        }
+        const bool split = !(at == cur.first && cur.end == cur.first + cur.tiles);
         const int slot = at == w0 ? 0 : 1;
         const size_t part = (size_t)cta * 2 + slot;
         auto finish = [&](int r, int d4, float4 sum, float mm, float ll) {
@@ -480,7 +633,7 @@ paged_attention_kernel(PagedAttnParams p) {
             uint2 out;
             out.x = pack_bf16x2(sum.x * inv, sum.y * inv);
             out.y = pack_bf16x2(sum.z * inv, sum.w * inv);
-            const int token = s.start + i;
+            const int token = cur.start + i;
             st_global_v2(p.o + (size_t)token * p.o_stride + (size_t)hh * D + d4 * 4, out);
             if (d4 == 0 && p.lse)
                 p.lse[(size_t)hh * p.tokens + token] = ll == 0.0f ? -INFINITY : 0.6931471805599453f * (mm - 15.0f + log2f(ll));
@@ -489,11 +642,11 @@ paged_attention_kernel(PagedAttnParams p) {
             const int r = x / (D / 4), d4 = x % (D / 4);
             float mm = -INFINITY, ll = 0.0f;
 #pragma unroll
-            for (int w = 0; w < NW; ++w) mm = fmaxf(mm, ml_s[w][r].x);
+            for (int w = 0; w < Cfg::WRITERS; ++w) mm = fmaxf(mm, ml_s[w][r].x);
             const float safe = mm == -INFINITY ? 0.0f : mm;
             float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
-            for (int w = 0; w < NW; ++w) {
+            for (int w = 0; w < Cfg::WRITERS; ++w) {
                 const float f = ex2(ml_s[w][r].x - safe);
                 const float4 v = *reinterpret_cast<const float4*>(acc_s + ((size_t)w * ROWS + r) * Cfg::PITCH + d4 * 4);
                 ll = fmaf(ml_s[w][r].y, f, ll);
@@ -509,7 +662,7 @@ paged_attention_kernel(PagedAttnParams p) {
         }
         if (split) {
             // CTAs of the item: from the one with its first unit to the one with its last
-            const long long last_unit = first + s.tiles - 1;
+            const long long first = cur.first, last_unit = first + cur.tiles - 1;
             auto owner = [&](long long u) { return (int)(((u + 1) * grid - 1) / total); };
             const int c0 = owner(first), c1 = owner(last_unit);
             __threadfence();
@@ -540,17 +693,40 @@ paged_attention_kernel(PagedAttnParams p) {
                 }
             }
         }
-        at = end;
-        first += s.tiles;
-        ++item;
+        at = cur.end;
+    }
+    if (abort_s) {                       // a wait gave up: copies may be in flight, a bounded time for them to land
+        const uint64_t until = tc::global_timer_ns() + 1000000ull;
+        while (tc::global_timer_ns() < until) {}
     }
 }
 
 template <int D, int NT>
-static int paged_grid() { return min(device_sm_count() * PagedCfg<D, NT>::CTAS, PA_MAX_GRID); }
+static int paged_grid() { return min(device_sm_count(), PA_MAX_GRID); }
 template <int D, int NT>
 static long long paged_workspace() {
     return 4 * PA_MAX_GRID + (long long)paged_grid<D, NT>() * 2 * PagedCfg<D, NT>::ROWS * (D + 2) * 4;
+}
+
+// A cache as a matrix of head_dim bytes a row; boxes of `box` rows x 128 bytes (64 for heads of 64), swizzled over that width.  Rows
+// behind the last one read as zeros.
+static int paged_map(CUtensorMap* out, const void* base, int rows, int d, int box) {
+    typedef CUresult (*Encode)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                               const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion,
+                               CUtensorMapFloatOOBfill);
+    static const Encode encode = [] {
+        void* fn = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        const cudaError_t e = cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &q);
+        return e == cudaSuccess && q == cudaDriverEntryPointSuccess ? reinterpret_cast<Encode>(fn) : nullptr;
+    }();
+    if (!encode) return FRT_ERR_UNSUPPORTED;
+    const cuuint64_t dims[2] = {(cuuint64_t)d, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)d};
+    const cuuint32_t boxes[2] = {(cuuint32_t)(d < 128 ? d : 128), (cuuint32_t)box}, ones[2] = {1, 1};
+    const CUresult r = encode(out, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, boxes, ones,
+                              CU_TENSOR_MAP_INTERLEAVE_NONE, d < 128 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
+                              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? FRT_OK : FRT_ERR_INVALID;
 }
 
 template <int D, int NT>
@@ -569,6 +745,11 @@ static int launch_paged_attention(PagedAttnParams p, void* work, long long work_
     p.counters = static_cast<unsigned*>(work);
     p.part_ml = reinterpret_cast<float2*>(static_cast<uint8_t*>(work) + 4 * PA_MAX_GRID);
     p.part_o = reinterpret_cast<float*>(p.part_ml + (size_t)grid * 2 * Cfg::ROWS);
+    CUtensorMap tmK, tmV;
+    const int box = Cfg::KT < p.block_size ? Cfg::KT : p.block_size;
+    int rc = paged_map(&tmK, p.k, p.pool_rows, D, box);
+    if (!rc) rc = paged_map(&tmV, p.v, p.pool_rows, D, box);
+    if (rc) return rc;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(grid);
     cfg.blockDim = dim3(Cfg::THREADS);
@@ -579,25 +760,44 @@ static int launch_paged_attention(PagedAttnParams p, void* work, long long work_
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, paged_attention_kernel<D, NT>, p);
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, paged_attention_kernel<D, NT>, tmK, tmV, p);
     return e == cudaSuccess ? FRT_OK : FRT_CUDA_ERR(e);
 }
 
 }  // namespace frt
 
-// Row tiles of 8 or 16: a decode step's group, or more rows, which then read the keys once per 16.
-static bool paged_two(long long max_new, int hq, int hkv) { return max_new * (hq / hkv) > 8; }
+// Row tiles of 8 NT rows, so that the keys are read and converted as few times as the registers of the accumulators allow (heads of
+// 256: 16 rows, else 32), and no wider than the rows need.
+static int paged_nt(long long max_new, int group, int d) {
+    const int most = d == 256 ? 2 : 4;
+    const long long rows = max_new * group, tiles = (rows + 8 * most - 1) / (8 * most);
+    return tiles < 1 ? 1 : tiles > 4 ? most : (int)((rows + 8 * tiles - 1) / (8 * tiles));
+}
+// f(kernel's head dim, row tile) for one of the instances
+template <typename F>
+static auto paged_dispatch(int d, int nt, F f) {
+    using std::integral_constant;
+    auto with = [&](auto D) {
+        if constexpr (D() != 256) {
+            if (nt == 4) return f(D, integral_constant<int, 4>());
+            if (nt == 3) return f(D, integral_constant<int, 3>());
+        }
+        if (nt == 2) return f(D, integral_constant<int, 2>());
+        return f(D, integral_constant<int, 1>());
+    };
+    if (d == 64) return with(integral_constant<int, 64>());
+    if (d == 128) return with(integral_constant<int, 128>());
+    return with(integral_constant<int, 256>());
+}
 
 extern "C" int frt_b200_paged_attention_workspace_bytes(int tokens, int batch, int max_new, int num_heads_q, int num_heads_kv,
                                                         int head_dim, long long* out_bytes) {
     using namespace frt;
     if (!out_bytes || tokens < 0 || batch < 0 || max_new < 0 || num_heads_q < 1 || num_heads_kv < 1) return FRT_ERR_INVALID;
     if (num_heads_q % num_heads_kv) return FRT_ERR_UNSUPPORTED;
-    const bool two = paged_two(max_new, num_heads_q, num_heads_kv);
-    if (head_dim == 64) *out_bytes = two ? paged_workspace<64, 2>() : paged_workspace<64, 1>();
-    else if (head_dim == 128) *out_bytes = two ? paged_workspace<128, 2>() : paged_workspace<128, 1>();
-    else if (head_dim == 256) *out_bytes = two ? paged_workspace<256, 2>() : paged_workspace<256, 1>();
-    else return FRT_ERR_UNSUPPORTED;
+    if (head_dim != 64 && head_dim != 128 && head_dim != 256) return FRT_ERR_UNSUPPORTED;
+    *out_bytes = paged_dispatch(head_dim, paged_nt(max_new, num_heads_q / num_heads_kv, head_dim),
+                                [](auto D, auto NT) { return paged_workspace<D(), NT()>(); });
     return FRT_OK;
 }
 
@@ -652,13 +852,11 @@ extern "C" int frt_b200_paged_attention_fp8(const void* Q, long long q_stride, v
     p.window = window;
     p.causal = causal;
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
-    const bool two = paged_two(max_new, num_heads_q, num_heads_kv);
-    if (head_dim == 64)
-        return two ? launch_paged_attention<64, 2>(p, workspace, workspace_bytes, st)
-                   : launch_paged_attention<64, 1>(p, workspace, workspace_bytes, st);
-    if (head_dim == 128)
-        return two ? launch_paged_attention<128, 2>(p, workspace, workspace_bytes, st)
-                   : launch_paged_attention<128, 1>(p, workspace, workspace_bytes, st);
-    return two ? launch_paged_attention<256, 2>(p, workspace, workspace_bytes, st)
-               : launch_paged_attention<256, 1>(p, workspace, workspace_bytes, st);
+    const long long pool_rows = (long long)num_blocks * num_heads_kv * block_size;
+    if (pool_rows > 0x7fffffffLL) return FRT_ERR_UNSUPPORTED;
+    p.pool_rows = (int)pool_rows;
+    p.status = attention_status_device_ptr();
+    if (!p.status) return FRT_ERR_UNSUPPORTED;
+    return paged_dispatch(head_dim, paged_nt(max_new, p.group, head_dim),
+                          [&](auto D, auto NT) { return launch_paged_attention<D(), NT()>(p, workspace, workspace_bytes, st); });
 }
