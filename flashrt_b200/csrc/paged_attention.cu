@@ -12,10 +12,9 @@
 // the row's largest lose bits).
 //
 // What bounds it: a decode step reads every key and value once and does 4 x group flops per byte, so memory does, and the kernel is
-// built to keep copies in flight.  Every warp works alone: it owns a ring of slots (KT keys and their values, 8 KB each) that it fills
-// itself by TMA, two or three tiles ahead and across the items of its work, so neither the join of an item's warps nor the set-up of
-// the next one lets the memory wait.  (The form before loaded into registers, one tile ahead: 64 sequences of 1500 .. 6000 tokens, 32
-// heads on 8 of 128: 142 us, memory 42 % busy, every second cycle of a warp spent on a load.)
+// built to keep copies in flight.  One warp copies -- a lane per block, by TMA, into a ring of stages, across the items of the CTA's
+// work, so that neither the join of an item's warps nor the set-up of the next lets the memory wait -- and the others take KT keys each
+// of every stage.
 // Codes go from shared memory to the tensor cores as fp16: keys are the M rows of K . Q^T and dimensions the M rows of V^T . P^T
 // (mma.sync m16n8k16), so a group of up to eight query rows fills the N side and no tensor work is wasted.  Which dimension a k index
 // stands for is free, hence a lane's 16 contiguous bytes serve four k steps; the pairs of keys that V^T wants side by side come from
@@ -33,11 +32,12 @@
 
 #include <cuda_fp16.h>
 
+#include <climits>
 #include <type_traits>
 
 namespace frt {
 
-constexpr int PA_MAX_GRID = 1024;                     // counters at the head of the workspace
+constexpr int PA_MAX_GRID = 256, PA_HEAD_BYTES = 4096;      // arrival counters at the head of the workspace
 
 struct PagedAttnParams {
     const __nv_bfloat16* q;
@@ -60,26 +60,29 @@ struct PagedAttnParams {
 template <int D, int NT>
 struct PagedCfg {
     static constexpr int ROWS = 8 * NT;
-    static constexpr int KT = 4096 / D;               // keys of a warp's tile: 4 KB of keys, 4 KB of values
-    static constexpr int ST = KT / 16;                // 16-key steps
-    static constexpr int NW = 8;
-    static constexpr int THREADS = 32 * NW;
-    static constexpr int SLOT_BYTES = 2 * KT * D;
-    static constexpr int SLOTS = NT == 1 && D <= 128 ? 3 : 2;
-    static constexpr int RING_BYTES = NW * SLOTS * SLOT_BYTES;
-    static constexpr int WRITERS = NT == 1 && D != 128 ? NW : NW / 2;      // warps whose accumulators are in shared memory at once
+    static constexpr int NW = 8;                  // warps that compute; one more copies
+    static constexpr int KT = D == 256 ? 16 : 32; // keys of a warp
+    static constexpr int ST = KT / 16;
+    static constexpr int UK = NW * KT;                // keys of a stage, and unit of the work line
+    static constexpr int THREADS = 32 * (NW + 1);
+    static constexpr int STAGE_BYTES = 2 * UK * D;
+    static constexpr int BUFS = 4;                    // warps whose accumulators are in shared memory at once
     static constexpr int PITCH = D + 4;               // floats of an accumulator row in shared memory
     static constexpr int Q_BYTES = NT * (D / 16) * 32 * 8;
-    static constexpr int ACC_BYTES = WRITERS * ROWS * PITCH * 4;
+    static constexpr int ACC_BYTES = BUFS * ROWS * PITCH * 4;
+    static constexpr int ROOM = 232448 - 1024 - 6 * 1024 - Q_BYTES - ACC_BYTES;
+    static constexpr int STAGES = ROOM / STAGE_BYTES < 6 ? ROOM / STAGE_BYTES : 6;
+    static constexpr int RING_BYTES = STAGES * STAGE_BYTES;
     static constexpr int SMEM_BYTES = 1024 + RING_BYTES + Q_BYTES + ACC_BYTES;
     static constexpr bool Q_REGS = NT == 1;           // query fragments stay in registers
-    static_assert(SMEM_BYTES <= 232448 - 6 * 1024, "dynamic and static shared memory of a CTA");
+    static_assert(STAGES >= 2, "shared memory");
+    static_assert(ACC_BYTES / 4 / ROWS >= PA_MAX_GRID, "weights of the pieces of an item");
 };
 
 // One sequence's share of the work line.
 struct PagedSeq { int start, n, len, row_tiles, t0, tiles; };
 
-template <int KT, int ROWS>
+template <int UK, int ROWS>
 __device__ __forceinline__ PagedSeq paged_seq(const PagedAttnParams& p, int b) {
     PagedSeq s;
     s.start = p.cu ? min(max(p.cu[b], 0), p.tokens) : b;
@@ -88,19 +91,29 @@ __device__ __forceinline__ PagedSeq paged_seq(const PagedAttnParams& p, int b) {
     s.len = min(max(p.lens[b], 0), (int)min((long long)p.table_stride << p.block_shift, 0x7fffff00LL));
     s.row_tiles = (int)(((long long)s.n * p.group + ROWS - 1) / ROWS);
     const int lo = p.window > 0 ? max(0, s.len - s.n - p.window + 1) : 0;
-    s.t0 = lo / KT;
-    s.tiles = max(1, (s.len + KT - 1) / KT - s.t0);             // an item without keys still writes its rows
+    s.t0 = lo / UK;
+    s.tiles = max(1, (s.len + UK - 1) / UK - s.t0);             // an item without keys still writes its rows
     return s;
 }
-template <int KT, int ROWS>
+template <int UK, int ROWS>
 __device__ __forceinline__ long long paged_units(const PagedAttnParams& p, int b) {
-    const PagedSeq s = paged_seq<KT, ROWS>(p, b);
+    const PagedSeq s = paged_seq<UK, ROWS>(p, b);
     return (long long)s.row_tiles * s.tiles * p.hkv;
 }
 
 __device__ __forceinline__ float ex2(float x) {
     float r;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+__device__ __forceinline__ float lg2(float x) {
+    float r;
+    asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+__device__ __forceinline__ float rcp(float x) {
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
     return r;
 }
 __device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
@@ -138,36 +151,49 @@ __device__ __forceinline__ float ld_shared_f(uint32_t a) {
     asm volatile("ld.shared.f32 %0, [%1];" : "=f"(r) : "r"(a) : "memory");
     return r;
 }
-// 4 bytes to shared memory (zero if !there); the thread's arrival at `bar` follows its copies
-__device__ __forceinline__ void copy_scale(uint32_t dst, const float* src, bool there, uint32_t bar) {
-    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(there ? 4 : 0) : "memory");
-    asm volatile("cp.async.mbarrier.arrive.noinc.shared.b64 [%0];" ::"r"(bar) : "memory");
-}
+__device__ __forceinline__ void st_shared_zero(uint32_t a) { asm volatile("st.shared.v4.u32 [%0], {%1,%1,%1,%1};" ::"r"(a), "r"(0) : "memory"); }
+// the warps that compute meet without the one that copies
+__device__ __forceinline__ void sync_threads(int n) { asm volatile("bar.sync 1, %0;" ::"r"(n) : "memory"); }
 
 // tanh through the hardware's exp2 and reciprocal: 2^-22 absolute, where tanh.approx has 2^-11
 __device__ __forceinline__ float soft_cap(float s, float cap, float inv_cap2) {
-    float r;
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + ex2(s * inv_cap2)));
-    return cap * (1.0f - 2.0f * r);
+    return cap * (1.0f - 2.0f * rcp(1.0f + ex2(s * inv_cap2)));
 }
 
-// A stretch of the work line inside one item: what a warp has to know to copy its tiles, and where the item's rows are.
+// The line cut into `grid` stretches whose lengths differ by one at most.
+struct PagedShare {
+    long long each;
+    int longer;                  // the first ones have one unit more
+    __device__ __forceinline__ PagedShare(long long total, int grid) {
+        each = total < 0x7fffffffLL ? (long long)((unsigned)total / (unsigned)grid) : total / grid;
+        longer = (int)(total - each * grid);
+    }
+    __device__ __forceinline__ long long begin(int cta) const { return each * cta + min(cta, longer); }
+    __device__ __forceinline__ int owner(long long unit) const {
+        const long long head = (each + 1) * longer;
+        if (unit < head) return head < 0x7fffffffLL ? (int)((unsigned)unit / (unsigned)(each + 1)) : (int)(unit / (each + 1));
+        return longer + (unit - head < 0x7fffffffLL && each < 0x7fffffffLL ? (int)((unsigned)(unit - head) / (unsigned)each)
+                                                                          : (int)((unit - head) / each));
+    }
+};
+
+// A stretch of the work line inside one item: the units to copy, and where the item's rows are.
 struct PagedSegment {
     int b, item;                 // sequence; (head, row tile) inside it
     long long first, end;        // line positions: of the item, behind the stretch
     int items, h, row0, rows, tiles;
     int len, n, start;
     int key_lo, key_hi;          // keys that any row sees
-    int tile_lo, tile_hi;        // tiles of the stretch with such keys
+    int unit_lo, unit_hi;        // units of the stretch with such keys
 };
 // the stretch that begins at line position `at` < w1; b, item, first are set
-template <int KT, int ROWS>
+template <int UK, int ROWS>
 __device__ __forceinline__ void paged_segment(const PagedAttnParams& p, PagedSegment& g, long long at, long long w1) {
-    PagedSeq s = paged_seq<KT, ROWS>(p, g.b);
+    PagedSeq s = paged_seq<UK, ROWS>(p, g.b);
     while (g.item >= s.row_tiles * p.hkv && g.b + 1 < p.batch) {             // through with the sequence, or one without new tokens
         ++g.b;
         g.item = 0;
-        s = paged_seq<KT, ROWS>(p, g.b);
+        s = paged_seq<UK, ROWS>(p, g.b);
     }
     g.items = s.row_tiles * p.hkv;
     g.h = g.item / s.row_tiles;
@@ -181,15 +207,16 @@ __device__ __forceinline__ void paged_segment(const PagedAttnParams& p, PagedSeg
     const int p0 = s.len - s.n + g.row0 / p.group, p1 = s.len - s.n + (g.row0 + g.rows - 1) / p.group;
     g.key_lo = p.window > 0 ? max(0, p0 - p.window + 1) : 0;
     g.key_hi = p.causal ? min(s.len, p1 + 1) : s.len;
-    g.tile_lo = max(s.t0 + (int)(at - g.first), g.key_lo / KT);
-    g.tile_hi = min(s.t0 + (int)(g.end - g.first), g.key_hi > 0 ? (g.key_hi + KT - 1) / KT : 0);
+    g.unit_lo = max(s.t0 + (int)(at - g.first), g.key_lo / UK);
+    g.unit_hi = min(s.t0 + (int)(g.end - g.first), g.key_hi > 0 ? (g.key_hi + UK - 1) / UK : 0);
 }
 
 template <int D, int NT>
-__global__ void __launch_bounds__(256, 1)
+__global__ void __launch_bounds__((PagedCfg<D, NT>::THREADS), 1)
 paged_attention_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, PagedAttnParams p) {
     using Cfg = PagedCfg<D, NT>;
-    constexpr int ST = Cfg::ST, KT = Cfg::KT, NW = Cfg::NW, ROWS = Cfg::ROWS, SEGS = D / 64, MT = D / 16, SLOTS = Cfg::SLOTS;
+    constexpr int ST = Cfg::ST, KT = Cfg::KT, UK = Cfg::UK, NW = Cfg::NW, ROWS = Cfg::ROWS, SEGS = D / 64, MT = D / 16;
+    constexpr int STAGES = Cfg::STAGES, SCAN = 256;
     constexpr float LOG2E = 1.4426950408889634f;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
@@ -197,137 +224,181 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
     float* acc_s = reinterpret_cast<float*>(smem + Cfg::RING_BYTES + Cfg::Q_BYTES);       // [warp][row][PITCH]
     __shared__ float2 ml_s[NW][ROWS];
     __shared__ float rf_s[ROWS];
-    __shared__ float scale_s[NW][SLOTS][ST][2];
-    __shared__ uint64_t full_s[NW][SLOTS];
-    __shared__ long long scan_s[256];
-    __shared__ long long warp_s[8];
+    __shared__ float2 scale_s[STAGES][UK / 16];                              // per 16 keys: of the keys, of the values
+    __shared__ uint64_t full_s[STAGES], empty_s[STAGES];
+    __shared__ long long warp_s[SCAN / 32], first_s;
+    __shared__ int begin_s[2];
     __shared__ unsigned last_s;
     __shared__ volatile int abort_s;
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
-    if (lane < SLOTS) tc::mbar_init(&full_s[warp][lane], 1 + 2 * ST);        // the copies' bytes, one arrival per scale
     if (tid == 0) {
+        for (int s = 0; s < STAGES; ++s) {
+            tc::mbar_init(&full_s[s], 2);                                    // the copies' bytes; the scales
+            tc::mbar_init(&empty_s[s], NW);
+        }
+        abort_s = 0;
+        tc::mbar_fence_init();
         tc::tma_prefetch_desc(&tmK);
         tc::tma_prefetch_desc(&tmV);
     }
-    tc::mbar_fence_init();
     const uint64_t deadline = tc::global_timer_ns() + FRT_KERNEL_DEADLINE_NS;
-    if (tid == 0) abort_s = 0;
     pdl_launch_dependents();
     pdl_wait();
 
     // ---------------- the work line: thread t counts the units of sequences [t * per, (t + 1) * per)
-    const int per = (p.batch + 255) / 256;
-    long long mine = 0;
-    for (int b = tid * per; b < min((tid + 1) * per, p.batch); ++b) mine += paged_units<KT, ROWS>(p, b);
-    long long incl = mine;
+    const int per = (p.batch + SCAN - 1) / SCAN;
+    long long mine = 0, incl;
+    if (tid < SCAN) {
+        for (int b = tid * per; b < min((tid + 1) * per, p.batch); ++b) mine += paged_units<UK, ROWS>(p, b);
+        incl = mine;
 #pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-        const long long o = __shfl_up_sync(0xffffffffu, incl, d);
-        if (lane >= d) incl += o;
+        for (int d = 1; d < 32; d <<= 1) {
+            const long long o = __shfl_up_sync(0xffffffffu, incl, d);
+            if (lane >= d) incl += o;
+        }
+        if (lane == 31) warp_s[warp] = incl;
     }
-    if (lane == 31) warp_s[warp] = incl;
     __syncthreads();
     long long before = 0, total = 0;
 #pragma unroll
-    for (int w = 0; w < 8; ++w) {
+    for (int w = 0; w < SCAN / 32; ++w) {
         if (w < warp) before += warp_s[w];
         total += warp_s[w];
     }
-    scan_s[tid] = before + incl - mine;                                      // exclusive
-    __syncthreads();
-    // few units: as many CTAs as give every warp one
-    const int grid = (int)max(1LL, min((long long)gridDim.x, (total + NW - 1) / NW));
+    const int grid = (int)max(1LL, min((long long)gridDim.x, total));
     const int cta = blockIdx.x;
     if (cta >= grid || total == 0) return;
-    const long long w0 = total * cta / grid, w1 = total * (cta + 1) / grid;
+    const PagedShare share(total, grid);
+    const long long w0 = share.begin(cta), w1 = share.begin(cta + 1);
+    if (tid < SCAN && mine > 0) {
+        long long first = before + incl - mine;
+        if (first <= w0 && w0 < first + mine) {                              // one thread's sequences hold the first unit
+            int b = tid * per;
+            for (;;) {
+                const long long u = per == 1 ? mine : paged_units<UK, ROWS>(p, b);
+                if (w0 < first + u) break;
+                first += u;
+                ++b;
+            }
+            const int units = paged_seq<UK, ROWS>(p, b).tiles;
+            const long long in = w0 - first;
+            const int item = in < 0x7fffffffLL ? (int)((unsigned)in / (unsigned)units) : (int)(in / units);
+            begin_s[0] = b;
+            begin_s[1] = item;
+            first_s = first + (long long)item * units;
+        }
+    }
+    __syncthreads();
     PagedSegment cur;
-    {
-        int lo = 0, hi = 256;
-        while (hi - lo > 1) {
-            const int mid = (lo + hi) >> 1;
-            if (scan_s[mid] <= w0) lo = mid; else hi = mid;
-        }
-        cur.b = lo * per;
-        cur.first = scan_s[lo];
-        for (;;) {                                                           // ends before the chunk does: w0 lies in it
-            const long long u = paged_units<KT, ROWS>(p, cur.b);
-            if (w0 < cur.first + u || cur.b + 1 >= p.batch) break;
-            cur.first += u;
-            ++cur.b;
-        }
-        cur.item = (int)((w0 - cur.first) / paged_seq<KT, ROWS>(p, cur.b).tiles);
-        cur.first += (long long)cur.item * paged_seq<KT, ROWS>(p, cur.b).tiles;
-    }
-    paged_segment<KT, ROWS>(p, cur, w0, w1);
-
-    // ---------------- this warp's copies: `nx` runs ahead of the computation by the slots of the ring
-    const uint32_t ring = tc::smem_u32(smem) + (uint32_t)warp * (SLOTS * Cfg::SLOT_BYTES);
-    const uint32_t full_a = tc::smem_u32(&full_s[warp][0]), scale_a = tc::smem_u32(&scale_s[warp][0][0][0]);
-    PagedSegment nx = cur;
-    int nx_tile = cur.tile_lo + warp, nx_page = -1, nx_slot = 0;
-    // to the next tile there is for this warp; lanes 2 st, 2 st + 1 ask for the page of its st-th 16 keys
-    auto seek = [&] {
-        while (nx_tile >= nx.tile_hi) {
-            if (nx.end >= w1) { nx_tile = 0x7fffffff; return; }
-            const long long at = nx.end;
-            nx.first = at;                                                   // a stretch that does not end the work ends its item
-            ++nx.item;
-            paged_segment<KT, ROWS>(p, nx, at, w1);
-            nx_tile = nx.tile_lo + warp;
-        }
-        const int k0 = nx_tile * KT + (lane >> 1) * 16, box = min(KT, p.block_size), head = k0 & ~(box - 1);
-        nx_page = -1;                                                        // a box without keys of the item is not looked at
-        if (lane < 2 * ST && head < nx.key_hi && head + box > nx.key_lo)
-            nx_page = p.table[(size_t)nx.b * p.table_stride + (head >> p.block_shift)];
-        if (nx_page >= p.num_blocks) nx_page = -1;
-    };
-    auto copy = [&] {
-        if (nx_tile == 0x7fffffff) return;
-        const uint32_t bar = full_a + 8 * nx_slot, dst = ring + nx_slot * Cfg::SLOT_BYTES;
-        if (lane < 2 * ST) {
-            const float* src = lane & 1 ? p.v_scale : p.k_scale;
-            copy_scale(scale_a + (nx_slot * ST * 2 + lane) * 4, src + (size_t)max(nx_page, 0) * p.hkv + nx.h, nx_page >= 0, bar);
-        }
-        if (lane == 0) tc::mbar_arrive_expect_tx(bar, Cfg::SLOT_BYTES);
-        // one box per block (or per tile inside one): lane 2 st of its first 16 keys issues it; rows beyond the pool arrive as zeros
-        const int box = min(KT, p.block_size), st = lane >> 1;
-        if (lane < 2 * ST && (st * 16) % box == 0) {
-            const int k0 = nx_tile * KT + st * 16;
-            const int row = nx_page >= 0 ? (nx_page * p.hkv + nx.h) * p.block_size + (k0 & (p.block_size - 1)) : p.pool_rows;
-            const CUtensorMap* map = lane & 1 ? &tmV : &tmK;
-            constexpr int INNER = D < 128 ? D : 128;
-            const uint32_t to = dst + (lane & 1) * (KT * D) + st * 16 * INNER;
-#pragma unroll
-            for (int x = 0; x < D; x += INNER) tc::tma_load_2d(to + x * KT, map, bar, x, row);
-        }
-        if (++nx_slot == SLOTS) nx_slot = 0;
-        nx_tile += NW;
-    };
-    for (int i = 0; i < SLOTS; ++i) {
-        seek();
-        copy();
-    }
-    seek();
-    int slot = 0;
+    cur.b = begin_s[0];
+    cur.item = begin_s[1];
+    cur.first = first_s;
+    paged_segment<UK, ROWS>(p, cur, w0, w1);
+    int stage = 0;
     uint32_t phase = 0;
 
-    // where this lane's operands are in a slot (see the top: groups of lanes four rows or chunks apart)
+    if (warp == NW) {
+        // ---------------- copies: a lane takes a block (or the unit's part of one) of the keys or of the values.  Block numbers are asked for
+        // two units ahead and scales one, so that the wait for a free stage covers their latency (asked for when they were needed,
+        // two trips to memory a stage, they held 64 sequences of 1500 .. 6000 tokens to 4.5 TB/s with nothing computed)
+        const uint32_t ring = tc::smem_u32(smem), full_a = tc::smem_u32(full_s), empty_a = tc::smem_u32(empty_s);
+        const int box = min(UK, p.block_size), boxes = UK / box;
+        constexpr int INNER = D < 128 ? D : 128;
+        constexpr int PER_LANE = UK / 16 * 2 / 32 > 0 ? UK / 16 * 2 / 32 : 1;       // copies of a lane at most
+        const float* my_scale = lane & 1 ? p.v_scale : p.k_scale;
+        const CUtensorMap* map = lane & 1 ? &tmV : &tmK;
+        struct Unit {
+            int page[PER_LANE];      // table entry; INT_MIN: no key of the item there
+            int h, k0;               // key/value head, first key
+            bool there;
+        };
+        int u = cur.unit_lo - 1;
+        auto ask_pages = [&](Unit& n) {
+            n.there = false;
+            if (u == INT_MAX) return;
+            ++u;
+            while (u >= cur.unit_hi) {
+                if (cur.end >= w1) { u = INT_MAX; return; }
+                const long long at = cur.end;                                // a stretch that does not end the work ends its item
+                cur.first = at;
+                ++cur.item;
+                paged_segment<UK, ROWS>(p, cur, at, w1);
+                u = cur.unit_lo;
+            }
+            n.there = true;
+            n.h = cur.h;
+            n.k0 = u * UK;
+#pragma unroll
+            for (int i = 0; i < PER_LANE; ++i) {
+                const int k0 = u * UK + ((lane + 32 * i) >> 1) * box;
+                const bool want = (lane + 32 * i) >> 1 < boxes && k0 < cur.key_hi && k0 + box > cur.key_lo;
+                n.page[i] = want ? max(p.table[(size_t)cur.b * p.table_stride + (k0 >> p.block_shift)], -1) : INT_MIN;
+            }
+        };
+        Unit now, next;
+        float scale[PER_LANE];
+        auto ask_scales = [&] {
+#pragma unroll
+            for (int i = 0; i < PER_LANE; ++i) {
+                if (now.page[i] >= p.num_blocks) now.page[i] = -1;
+                if (now.there && now.page[i] >= 0) scale[i] = my_scale[(size_t)now.page[i] * p.hkv + now.h];
+            }
+        };
+        ask_pages(now);
+        ask_pages(next);
+        ask_scales();
+        while (now.there) {
+            unsigned wanted = 0;
+#pragma unroll
+            for (int i = 0; i < PER_LANE; ++i) wanted += __popc(__ballot_sync(0xffffffffu, now.page[i] != INT_MIN));
+            if (!tc::warp_wait(empty_a + 8 * stage, phase ^ 1, false, deadline, &abort_s)) {
+                if (lane == 0 && !abort_s) atomicCAS(p.status, 0, 1 | (blockIdx.x << 8));
+                abort_s = 1;
+                return;
+            }
+            const uint32_t bar = full_a + 8 * stage, dst = ring + stage * Cfg::STAGE_BYTES;
+            if (lane == 0) tc::mbar_arrive_expect_tx(bar, wanted * (unsigned)(box * D));
+            __syncwarp();
+#pragma unroll
+            for (int i = 0; i < PER_LANE; ++i) {
+                if (now.page[i] == INT_MIN) continue;
+                const int n = (lane + 32 * i) >> 1, in_block = (now.k0 + n * box) & (p.block_size - 1);
+                // no block of the pool: rows behind its end, which arrive as zeros
+                const int row = now.page[i] >= 0 ? (now.page[i] * p.hkv + now.h) * p.block_size + in_block : p.pool_rows;
+                const uint32_t to = dst + (lane & 1) * (UK * D) + n * box * INNER;
+#pragma unroll
+                for (int x = 0; x < D; x += INNER) tc::tma_load_2d(to + x * UK, map, bar, x, row);
+                for (int j = 0; j < box / 16; ++j) (&scale_s[stage][n * (box / 16) + j].x)[lane & 1] = now.page[i] >= 0 ? fmaxf(scale[i], 1e-30f) : 0.0f;
+            }
+            __syncwarp();
+            if (lane == 0) tc::mbar_arrive(&full_s[stage]);
+            if (++stage == STAGES) { stage = 0; phase ^= 1; }
+            now = next;
+            ask_scales();
+            ask_pages(next);
+        }
+        return;
+    }
+
+    // where this lane's operands are in its warp's part of a stage (see the top: groups of lanes four rows or chunks apart)
     const int krow = D == 64 ? g : (g >> 1) | ((g & 1) << 2), dchunk = krow;
     const uint32_t k_off = D == 64 ? g * 64 + ((c ^ ((g >> 1) & 3)) << 4) : krow * 128 + ((c ^ krow) << 4);
-    const uint32_t v_off = KT * D + (D == 64 ? 2 * c * 64 + (((g >> 1) ^ c) << 4) + (g & 1) * 8 : c * 128 + ((dchunk ^ c) << 4));
+    const uint32_t v_off = (D == 64 ? 2 * c * 64 + (((g >> 1) ^ c) << 4) + (g & 1) * 8 : c * 128 + ((dchunk ^ c) << 4));
     constexpr int STEP = D == 64 ? 64 : 128;                                 // bytes from row to row
+    const bool capped = p.cap > 0.0f;
+    const float inv_cap2 = capped ? 2.0f * LOG2E / p.cap : 0.0f;
 
     for (long long at = w0; at < w1;) {
         if (at != w0) {
             cur.first = at;
             ++cur.item;
-            paged_segment<KT, ROWS>(p, cur, at, w1);
+            paged_segment<UK, ROWS>(p, cur, at, w1);
         }
         const int rows = cur.rows, row0 = cur.row0, h = cur.h;
 
         // queries -> fp16 operand fragments, at most 1 in magnitude: one warp per row
-        __syncthreads();                                                     // the item before is through with shared memory
+        sync_threads(32 * NW);                                               // the item before is through with shared memory
         for (int r = warp; r < ROWS; r += NW) {
             constexpr int PL = D / 32;                                       // dimensions of a lane
             float x[PL];
@@ -356,7 +427,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
                 dst[((step * 32 + (r & 7) * 4 + cc) << 2) + place] = __float2half_rn(x[j] * down);
             }
         }
-        __syncthreads();
+        sync_threads(32 * NW);
 
         // this lane's rows: 2c, 2c + 1 of every n tile
         float rf[NT][2];
@@ -366,7 +437,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
                 const int r = nt * 8 + 2 * c + x;
-                rf[nt][x] = rf_s[r] * p.scale * (p.cap > 0.0f ? 1.0f : LOG2E);
+                rf[nt][x] = rf_s[r] * p.scale * (capped ? 1.0f : LOG2E);
                 const int pos = cur.len - cur.n + (row0 + min(r, rows - 1)) / p.group;
                 row_hi[nt][x] = p.causal ? min(pos + 1, cur.len) : cur.len;
                 row_lo[nt][x] = p.window > 0 ? max(0, pos - p.window + 1) : 0;
@@ -391,13 +462,15 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
                 for (int x = 0; x < 4; ++x) acc[nt][j][x] = 0.0f;
         }
 
-        for (int tile = cur.tile_lo + warp; tile < cur.tile_hi; tile += NW) {
-            const uint32_t base = ring + slot * Cfg::SLOT_BYTES;
-            if (!tc::mbar_wait_until(full_a + 8 * slot, phase, deadline, &abort_s)) {
-                if (!abort_s && lane == 0) atomicCAS(p.status, 0, 1 | (blockIdx.x << 8));
+        for (int unit = cur.unit_lo; unit < cur.unit_hi; ++unit) {
+            const int key0 = unit * UK + warp * KT;
+            if (!tc::mbar_wait_until(&full_s[stage], phase, deadline, &abort_s)) {
+                if (!abort_s && lane == 0) atomicCAS(p.status, 0, 2 | (blockIdx.x << 8));
                 abort_s = 1;
             }
             __syncwarp();
+            if (key0 < cur.key_hi && key0 + KT > cur.key_lo) {
+            const uint32_t base = tc::smem_u32(smem) + stage * Cfg::STAGE_BYTES + warp * (KT * STEP), base_v = base + UK * D;
             // ---- scores: [key][row]
             float sc[ST][NT][4];
 #pragma unroll
@@ -409,7 +482,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
 #pragma unroll
             for (int sg = 0; sg < SEGS; ++sg) {
                 uint32_t kw[ST][2][4];
-                const uint32_t kb = base + (sg >> 1) * (KT * 128) + (sg & 1 ? k_off ^ 64 : k_off);
+                const uint32_t kb = base + (sg >> 1) * (UK * 128) + (sg & 1 ? k_off ^ 64 : k_off);
 #pragma unroll
                 for (int st = 0; st < ST; ++st)
 #pragma unroll
@@ -433,32 +506,45 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
                 }
             }
             // ---- base-2 logits with the values' scale, mask, running maximum
-            const int key0 = tile * KT;
             bool open = key0 >= all_lo && key0 + KT <= all_hi;
             float ks[ST], lv[ST], inv_vs[ST], top[NT][2];
 #pragma unroll
             for (int st = 0; st < ST; ++st) {
-                ks[st] = ld_shared_f(scale_a + ((slot * ST + st) * 2) * 4);
-                const float vs = ld_shared_f(scale_a + ((slot * ST + st) * 2 + 1) * 4);
-                open = open && vs != 0.0f;                                   // zero: an absent page
-                lv[st] = __log2f(fmaxf(vs, 1e-30f));
-                inv_vs[st] = vs != 0.0f ? __frcp_rn(fmaxf(vs, 1e-30f)) : 0.0f;
+                // a step without keys of the item has no scales: anything, all of it masked
+                const float2 s = scale_s[stage][warp * ST + st];
+                const bool there = s.y != 0.0f && key0 + st * 16 < cur.key_hi && key0 + st * 16 + 16 > cur.key_lo;
+                open = open && there;
+                ks[st] = there ? s.x : 0.0f;
+                lv[st] = there ? lg2(s.y) : 0.0f;
+                inv_vs[st] = there ? rcp(s.y) : 0.0f;
             }
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) top[nt][0] = top[nt][1] = -INFINITY;
 #pragma unroll
             for (int st = 0; st < ST; ++st)
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
+                for (int nt = 0; nt < NT; ++nt) {
+                    const float f[2] = {rf[nt][0] * ks[st], rf[nt][1] * ks[st]};
 #pragma unroll
-                    for (int x = 0; x < 4; ++x) {
-                        const float f = rf[nt][x & 1] * ks[st];
-                        float u;
-                        if (p.cap > 0.0f) u = fmaf(soft_cap(sc[st][nt][x] * f, p.cap, 2.0f * LOG2E / p.cap), LOG2E, lv[st]);
-                        else u = fmaf(sc[st][nt][x], f, lv[st]);
-                        sc[st][nt][x] = u;
-                    }
+                    for (int x = 0; x < 4; ++x) sc[st][nt][x] = fmaf(sc[st][nt][x], f[x & 1], capped ? 0.0f : lv[st]);
+                }
+            if (capped) {
+#pragma unroll
+                for (int st = 0; st < ST; ++st)
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                        for (int x = 0; x < 4; ++x) sc[st][nt][x] = fmaf(soft_cap(sc[st][nt][x], p.cap, inv_cap2), LOG2E, lv[st]);
+            }
             if (!open) {
+                // values outside the item's keys may be anything, and 0 x NaN is NaN: zero their rows, 16 bytes a lane
+                for (int i = lane; i < KT * (D / 16); i += 32) {
+                    const int r = i / (D / 16), ch = i % (D / 16);
+                    if (key0 + r >= cur.key_hi || key0 + r < cur.key_lo)
+                        st_shared_zero(base_v + (D == 256 ? (ch >> 3) * (UK * 128) + r * 128 + (ch & 7) * 16 : r * STEP + ch * 16));
+                }
+                tc::fence_proxy_async_smem();                                // before the next copy of this stage
+                __syncwarp();
 #pragma unroll
                 for (int st = 0; st < ST; ++st)
 #pragma unroll
@@ -466,7 +552,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
 #pragma unroll
                         for (int x = 0; x < 4; ++x) {
                             const int key = key0 + st * 16 + krow + 8 * (x >> 1);
-                            if (inv_vs[st] == 0.0f || key >= row_hi[nt][x & 1] || key < row_lo[nt][x & 1]) sc[st][nt][x] = -INFINITY;
+                            if (ks[st] == 0.0f || key >= row_hi[nt][x & 1] || key < row_lo[nt][x & 1]) sc[st][nt][x] = -INFINITY;
                         }
             }
 #pragma unroll
@@ -531,20 +617,12 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
 #pragma unroll
                     for (int x = 0; x < 4; ++x) {                            // k indices 2c, 2c + 1, 2c + 8, 2c + 9
                         if constexpr (D == 64) {
-                            const uint2 w = ld_shared_v2(base + v_off + (st * 16 + (x & 1) + 8 * (x >> 1)) * 64);
+                            const uint2 w = ld_shared_v2(base_v + v_off + (st * 16 + (x & 1) + 8 * (x >> 1)) * 64);
                             vw[x][0] = w.x; vw[x][1] = w.y;
                         } else {
-                            const uint4 w = ld_shared_v4(base + (x & 1 ? (v_off ^ 64) + 512 : v_off) + (st * 16 + 8 * (x >> 1)) * 128 +
-                                                         half * (KT * 128));
+                            const uint4 w = ld_shared_v4(base_v + (x & 1 ? (v_off ^ 64) + 512 : v_off) + (st * 16 + 8 * (x >> 1)) * 128 +
+                                                         half * (UK * 128));
                             vw[x][0] = w.x; vw[x][1] = w.y; vw[x][2] = w.z; vw[x][3] = w.w;
-                        }
-                        if (!open) {
-                            // what lies outside the item's keys may be anything, and 0 x NaN is NaN
-                            const int key = key0 + st * 16 + (D == 64 ? 2 * c + (x & 1) : c + 4 * (x & 1)) + 8 * (x >> 1);
-                            if (key >= cur.key_hi || key < cur.key_lo) {
-#pragma unroll
-                                for (int y = 0; y < W; ++y) vw[x][y] = 0;
-                            }
                         }
                     }
 #pragma unroll
@@ -563,10 +641,10 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
                     }
                 }
             }
-            __syncwarp();                                                    // the slot is read: the next tile may land there
-            copy();
-            seek();
-            if (++slot == SLOTS) { slot = 0; phase ^= 1; }
+            }
+            __syncwarp();
+            if (lane == 0) tc::mbar_arrive(&empty_s[stage]);
+            if (++stage == STAGES) { stage = 0; phase ^= 1; }
         }
 
         // ---------------- the warps' results
@@ -594,24 +672,23 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
                     for (int i = 0; i < MT / 2; ++i)
                         *place(w, nt, x, i) = make_float4(acc[nt][2 * i][x], acc[nt][2 * i][2 + x], acc[nt][2 * i + 1][x], acc[nt][2 * i + 1][2 + x]);
         };
-        if constexpr (Cfg::WRITERS == NW) {
-            put(warp);
-            __syncthreads();
-        } else {
-            // the upper half's accumulators first, each into the registers of a warp of the lower half
-            if (warp >= NW / 2) put(warp - NW / 2);
-            __syncthreads();
-            if (warp < NW / 2) {
+        // four warps at a time hand theirs to the four below, until four are left
+        constexpr int BUFS = Cfg::BUFS;
+#pragma unroll 1
+        for (int top_warp = NW; top_warp > BUFS; top_warp -= BUFS) {
+            if (warp >= top_warp - BUFS && warp < top_warp) put(warp & (BUFS - 1));
+            sync_threads(32 * NW);
+            if (warp >= top_warp - 2 * BUFS && warp < top_warp - BUFS) {
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                     for (int x = 0; x < 2; ++x) {
                         const int r = nt * 8 + 2 * c + x;
-                        const float2 a = ml_s[warp][r], b = ml_s[warp + NW / 2][r];
+                        const float2 a = ml_s[warp][r], b = ml_s[warp + BUFS][r];
                         const float mm = fmaxf(a.x, b.x), safe = mm == -INFINITY ? 0.0f : mm, fa = ex2(a.x - safe), fb = ex2(b.x - safe);
 #pragma unroll
                         for (int i = 0; i < MT / 2; ++i) {
-                            const float4 o = *place(warp, nt, x, i);
+                            const float4 o = *place(warp & (BUFS - 1), nt, x, i);
                             acc[nt][2 * i][x] = acc[nt][2 * i][x] * fa + o.x * fb;
                             acc[nt][2 * i][2 + x] = acc[nt][2 * i][2 + x] * fa + o.y * fb;
                             acc[nt][2 * i + 1][x] = acc[nt][2 * i + 1][x] * fa + o.z * fb;
@@ -620,10 +697,10 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
                         __syncwarp();
                         if (g == 0) ml_s[warp][r] = make_float2(mm, a.y * fa + b.y * fb);
                     }
-                put(warp);
             }
-            __syncthreads();
         }
+        if (warp < BUFS) put(warp);
+        sync_threads(32 * NW);
         const bool split = !(at == cur.first && cur.end == cur.first + cur.tiles);
         const int slot = at == w0 ? 0 : 1;
         const size_t part = (size_t)cta * 2 + slot;
@@ -638,15 +715,15 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
             if (d4 == 0 && p.lse)
                 p.lse[(size_t)hh * p.tokens + token] = ll == 0.0f ? -INFINITY : 0.6931471805599453f * (mm - 15.0f + log2f(ll));
         };
-        for (int x = tid; x < rows * (D / 4); x += Cfg::THREADS) {
+        for (int x = tid; x < rows * (D / 4); x += 32 * NW) {
             const int r = x / (D / 4), d4 = x % (D / 4);
             float mm = -INFINITY, ll = 0.0f;
 #pragma unroll
-            for (int w = 0; w < Cfg::WRITERS; ++w) mm = fmaxf(mm, ml_s[w][r].x);
+            for (int w = 0; w < BUFS; ++w) mm = fmaxf(mm, ml_s[w][r].x);
             const float safe = mm == -INFINITY ? 0.0f : mm;
             float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
-            for (int w = 0; w < Cfg::WRITERS; ++w) {
+            for (int w = 0; w < BUFS; ++w) {
                 const float f = ex2(ml_s[w][r].x - safe);
                 const float4 v = *reinterpret_cast<const float4*>(acc_s + ((size_t)w * ROWS + r) * Cfg::PITCH + d4 * 4);
                 ll = fmaf(ml_s[w][r].y, f, ll);
@@ -663,33 +740,62 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
         if (split) {
             // CTAs of the item: from the one with its first unit to the one with its last
             const long long first = cur.first, last_unit = first + cur.tiles - 1;
-            auto owner = [&](long long u) { return (int)(((u + 1) * grid - 1) / total); };
-            const int c0 = owner(first), c1 = owner(last_unit);
-            __threadfence();
-            __syncthreads();
-            if (tid == 0) last_s = atomicInc(p.counters + c0, (unsigned)(c1 - c0)) == (unsigned)(c1 - c0);
-            __syncthreads();
-            if (last_s) {
+            const int c0 = share.owner(first), c1 = share.owner(last_unit);
+            sync_threads(32 * NW);
+            if (tid == 0) {
+                __threadfence();                                             // the whole CTA's stores (it met at the barrier)
+                last_s = atomicInc(p.counters + c0, (unsigned)(c1 - c0)) == (unsigned)(c1 - c0);
                 __threadfence();
-                const int slot0 = total * c0 / grid < first;                 // the first CTA had another item in front
-                for (int x = tid; x < rows * (D / 4); x += Cfg::THREADS) {
-                    const int r = x / (D / 4), d4 = x % (D / 4);
-                    auto piece = [&](int q) { return (size_t)q * 2 + (q == c0 ? slot0 : 0); };
+            }
+            sync_threads(32 * NW);
+            if (last_s) {
+                const int slot0 = share.begin(c0) < first;                   // the first CTA had another item in front
+                const int pieces = c1 - c0 + 1;
+                const size_t part0 = (size_t)c0 * 2 + slot0;                 // the others' are at 2 (c0 + q)
+                // a warp per row: maximum, weights of the pieces (in the accumulators' space), sum
+                float* weight_s = acc_s;
+                const int cap = Cfg::ACC_BYTES / 4 / ROWS;                   // pieces whose weights fit; all, where a CTA per SM is the grid
+                for (int r = warp; r < rows; r += NW) {
                     float mm = -INFINITY, ll = 0.0f;
-                    for (int q = c0; q <= c1; ++q) mm = fmaxf(mm, __ldcg(p.part_ml + piece(q) * ROWS + r).x);
+                    for (int q = lane; q < pieces; q += 32) mm = fmaxf(mm, __ldcg(p.part_ml + (q ? ((size_t)c0 + q) * 2 : part0) * ROWS + r).x);
+                    mm = warp_max_butterfly(mm);
                     const float safe = mm == -INFINITY ? 0.0f : mm;
-                    float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 4
-                    for (int q = c0; q <= c1; ++q) {
-                        const size_t at_q = piece(q) * ROWS + r;
-                        const float2 ml = __ldcg(p.part_ml + at_q);
-                        const float4 v = __ldcg(reinterpret_cast<const float4*>(p.part_o + at_q * D + d4 * 4));
+                    for (int q = lane; q < pieces; q += 32) {
+                        const float2 ml = __ldcg(p.part_ml + (q ? ((size_t)c0 + q) * 2 : part0) * ROWS + r);
                         const float f = ex2(ml.x - safe);
+                        weight_s[r * cap + q] = f;
                         ll = fmaf(ml.y, f, ll);
+                    }
+                    ll = warp_sum_butterfly(ll);
+                    if (lane == 0) ml_s[0][r] = make_float2(mm, ll);
+                }
+                sync_threads(32 * NW);
+                for (int x = tid; x < rows * (D / 4); x += 32 * NW) {
+                    const int r = x / (D / 4), d4 = x % (D / 4);
+                    float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                    auto add = [&](float4 v, float f) {
                         sum.x = fmaf(v.x, f, sum.x); sum.y = fmaf(v.y, f, sum.y);
                         sum.z = fmaf(v.z, f, sum.z); sum.w = fmaf(v.w, f, sum.w);
+                    };
+                    const float* src = p.part_o + (size_t)r * D + d4 * 4;
+                    const float* w = weight_s + r * cap;
+                    add(__ldcg(reinterpret_cast<const float4*>(src + part0 * (ROWS * D))), w[0]);
+                    int q = 1;
+                    for (; q + 8 <= pieces; q += 8) {                        // eight loads in flight
+                        float4 v[8];
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) v[i] = __ldcg(reinterpret_cast<const float4*>(src + ((size_t)c0 + q + i) * (2 * ROWS * D)));
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) add(v[i], w[q + i]);
                     }
-                    finish(r, d4, sum, mm, ll);
+                    float4 v[8];
+#pragma unroll
+                    for (int i = 0; i < 7; ++i)
+                        if (q + i < pieces) v[i] = __ldcg(reinterpret_cast<const float4*>(src + ((size_t)c0 + q + i) * (2 * ROWS * D)));
+#pragma unroll
+                    for (int i = 0; i < 7; ++i)
+                        if (q + i < pieces) add(v[i], w[q + i]);
+                    finish(r, d4, sum, ml_s[0][r].x, ml_s[0][r].y);
                 }
             }
         }
@@ -705,7 +811,7 @@ template <int D, int NT>
 static int paged_grid() { return min(device_sm_count(), PA_MAX_GRID); }
 template <int D, int NT>
 static long long paged_workspace() {
-    return 4 * PA_MAX_GRID + (long long)paged_grid<D, NT>() * 2 * PagedCfg<D, NT>::ROWS * (D + 2) * 4;
+    return PA_HEAD_BYTES + (long long)paged_grid<D, NT>() * 2 * PagedCfg<D, NT>::ROWS * (D + 2) * 4;
 }
 
 // A cache as a matrix of head_dim bytes a row; boxes of `box` rows x 128 bytes (64 for heads of 64), swizzled over that width.  Rows
@@ -743,10 +849,10 @@ static int launch_paged_attention(PagedAttnParams p, void* work, long long work_
     const int grid = paged_grid<D, NT>();
     if (work_bytes < paged_workspace<D, NT>()) return FRT_ERR_INVALID;
     p.counters = static_cast<unsigned*>(work);
-    p.part_ml = reinterpret_cast<float2*>(static_cast<uint8_t*>(work) + 4 * PA_MAX_GRID);
+    p.part_ml = reinterpret_cast<float2*>(static_cast<uint8_t*>(work) + PA_HEAD_BYTES);
     p.part_o = reinterpret_cast<float*>(p.part_ml + (size_t)grid * 2 * Cfg::ROWS);
     CUtensorMap tmK, tmV;
-    const int box = Cfg::KT < p.block_size ? Cfg::KT : p.block_size;
+    const int box = Cfg::UK < p.block_size ? Cfg::UK : p.block_size;
     int rc = paged_map(&tmK, p.k, p.pool_rows, D, box);
     if (!rc) rc = paged_map(&tmV, p.v, p.pool_rows, D, box);
     if (rc) return rc;
