@@ -12,9 +12,9 @@
 // the row's largest lose bits).
 //
 // What bounds it: a decode step reads every key and value once and does 4 x group flops per byte, so memory does, and the kernel is
-// built to keep copies in flight.  One warp copies -- a lane per block, by TMA, into a ring of stages, across the items of the CTA's
-// work, so that neither the join of an item's warps nor the set-up of the next lets the memory wait -- and the others take KT keys each
-// of every stage.
+// built to keep copies in flight.  Up to four warps copy -- a lane per block, by TMA, into a ring of stages, across the items of the CTA's
+// work, so that neither the join of an item's warps nor the set-up of the next lets the memory wait -- and two or three groups of four
+// take the stages in turn, a warp KT keys.
 // Codes go from shared memory to the tensor cores as fp16: keys are the M rows of K . Q^T and dimensions the M rows of V^T . P^T
 // (mma.sync m16n8k16), so a group of up to eight query rows fills the N side and no tensor work is wasted.  Which dimension a k index
 // stands for is free, hence a lane's 16 contiguous bytes serve four k steps; the pairs of keys that V^T wants side by side come from
@@ -37,7 +37,7 @@
 
 namespace frt {
 
-constexpr int PA_MAX_GRID = 256, PA_HEAD_BYTES = 4096;      // arrival counters at the head of the workspace
+constexpr int PA_MAX_GRID = 512, PA_HEAD_BYTES = 4096;      // arrival counters at the head of the workspace
 
 struct PagedAttnParams {
     const __nv_bfloat16* q;
@@ -60,23 +60,36 @@ struct PagedAttnParams {
 template <int D, int NT>
 struct PagedCfg {
     static constexpr int ROWS = 8 * NT;
-    static constexpr int NW = 8;                  // warps that compute; one more copies
-    static constexpr int KT = D == 256 ? 16 : 32; // keys of a warp
+    // Warps that compute, in groups of four: a group takes a stage, a warp KT of its keys.  With eight rows two CTAs share an SM, each
+    // with a group and a share of the line of its own: one joins an item while the other streams (64 sequences of 1500 .. 6000 tokens
+    // 98.7 -> 90.4 us; heads of 256 on one short sequence 11.8 -> 16.7, so they keep one CTA).
+    static constexpr int CTAS = NT == 1 && D <= 128 ? 2 : 1;
+    static constexpr int GROUPS = CTAS == 2 ? 1 : 2;
+    static constexpr int NW = 4 * GROUPS;
+    static constexpr int KT = D == 256 ? 16 : 32;
     static constexpr int ST = KT / 16;
-    static constexpr int UK = NW * KT;                // keys of a stage, and unit of the work line
-    static constexpr int THREADS = 32 * (NW + 1);
+    static constexpr int UK = 4 * KT;                 // keys of a stage, and unit of the work line
+    static constexpr int THREADS = 32 * (NW + 4);     // and a group that copies
+    // registers of a thread: 128 or 168 at launch; the warps that compute take what the others give (4 x 176 + 4 x 80 = 8 x 128,
+    // 8 x 200 + 4 x 104 = 12 x 168)
+    static constexpr int REGS_COMPUTE = CTAS == 2 ? 176 : 200, REGS_COPY = CTAS == 2 ? 80 : 104;
     static constexpr int STAGE_BYTES = 2 * UK * D;
-    static constexpr int BUFS = 4;                    // warps whose accumulators are in shared memory at once
+    static constexpr int BUFS = CTAS == 2 ? 2 : 4;    // warps whose accumulators are in shared memory at once
     static constexpr int PITCH = D + 4;               // floats of an accumulator row in shared memory
     static constexpr int Q_BYTES = NT * (D / 16) * 32 * 8;
     static constexpr int ACC_BYTES = BUFS * ROWS * PITCH * 4;
-    static constexpr int ROOM = 232448 - 1024 - 6 * 1024 - Q_BYTES - ACC_BYTES;
-    static constexpr int STAGES = ROOM / STAGE_BYTES < 6 ? ROOM / STAGE_BYTES : 6;
+    static constexpr int ROOM = (CTAS == 2 ? 115200 - 1024 - 1536 : 232448 - 1024 - 6 * 1024) - Q_BYTES - ACC_BYTES;    // static: below 1536 or 6 K
+    static constexpr int FIT = ROOM / STAGE_BYTES < 12 ? ROOM / STAGE_BYTES : 12;
+    static constexpr int STAGES = FIT / GROUPS * GROUPS;
+    // Warps that copy, each every COPIERS-th unit.  A warp that waits for a stage's k-th release tells it by the phase's parity, which is
+    // right as long as the release before the last has happened.  Its own unit before, COPIERS back, found a stage whose unit
+    // before, STAGES further back, was released, and one group's releases are in order: the same group as this stage's, if
+    // COPIERS and STAGES are multiples of GROUPS, and a later unit than the one in question, if COPIERS <= STAGES.
+    static constexpr int COPIERS = STAGES < 4 ? STAGES / GROUPS * GROUPS : 4;
+    static_assert(COPIERS <= STAGES && COPIERS % GROUPS == 0 && STAGES % GROUPS == 0 && STAGES >= 2, "parity of a stage's releases");
     static constexpr int RING_BYTES = STAGES * STAGE_BYTES;
     static constexpr int SMEM_BYTES = 1024 + RING_BYTES + Q_BYTES + ACC_BYTES;
     static constexpr bool Q_REGS = NT == 1;           // query fragments stay in registers
-    static_assert(STAGES >= 2, "shared memory");
-    static_assert(ACC_BYTES / 4 / ROWS >= PA_MAX_GRID, "weights of the pieces of an item");
 };
 
 // One sequence's share of the work line.
@@ -151,8 +164,15 @@ __device__ __forceinline__ float ld_shared_f(uint32_t a) {
     asm volatile("ld.shared.f32 %0, [%1];" : "=f"(r) : "r"(a) : "memory");
     return r;
 }
+// a box that nobody reads again soon: with the default policy a cache larger than L2 pushes itself through it (96.6 us for 90.4, above)
+__device__ __forceinline__ void tma_load_once(uint32_t dst, const CUtensorMap* m, uint32_t bar, int x, int y, uint64_t policy) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1, {%3, %4}], [%2], %5;"
+        ::"r"(dst), "l"(m), "r"(bar), "r"(x), "r"(y), "l"(policy)
+        : "memory");
+}
 __device__ __forceinline__ void st_shared_zero(uint32_t a) { asm volatile("st.shared.v4.u32 [%0], {%1,%1,%1,%1};" ::"r"(a), "r"(0) : "memory"); }
-// the warps that compute meet without the one that copies
+// the warps that compute meet without those that copy
 __device__ __forceinline__ void sync_threads(int n) { asm volatile("bar.sync 1, %0;" ::"r"(n) : "memory"); }
 
 // tanh through the hardware's exp2 and reciprocal: 2^-22 absolute, where tanh.approx has 2^-11
@@ -212,7 +232,7 @@ __device__ __forceinline__ void paged_segment(const PagedAttnParams& p, PagedSeg
 }
 
 template <int D, int NT>
-__global__ void __launch_bounds__((PagedCfg<D, NT>::THREADS), 1)
+__global__ void __launch_bounds__((PagedCfg<D, NT>::THREADS), (PagedCfg<D, NT>::CTAS))
 paged_attention_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, PagedAttnParams p) {
     using Cfg = PagedCfg<D, NT>;
     constexpr int ST = Cfg::ST, KT = Cfg::KT, UK = Cfg::UK, NW = Cfg::NW, ROWS = Cfg::ROWS, SEGS = D / 64, MT = D / 16;
@@ -235,7 +255,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
     if (tid == 0) {
         for (int s = 0; s < STAGES; ++s) {
             tc::mbar_init(&full_s[s], 2);                                    // the copies' bytes; the scales
-            tc::mbar_init(&empty_s[s], NW);
+            tc::mbar_init(&empty_s[s], 4);
         }
         abort_s = 0;
         tc::mbar_fence_init();
@@ -266,7 +286,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
         if (w < warp) before += warp_s[w];
         total += warp_s[w];
     }
-    const int grid = (int)max(1LL, min((long long)gridDim.x, total));
+    const int grid = (int)max(1LL, min((long long)gridDim.x, (total + Cfg::GROUPS - 1) / Cfg::GROUPS));   // a unit for every group
     const int cta = blockIdx.x;
     if (cta >= grid || total == 0) return;
     const PagedShare share(total, grid);
@@ -298,34 +318,44 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
     int stage = 0;
     uint32_t phase = 0;
 
-    if (warp == NW) {
-        // ---------------- copies: a lane takes a block (or the unit's part of one) of the keys or of the values.  Block numbers are asked for
-        // two units ahead and scales one, so that the wait for a free stage covers their latency (asked for when they were needed,
-        // two trips to memory a stage, they held 64 sequences of 1500 .. 6000 tokens to 4.5 TB/s with nothing computed)
+    auto next_segment = [&] {                                                // a stretch that does not end the work ends its item
+        const long long at = cur.end;
+        cur.first = at;
+        ++cur.item;
+        paged_segment<UK, ROWS>(p, cur, at, w1);
+    };
+    if (warp >= NW) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Cfg::REGS_COPY));
+        if (warp >= NW + Cfg::COPIERS) return;
+        // ---------------- copies: a warp takes every COPIERS-th unit, a lane a block (or the unit's part of one) of its keys or of its values.
+        // A unit costs its warp 1800 to 2600 clocks -- two dependent trips to memory for block number and scale, and some 100 a copy,
+        // which its uniform operands make the lanes issue one by one -- where a stage takes 2700 to arrive (of 256 keys then): with one warp, 64 sequences
+        // of 1500 .. 6000 tokens in blocks of 32 took 99.6 us
         const uint32_t ring = tc::smem_u32(smem), full_a = tc::smem_u32(full_s), empty_a = tc::smem_u32(empty_s);
         const int box = min(UK, p.block_size), boxes = UK / box;
         constexpr int INNER = D < 128 ? D : 128;
         constexpr int PER_LANE = UK / 16 * 2 / 32 > 0 ? UK / 16 * 2 / 32 : 1;       // copies of a lane at most
         const float* my_scale = lane & 1 ? p.v_scale : p.k_scale;
         const CUtensorMap* map = lane & 1 ? &tmV : &tmK;
+        const uint64_t once = tc::l2_policy_evict_first();
         struct Unit {
             int page[PER_LANE];      // table entry; INT_MIN: no key of the item there
             int h, k0;               // key/value head, first key
             bool there;
         };
-        int u = cur.unit_lo - 1;
+        int u = cur.unit_lo, skip = warp - NW;                               // this warp's next unit is `skip` behind u
         auto ask_pages = [&](Unit& n) {
             n.there = false;
-            if (u == INT_MAX) return;
-            ++u;
-            while (u >= cur.unit_hi) {
-                if (cur.end >= w1) { u = INT_MAX; return; }
-                const long long at = cur.end;                                // a stretch that does not end the work ends its item
-                cur.first = at;
-                ++cur.item;
-                paged_segment<UK, ROWS>(p, cur, at, w1);
+            for (;;) {
+                const int left = max(cur.unit_hi - u, 0);
+                if (skip < left) break;
+                skip -= left;
+                if (cur.end >= w1) { u = cur.unit_hi; return; }
+                next_segment();
                 u = cur.unit_lo;
             }
+            u += skip;
+            skip = Cfg::COPIERS;
             n.there = true;
             n.h = cur.h;
             n.k0 = u * UK;
@@ -345,6 +375,11 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
                 if (now.there && now.page[i] >= 0) scale[i] = my_scale[(size_t)now.page[i] * p.hkv + now.h];
             }
         };
+        auto step = [&](int n) {                                             // units -> stages
+            stage += n;
+            while (stage >= STAGES) { stage -= STAGES; phase ^= 1; }
+        };
+        step(warp - NW);
         ask_pages(now);
         ask_pages(next);
         ask_scales();
@@ -368,12 +403,12 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
                 const int row = now.page[i] >= 0 ? (now.page[i] * p.hkv + now.h) * p.block_size + in_block : p.pool_rows;
                 const uint32_t to = dst + (lane & 1) * (UK * D) + n * box * INNER;
 #pragma unroll
-                for (int x = 0; x < D; x += INNER) tc::tma_load_2d(to + x * UK, map, bar, x, row);
+                for (int x = 0; x < D; x += INNER) tma_load_once(to + x * UK, map, bar, x, row, once);
                 for (int j = 0; j < box / 16; ++j) (&scale_s[stage][n * (box / 16) + j].x)[lane & 1] = now.page[i] >= 0 ? fmaxf(scale[i], 1e-30f) : 0.0f;
             }
             __syncwarp();
             if (lane == 0) tc::mbar_arrive(&full_s[stage]);
-            if (++stage == STAGES) { stage = 0; phase ^= 1; }
+            step(Cfg::COPIERS);
             now = next;
             ask_scales();
             ask_pages(next);
@@ -381,20 +416,20 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
         return;
     }
 
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(Cfg::REGS_COMPUTE));
+
     // where this lane's operands are in its warp's part of a stage (see the top: groups of lanes four rows or chunks apart)
     const int krow = D == 64 ? g : (g >> 1) | ((g & 1) << 2), dchunk = krow;
     const uint32_t k_off = D == 64 ? g * 64 + ((c ^ ((g >> 1) & 3)) << 4) : krow * 128 + ((c ^ krow) << 4);
     const uint32_t v_off = (D == 64 ? 2 * c * 64 + (((g >> 1) ^ c) << 4) + (g & 1) * 8 : c * 128 + ((dchunk ^ c) << 4));
     constexpr int STEP = D == 64 ? 64 : 128;                                 // bytes from row to row
+    const int group = warp >> 2, part_w = warp & 3;
+    int turn = 0;
     const bool capped = p.cap > 0.0f;
     const float inv_cap2 = capped ? 2.0f * LOG2E / p.cap : 0.0f;
 
     for (long long at = w0; at < w1;) {
-        if (at != w0) {
-            cur.first = at;
-            ++cur.item;
-            paged_segment<UK, ROWS>(p, cur, at, w1);
-        }
+        if (at != w0) next_segment();
         const int rows = cur.rows, row0 = cur.row0, h = cur.h;
 
         // queries -> fp16 operand fragments, at most 1 in magnitude: one warp per row
@@ -462,15 +497,25 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
                 for (int x = 0; x < 4; ++x) acc[nt][j][x] = 0.0f;
         }
 
-        for (int unit = cur.unit_lo; unit < cur.unit_hi; ++unit) {
-            const int key0 = unit * UK + warp * KT;
-            if (!tc::mbar_wait_until(&full_s[stage], phase, deadline, &abort_s)) {
+        // the group's units of the stretch; `stage`, `phase`, `turn`: of the stretch's first
+        const int units = max(cur.unit_hi - cur.unit_lo, 0);
+        int off = group - turn;
+        if (off < 0) off += Cfg::GROUPS;
+        int st_i = stage + off;
+        uint32_t ph_i = phase;
+        if (st_i >= STAGES) { st_i -= STAGES; ph_i ^= 1; }
+        turn = (turn + units) % Cfg::GROUPS;
+        phase ^= (uint32_t)((stage + units) / STAGES) & 1u;
+        stage = (stage + units) % STAGES;
+        for (; off < units; off += Cfg::GROUPS) {
+            const int key0 = (cur.unit_lo + off) * UK + part_w * KT;
+            if (!tc::mbar_wait_until(&full_s[st_i], ph_i, deadline, &abort_s)) {
                 if (!abort_s && lane == 0) atomicCAS(p.status, 0, 2 | (blockIdx.x << 8));
                 abort_s = 1;
             }
             __syncwarp();
             if (key0 < cur.key_hi && key0 + KT > cur.key_lo) {
-            const uint32_t base = tc::smem_u32(smem) + stage * Cfg::STAGE_BYTES + warp * (KT * STEP), base_v = base + UK * D;
+            const uint32_t base = tc::smem_u32(smem) + st_i * Cfg::STAGE_BYTES + part_w * (KT * STEP), base_v = base + UK * D;
             // ---- scores: [key][row]
             float sc[ST][NT][4];
 #pragma unroll
@@ -511,7 +556,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
 #pragma unroll
             for (int st = 0; st < ST; ++st) {
                 // a step without keys of the item has no scales: anything, all of it masked
-                const float2 s = scale_s[stage][warp * ST + st];
+                const float2 s = scale_s[st_i][part_w * ST + st];
                 const bool there = s.y != 0.0f && key0 + st * 16 < cur.key_hi && key0 + st * 16 + 16 > cur.key_lo;
                 open = open && there;
                 ks[st] = there ? s.x : 0.0f;
@@ -643,8 +688,9 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
             }
             }
             __syncwarp();
-            if (lane == 0) tc::mbar_arrive(&empty_s[stage]);
-            if (++stage == STAGES) { stage = 0; phase ^= 1; }
+            if (lane == 0) tc::mbar_arrive(&empty_s[st_i]);
+            st_i += Cfg::GROUPS;
+            if (st_i >= STAGES) { st_i -= STAGES; ph_i ^= 1; }
         }
 
         // ---------------- the warps' results
@@ -754,16 +800,17 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
                 const size_t part0 = (size_t)c0 * 2 + slot0;                 // the others' are at 2 (c0 + q)
                 // a warp per row: maximum, weights of the pieces (in the accumulators' space), sum
                 float* weight_s = acc_s;
-                const int cap = Cfg::ACC_BYTES / 4 / ROWS;                   // pieces whose weights fit; all, where a CTA per SM is the grid
+                constexpr int CAP = Cfg::ACC_BYTES / 4 / ROWS;               // pieces whose weights fit; the others' are formed again
+                auto part_of = [&](int q) { return (q ? ((size_t)c0 + q) * 2 : part0) * ROWS; };
                 for (int r = warp; r < rows; r += NW) {
                     float mm = -INFINITY, ll = 0.0f;
-                    for (int q = lane; q < pieces; q += 32) mm = fmaxf(mm, __ldcg(p.part_ml + (q ? ((size_t)c0 + q) * 2 : part0) * ROWS + r).x);
+                    for (int q = lane; q < pieces; q += 32) mm = fmaxf(mm, __ldcg(p.part_ml + part_of(q) + r).x);
                     mm = warp_max_butterfly(mm);
                     const float safe = mm == -INFINITY ? 0.0f : mm;
                     for (int q = lane; q < pieces; q += 32) {
-                        const float2 ml = __ldcg(p.part_ml + (q ? ((size_t)c0 + q) * 2 : part0) * ROWS + r);
+                        const float2 ml = __ldcg(p.part_ml + part_of(q) + r);
                         const float f = ex2(ml.x - safe);
-                        weight_s[r * cap + q] = f;
+                        if (q < CAP) weight_s[r * CAP + q] = f;
                         ll = fmaf(ml.y, f, ll);
                     }
                     ll = warp_sum_butterfly(ll);
@@ -772,29 +819,21 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
                 sync_threads(32 * NW);
                 for (int x = tid; x < rows * (D / 4); x += 32 * NW) {
                     const int r = x / (D / 4), d4 = x % (D / 4);
+                    const float safe = ml_s[0][r].x == -INFINITY ? 0.0f : ml_s[0][r].x;
                     float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                    auto add = [&](float4 v, float f) {
-                        sum.x = fmaf(v.x, f, sum.x); sum.y = fmaf(v.y, f, sum.y);
-                        sum.z = fmaf(v.z, f, sum.z); sum.w = fmaf(v.w, f, sum.w);
-                    };
-                    const float* src = p.part_o + (size_t)r * D + d4 * 4;
-                    const float* w = weight_s + r * cap;
-                    add(__ldcg(reinterpret_cast<const float4*>(src + part0 * (ROWS * D))), w[0]);
-                    int q = 1;
-                    for (; q + 8 <= pieces; q += 8) {                        // eight loads in flight
+                    for (int q = 0; q < pieces; q += 8) {                    // eight loads in flight
                         float4 v[8];
 #pragma unroll
-                        for (int i = 0; i < 8; ++i) v[i] = __ldcg(reinterpret_cast<const float4*>(src + ((size_t)c0 + q + i) * (2 * ROWS * D)));
+                        for (int i = 0; i < 8; ++i)
+                            if (q + i < pieces) v[i] = __ldcg(reinterpret_cast<const float4*>(p.part_o + (part_of(q + i) + r) * D + d4 * 4));
 #pragma unroll
-                        for (int i = 0; i < 8; ++i) add(v[i], w[q + i]);
+                        for (int i = 0; i < 8; ++i)
+                            if (q + i < pieces) {
+                                const float f = q + i < CAP ? weight_s[r * CAP + q + i] : ex2(__ldcg(p.part_ml + part_of(q + i) + r).x - safe);
+                                sum.x = fmaf(v[i].x, f, sum.x); sum.y = fmaf(v[i].y, f, sum.y);
+                                sum.z = fmaf(v[i].z, f, sum.z); sum.w = fmaf(v[i].w, f, sum.w);
+                            }
                     }
-                    float4 v[8];
-#pragma unroll
-                    for (int i = 0; i < 7; ++i)
-                        if (q + i < pieces) v[i] = __ldcg(reinterpret_cast<const float4*>(src + ((size_t)c0 + q + i) * (2 * ROWS * D)));
-#pragma unroll
-                    for (int i = 0; i < 7; ++i)
-                        if (q + i < pieces) add(v[i], w[q + i]);
                     finish(r, d4, sum, ml_s[0][r].x, ml_s[0][r].y);
                 }
             }
@@ -808,7 +847,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
 }
 
 template <int D, int NT>
-static int paged_grid() { return min(device_sm_count(), PA_MAX_GRID); }
+static int paged_grid() { return min(device_sm_count() * PagedCfg<D, NT>::CTAS, PA_MAX_GRID); }
 template <int D, int NT>
 static long long paged_workspace() {
     return PA_HEAD_BYTES + (long long)paged_grid<D, NT>() * 2 * PagedCfg<D, NT>::ROWS * (D + 2) * 4;
