@@ -50,6 +50,7 @@ struct PagedAttnParams {
     int table_stride, tokens, batch, num_blocks, block_size, block_shift, hq, hkv, group;
     float scale, cap;
     int window, causal;
+    int few_rows;                // sequences with more query rows than this are the other kernel's
     int pool_rows;               // rows of a cache seen as a matrix of head_dim columns
     int* status;
     unsigned* counters;
@@ -101,6 +102,7 @@ __device__ __forceinline__ PagedSeq paged_seq(const PagedAttnParams& p, int b) {
     s.start = p.cu ? min(max(p.cu[b], 0), p.tokens) : b;
     const int end = p.cu ? min(max(p.cu[b + 1], s.start), p.tokens) : b + 1;
     s.n = end - s.start;
+    if ((long long)s.n * p.group > p.few_rows) s.n = 0;
     s.len = min(max(p.lens[b], 0), (int)min((long long)p.table_stride << p.block_shift, 0x7fffff00LL));
     s.row_tiles = (int)(((long long)s.n * p.group + ROWS - 1) / ROWS);
     const int lo = p.window > 0 ? max(0, s.len - s.n - p.window + 1) : 0;
@@ -171,10 +173,18 @@ __device__ __forceinline__ void tma_load_once(uint32_t dst, const CUtensorMap* m
         ::"r"(dst), "l"(m), "r"(bar), "r"(x), "r"(y), "l"(policy)
         : "memory");
 }
+__device__ __forceinline__ void st_shared_v4(uint32_t a, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
+    asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(a), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
+}
 __device__ __forceinline__ void st_shared_zero(uint32_t a) { asm volatile("st.shared.v4.u32 [%0], {%1,%1,%1,%1};" ::"r"(a), "r"(0) : "memory"); }
 // the warps that compute meet without those that copy
 __device__ __forceinline__ void sync_threads(int n) { asm volatile("bar.sync 1, %0;" ::"r"(n) : "memory"); }
 
+__device__ __forceinline__ float inverse_sum(float l) { return l > 0.0f ? __frcp_rn(l) : l; }
+// e with 2^e > top for a row whose largest magnitude is top (zero, tiny: 0; infinite: 0 too, the row is NaN or infinite as it should be)
+__device__ __forceinline__ int query_exponent(float top) {
+    return top > 1e-30f && top < INFINITY ? min((int)((__float_as_uint(top) >> 23) & 255) - 126, 126) : 0;
+}
 // tanh through the hardware's exp2 and reciprocal: 2^-22 absolute, where tanh.approx has 2^-11
 __device__ __forceinline__ float soft_cap(float s, float cap, float inv_cap2) {
     return cap * (1.0f - 2.0f * rcp(1.0f + ex2(s * inv_cap2)));
@@ -450,8 +460,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
 #pragma unroll
             for (int j = 0; j < PL; ++j) top = fmaxf(top, fabsf(x[j]));
             top = warp_max_butterfly(top);
-            // 2^-e with 2^e > top (zero, tiny: no scaling; infinite: neither, the row is NaN or infinite as it should be)
-            const int e = top > 1e-30f && top < INFINITY ? min((int)((__float_as_uint(top) >> 23) & 255) - 126, 126) : 0;
+            const int e = query_exponent(top);
             const float down = __uint_as_float((uint32_t)(127 - e) << 23);
             if (lane == 0) rf_s[r] = __uint_as_float((uint32_t)(127 + e) << 23);
             __half* dst = reinterpret_cast<__half*>(q_s + (r >> 3) * MT * 32);
@@ -752,7 +761,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
         const size_t part = (size_t)cta * 2 + slot;
         auto finish = [&](int r, int d4, float4 sum, float mm, float ll) {
             const int i = (row0 + r) / p.group, hh = h * p.group + (row0 + r) % p.group;
-            const float inv = ll > 0.0f ? __frcp_rn(ll) : (ll == 0.0f ? 0.0f : ll);       // no key: zero; NaN stays
+            const float inv = inverse_sum(ll);
             uint2 out;
             out.x = pack_bf16x2(sum.x * inv, sum.y * inv);
             out.y = pack_bf16x2(sum.z * inv, sum.w * inv);
@@ -853,9 +862,10 @@ static long long paged_workspace() {
     return PA_HEAD_BYTES + (long long)paged_grid<D, NT>() * 2 * PagedCfg<D, NT>::ROWS * (D + 2) * 4;
 }
 
-// A cache as a matrix of head_dim bytes a row; boxes of `box` rows x 128 bytes (64 for heads of 64), swizzled over that width.  Rows
+// A cache as a matrix of head_dim bytes a row; boxes of `box` rows x 128 bytes (64 for heads of 64), swizzled over that width, or of whole
+// rows as they are.  Rows
 // behind the last one read as zeros.
-static int paged_map(CUtensorMap* out, const void* base, int rows, int d, int box) {
+static int paged_map(CUtensorMap* out, const void* base, int rows, int d, int box, bool swizzled) {
     typedef CUresult (*Encode)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
                                const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion,
                                CUtensorMapFloatOOBfill);
@@ -867,15 +877,16 @@ static int paged_map(CUtensorMap* out, const void* base, int rows, int d, int bo
     }();
     if (!encode) return FRT_ERR_UNSUPPORTED;
     const cuuint64_t dims[2] = {(cuuint64_t)d, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)d};
-    const cuuint32_t boxes[2] = {(cuuint32_t)(d < 128 ? d : 128), (cuuint32_t)box}, ones[2] = {1, 1};
+    const cuuint32_t boxes[2] = {(cuuint32_t)(swizzled && d > 128 ? 128 : d), (cuuint32_t)box}, ones[2] = {1, 1};
     const CUresult r = encode(out, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, boxes, ones,
-                              CU_TENSOR_MAP_INTERLEAVE_NONE, d < 128 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
+                              CU_TENSOR_MAP_INTERLEAVE_NONE,
+                              !swizzled ? CU_TENSOR_MAP_SWIZZLE_NONE : d < 128 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
                               CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     return r == CUDA_SUCCESS ? FRT_OK : FRT_ERR_INVALID;
 }
 
 template <int D, int NT>
-static int launch_paged_attention(PagedAttnParams p, void* work, long long work_bytes, cudaStream_t stream) {
+static int launch_paged_attention(PagedAttnParams p, void* work, cudaStream_t stream) {
     using Cfg = PagedCfg<D, NT>;
     static PerDeviceOnce attr_once;
     int attr_dev = 0;
@@ -886,14 +897,13 @@ static int launch_paged_attention(PagedAttnParams p, void* work, long long work_
         attr_once.set(attr_dev);
     }
     const int grid = paged_grid<D, NT>();
-    if (work_bytes < paged_workspace<D, NT>()) return FRT_ERR_INVALID;
     p.counters = static_cast<unsigned*>(work);
     p.part_ml = reinterpret_cast<float2*>(static_cast<uint8_t*>(work) + PA_HEAD_BYTES);
     p.part_o = reinterpret_cast<float*>(p.part_ml + (size_t)grid * 2 * Cfg::ROWS);
     CUtensorMap tmK, tmV;
     const int box = Cfg::UK < p.block_size ? Cfg::UK : p.block_size;
-    int rc = paged_map(&tmK, p.k, p.pool_rows, D, box);
-    if (!rc) rc = paged_map(&tmV, p.v, p.pool_rows, D, box);
+    int rc = paged_map(&tmK, p.k, p.pool_rows, D, box, true);
+    if (!rc) rc = paged_map(&tmV, p.v, p.pool_rows, D, box, true);
     if (rc) return rc;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(grid);
@@ -909,14 +919,28 @@ static int launch_paged_attention(PagedAttnParams p, void* work, long long work_
     return e == cudaSuccess ? FRT_OK : FRT_CUDA_ERR(e);
 }
 
+#include "paged_prefill.cuh"
+
 }  // namespace frt
 
 // Row tiles of 8 NT rows, so that the keys are read and converted as few times as the registers of the accumulators allow (heads of
 // 256: 16 rows, else 32), and no wider than the rows need.
-static int paged_nt(long long max_new, int group, int d) {
+static int paged_nt(long long rows, int d) {
     const int most = d == 256 ? 2 : 4;
-    const long long rows = max_new * group, tiles = (rows + 8 * most - 1) / (8 * most);
+    const long long tiles = (rows + 8 * most - 1) / (8 * most);
     return tiles < 1 ? 1 : tiles > 4 ? most : (int)((rows + 8 * tiles - 1) / (8 * tiles));
+}
+// Query rows of a sequence up to which the kernel for few rows takes it.
+static int paged_few(int d) { return d == 256 ? 16 : 32; }
+// f(head dim, row tiles of a CTA)
+template <typename F>
+static auto prefill_dispatch(int d, long long rows, F f) {
+    using std::integral_constant;
+    if (d == 256) return f(integral_constant<int, 256>(), integral_constant<int, 1>());
+    if (d == 128) return rows > 128 ? f(integral_constant<int, 128>(), integral_constant<int, 2>())
+                                    : f(integral_constant<int, 128>(), integral_constant<int, 1>());
+    return rows > 128 ? f(integral_constant<int, 64>(), integral_constant<int, 2>())
+                      : f(integral_constant<int, 64>(), integral_constant<int, 1>());
 }
 // f(kernel's head dim, row tile) for one of the instances
 template <typename F>
@@ -941,8 +965,13 @@ extern "C" int frt_b200_paged_attention_workspace_bytes(int tokens, int batch, i
     if (!out_bytes || tokens < 0 || batch < 0 || max_new < 0 || num_heads_q < 1 || num_heads_kv < 1) return FRT_ERR_INVALID;
     if (num_heads_q % num_heads_kv) return FRT_ERR_UNSUPPORTED;
     if (head_dim != 64 && head_dim != 128 && head_dim != 256) return FRT_ERR_UNSUPPORTED;
-    *out_bytes = paged_dispatch(head_dim, paged_nt(max_new, num_heads_q / num_heads_kv, head_dim),
-                                [](auto D, auto NT) { return paged_workspace<D(), NT()>(); });
+    const int group = num_heads_q / num_heads_kv, few = paged_few(head_dim);
+    const long long rows = (long long)max_new * group;
+    *out_bytes = paged_dispatch(head_dim, paged_nt(rows < few ? rows : few, head_dim), [](auto D, auto NT) { return paged_workspace<D(), NT()>(); });
+    if (rows > few)
+        *out_bytes += prefill_dispatch(head_dim, rows, [&](auto D, auto T) {
+            return prefill_workspace<D(), T()>(tokens, batch, group, num_heads_kv);
+        });
     return FRT_OK;
 }
 
@@ -955,7 +984,7 @@ extern "C" int frt_b200_paged_attention_fp8(const void* Q, long long q_stride, v
     using namespace frt;
     auto off = [](const void* a, uintptr_t n) { return (reinterpret_cast<uintptr_t>(a) & (n - 1)) != 0; };
     if (tokens < 0 || batch < 0 || max_new < 0 || num_blocks < 0 || table_stride < 0 || num_heads_q < 1 || num_heads_kv < 1 ||
-        window < 0 || !(softcap >= 0.0f) || softcap > 1e30f || !(softmax_scale > -1e30f && softmax_scale < 1e30f))
+        window < 0 || !(softcap >= 0.0f) || softcap > 1e30f || !(softmax_scale > 0.0f && softmax_scale < 1e30f))
         return FRT_ERR_INVALID;
     if (head_dim != 64 && head_dim != 128 && head_dim != 256) return FRT_ERR_UNSUPPORTED;
     if (block_size < 16 || block_size > 128 || (block_size & (block_size - 1))) return FRT_ERR_UNSUPPORTED;
@@ -996,12 +1025,27 @@ extern "C" int frt_b200_paged_attention_fp8(const void* Q, long long q_stride, v
     p.cap = softcap;
     p.window = window;
     p.causal = causal;
-    const cudaStream_t st = static_cast<cudaStream_t>(stream);
+    const cudaStream_t stream_of = static_cast<cudaStream_t>(stream);
     const long long pool_rows = (long long)num_blocks * num_heads_kv * block_size;
     if (pool_rows > 0x7fffffffLL) return FRT_ERR_UNSUPPORTED;
     p.pool_rows = (int)pool_rows;
     p.status = attention_status_device_ptr();
     if (!p.status) return FRT_ERR_UNSUPPORTED;
-    return paged_dispatch(head_dim, paged_nt(max_new, p.group, head_dim),
-                          [&](auto D, auto NT) { return launch_paged_attention<D(), NT()>(p, workspace, workspace_bytes, st); });
+    // Sequences of few rows and of many go to different kernels; a batch whose sequences all bring max_new tokens needs one of them.
+    const int few = paged_few(head_dim);
+    const long long rows = (long long)max_new * p.group;
+    const bool many = rows > few, some_few = !many || (long long)batch * max_new != tokens;
+    p.few_rows = many ? few : INT_MAX;
+    uint8_t* work = static_cast<uint8_t*>(workspace);
+    int rc = FRT_OK;
+    rc = paged_dispatch(head_dim, paged_nt(rows < few ? rows : few, head_dim), [&](auto D, auto NT) {
+            const long long need = paged_workspace<D(), NT()>();
+            if (workspace_bytes < need) return (int)FRT_ERR_INVALID;
+            const int r = some_few ? launch_paged_attention<D(), NT()>(p, work, stream_of) : FRT_OK;
+            work += need;
+            workspace_bytes -= need;
+            return r;
+        });
+    if (rc || !many) return rc;
+    return prefill_dispatch(head_dim, rows, [&](auto D, auto T) { return launch_prefill<D(), T()>(p, work, workspace_bytes, stream_of); });
 }

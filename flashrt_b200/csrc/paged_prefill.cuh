@@ -1,0 +1,617 @@
+#pragma once
+
+// Many query rows over the paged E4M3 cache: chunks of prompts.  Included by paged_attention.cu inside namespace frt.
+//
+// Same formulas as the kernel for few rows.  128 query rows (tokens x the group's heads) are the lanes of a tcgen05 tile; two tiles share
+// every converted tile of keys and values and take turns: the tensor core works for one while the softmax warps of the other work.
+//   S = Q . K^T    kind::f16, queries and codes as fp16 (both exact, see the top of paged_attention.cu) in shared memory
+//   O += P . V     P fp16 from tensor memory, written over S
+// The block's scales stay out of the operands: a column of S has the factor softmax_scale * log2(e) * ks of its 16 keys and the addend
+// log2(vs), which replace the one factor that a softmax has anyway; the sum takes 1 / vs per 16 keys.
+// O is rescaled only when a row's maximum grows by more than 2^8: weights are 2^(u - m + 7) with the stale m, at most 2^15.
+// Warps: 0-3 and 4-7 softmax (thread = row), 8-11 turn E4M3 bytes into swizzled fp16 operands, 12 issues the MMAs, 13 the copies.
+// Heads of 256 (an O of 256 columns) and calls of at most 128 rows have one tile; then two S buffers alternate.
+// Bound by: the tensor pipe (4 x 128 x 128 x 128 products a key tile and pair: some 2050 clocks) and, close to it, the exponentials
+// (2 x 128 x 128 at 16 a clock: 2048).
+template <int D, int T>
+struct PrefillCfg {
+    static_assert(T == 1 || D <= 128, "tensor memory: two tiles of S and O");
+    static constexpr int BKV = D == 256 ? 64 : 128;       // keys of a tile
+    static constexpr int GR = BKV / 16;                   // groups of 16 keys: one block each
+    static constexpr int Q_BYTES = 128 * D * 2, KV_BYTES = BKV * D * 2, RAW_BYTES = BKV * D;
+    static constexpr int OFF_K = T * Q_BYTES, OFF_V = OFF_K + 2 * KV_BYTES, OFF_RAW = OFF_V + 2 * KV_BYTES;
+    static constexpr int SMEM_BYTES = OFF_RAW + 2 * RAW_BYTES + 1024;
+    static constexpr int O_COL = 2 * BKV;                 // accumulators behind the two S
+    static constexpr int THREADS = 512;
+    // registers of a thread: 128 at launch (8 x 184 + 4 x 88 + 4 x 56 = 16 x 128)
+    static constexpr int REGS_SOFTMAX = 184, REGS_CONVERT = 88, REGS_ISSUE = 56;
+    static constexpr int RING = 8;                        // scales of tiles; copies run at most four tiles ahead of the softmax
+    static constexpr float OFFSET = 7.0f, GROWTH = 8.0f;
+};
+
+struct PrefillParams {
+    PagedAttnParams a;
+    int splits;                  // along the keys; pieces joined by the CTA that arrives last at an item
+    unsigned* counters;          // one per item
+    float* part_o;               // [item][split][tile][D][128]
+    float2* part_ml;             // [item][split][tile][128]
+};
+
+template <int D, int T>
+__global__ void __launch_bounds__(512, 1)
+paged_prefill_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const PrefillParams pp) {
+    using Cfg = PrefillCfg<D, T>;
+    constexpr int BKV = Cfg::BKV, GR = Cfg::GR;
+    constexpr float LOG2E = 1.4426950408889634f;
+    const PagedAttnParams& p = pp.a;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+    __shared__ uint64_t raw_full[2], raw_empty[2], k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_half[2], p_ready[2], q_full, o_done;
+    __shared__ float4 scale_s[Cfg::RING][GR];               // per 16 keys: ks, log2 vs, 1 / vs
+    __shared__ int warp_s[16], item_s[2];
+    __shared__ uint32_t tmem_slot;
+    __shared__ unsigned last_s;
+    __shared__ volatile int abort_s;
+
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    if (tid == 0) {
+        for (int i = 0; i < 2; ++i) {
+            tc::mbar_init(&raw_full[i], 2);                 // bytes; scales
+            tc::mbar_init(&raw_empty[i], 4);
+            tc::mbar_init(&k_full[i], 4);
+            tc::mbar_init(&k_empty[i], 1);
+            tc::mbar_init(&v_full[i], 4);
+            tc::mbar_init(&v_empty[i], 1);
+            tc::mbar_init(&s_full[i], 1);
+            tc::mbar_init(&p_half[i], 128);
+            tc::mbar_init(&p_ready[i], 128);
+        }
+        tc::mbar_init(&q_full, 128 * T);
+        tc::mbar_init(&o_done, T);
+        abort_s = 0;
+        tc::mbar_fence_init();
+        tc::tma_prefetch_desc(&tmK);
+        tc::tma_prefetch_desc(&tmV);
+    }
+    if (warp == 12) {
+        tc::tmem_alloc(&tmem_slot, 512);
+        tc::tmem_relinquish();
+    }
+    const uint64_t deadline = tc::global_timer_ns() + FRT_KERNEL_DEADLINE_NS;
+    pdl_launch_dependents();
+    pdl_wait();
+
+    // ---------------- this CTA's item: tiles of the sequences with more than few_rows rows, a sequence's last (most keys) first
+    const int per = (p.batch + 511) / 512;
+    auto tiles_of = [&](int b) {
+        const int start = p.cu ? min(max(p.cu[b], 0), p.tokens) : b, end = p.cu ? min(max(p.cu[b + 1], start), p.tokens) : b + 1;
+        const long long rows = (long long)(end - start) * p.group;
+        return rows > p.few_rows ? (int)((rows + 128 * T - 1) / (128 * T)) : 0;
+    };
+    int mine = 0;
+    for (int b = tid * per; b < min((tid + 1) * per, p.batch); ++b) mine += tiles_of(b);
+    int incl = mine;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+        const int o = __shfl_up_sync(0xffffffffu, incl, d);
+        if (lane >= d) incl += o;
+    }
+    if (lane == 31) warp_s[warp] = incl;
+    if (tid == 0) item_s[0] = -1;
+    tc::tc_fence_before_sync();
+    __syncthreads();
+    tc::tc_fence_after_sync();
+    int first = incl - mine;
+    for (int w = 0; w < warp; ++w) first += warp_s[w];
+    const int want = (int)blockIdx.x;
+    if (mine > 0 && first <= want && want < first + mine) {
+        int b = tid * per;
+        for (;; ++b) {
+            const int n = tiles_of(b);
+            if (want < first + n) {
+                item_s[1] = n - 1 - (want - first);
+                break;
+            }
+            first += n;
+        }
+        item_s[0] = b;
+    }
+    __syncthreads();
+    const int b = item_s[0];
+    const uint32_t tmem = tmem_slot;
+    if (b < 0) {                                            // fewer items than the grid's bound
+        if (warp == 12) tc::tmem_dealloc(tmem, 512);
+        return;
+    }
+    const int start = p.cu ? min(max(p.cu[b], 0), p.tokens) : b, stop = p.cu ? min(max(p.cu[b + 1], start), p.tokens) : b + 1;
+    const int n_new = stop - start, h = (int)blockIdx.y, row0 = item_s[1] * (128 * T);
+    const int rows = (int)min((long long)128 * T, (long long)n_new * p.group - row0);
+    const int len = min(max(p.lens[b], 0), (int)min((long long)p.table_stride << p.block_shift, 0x7fffff00LL));
+    const int p0 = len - n_new + row0 / p.group, p1 = len - n_new + (row0 + rows - 1) / p.group;
+    const int key_lo = p.window > 0 ? max(0, p0 - p.window + 1) : 0;
+    const int key_hi = p.causal ? min(len, p1 + 1) : len;
+    const int jl = key_lo / BKV, jn = max(key_hi > 0 ? (key_hi + BKV - 1) / BKV - jl : 0, 0);
+    const int split = (int)blockIdx.z;
+    const int j0 = jl + (int)((long long)jn * split / pp.splits), j1 = jl + (int)((long long)jn * (split + 1) / pp.splits);
+    const int nt = j1 - j0;
+    const int* table = p.table + (size_t)b * p.table_stride;
+    const uint32_t sm = tc::smem_u32(smem);
+    auto gave_up = [&](int code) {
+        if (!abort_s && lane == 0) atomicCAS(p.status, 0, code | (blockIdx.x << 8));
+        abort_s = 1;
+    };
+
+    if (warp >= 12) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Cfg::REGS_ISSUE));
+        if (warp == 12) {
+            // ---------------- MMA issuer (whole warp)
+            constexpr uint32_t idesc_s = tc::make_idesc(0, 0, 0, 0, 128, BKV);      // fp16, both K-major
+            constexpr uint32_t idesc_o = tc::make_idesc(0, 0, 0, 1, 128, D);        // P from tensor memory, V MN-major
+            const uint64_t dq0 = tc::make_desc_kmajor_sw128(sm), dk0 = tc::make_desc_kmajor_sw128(sm + Cfg::OFF_K);
+            const uint64_t dv0 = tc::make_desc_mnmajor_sw128(sm + Cfg::OFF_V, BKV * 128);
+            // S and its barriers: tile t's own, or the buffers in turn
+            auto buf = [&](int t, int i) { return T == 2 ? t : i & 1; };
+            auto par = [&](int i) { return (uint32_t)((T == 2 ? i : i >> 1) & 1); };
+            auto qk = [&](int t, int i) {
+                const uint64_t dq = dq0 + (uint64_t)(t * (Cfg::Q_BYTES >> 4)), dk = dk0 + (uint64_t)((i & 1) * (Cfg::KV_BYTES >> 4));
+                if (tc::elect_one()) {
+#pragma unroll
+                    for (int k = 0; k < D / 16; ++k)        // 64-element blocks, 32 bytes per step inside
+                        tc::mma_f16(tmem + buf(t, i) * BKV, dq + (uint64_t)((k / 4) * ((128 * 128) >> 4) + 2 * (k % 4)),
+                                    dk + (uint64_t)((k / 4) * ((BKV * 128) >> 4) + 2 * (k % 4)), idesc_s, k > 0 ? 1u : 0u);
+                    tc::mma_commit(&s_full[buf(t, i)]);
+                    if (t == T - 1) tc::mma_commit(&k_empty[i & 1]);
+                }
+                __syncwarp();
+            };
+            auto pv = [&](int t, int i, int half) {
+                const uint64_t dv = dv0 + (uint64_t)((i & 1) * (Cfg::KV_BYTES >> 4));
+                if (tc::elect_one()) {
+#pragma unroll
+                    for (int k = half * (BKV / 32); k < (half + 1) * (BKV / 32); ++k)
+                        tc::mma_f16_ts(tmem + Cfg::O_COL + t * D, tmem + buf(t, i) * BKV + 8 * k, dv + (uint64_t)(k * ((16 * 128) >> 4)),
+                                       idesc_o, i > 0 || k > 0 ? 1u : 0u);
+                    if (half == 1) {
+                        if (t == T - 1) tc::mma_commit(&v_empty[i & 1]);
+                        if (T == 1 || i == nt - 1) tc::mma_commit(&o_done);       // T == 2: once per row tile, at the end
+                    }
+                }
+                __syncwarp();
+            };
+            auto p_step = [&](int t, int i) {
+                if (!tc::warp_wait(tc::smem_u32(&p_half[buf(t, i)]), par(i), false, deadline, &abort_s)) return false;
+                tc::tc_fence_after_sync();
+                pv(t, i, 0);
+                if (!tc::warp_wait(tc::smem_u32(&p_ready[buf(t, i)]), par(i), false, deadline, &abort_s)) return false;
+                tc::tc_fence_after_sync();
+                pv(t, i, 1);
+                return true;
+            };
+            auto k_there = [&](int i) {
+                const bool ok = tc::warp_wait(tc::smem_u32(&k_full[i & 1]), (uint32_t)((i >> 1) & 1), false, deadline, &abort_s);
+                tc::tc_fence_after_sync();
+                return ok;
+            };
+            bool ok = nt == 0 || (tc::warp_wait(tc::smem_u32(&q_full), 0u, false, deadline, &abort_s) && k_there(0));
+            if (ok && nt > 0) {
+                qk(0, 0);
+                if constexpr (T == 2) qk(1, 0);
+            }
+            for (int i = 0; ok && i < nt; ++i) {
+                const bool more = i + 1 < nt;
+                if constexpr (T == 1) {
+                    if (more) {
+                        ok = k_there(i + 1);
+                        if (!ok) break;
+                        qk(0, i + 1);
+                    }
+                }
+                ok = tc::warp_wait(tc::smem_u32(&v_full[i & 1]), (uint32_t)((i >> 1) & 1), false, deadline, &abort_s) && p_step(0, i);
+                if (!ok) break;
+                if constexpr (T == 2) {
+                    if (more) {
+                        ok = k_there(i + 1);
+                        if (!ok) break;
+                        qk(0, i + 1);
+                    }
+                    ok = p_step(1, i);
+                    if (!ok) break;
+                    if (more) qk(1, i + 1);
+                }
+            }
+            if (!ok) gave_up(3);
+        } else if (warp == 13) {
+            // ---------------- copies: lane = (box of a block, keys or values); scales by the lanes of 16 keys each
+            const int box = min(BKV, p.block_size), boxes = BKV / box;
+            const CUtensorMap* map = lane & 1 ? &tmV : &tmK;
+            auto page_of = [&](int j, int k) {              // k: first key of the box in the tile; INT_MIN: no key of the item there
+                const int k0 = j * BKV + k;
+                if (k0 >= key_hi || k0 + box <= key_lo) return INT_MIN;
+                const int page = table[k0 >> p.block_shift];
+                return page < 0 || page >= p.num_blocks ? -1 : page;
+            };
+            int page = INT_MIN;
+            const int my_k = (lane >> 1) * box;
+            auto group_scales = [&](int j) {                // of group lane / 2: this lane's tensor
+                const int pg = lane < 2 * GR ? page_of(j, (lane >> 1) * 16 / box * box) : INT_MIN;
+                return pg >= 0 ? fmaxf((lane & 1 ? p.v_scale : p.k_scale)[(size_t)pg * p.hkv + h], 1e-30f) : 0.0f;
+            };
+            if (nt > 0 && (lane >> 1) < boxes) page = page_of(j0, my_k);
+            float scale = nt > 0 ? group_scales(j0) : 0.0f;
+            for (int i = 0; i < nt; ++i) {
+                const int j = j0 + i;
+                const int wanted = __popc(__ballot_sync(0xffffffffu, page != INT_MIN)) / 2;       // boxes of each tensor
+#pragma unroll
+                for (int x = 0; x < 2; ++x) {
+                    if (!tc::warp_wait(tc::smem_u32(&raw_empty[x]), (uint32_t)((i & 1) ^ 1), false, deadline, &abort_s)) {
+                        gave_up(1);
+                        i = nt;
+                        break;
+                    }
+                    if (lane == 0) tc::mbar_arrive_expect_tx(&raw_full[x], (unsigned)(wanted * box * D));
+                    __syncwarp();
+                    if (page != INT_MIN && (lane & 1) == x) {
+                        const int row = page >= 0 ? (page * p.hkv + h) * p.block_size + ((j * BKV + my_k) & (p.block_size - 1)) : p.pool_rows;
+                        tc::tma_load_2d(sm + Cfg::OFF_RAW + x * Cfg::RAW_BYTES + my_k * D, map, tc::smem_u32(&raw_full[x]), 0, row);
+                    }
+                    if (x == 0) {
+                        const float vs = __shfl_down_sync(0xffffffffu, scale, 1);
+                        if (lane < 2 * GR && !(lane & 1))
+                            scale_s[i % Cfg::RING][lane >> 1] = scale > 0.0f ? make_float4(scale, lg2(vs), rcp(vs), 0.0f)
+                                                                             : make_float4(0.0f, -INFINITY, 0.0f, 0.0f);
+                        __syncwarp();
+                    }
+                    if (lane == 0) tc::mbar_arrive(&raw_full[x]);
+                }
+                if (i + 1 < nt) {
+                    page = (lane >> 1) < boxes ? page_of(j + 1, my_k) : INT_MIN;
+                    scale = group_scales(j + 1);
+                }
+            }
+        }
+    } else if (warp >= 8) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Cfg::REGS_CONVERT));
+        // ---------------- E4M3 bytes -> fp16 operand rows of 128 bytes (64 dimensions), 128-byte swizzle.  A thread takes 16 bytes; the blocks
+        // of 64 that neighbouring rows take differ, so that neither the reads nor the writes of eight lanes share banks.
+        constexpr int BL = D / 64, PASSES = BKV / 32 * BL;
+        const int c = tid - 256, sub = c & 3, r_in = c >> 2;
+        for (int i = 0; i < nt; ++i) {
+            const int key0 = (j0 + i) * BKV, st = i & 1;
+            const bool inside = key0 >= key_lo && key0 + BKV <= key_hi;
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+                const uint32_t src = sm + Cfg::OFF_RAW + x * Cfg::RAW_BYTES;
+                const uint32_t dst = sm + (x ? Cfg::OFF_V : Cfg::OFF_K) + st * Cfg::KV_BYTES;
+                bool ok = tc::mbar_wait_until(&raw_full[x], (uint32_t)(i & 1), deadline, &abort_s);
+                ok = ok && tc::mbar_wait_until(x ? &v_empty[st] : &k_empty[st], (uint32_t)(((i >> 1) & 1) ^ 1), deadline, &abort_s);
+                if (!__all_sync(0xffffffffu, ok)) { gave_up(2); i = nt; break; }
+#pragma unroll
+                for (int q0 = 0; q0 < PASSES; q0 += 4) {
+                    uint4 w[4];
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        const int r = r_in + 32 * ((q0 + q) / BL), bl = BL == 1 ? 0 : ((q0 + q) % BL) ^ (r & 1);
+                        w[q] = ld_shared_v4(src + r * D + (bl * 4 + sub) * 16);
+                        // rows outside the item's keys may be anything, and 0 x NaN is NaN
+                        if (!inside && (key0 + r < key_lo || key0 + r >= key_hi)) w[q] = make_uint4(0, 0, 0, 0);
+                    }
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        const int r = r_in + 32 * ((q0 + q) / BL), bl = BL == 1 ? 0 : ((q0 + q) % BL) ^ (r & 1);
+                        uint32_t f[8];
+                        e4m3x4_to_f16(w[q].x, f[0], f[1]);
+                        e4m3x4_to_f16(w[q].y, f[2], f[3]);
+                        e4m3x4_to_f16(w[q].z, f[4], f[5]);
+                        e4m3x4_to_f16(w[q].w, f[6], f[7]);
+                        const uint32_t row = dst + bl * (BKV * 128) + r * 128;
+                        st_shared_v4(row + (((2 * sub) ^ (r & 7)) << 4), f[0], f[1], f[2], f[3]);
+                        st_shared_v4(row + (((2 * sub + 1) ^ (r & 7)) << 4), f[4], f[5], f[6], f[7]);
+                    }
+                }
+                tc::fence_proxy_async_smem();               // operands are read by the tensor core, the bytes written by the next copy
+                __syncwarp();
+                if (lane == 0) {
+                    tc::mbar_arrive(&raw_empty[x]);
+                    tc::mbar_arrive(x ? &v_full[st] : &k_full[st]);
+                }
+            }
+        }
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(Cfg::REGS_SOFTMAX));
+        const int t = warp >> 2;
+        if (t < T) {
+            // ---------------- softmax: thread = row
+            const int row = (warp & 3) * 32 + lane, r = t * 128 + row;             // in the tile, in the item
+            const bool real = r < rows;
+            const int i_tok = (row0 + (real ? r : 0)) / p.group, hh = h * p.group + (row0 + (real ? r : 0)) % p.group, token = start + i_tok;
+            const int pos = len - n_new + i_tok;
+            const int hi = !real ? 0 : p.causal ? max(0, min(pos + 1, len)) : len, lo = p.window > 0 ? max(0, pos - p.window + 1) : 0;
+            // this row's query: fp16 at most 1 in magnitude, 16-byte chunks at chunk xor row % 8
+            float rf;
+            {
+                const uint4* src = reinterpret_cast<const uint4*>(p.q + (size_t)token * p.q_stride + (size_t)hh * D);
+                float top = 0.0f;
+                if (real) {
+#pragma unroll 8
+                    for (int k = 0; k < D / 8; ++k) {
+                        const uint4 w = src[k];
+                        const uint32_t* ww = &w.x;
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            float x, y;
+                            unpack_bf16x2(ww[e], x, y);
+                            top = fmaxf(top, fmaxf(fabsf(x), fabsf(y)));
+                        }
+                    }
+                }
+                const int e = query_exponent(top);
+                const float down = __uint_as_float((uint32_t)(127 - e) << 23);
+                rf = __uint_as_float((uint32_t)(127 + e) << 23) * p.scale * (p.cap > 0.0f ? 1.0f : LOG2E);
+                const uint32_t dst = sm + t * Cfg::Q_BYTES + row * 128;
+#pragma unroll 8
+                for (int k = 0; k < D / 8; ++k) {
+                    uint32_t f[4] = {0, 0, 0, 0};
+                    if (real) {
+                        const uint4 w = src[k];
+                        const uint32_t* ww = &w.x;
+#pragma unroll
+                        for (int e2 = 0; e2 < 4; ++e2) {
+                            float x, y;
+                            unpack_bf16x2(ww[e2], x, y);
+                            f[e2] = pack_f16x2(x * down, y * down);
+                        }
+                    }
+                    st_shared_v4(dst + (k >> 3) * (128 * 128) + (((k & 7) ^ (row & 7)) << 4), f[0], f[1], f[2], f[3]);
+                }
+                tc::fence_proxy_async_smem();
+                tc::mbar_arrive(&q_full);
+            }
+            const uint32_t lane_off = (uint32_t)((warp & 3) * 32) << 16;
+            const uint32_t tmem_O = tmem + Cfg::O_COL + t * D + lane_off;
+            const bool capped = p.cap > 0.0f;
+            const float inv_cap2 = capped ? 2.0f * LOG2E / p.cap : 0.0f;
+            // keys that every row of the warp sees
+            const int w_hi = (int)__reduce_min_sync(0xffffffffu, (unsigned)hi), w_lo = (int)__reduce_max_sync(0xffffffffu, (unsigned)lo);
+            float m = -INFINITY, l = 0.0f;
+            bool alive = true;
+            for (int i = 0; i < nt; ++i) {
+                const int sb = T == 2 ? t : i & 1;
+                const uint32_t par = (uint32_t)((T == 2 ? i : i >> 1) & 1), tmem_S = tmem + sb * BKV + lane_off;
+                const bool ok = tc::mbar_wait_until(&s_full[sb], par, deadline, &abort_s);
+                if (!__all_sync(0xffffffffu, ok)) { gave_up(4); alive = false; break; }
+                tc::tc_fence_after_sync();
+                uint32_t sv[BKV];
+#pragma unroll
+                for (int k = 0; k < BKV; k += 32) tc::tmem_ld32(tmem_S + k, sv + k);
+                tc::tmem_ld_wait();
+                const int key0 = (j0 + i) * BKV;
+                const float4* sc = scale_s[i % Cfg::RING];
+                const bool plain = !capped && key0 >= w_lo && key0 + BKV <= w_hi;     // warp-uniform
+                if (!plain) {
+                    // the base-2 logits themselves, masked: factor 1 and addend 0 below
+#pragma unroll
+                    for (int k = 0; k < BKV; ++k) {
+                        const float4 g = sc[k / 16];
+                        float u = __uint_as_float(sv[k]) * (rf * g.x);
+                        if (capped) u = soft_cap(u, p.cap, inv_cap2) * LOG2E;
+                        sv[k] = __float_as_uint(key0 + k < hi && key0 + k >= lo ? u + g.y : -INFINITY);
+                    }
+                }
+                float mx = -INFINITY;
+#pragma unroll
+                for (int g = 0; g < GR; ++g) {
+                    float a = -INFINITY, c = -INFINITY;
+#pragma unroll
+                    for (int k = 0; k < 16; k += 2) {
+                        a = fmaxf(a, __uint_as_float(sv[g * 16 + k]));
+                        c = fmaxf(c, __uint_as_float(sv[g * 16 + k + 1]));
+                    }
+                    const float4 s = sc[g];
+                    mx = fmaxf(mx, plain ? fmaf(fmaxf(a, c), rf * s.x, s.y) : fmaxf(a, c));
+                }
+                const bool grow = mx > m + Cfg::GROWTH;
+                if (__any_sync(0xffffffffu, grow && i > 0)) {                     // warp-uniform: tensor-memory loads are collective
+                    if constexpr (T == 1) {                                       // the product before may still run: S came in front of it
+                        const bool done = tc::mbar_wait_until(&o_done, (uint32_t)((i - 1) & 1), deadline, &abort_s);
+                        if (!__all_sync(0xffffffffu, done)) { gave_up(5); alive = false; break; }
+                        tc::tc_fence_after_sync();
+                    }
+                    const float f = grow ? ex2(m - mx) : 1.0f;
+                    l *= f;
+#pragma unroll 1
+                    for (int k = 0; k < D; k += 32) {
+                        uint32_t v[32];
+                        tc::tmem_ld32(tmem_O + k, v);
+                        tc::tmem_ld_wait();
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) v[e] = __float_as_uint(__uint_as_float(v[e]) * f);
+                        tc::tmem_st32(tmem_O + k, v);
+                    }
+                    tc::tmem_st_wait();
+                }
+                if (grow) m = mx;
+                const float ref = Cfg::OFFSET - (m == -INFINITY ? 0.0f : m);
+#pragma unroll
+                for (int k = 0; k < BKV; k += 32) {
+                    uint32_t u[16];
+#pragma unroll
+                    for (int gg = 0; gg < 2; ++gg) {
+                        const float4 s = sc[k / 16 + gg];
+                        const float f = plain ? rf * s.x : 1.0f, add = plain ? s.y + ref : ref;
+                        const uint64_t f2 = f32x2(f, f), a2 = f32x2(add, add);
+                        uint64_t sum = 0;
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) {
+                            const int at = k + gg * 16 + 2 * e;
+                            float x, y;
+                            f32x2_parts(fma_f32x2(f32x2(__uint_as_float(sv[at]), __uint_as_float(sv[at + 1])), f2, a2), x, y);
+                            x = ex2(x);
+                            y = ex2(y);
+                            sum = add_f32x2(sum, f32x2(x, y));
+                            u[gg * 8 + e] = pack_f16x2(x, y);
+                        }
+                        float s0, s1;
+                        f32x2_parts(sum, s0, s1);
+                        l = fmaf(s0 + s1, s.z, l);
+                    }
+                    tc::tmem_st16(tmem_S + (k >> 1), u);
+                    if (k == BKV / 2 - 32) {
+                        tc::tmem_st_wait();
+                        tc::tc_fence_before_sync();
+                        tc::mbar_arrive(&p_half[sb]);
+                    }
+                }
+                tc::tmem_st_wait();
+                tc::tc_fence_before_sync();
+                tc::mbar_arrive(&p_ready[sb]);
+            }
+            if (alive && nt > 0) {
+                const bool ok = tc::mbar_wait_until(&o_done, (uint32_t)(T == 1 ? (nt - 1) & 1 : 0), deadline, &abort_s);
+                alive = __all_sync(0xffffffffu, ok) != 0;
+                if (!alive) gave_up(6);
+                tc::tc_fence_after_sync();
+            }
+            const int item = (int)(blockIdx.y * gridDim.x + blockIdx.x);
+            const size_t part = (size_t)(item * pp.splits + split) * T + t;
+            if (alive) {
+                const float inv = inverse_sum(l);
+#pragma unroll 1
+                for (int k = 0; k < D; k += 32) {
+                    uint32_t v[32];
+                    __syncwarp();                               // the lanes part in the store
+                    if (nt > 0) {
+                        tc::tmem_ld32(tmem_O + k, v);
+                        tc::tmem_ld_wait();
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) v[e] = 0u;
+                    }
+                    if (!real) continue;
+                    if (pp.splits > 1) {
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) __stcg(pp.part_o + (part * D + k + e) * 128 + row, __uint_as_float(v[e]));
+                    } else {
+                        __nv_bfloat16* dst = p.o + (size_t)token * p.o_stride + (size_t)hh * D + k;
+#pragma unroll
+                        for (int e = 0; e < 32; e += 8)
+                            st_global_v4(dst + e, make_uint4(pack_bf16x2(__uint_as_float(v[e]) * inv, __uint_as_float(v[e + 1]) * inv),
+                                                             pack_bf16x2(__uint_as_float(v[e + 2]) * inv, __uint_as_float(v[e + 3]) * inv),
+                                                             pack_bf16x2(__uint_as_float(v[e + 4]) * inv, __uint_as_float(v[e + 5]) * inv),
+                                                             pack_bf16x2(__uint_as_float(v[e + 6]) * inv, __uint_as_float(v[e + 7]) * inv)));
+                    }
+                }
+                if (real) {
+                    if (pp.splits > 1) __stcg(pp.part_ml + part * 128 + row, make_float2(m, l));
+                    else if (p.lse) p.lse[(size_t)hh * p.tokens + token] = l == 0.0f ? -INFINITY : 0.6931471805599453f * (m - Cfg::OFFSET + log2f(l));
+                }
+            }
+            if (pp.splits > 1) {
+                sync_threads(128 * T);
+                if (tid == 0) {
+                    __threadfence();                            // the whole CTA's stores (its softmax warps met at the barrier)
+                    last_s = atomicInc(pp.counters + item, (unsigned)(pp.splits - 1)) == (unsigned)(pp.splits - 1);
+                    __threadfence();
+                }
+                sync_threads(128 * T);
+                if (last_s && real) {
+                    const size_t p_first = (size_t)item * pp.splits * T + t;
+                    float mm = -INFINITY, ll = 0.0f;
+                    for (int z = 0; z < pp.splits; ++z) mm = fmaxf(mm, __ldcg(pp.part_ml + (p_first + (size_t)z * T) * 128 + row).x);
+                    const float safe = mm == -INFINITY ? 0.0f : mm;
+                    for (int z = 0; z < pp.splits; ++z) {
+                        const float2 ml = __ldcg(pp.part_ml + (p_first + (size_t)z * T) * 128 + row);
+                        ll = fmaf(ml.y, ex2(ml.x - safe), ll);
+                    }
+                    const float inv = inverse_sum(ll);
+#pragma unroll 1
+                    for (int k = 0; k < D; k += 16) {
+                        float sum[16];
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) sum[e] = 0.0f;
+#pragma unroll 1
+                        for (int z = 0; z < pp.splits; ++z) {
+                            const size_t at = p_first + (size_t)z * T;
+                            const float f = ex2(__ldcg(pp.part_ml + at * 128 + row).x - safe);
+                            float v[16];
+#pragma unroll
+                            for (int e = 0; e < 16; ++e) v[e] = __ldcg(pp.part_o + (at * D + k + e) * 128 + row);
+#pragma unroll
+                            for (int e = 0; e < 16; ++e) sum[e] = fmaf(v[e], f, sum[e]);
+                        }
+                        __nv_bfloat16* dst = p.o + (size_t)token * p.o_stride + (size_t)hh * D + k;
+#pragma unroll
+                        for (int e = 0; e < 16; e += 8)
+                            st_global_v4(dst + e, make_uint4(pack_bf16x2(sum[e] * inv, sum[e + 1] * inv), pack_bf16x2(sum[e + 2] * inv, sum[e + 3] * inv),
+                                                             pack_bf16x2(sum[e + 4] * inv, sum[e + 5] * inv), pack_bf16x2(sum[e + 6] * inv, sum[e + 7] * inv)));
+                    }
+                    if (p.lse) p.lse[(size_t)hh * p.tokens + token] = ll == 0.0f ? -INFINITY : 0.6931471805599453f * (mm - Cfg::OFFSET + log2f(ll));
+                }
+            }
+        }
+    }
+    if (abort_s && warp == 13) {                            // a wait gave up: copies may be in flight, a bounded time for them to land
+        const uint64_t until = tc::global_timer_ns() + 1000000ull;
+        while (tc::global_timer_ns() < until) {}
+    }
+    __syncwarp();
+    tc::tc_fence_before_sync();
+    __syncthreads();
+    tc::tc_fence_after_sync();
+    if (warp == 12) tc::tmem_dealloc(tmem, 512);
+}
+
+// Row tiles of all sequences, at most: a sequence adds less than one to its rows' share.
+static long long prefill_items(long long tokens, long long batch, int group, int hkv, int tile_rows) {
+    return (tokens * group / tile_rows + batch) * hkv;
+}
+// Splits of the keys where the items leave SMs idle; at most 8, since a CTA joins them.
+static int prefill_splits(long long items, int sms) {
+    const long long s = sms / (items < 1 ? 1 : items);
+    return s < 1 ? 1 : s > 8 ? 8 : (int)s;
+}
+template <int D, int T>
+static long long prefill_workspace(long long tokens, long long batch, int group, int hkv) {
+    const long long items = prefill_items(tokens, batch, group, hkv, 128 * T);
+    const int splits = prefill_splits(items, device_sm_count());
+    return splits == 1 ? 0 : (items * 4 + 15) / 16 * 16 + items * splits * T * 128 * (8 + 4 * D);
+}
+
+template <int D, int T>
+static int launch_prefill(const PagedAttnParams& a, void* work, long long work_bytes, cudaStream_t stream) {
+    using Cfg = PrefillCfg<D, T>;
+    static PerDeviceOnce attr_once;
+    int attr_dev = 0;
+    if (attr_once.need(attr_dev)) {
+        const cudaError_t e = cudaFuncSetAttribute(paged_prefill_kernel<D, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::SMEM_BYTES);
+        if (e != cudaSuccess) return FRT_CUDA_ERR(e);
+        attr_once.set(attr_dev);
+    }
+    if (work_bytes < prefill_workspace<D, T>(a.tokens, a.batch, a.group, a.hkv)) return FRT_ERR_INVALID;
+    const long long items = prefill_items(a.tokens, a.batch, a.group, a.hkv, 128 * T), tiles = items / a.hkv;
+    if (tiles > 0x7fffffffLL / a.hkv) return FRT_ERR_UNSUPPORTED;
+    PrefillParams pp = {};
+    pp.a = a;
+    pp.splits = prefill_splits(items, device_sm_count());
+    uint8_t* w = static_cast<uint8_t*>(work);
+    pp.counters = reinterpret_cast<unsigned*>(w);
+    w += (items * 4 + 15) / 16 * 16;
+    pp.part_ml = reinterpret_cast<float2*>(w);
+    pp.part_o = reinterpret_cast<float*>(w + items * pp.splits * T * 128 * 8);
+    CUtensorMap tmK, tmV;
+    const int box = Cfg::BKV < a.block_size ? Cfg::BKV : a.block_size;
+    int rc = paged_map(&tmK, a.k, a.pool_rows, D, box, false);
+    if (!rc) rc = paged_map(&tmV, a.v, a.pool_rows, D, box, false);
+    if (rc) return rc;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)tiles, (unsigned)a.hkv, (unsigned)pp.splits);
+    cfg.blockDim = dim3(Cfg::THREADS);
+    cfg.dynamicSmemBytes = Cfg::SMEM_BYTES;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, paged_prefill_kernel<D, T>, tmK, tmV, pp);
+    return e == cudaSuccess ? FRT_OK : FRT_CUDA_ERR(e);
+}
