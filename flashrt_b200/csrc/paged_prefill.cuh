@@ -3,29 +3,34 @@
 // Many query rows over the paged E4M3 cache: chunks of prompts.  Included by paged_attention.cu inside namespace frt.
 //
 // Same formulas as the kernel for few rows.  128 query rows (tokens x the group's heads) are the lanes of a tcgen05 tile; two tiles share
-// every converted tile of keys and values and take turns: the tensor core works for one while the softmax warps of the other work.
+// every converted tile of keys and values.
 //   S = Q . K^T    kind::f16, queries and codes as fp16 (both exact, see the top of paged_attention.cu) in shared memory
 //   O += P . V     P fp16 from tensor memory, written over S
 // The block's scales stay out of the operands: a column of S has the factor softmax_scale * log2(e) * ks of its 16 keys and the addend
 // log2(vs), which replace the one factor that a softmax has anyway; the sum takes 1 / vs per 16 keys.
-// O is rescaled only when a row's maximum grows by more than 2^8: weights are 2^(u - m + 7) with the stale m, at most 2^15.
-// Warps: 0-3 and 4-7 softmax (thread = row), 8-11 turn E4M3 bytes into swizzled fp16 operands, 12 issues the MMAs, 13 the copies.
-// Heads of 256 (an O of 256 columns) and calls of at most 128 rows have one tile; then two S buffers alternate.
+// Every row tile has two S: the next scores are issued in front of this tile's P . V and stand when the softmax is through.  O is rescaled only when a row's maximum grows by more than 2^8: weights are 2^(u - m + 7) with the stale m, at most 2^15.
+// Warps: 0-3 and 4-7 softmax (thread = row), 8-11 turn E4M3 bytes into swizzled fp16 operands, 12 and 14 issue a row tile's MMAs, 13 the copies.
+// Heads of 256 (an O of 256 columns) and calls of at most 128 rows have one tile.
 // Bound by: the tensor pipe (4 x 128 x 128 x 128 products a key tile and pair: some 2050 clocks) and, close to it, the exponentials
 // (2 x 128 x 128 at 16 a clock: 2048).
 template <int D, int T>
 struct PrefillCfg {
     static_assert(T == 1 || D <= 128, "tensor memory: two tiles of S and O");
-    static constexpr int BKV = D == 256 ? 64 : 128;       // keys of a tile
+    static constexpr int BKV = T == 2 || D == 256 ? 64 : 128;      // keys of a tile: two S a row tile beside its O
     static constexpr int GR = BKV / 16;                   // groups of 16 keys: one block each
     static constexpr int Q_BYTES = 128 * D * 2, KV_BYTES = BKV * D * 2, RAW_BYTES = BKV * D;
-    static constexpr int OFF_K = T * Q_BYTES, OFF_V = OFF_K + 2 * KV_BYTES, OFF_RAW = OFF_V + 2 * KV_BYTES;
-    static constexpr int SMEM_BYTES = OFF_RAW + 2 * RAW_BYTES + 1024;
-    static constexpr int O_COL = 2 * BKV;                 // accumulators behind the two S
+    // Keys and values alternate in both rings (operand 2 i: the keys of tile i, 2 i + 1: its values): slots of bytes, so that copies run
+    // ahead, and of fp16 operands.
+    static constexpr int RAWS = BKV == 64 && D <= 128 ? 6 : 4, OPS = BKV == 64 && D <= 128 ? 6 : 3;
+    static constexpr int OFF_OP = T * Q_BYTES, OFF_RAW = OFF_OP + OPS * KV_BYTES;
+    static constexpr int SMEM_BYTES = OFF_RAW + RAWS * RAW_BYTES + 1024;
+    static_assert(SMEM_BYTES <= 232448 - (D == 256 ? 2048 : 3072), "dynamic and static shared memory of a CTA");
+    static constexpr int O_COL = T * 2 * BKV;             // accumulators behind the S
+    static_assert(O_COL + T * D <= 512, "tensor memory");
     static constexpr int THREADS = 512;
-    // registers of a thread: 128 at launch (8 x 184 + 4 x 88 + 4 x 56 = 16 x 128)
-    static constexpr int REGS_SOFTMAX = 184, REGS_CONVERT = 88, REGS_ISSUE = 56;
-    static constexpr int RING = 8;                        // scales of tiles; copies run at most four tiles ahead of the softmax
+    // registers of a thread: 128 at launch (8 x 192 + 4 x 80 + 4 x 48 = 16 x 128)
+    static constexpr int REGS_SOFTMAX = 192, REGS_CONVERT = 80, REGS_ISSUE = 48;
+    static constexpr int RING = 16;                       // scales of tiles; copies run at most RAWS / 2 + OPS / 2 + 2 tiles ahead of the softmax
     static constexpr float OFFSET = 7.0f, GROWTH = 8.0f;
 };
 
@@ -46,8 +51,9 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
     const PagedAttnParams& p = pp.a;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-    __shared__ uint64_t raw_full[2], raw_empty[2], k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_half[2], p_ready[2], q_full, o_done;
+    __shared__ uint64_t raw_full[Cfg::RAWS], raw_empty[Cfg::RAWS], op_full[Cfg::OPS], op_empty[Cfg::OPS], s_full[2 * T], p_half[2 * T], p_ready[2 * T], q_full, o_done[T];
     __shared__ float4 scale_s[Cfg::RING][GR];               // per 16 keys: ks, log2 vs, 1 / vs
+    __shared__ float rf_s[T * 128];
     __shared__ int warp_s[16], item_s[2];
     __shared__ uint32_t tmem_slot;
     __shared__ unsigned last_s;
@@ -55,19 +61,21 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     if (tid == 0) {
-        for (int i = 0; i < 2; ++i) {
+        for (int i = 0; i < Cfg::RAWS; ++i) {
             tc::mbar_init(&raw_full[i], 2);                 // bytes; scales
             tc::mbar_init(&raw_empty[i], 4);
-            tc::mbar_init(&k_full[i], 4);
-            tc::mbar_init(&k_empty[i], 1);
-            tc::mbar_init(&v_full[i], 4);
-            tc::mbar_init(&v_empty[i], 1);
+        }
+        for (int i = 0; i < Cfg::OPS; ++i) {
+            tc::mbar_init(&op_full[i], 4);
+            tc::mbar_init(&op_empty[i], T);
+        }
+        for (int i = 0; i < 2 * T; ++i) {
             tc::mbar_init(&s_full[i], 1);
             tc::mbar_init(&p_half[i], 128);
             tc::mbar_init(&p_ready[i], 128);
         }
         tc::mbar_init(&q_full, 128 * T);
-        tc::mbar_init(&o_done, T);
+        for (int i = 0; i < T; ++i) tc::mbar_init(&o_done[i], 1);
         abort_s = 0;
         tc::mbar_fence_init();
         tc::tma_prefetch_desc(&tmK);
@@ -143,81 +151,67 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
 
     if (warp >= 12) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Cfg::REGS_ISSUE));
-        if (warp == 12) {
-            // ---------------- MMA issuer (whole warp)
+        if (warp == 12 || (T == 2 && warp == 14)) {
+            // ---------------- MMA issuer of a row tile (whole warp).  One warp for both tiles took some 80 clocks an MMA, 2900 of a pair's 4220
+            // for a tile of keys, and made each tile wait for the other's turn.
             constexpr uint32_t idesc_s = tc::make_idesc(0, 0, 0, 0, 128, BKV);      // fp16, both K-major
             constexpr uint32_t idesc_o = tc::make_idesc(0, 0, 0, 1, 128, D);        // P from tensor memory, V MN-major
-            const uint64_t dq0 = tc::make_desc_kmajor_sw128(sm), dk0 = tc::make_desc_kmajor_sw128(sm + Cfg::OFF_K);
-            const uint64_t dv0 = tc::make_desc_mnmajor_sw128(sm + Cfg::OFF_V, BKV * 128);
-            // S and its barriers: tile t's own, or the buffers in turn
-            auto buf = [&](int t, int i) { return T == 2 ? t : i & 1; };
-            auto par = [&](int i) { return (uint32_t)((T == 2 ? i : i >> 1) & 1); };
-            auto qk = [&](int t, int i) {
-                const uint64_t dq = dq0 + (uint64_t)(t * (Cfg::Q_BYTES >> 4)), dk = dk0 + (uint64_t)((i & 1) * (Cfg::KV_BYTES >> 4));
+            const int t = (warp - 12) >> 1;
+            const uint64_t dq = tc::make_desc_kmajor_sw128(sm + t * Cfg::Q_BYTES), dk0 = tc::make_desc_kmajor_sw128(sm + Cfg::OFF_OP);
+            const uint64_t dv0 = tc::make_desc_mnmajor_sw128(sm + Cfg::OFF_OP, BKV * 128);
+            const uint32_t tmem_o = tmem + Cfg::O_COL + t * D;
+            auto buf = [&](int i) { return 2 * t + (i & 1); };              // S and its barriers: two in turn
+            auto par = [&](int i) { return (uint32_t)((i >> 1) & 1); };
+            auto qk = [&](int i) {
+                const uint64_t dk = dk0 + (uint64_t)((2 * i % Cfg::OPS) * (Cfg::KV_BYTES >> 4));
+                const uint32_t tmem_s = tmem + buf(i) * BKV;
                 if (tc::elect_one()) {
 #pragma unroll
                     for (int k = 0; k < D / 16; ++k)        // 64-element blocks, 32 bytes per step inside
-                        tc::mma_f16(tmem + buf(t, i) * BKV, dq + (uint64_t)((k / 4) * ((128 * 128) >> 4) + 2 * (k % 4)),
+                        tc::mma_f16(tmem_s, dq + (uint64_t)((k / 4) * ((128 * 128) >> 4) + 2 * (k % 4)),
                                     dk + (uint64_t)((k / 4) * ((BKV * 128) >> 4) + 2 * (k % 4)), idesc_s, k > 0 ? 1u : 0u);
-                    tc::mma_commit(&s_full[buf(t, i)]);
-                    if (t == T - 1) tc::mma_commit(&k_empty[i & 1]);
+                    tc::mma_commit(&s_full[buf(i)]);
+                    tc::mma_commit(&op_empty[2 * i % Cfg::OPS]);
                 }
                 __syncwarp();
             };
-            auto pv = [&](int t, int i, int half) {
-                const uint64_t dv = dv0 + (uint64_t)((i & 1) * (Cfg::KV_BYTES >> 4));
+            auto pv = [&](int i, int half) {
+                const uint64_t dv = dv0 + (uint64_t)(((2 * i + 1) % Cfg::OPS) * (Cfg::KV_BYTES >> 4));
+                const uint32_t tmem_p = tmem + buf(i) * BKV;
                 if (tc::elect_one()) {
 #pragma unroll
                     for (int k = half * (BKV / 32); k < (half + 1) * (BKV / 32); ++k)
-                        tc::mma_f16_ts(tmem + Cfg::O_COL + t * D, tmem + buf(t, i) * BKV + 8 * k, dv + (uint64_t)(k * ((16 * 128) >> 4)),
-                                       idesc_o, i > 0 || k > 0 ? 1u : 0u);
+                        tc::mma_f16_ts(tmem_o, tmem_p + 8 * k, dv + (uint64_t)(k * ((16 * 128) >> 4)), idesc_o, i > 0 || k > 0 ? 1u : 0u);
                     if (half == 1) {
-                        if (t == T - 1) tc::mma_commit(&v_empty[i & 1]);
-                        if (T == 1 || i == nt - 1) tc::mma_commit(&o_done);       // T == 2: once per row tile, at the end
+                        tc::mma_commit(&op_empty[(2 * i + 1) % Cfg::OPS]);
+                        tc::mma_commit(&o_done[t]);
                     }
                 }
                 __syncwarp();
             };
-            auto p_step = [&](int t, int i) {
-                if (!tc::warp_wait(tc::smem_u32(&p_half[buf(t, i)]), par(i), false, deadline, &abort_s)) return false;
+            auto p_step = [&](int i) {
+                if (!tc::warp_wait(tc::smem_u32(&p_half[buf(i)]), par(i), false, deadline, &abort_s)) return false;
                 tc::tc_fence_after_sync();
-                pv(t, i, 0);
-                if (!tc::warp_wait(tc::smem_u32(&p_ready[buf(t, i)]), par(i), false, deadline, &abort_s)) return false;
+                pv(i, 0);
+                if (!tc::warp_wait(tc::smem_u32(&p_ready[buf(i)]), par(i), false, deadline, &abort_s)) return false;
                 tc::tc_fence_after_sync();
-                pv(t, i, 1);
+                pv(i, 1);
                 return true;
             };
-            auto k_there = [&](int i) {
-                const bool ok = tc::warp_wait(tc::smem_u32(&k_full[i & 1]), (uint32_t)((i >> 1) & 1), false, deadline, &abort_s);
+            auto there = [&](int n) {
+                const bool ok = tc::warp_wait(tc::smem_u32(&op_full[n % Cfg::OPS]), (uint32_t)((n / Cfg::OPS) & 1), false, deadline, &abort_s);
                 tc::tc_fence_after_sync();
                 return ok;
             };
-            bool ok = nt == 0 || (tc::warp_wait(tc::smem_u32(&q_full), 0u, false, deadline, &abort_s) && k_there(0));
-            if (ok && nt > 0) {
-                qk(0, 0);
-                if constexpr (T == 2) qk(1, 0);
-            }
+            bool ok = nt == 0 || (tc::warp_wait(tc::smem_u32(&q_full), 0u, false, deadline, &abort_s) && there(0));
+            if (ok && nt > 0) qk(0);
             for (int i = 0; ok && i < nt; ++i) {
-                const bool more = i + 1 < nt;
-                if constexpr (T == 1) {
-                    if (more) {
-                        ok = k_there(i + 1);
-                        if (!ok) break;
-                        qk(0, i + 1);
-                    }
-                }
-                ok = tc::warp_wait(tc::smem_u32(&v_full[i & 1]), (uint32_t)((i >> 1) & 1), false, deadline, &abort_s) && p_step(0, i);
-                if (!ok) break;
-                if constexpr (T == 2) {
-                    if (more) {
-                        ok = k_there(i + 1);
-                        if (!ok) break;
-                        qk(0, i + 1);
-                    }
-                    ok = p_step(1, i);
+                if (i + 1 < nt) {                            // the next scores first: the softmax finds them when it is through with these
+                    ok = there(2 * i + 2);
                     if (!ok) break;
-                    if (more) qk(1, i + 1);
+                    qk(i + 1);
                 }
+                ok = there(2 * i + 1) && p_step(i);
             }
             if (!ok) gave_up(3);
         } else if (warp == 13) {
@@ -243,16 +237,17 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
                 const int wanted = __popc(__ballot_sync(0xffffffffu, page != INT_MIN)) / 2;       // boxes of each tensor
 #pragma unroll
                 for (int x = 0; x < 2; ++x) {
-                    if (!tc::warp_wait(tc::smem_u32(&raw_empty[x]), (uint32_t)((i & 1) ^ 1), false, deadline, &abort_s)) {
+                    const int slot = (2 * i + x) % Cfg::RAWS;
+                    if (!tc::warp_wait(tc::smem_u32(&raw_empty[slot]), (uint32_t)(((2 * i + x) / Cfg::RAWS) & 1) ^ 1u, false, deadline, &abort_s)) {
                         gave_up(1);
                         i = nt;
                         break;
                     }
-                    if (lane == 0) tc::mbar_arrive_expect_tx(&raw_full[x], (unsigned)(wanted * box * D));
+                    if (lane == 0) tc::mbar_arrive_expect_tx(&raw_full[slot], (unsigned)(wanted * box * D));
                     __syncwarp();
                     if (page != INT_MIN && (lane & 1) == x) {
                         const int row = page >= 0 ? (page * p.hkv + h) * p.block_size + ((j * BKV + my_k) & (p.block_size - 1)) : p.pool_rows;
-                        tc::tma_load_2d(sm + Cfg::OFF_RAW + x * Cfg::RAW_BYTES + my_k * D, map, tc::smem_u32(&raw_full[x]), 0, row);
+                        tc::tma_load_2d(sm + Cfg::OFF_RAW + slot * Cfg::RAW_BYTES + my_k * D, map, tc::smem_u32(&raw_full[slot]), 0, row);
                     }
                     if (x == 0) {
                         const float vs = __shfl_down_sync(0xffffffffu, scale, 1);
@@ -261,7 +256,7 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
                                                                              : make_float4(0.0f, -INFINITY, 0.0f, 0.0f);
                         __syncwarp();
                     }
-                    if (lane == 0) tc::mbar_arrive(&raw_full[x]);
+                    if (lane == 0) tc::mbar_arrive(&raw_full[slot]);
                 }
                 if (i + 1 < nt) {
                     page = (lane >> 1) < boxes ? page_of(j + 1, my_k) : INT_MIN;
@@ -273,30 +268,30 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Cfg::REGS_CONVERT));
         // ---------------- E4M3 bytes -> fp16 operand rows of 128 bytes (64 dimensions), 128-byte swizzle.  A thread takes 16 bytes; the blocks
         // of 64 that neighbouring rows take differ, so that neither the reads nor the writes of eight lanes share banks.
-        constexpr int BL = D / 64, PASSES = BKV / 32 * BL;
+        constexpr int BL = D / 64, PASSES = BKV / 32 * BL, AT_ONCE = PASSES < 4 ? PASSES : 4;
         const int c = tid - 256, sub = c & 3, r_in = c >> 2;
         for (int i = 0; i < nt; ++i) {
-            const int key0 = (j0 + i) * BKV, st = i & 1;
+            const int key0 = (j0 + i) * BKV;
             const bool inside = key0 >= key_lo && key0 + BKV <= key_hi;
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
-                const uint32_t src = sm + Cfg::OFF_RAW + x * Cfg::RAW_BYTES;
-                const uint32_t dst = sm + (x ? Cfg::OFF_V : Cfg::OFF_K) + st * Cfg::KV_BYTES;
-                bool ok = tc::mbar_wait_until(&raw_full[x], (uint32_t)(i & 1), deadline, &abort_s);
-                ok = ok && tc::mbar_wait_until(x ? &v_empty[st] : &k_empty[st], (uint32_t)(((i >> 1) & 1) ^ 1), deadline, &abort_s);
+                const int n = 2 * i + x, slot = n % Cfg::RAWS, op = n % Cfg::OPS;
+                const uint32_t src = sm + Cfg::OFF_RAW + slot * Cfg::RAW_BYTES, dst = sm + Cfg::OFF_OP + op * Cfg::KV_BYTES;
+                bool ok = tc::mbar_wait_until(&raw_full[slot], (uint32_t)((n / Cfg::RAWS) & 1), deadline, &abort_s);
+                ok = ok && tc::mbar_wait_until(&op_empty[op], (uint32_t)((n / Cfg::OPS) & 1) ^ 1u, deadline, &abort_s);
                 if (!__all_sync(0xffffffffu, ok)) { gave_up(2); i = nt; break; }
 #pragma unroll
-                for (int q0 = 0; q0 < PASSES; q0 += 4) {
-                    uint4 w[4];
+                for (int q0 = 0; q0 < PASSES; q0 += AT_ONCE) {
+                    uint4 w[AT_ONCE];
 #pragma unroll
-                    for (int q = 0; q < 4; ++q) {
+                    for (int q = 0; q < AT_ONCE; ++q) {
                         const int r = r_in + 32 * ((q0 + q) / BL), bl = BL == 1 ? 0 : ((q0 + q) % BL) ^ (r & 1);
                         w[q] = ld_shared_v4(src + r * D + (bl * 4 + sub) * 16);
                         // rows outside the item's keys may be anything, and 0 x NaN is NaN
                         if (!inside && (key0 + r < key_lo || key0 + r >= key_hi)) w[q] = make_uint4(0, 0, 0, 0);
                     }
 #pragma unroll
-                    for (int q = 0; q < 4; ++q) {
+                    for (int q = 0; q < AT_ONCE; ++q) {
                         const int r = r_in + 32 * ((q0 + q) / BL), bl = BL == 1 ? 0 : ((q0 + q) % BL) ^ (r & 1);
                         uint32_t f[8];
                         e4m3x4_to_f16(w[q].x, f[0], f[1]);
@@ -311,8 +306,8 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
                 tc::fence_proxy_async_smem();               // operands are read by the tensor core, the bytes written by the next copy
                 __syncwarp();
                 if (lane == 0) {
-                    tc::mbar_arrive(&raw_empty[x]);
-                    tc::mbar_arrive(x ? &v_full[st] : &k_full[st]);
+                    tc::mbar_arrive(&raw_empty[slot]);
+                    tc::mbar_arrive(&op_full[op]);
                 }
             }
         }
@@ -323,47 +318,48 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
             // ---------------- softmax: thread = row
             const int row = (warp & 3) * 32 + lane, r = t * 128 + row;             // in the tile, in the item
             const bool real = r < rows;
-            const int i_tok = (row0 + (real ? r : 0)) / p.group, hh = h * p.group + (row0 + (real ? r : 0)) % p.group, token = start + i_tok;
+            const int at_row = row0 + min(r, rows - 1);             // rows behind the last go along with it
+            const int i_tok = at_row / p.group, hh = h * p.group + at_row % p.group, token = start + i_tok;
             const int pos = len - n_new + i_tok;
-            const int hi = !real ? 0 : p.causal ? max(0, min(pos + 1, len)) : len, lo = p.window > 0 ? max(0, pos - p.window + 1) : 0;
-            // this row's query: fp16 at most 1 in magnitude, 16-byte chunks at chunk xor row % 8
+            const int hi = p.causal ? max(0, min(pos + 1, len)) : len, lo = p.window > 0 ? max(0, pos - p.window + 1) : 0;
+            // the warp's 32 queries, 16 bytes a lane: fp16 at most 1 in magnitude, 16-byte chunks at chunk xor row % 8
             float rf;
             {
-                const uint4* src = reinterpret_cast<const uint4*>(p.q + (size_t)token * p.q_stride + (size_t)hh * D);
-                float top = 0.0f;
-                if (real) {
-#pragma unroll 8
-                    for (int k = 0; k < D / 8; ++k) {
-                        const uint4 w = src[k];
-                        const uint32_t* ww = &w.x;
+                constexpr int CH = D / 8, RP = 32 / CH;                // chunks of a row, rows of a step
+                const int ch = lane % CH;
+#pragma unroll 1
+                for (int s0 = 0; s0 < 32; s0 += 8 * RP) {
+                    uint4 w[8];
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            float x, y;
-                            unpack_bf16x2(ww[e], x, y);
-                            top = fmaxf(top, fmaxf(fabsf(x), fabsf(y)));
-                        }
+                    for (int s = 0; s < 8; ++s) {
+                        const int q_row = t * 128 + (warp & 3) * 32 + s0 + s * RP + lane / CH, q_at = row0 + min(q_row, rows - 1);
+                        w[s] = make_uint4(0, 0, 0, 0);
+                        if (q_row < rows)
+                            w[s] = ld_global_v4(p.q + (size_t)(start + q_at / p.group) * p.q_stride + (size_t)(h * p.group + q_at % p.group) * D + ch * 8);
                     }
-                }
-                const int e = query_exponent(top);
-                const float down = __uint_as_float((uint32_t)(127 - e) << 23);
-                rf = __uint_as_float((uint32_t)(127 + e) << 23) * p.scale * (p.cap > 0.0f ? 1.0f : LOG2E);
-                const uint32_t dst = sm + t * Cfg::Q_BYTES + row * 128;
-#pragma unroll 8
-                for (int k = 0; k < D / 8; ++k) {
-                    uint32_t f[4] = {0, 0, 0, 0};
-                    if (real) {
-                        const uint4 w = src[k];
-                        const uint32_t* ww = &w.x;
 #pragma unroll
-                        for (int e2 = 0; e2 < 4; ++e2) {
-                            float x, y;
-                            unpack_bf16x2(ww[e2], x, y);
-                            f[e2] = pack_f16x2(x * down, y * down);
-                        }
+                    for (int s = 0; s < 8; ++s) {
+                        const int r_w = s0 + s * RP + lane / CH;      // in the warp
+                        const uint32_t* ww = &w[s].x;
+                        float x[8], top = 0.0f;
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) unpack_bf16x2(ww[e], x[2 * e], x[2 * e + 1]);
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(x[e]));
+#pragma unroll
+                        for (int d = 1; d < CH; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+                        const int e2 = query_exponent(top);
+                        const float down = __uint_as_float((uint32_t)(127 - e2) << 23);
+                        const int q_row = (warp & 3) * 32 + r_w;
+                        st_shared_v4(sm + t * Cfg::Q_BYTES + (ch >> 3) * (128 * 128) + q_row * 128 + (((ch & 7) ^ (q_row & 7)) << 4),
+                                     pack_f16x2(x[0] * down, x[1] * down), pack_f16x2(x[2] * down, x[3] * down),
+                                     pack_f16x2(x[4] * down, x[5] * down), pack_f16x2(x[6] * down, x[7] * down));
+                        if (ch == 0) rf_s[t * 128 + q_row] = __uint_as_float((uint32_t)(127 + e2) << 23);
                     }
-                    st_shared_v4(dst + (k >> 3) * (128 * 128) + (((k & 7) ^ (row & 7)) << 4), f[0], f[1], f[2], f[3]);
                 }
                 tc::fence_proxy_async_smem();
+                __syncwarp();
+                rf = rf_s[r] * p.scale * (p.cap > 0.0f ? 1.0f : LOG2E);
                 tc::mbar_arrive(&q_full);
             }
             const uint32_t lane_off = (uint32_t)((warp & 3) * 32) << 16;
@@ -372,50 +368,76 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
             const float inv_cap2 = capped ? 2.0f * LOG2E / p.cap : 0.0f;
             // keys that every row of the warp sees
             const int w_hi = (int)__reduce_min_sync(0xffffffffu, (unsigned)hi), w_lo = (int)__reduce_max_sync(0xffffffffu, (unsigned)lo);
+            const bool idle = t * 128 + (warp & 3) * 32 >= rows;    // a warp behind the last row only signs
             float m = -INFINITY, l = 0.0f;
             bool alive = true;
             for (int i = 0; i < nt; ++i) {
-                const int sb = T == 2 ? t : i & 1;
-                const uint32_t par = (uint32_t)((T == 2 ? i : i >> 1) & 1), tmem_S = tmem + sb * BKV + lane_off;
-                const bool ok = tc::mbar_wait_until(&s_full[sb], par, deadline, &abort_s);
-                if (!__all_sync(0xffffffffu, ok)) { gave_up(4); alive = false; break; }
-                tc::tc_fence_after_sync();
-                uint32_t sv[BKV];
-#pragma unroll
-                for (int k = 0; k < BKV; k += 32) tc::tmem_ld32(tmem_S + k, sv + k);
-                tc::tmem_ld_wait();
+                const int sb = 2 * t + (i & 1);
+                const uint32_t par = (uint32_t)((i >> 1) & 1), tmem_S = tmem + sb * BKV + lane_off;
                 const int key0 = (j0 + i) * BKV;
                 const float4* sc = scale_s[i % Cfg::RING];
                 const bool plain = !capped && key0 >= w_lo && key0 + BKV <= w_hi;     // warp-uniform
-                if (!plain) {
-                    // the base-2 logits themselves, masked: factor 1 and addend 0 below
-#pragma unroll
-                    for (int k = 0; k < BKV; ++k) {
-                        const float4 g = sc[k / 16];
-                        float u = __uint_as_float(sv[k]) * (rf * g.x);
-                        if (capped) u = soft_cap(u, p.cap, inv_cap2) * LOG2E;
-                        sv[k] = __float_as_uint(key0 + k < hi && key0 + k >= lo ? u + g.y : -INFINITY);
-                    }
+                const bool ok = tc::mbar_wait_until(&s_full[sb], par, deadline, &abort_s);
+                if (!__all_sync(0xffffffffu, ok)) { gave_up(4); alive = false; break; }
+                tc::tc_fence_after_sync();
+                if (idle) {
+                    tc::tc_fence_before_sync();
+                    tc::mbar_arrive(&p_half[sb]);
+                    tc::mbar_arrive(&p_ready[sb]);
+                    continue;
                 }
+                if (!plain) {
+                    // the base-2 logits themselves, masked, over S; factor 1 and addend 0 from here on.  In a loop of 32 columns: written out
+                    // over a row of registers this was 40 KB of instructions, fetched anew for every tile
+#pragma unroll 1
+                    for (int k = 0; k < BKV; k += 32) {
+                        uint32_t v[32];
+                        tc::tmem_ld32(tmem_S + k, v);
+                        const float2 s0 = *reinterpret_cast<const float2*>(&sc[k / 16]), s1 = *reinterpret_cast<const float2*>(&sc[k / 16 + 1]);
+                        tc::tmem_ld_wait();
+                        if (capped) {
+#pragma unroll
+                            for (int e = 0; e < 32; ++e)
+                                v[e] = __float_as_uint(soft_cap(__uint_as_float(v[e]) * (rf * (e < 16 ? s0.x : s1.x)), p.cap, inv_cap2) * LOG2E);
+                        } else {
+#pragma unroll
+                            for (int e = 0; e < 32; ++e) v[e] = __float_as_uint(__uint_as_float(v[e]) * (rf * (e < 16 ? s0.x : s1.x)));
+                        }
+                        const int from = lo - key0 - k, to = hi - key0 - k;
+#pragma unroll
+                        for (int e = 0; e < 32; ++e)
+                            v[e] = __float_as_uint(e >= from && e < to ? __uint_as_float(v[e]) + (e < 16 ? s0.y : s1.y) : -INFINITY);
+                        tc::tmem_st32(tmem_S + k, v);
+                    }
+                    tc::tmem_st_wait();
+                }
+                uint32_t sv[BKV];
+#pragma unroll
+                for (int k = 0; k < BKV; k += 32) tc::tmem_ld32(tmem_S + k, sv + k);
+                // factor and addend of each 16 keys, while the scores arrive
+                float fac[GR], add[GR];
+#pragma unroll
+                for (int g = 0; g < GR; ++g) {
+                    const float2 s = *reinterpret_cast<const float2*>(&sc[g]);
+                    fac[g] = plain ? rf * s.x : 1.0f;
+                    add[g] = plain ? s.y : 0.0f;
+                }
+                tc::tmem_ld_wait();
                 float mx = -INFINITY;
 #pragma unroll
                 for (int g = 0; g < GR; ++g) {
-                    float a = -INFINITY, c = -INFINITY;
-#pragma unroll
-                    for (int k = 0; k < 16; k += 2) {
-                        a = fmaxf(a, __uint_as_float(sv[g * 16 + k]));
-                        c = fmaxf(c, __uint_as_float(sv[g * 16 + k + 1]));
-                    }
-                    const float4 s = sc[g];
-                    mx = fmaxf(mx, plain ? fmaf(fmaxf(a, c), rf * s.x, s.y) : fmaxf(a, c));
+                    const uint32_t* s = sv + g * 16;
+                    auto v = [&](int e) { return __uint_as_float(s[e]); };
+                    const float a = max3(max3(v(0), v(1), v(2)), v(3), v(4)), c = max3(max3(v(5), v(6), v(7)), v(8), v(9));
+                    const float d = max3(max3(v(10), v(11), v(12)), max3(v(13), v(14), v(15)), a);
+                    mx = fmaxf(mx, fmaf(fmaxf(c, d), fac[g], add[g]));
                 }
                 const bool grow = mx > m + Cfg::GROWTH;
                 if (__any_sync(0xffffffffu, grow && i > 0)) {                     // warp-uniform: tensor-memory loads are collective
-                    if constexpr (T == 1) {                                       // the product before may still run: S came in front of it
-                        const bool done = tc::mbar_wait_until(&o_done, (uint32_t)((i - 1) & 1), deadline, &abort_s);
-                        if (!__all_sync(0xffffffffu, done)) { gave_up(5); alive = false; break; }
-                        tc::tc_fence_after_sync();
-                    }
+                    // the product before may still run: these scores were issued in front of it
+                    const bool done = tc::mbar_wait_until(&o_done[t], (uint32_t)((i - 1) & 1), deadline, &abort_s);
+                    if (!__all_sync(0xffffffffu, done)) { gave_up(5); alive = false; break; }
+                    tc::tc_fence_after_sync();
                     const float f = grow ? ex2(m - mx) : 1.0f;
                     l *= f;
 #pragma unroll 1
@@ -436,9 +458,8 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
                     uint32_t u[16];
 #pragma unroll
                     for (int gg = 0; gg < 2; ++gg) {
-                        const float4 s = sc[k / 16 + gg];
-                        const float f = plain ? rf * s.x : 1.0f, add = plain ? s.y + ref : ref;
-                        const uint64_t f2 = f32x2(f, f), a2 = f32x2(add, add);
+                        const int g = k / 16 + gg;
+                        const uint64_t f2 = f32x2(fac[g], fac[g]), a2 = f32x2(add[g] + ref, add[g] + ref);
                         uint64_t sum = 0;
 #pragma unroll
                         for (int e = 0; e < 8; ++e) {
@@ -452,7 +473,7 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
                         }
                         float s0, s1;
                         f32x2_parts(sum, s0, s1);
-                        l = fmaf(s0 + s1, s.z, l);
+                        l = fmaf(s0 + s1, sc[g].z, l);
                     }
                     tc::tmem_st16(tmem_S + (k >> 1), u);
                     if (k == BKV / 2 - 32) {
@@ -466,7 +487,7 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
                 tc::mbar_arrive(&p_ready[sb]);
             }
             if (alive && nt > 0) {
-                const bool ok = tc::mbar_wait_until(&o_done, (uint32_t)(T == 1 ? (nt - 1) & 1 : 0), deadline, &abort_s);
+                const bool ok = tc::mbar_wait_until(&o_done[t], (uint32_t)((nt - 1) & 1), deadline, &abort_s);
                 alive = __all_sync(0xffffffffu, ok) != 0;
                 if (!alive) gave_up(6);
                 tc::tc_fence_after_sync();
