@@ -975,7 +975,7 @@ extern "C" int frt_b200_paged_attention_workspace_bytes(int tokens, int batch, i
     *out_bytes = paged_dispatch(head_dim, paged_nt(rows < few ? rows : few, head_dim), [](auto D, auto NT) { return paged_workspace<D(), NT()>(); });
     if (rows > few)
         *out_bytes += prefill_dispatch(head_dim, rows, [&](auto D, auto T) {
-            return prefill_workspace<D(), T()>(tokens, batch, group, num_heads_kv);
+            return prefill_workspace<D(), T()>(tokens, batch, max_new, group, num_heads_kv);
         });
     return FRT_OK;
 }
@@ -1052,5 +1052,5 @@ extern "C" int frt_b200_paged_attention_fp8(const void* Q, long long q_stride, v
             return r;
         });
     if (rc || !many) return rc;
-    return prefill_dispatch(head_dim, rows, [&](auto D, auto T) { return launch_prefill<D(), T()>(p, work, workspace_bytes, stream_of); });
+    return prefill_dispatch(head_dim, rows, [&](auto D, auto T) { return launch_prefill<D(), T()>(p, max_new, work, workspace_bytes, stream_of); });
 }

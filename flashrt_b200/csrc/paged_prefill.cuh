@@ -581,9 +581,10 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
     if (warp == 12) tc::tmem_dealloc(tmem, 512);
 }
 
-// Row tiles of all sequences, at most: a sequence adds less than one to its rows' share.
-static long long prefill_items(long long tokens, long long batch, int group, int hkv, int tile_rows) {
-    return (tokens * group / tile_rows + batch) * hkv;
+// Row tiles of all sequences, at most: a sequence adds less than one to its rows' share, and has no more than max_new tokens.
+static long long prefill_tiles(long long tokens, long long batch, long long max_new, int group, int tile_rows) {
+    const long long by_rows = tokens * group / tile_rows + batch, by_sequence = batch * ((max_new * group + tile_rows - 1) / tile_rows);
+    return by_rows < by_sequence ? by_rows : by_sequence;
 }
 // Splits of the keys where the items leave SMs idle; at most 8, since a CTA joins them.
 static int prefill_splits(long long items, int sms) {
@@ -591,14 +592,14 @@ static int prefill_splits(long long items, int sms) {
     return s < 1 ? 1 : s > 8 ? 8 : (int)s;
 }
 template <int D, int T>
-static long long prefill_workspace(long long tokens, long long batch, int group, int hkv) {
-    const long long items = prefill_items(tokens, batch, group, hkv, 128 * T);
+static long long prefill_workspace(long long tokens, long long batch, long long max_new, int group, int hkv) {
+    const long long items = prefill_tiles(tokens, batch, max_new, group, 128 * T) * hkv;
     const int splits = prefill_splits(items, device_sm_count());
     return splits == 1 ? 0 : (items * 4 + 15) / 16 * 16 + items * splits * T * 128 * (8 + 4 * D);
 }
 
 template <int D, int T>
-static int launch_prefill(const PagedAttnParams& a, void* work, long long work_bytes, cudaStream_t stream) {
+static int launch_prefill(const PagedAttnParams& a, int max_new, void* work, long long work_bytes, cudaStream_t stream) {
     using Cfg = PrefillCfg<D, T>;
     static PerDeviceOnce attr_once;
     int attr_dev = 0;
@@ -607,9 +608,9 @@ static int launch_prefill(const PagedAttnParams& a, void* work, long long work_b
         if (e != cudaSuccess) return FRT_CUDA_ERR(e);
         attr_once.set(attr_dev);
     }
-    if (work_bytes < prefill_workspace<D, T>(a.tokens, a.batch, a.group, a.hkv)) return FRT_ERR_INVALID;
-    const long long items = prefill_items(a.tokens, a.batch, a.group, a.hkv, 128 * T), tiles = items / a.hkv;
-    if (tiles > 0x7fffffffLL / a.hkv) return FRT_ERR_UNSUPPORTED;
+    if (work_bytes < prefill_workspace<D, T>(a.tokens, a.batch, max_new, a.group, a.hkv)) return FRT_ERR_INVALID;
+    const long long tiles = prefill_tiles(a.tokens, a.batch, max_new, a.group, 128 * T), items = tiles * a.hkv;
+    if (items > 0x7fffffffLL) return FRT_ERR_UNSUPPORTED;
     PrefillParams pp = {};
     pp.a = a;
     pp.splits = prefill_splits(items, device_sm_count());

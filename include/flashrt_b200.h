@@ -539,7 +539,8 @@ int frt_b200_paged_kv_append_fp8(const void* qkv, long long qkv_stride, const fl
  *   flags bit 1 (no window then) all seq_lens.  softcap > 0: scores become softcap * tanh(s / softcap).  Keys whose page is no
  *   block of the pool are absent.  A row that sees no key is zero, its lse -infinity.  Codes and scales are finite, scales
  *   positive, as the append leaves them; nothing is read behind a sequence's end or in front of its window.
- *   max_new: new tokens of the longest sequence, or more; a choice of the kernel, whose results agree to rounding.
+ *   max_new: new tokens of the longest sequence, or more: by it the kernels are chosen, whose results agree to rounding, and their
+ *   grid; rows of a sequence with more may be left out.
  *   workspace: frt_b200_paged_attention_workspace_bytes bytes for the same figures, 16-byte aligned, zeroed once; every launch
  *   leaves it ready for the next, of any shape that it is large enough for.  Launches that share one must not overlap. */
 int frt_b200_paged_attention_fp8(const void* Q, long long q_stride, void* O, long long o_stride, float* lse,
