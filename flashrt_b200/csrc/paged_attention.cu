@@ -928,15 +928,12 @@ static int launch_paged_attention(PagedAttnParams p, void* work, cudaStream_t st
 
 }  // namespace frt
 
-// Row tiles of 8 NT rows, so that the keys are read and converted as few times as the registers of the accumulators allow (heads of
-// 256: 16 rows, else 32), and no wider than the rows need.
-static int paged_nt(long long rows, int d) {
-    const int most = d == 256 ? 2 : 4;
-    const long long tiles = (rows + 8 * most - 1) / (8 * most);
-    return tiles < 1 ? 1 : tiles > 4 ? most : (int)((rows + 8 * tiles - 1) / (8 * tiles));
-}
-// Query rows of a sequence up to which the kernel for few rows takes it.
-static int paged_few(int d) { return d == 256 ? 16 : 32; }
+// Row tiles of 8 NT rows, no wider than the rows need (at most paged_few of them).
+static int paged_nt(long long rows) { return rows > 16 ? 3 : rows > 8 ? 2 : 1; }
+// Query rows of a sequence up to which the kernel for few rows takes it.  16 sequences x 4 key/value heads on 4000 keys, this kernel and the
+// other: heads of 128, 16 rows 28 and 45 us, 24 rows 40 and 45, 32 rows 66 and 42; of 64, 24 rows 27 and 34, 32 rows 36 and 33; of 256,
+// 16 rows 54 and 75, 24 rows 108 and 76.
+static int paged_few(int d) { return d == 256 ? 16 : 24; }
 // f(head dim, row tiles of a CTA)
 template <typename F>
 static auto prefill_dispatch(int d, long long rows, F f) {
@@ -953,7 +950,6 @@ static auto paged_dispatch(int d, int nt, F f) {
     using std::integral_constant;
     auto with = [&](auto D) {
         if constexpr (D() != 256) {
-            if (nt == 4) return f(D, integral_constant<int, 4>());
             if (nt == 3) return f(D, integral_constant<int, 3>());
         }
         if (nt == 2) return f(D, integral_constant<int, 2>());
@@ -972,7 +968,7 @@ extern "C" int frt_b200_paged_attention_workspace_bytes(int tokens, int batch, i
     if (head_dim != 64 && head_dim != 128 && head_dim != 256) return FRT_ERR_UNSUPPORTED;
     const int group = num_heads_q / num_heads_kv, few = paged_few(head_dim);
     const long long rows = (long long)max_new * group;
-    *out_bytes = paged_dispatch(head_dim, paged_nt(rows < few ? rows : few, head_dim), [](auto D, auto NT) { return paged_workspace<D(), NT()>(); });
+    *out_bytes = paged_dispatch(head_dim, paged_nt(rows < few ? rows : few), [](auto D, auto NT) { return paged_workspace<D(), NT()>(); });
     if (rows > few)
         *out_bytes += prefill_dispatch(head_dim, rows, [&](auto D, auto T) {
             return prefill_workspace<D(), T()>(tokens, batch, max_new, group, num_heads_kv);
@@ -1043,7 +1039,7 @@ extern "C" int frt_b200_paged_attention_fp8(const void* Q, long long q_stride, v
     p.few_rows = many ? few : INT_MAX;
     uint8_t* work = static_cast<uint8_t*>(workspace);
     int rc = FRT_OK;
-    rc = paged_dispatch(head_dim, paged_nt(rows < few ? rows : few, head_dim), [&](auto D, auto NT) {
+    rc = paged_dispatch(head_dim, paged_nt(rows < few ? rows : few), [&](auto D, auto NT) {
             const long long need = paged_workspace<D(), NT()>();
             if (workspace_bytes < need) return (int)FRT_ERR_INVALID;
             const int r = some_few ? launch_paged_attention<D(), NT()>(p, work, stream_of) : FRT_OK;
