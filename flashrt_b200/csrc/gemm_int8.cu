@@ -143,10 +143,10 @@ __device__ __forceinline__ void tma_load_pair(uint32_t dst, const CUtensorMap* m
         ::"r"(dst), "l"(m), "r"(bar_cluster_addr), "r"(x), "r"(y)
         : "memory");
 }
-__device__ __forceinline__ void commit_both(uint32_t bar_addr) {
+__device__ __forceinline__ void commit_both(uint32_t bar_addr, uint32_t leader) {
     asm volatile(
         "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar_addr),
-        "h"((uint16_t)3)
+        "h"((uint16_t)(3u << leader))
         : "memory");
 }
 __device__ __forceinline__ float finish(int acc, float ts, float cs, float bias, bool has_bias) {
@@ -290,10 +290,12 @@ gemm_int8_lane_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
                 tc::tmem_ld16(t_src + c0, v);
                 tc::tmem_ld_wait();
                 if (S > 1) {
-                    // [token][channel]: a warp's store is 128 contiguous bytes
-                    uint32_t* red = reinterpret_cast<uint32_t*>(smem) + q * 32 + lane;
+                    // [four tokens][channel]: a warp's store is 512 contiguous bytes
+                    const uint32_t red = tc::smem_u32(smem) + (uint32_t)(c0 / 4 * 128 + q * 32 + lane) * 16;
 #pragma unroll
-                    for (int j = 0; j < 16; ++j) red[(c0 + j) * 128] = v[j];
+                    for (int j = 0; j < 16; j += 4)
+                        asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(red + j * 512), "r"(v[j]), "r"(v[j + 1]), "r"(v[j + 2]),
+                                     "r"(v[j + 3]) : "memory");
                     continue;
                 }
 #pragma unroll
@@ -311,12 +313,26 @@ gemm_int8_lane_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
             const bool in = n < p.N;
             const float cs = in ? p.channel_scale[n] : 0.0f;
             const float bias = in && p.bias ? __bfloat162float(p.bias[n]) : 0.0f;
-            const uint32_t red = tc::smem_u32(smem) + (uint32_t)(q * 32 + lane) * 4;
-            for (int m = rank; m < p.M; m += S) {
-                int sum = 0;
-                for (int r = 0; r < S; ++r)
-                    sum += __float_as_int(tc::dsmem_ld_f32(tc::dsmem_map(red + (uint32_t)m * 512, (uint32_t)r)));
-                if (in) p.out[(size_t)m * p.N + n] = __float2bfloat16_rn(finish(sum, p.token_scale[m], cs, bias, p.bias != nullptr));
+            const uint32_t red = tc::smem_u32(smem) + (uint32_t)(q * 32 + lane) * 16;
+            for (int g = rank; 4 * g < p.M; g += S) {        // four tokens; the ranks' partials are all on their way before the first is added
+                float4 w[8];
+#pragma unroll
+                for (int r = 0; r < 8; ++r)
+                    if (r < S) w[r] = tc::dsmem_ld_f32x4(tc::dsmem_map(red + (uint32_t)g * 2048, (uint32_t)r));
+                int sum[4] = {0, 0, 0, 0};
+#pragma unroll
+                for (int r = 0; r < 8; ++r)
+                    if (r < S) {
+                        sum[0] += __float_as_int(w[r].x);
+                        sum[1] += __float_as_int(w[r].y);
+                        sum[2] += __float_as_int(w[r].z);
+                        sum[3] += __float_as_int(w[r].w);
+                    }
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int m = 4 * g + e;
+                    if (in && m < p.M) p.out[(size_t)m * p.N + n] = __float2bfloat16_rn(finish(sum[e], p.token_scale[m], cs, bias, p.bias != nullptr));
+                }
             }
         }
         tc::cluster_sync_all();                              // nobody leaves while its partial is read
@@ -399,11 +415,14 @@ __device__ __forceinline__ void store_block(const Params& p, const uint32_t* v, 
     __syncwarp();
 }
 
-template <int BN>
+// S > 1: a cluster of S pairs takes one tile, a pair the k-blocks [kb s / S, kb (s + 1) / S); the pairs then lay their integer partials into
+// shared memory, where their rings were, and each finishes BN / S of the columns.
+template <int BN, int S>
 __global__ void __launch_bounds__(320, 1)
 gemm_int8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmW, Params p) {
     using Cfg = PairCfg<BN>;
     constexpr int STAGES = Cfg::STAGES;
+    static_assert(S == 1 || (BN / S >= 64 && 128 * BN * 4 <= STAGES * Cfg::STAGE_BYTES), "columns of a half of the warps, partials in the ring");
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
     uint64_t* full = reinterpret_cast<uint64_t*>(smem + STAGES * Cfg::STAGE_BYTES);   // the leader's count both CTAs' bytes
@@ -414,8 +433,10 @@ gemm_int8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
     const uint64_t deadline = tc::global_timer_ns() + FRT_KERNEL_DEADLINE_NS;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const uint32_t rank = tc::cluster_ctarank();
-    const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+    const uint32_t cluster_rank = tc::cluster_ctarank(), rank = cluster_rank & 1, leader = cluster_rank & ~1u;
+    const int split = (int)(cluster_rank >> 1);
+    const int pair = (int)blockIdx.x / (2 * S), pairs = (int)gridDim.x / (2 * S);     // S > 1: as many as tiles
+    const int kb0 = S == 1 ? 0 : (int)((long long)p.kb * split / S), kb1 = S == 1 ? p.kb : (int)((long long)p.kb * (split + 1) / S);
     const int m_tiles = (p.M + 255) / 256, n_tiles = (p.N + BN - 1) / BN, total = m_tiles * n_tiles;
 
     if (threadIdx.x == 0) {
@@ -442,7 +463,7 @@ gemm_int8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
     if (warp == 0) {
         // ---------------- producer of this CTA's rows, bytes counted at the leader
         const uint32_t ring = tc::smem_u32(smem), empty_a = tc::smem_u32(empty), full_a = tc::smem_u32(full);
-        const uint32_t lead_full = tc::dsmem_map(full_a, 0);
+        const uint32_t lead_full = tc::dsmem_map(full_a, leader);
         pdl_wait();
         int s = 0;
         uint32_t ph = 1;
@@ -451,7 +472,7 @@ gemm_int8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
             int mt, nt;
             tile_at(t, p.gm, m_tiles, n_tiles, mt, nt);
             const int m0 = mt * 256 + (int)rank * 128, n0 = nt * BN + (int)rank * (BN / 2);
-            for (int kb = 0; kb < p.kb; ++kb) {
+            for (int kb = kb0; kb < kb1; ++kb) {
                 if (!tc::warp_wait(empty_a + 8 * s, ph, ready, deadline, abort_flag)) {
                     if (lane == 0) gave_up(p.status, abort_flag, ERR_PRODUCER);
                     t = total;
@@ -485,7 +506,7 @@ gemm_int8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
             }
             tc::tc_fence_after_sync();
             const uint32_t d_tm = tmem + buf * BN;
-            for (int kb = 0; kb < p.kb; ++kb) {
+            for (int kb = kb0; kb < kb1; ++kb) {
                 if (!tc::warp_wait(full_a + 8 * s, ph, ready, deadline, abort_flag)) {
                     if (lane == 0) gave_up(p.status, abort_flag, ERR_MMA);
                     failed = true;
@@ -498,9 +519,9 @@ gemm_int8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
                 ready = tc::mbar_test(full_a + 8 * s, ph);
                 if (tc::elect_one()) {
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) mma_pair(d_tm, dA0 + so + 2 * k, dB0 + so + 2 * k, idesc, kb > 0 || k > 0 ? 1u : 0u);
-                    commit_both(done);
-                    if (kb == p.kb - 1) commit_both(accF_a + 8 * buf);
+                    for (int k = 0; k < 4; ++k) mma_pair(d_tm, dA0 + so + 2 * k, dB0 + so + 2 * k, idesc, kb > kb0 || k > 0 ? 1u : 0u);
+                    commit_both(done, leader);
+                    if (kb == kb1 - 1) commit_both(accF_a + 8 * buf, leader);
                 }
             }
         }
@@ -531,10 +552,51 @@ gemm_int8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
                 __syncwarp();
                 tc::tmem_ld32(t_acc + c, v);
                 tc::tmem_ld_wait();
-                if (m_base < p.M && n_base + c < p.N) store_block(p, v, m_base, n_base + c, stg, ts, vec);
+                if constexpr (S > 1) {                       // [four columns][row]: a warp's store is 512 contiguous bytes
+                    const uint32_t red = tc::smem_u32(smem) + ((half * (BN / 2) + c) / 4 * 128 + q * 32 + lane) * 16;
+#pragma unroll
+                    for (int j = 0; j < 32; j += 4)
+                        asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(red + j * 512), "r"(v[j]), "r"(v[j + 1]), "r"(v[j + 2]),
+                                     "r"(v[j + 3]) : "memory");
+                } else if (m_base < p.M && n_base + c < p.N) store_block(p, v, m_base, n_base + c, stg, ts, vec);
             }
+            if constexpr (S > 1) break;
             tc::tc_fence_before_sync();
-            tc::mbar_arrive_cluster(tc::dsmem_map(tc::smem_u32(&acc_empty[buf]), 0));
+            tc::mbar_arrive_cluster(tc::dsmem_map(tc::smem_u32(&acc_empty[buf]), leader));
+        }
+    }
+    if constexpr (S > 1) {
+        tc::cluster_sync_all();                // all partials are there
+        if (warp >= 2 && !*abort_flag) {
+            constexpr int W = BN / S / 2;      // columns of this warp
+            const int q = warp & 3, half = (warp - 2) >> 2, col = split * (BN / S) + half * W;
+            int mt, nt;
+            tile_at(pair, p.gm, m_tiles, n_tiles, mt, nt);
+            const int m_base = mt * 256 + (int)rank * 128 + q * 32, n_base = nt * BN + col;
+            const float ts = m_base + lane < p.M ? p.token_scale[m_base + lane] : 0.0f;
+            uint8_t* stg = smem + STAGES * Cfg::STAGE_BYTES + 256 + (warp - 2) * (32 * 128);
+            const uint32_t red = tc::smem_u32(smem) + (uint32_t)(col / 4 * 128 + q * 32 + lane) * 16;
+#pragma unroll 1
+            for (int c = 0; c < W; c += 32) {
+                uint32_t v[32];
+#pragma unroll
+                for (int j = 0; j < 32; ++j) v[j] = 0;
+#pragma unroll
+                for (int s = 0; s < S; ++s) {
+                    const uint32_t from = tc::dsmem_map(red + (uint32_t)c * 512, (uint32_t)(2 * s) + rank);
+                    float4 w[8];
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) w[j] = tc::dsmem_ld_f32x4(from + (uint32_t)j * 2048);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        v[4 * j] += __float_as_uint(w[j].x);
+                        v[4 * j + 1] += __float_as_uint(w[j].y);
+                        v[4 * j + 2] += __float_as_uint(w[j].z);
+                        v[4 * j + 3] += __float_as_uint(w[j].w);
+                    }
+                }
+                if (m_base < p.M && n_base + c < p.N) store_block(p, v, m_base, n_base + c, stg, ts, (p.N & 3) == 0);
+            }
         }
     }
     if (*abort_flag && threadIdx.x == 0) let_copies_land();
@@ -577,14 +639,14 @@ static int launch_lane(const void* A, const void* W, Params p, int K, int splits
     return e == cudaSuccess ? FRT_OK : FRT_CUDA_ERR(e);
 }
 
-template <int BN>
+template <int BN, int S>
 static int launch_pair(const void* A, const void* W, Params p, int K, cudaStream_t stream) {
     using Cfg = PairCfg<BN>;
     static PerDeviceOnce once;
     CUtensorMap tmA, tmW;
     int dev = 0;
     if (once.need(dev)) {
-        const cudaError_t e = cudaFuncSetAttribute(gemm_int8_pair_kernel<BN>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::SMEM_BYTES);
+        const cudaError_t e = cudaFuncSetAttribute(gemm_int8_pair_kernel<BN, S>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::SMEM_BYTES);
         if (e != cudaSuccess) return FRT_CUDA_ERR(e);
         once.set(dev);
     }
@@ -600,21 +662,52 @@ static int launch_pair(const void* A, const void* W, Params p, int K, cudaStream
     else
         while (p.gm < m_tiles && (long long)(p.gm + 1) * (p.gm + 1) * 256 <= (long long)BN * workers) ++p.gm;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(2 * (unsigned)(total < workers ? total : workers));
+    cfg.gridDim = dim3(S > 1 ? 2 * S * (unsigned)total : 2 * (unsigned)(total < workers ? total : workers));
     cfg.blockDim = dim3(320);
     cfg.dynamicSmemBytes = Cfg::SMEM_BYTES;
     cfg.stream = stream;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = 2;
+    attr[0].val.clusterDim.x = 2 * S;
     attr[0].val.clusterDim.y = 1;
     attr[0].val.clusterDim.z = 1;
     attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 2;
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, gemm_int8_pair_kernel<BN>, tmA, tmW, p);
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, gemm_int8_pair_kernel<BN, S>, tmA, tmW, p);
     return e == cudaSuccess ? FRT_OK : FRT_CUDA_ERR(e);
+}
+
+// Clusters of the sharing form that the device holds at once (a cluster lies in one GPC, whose SMs its size need not divide): asked once.
+template <int BN, int S>
+static long long pair_clusters() {
+    using Cfg = PairCfg<BN>;
+    static int known[64] = {0};
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 0;
+    if (!known[dev]) {
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3(2 * S);
+        cfg.blockDim = dim3(320);
+        cfg.dynamicSmemBytes = Cfg::SMEM_BYTES;
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = 2 * S;
+        attr[0].val.clusterDim.y = 1;
+        attr[0].val.clusterDim.z = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = 1;
+        int n = 0;
+        cudaError_t e = cudaFuncSetAttribute(gemm_int8_pair_kernel<BN, S>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::SMEM_BYTES);
+        if (e == cudaSuccess) e = cudaOccupancyMaxActiveClusters(&n, gemm_int8_pair_kernel<BN, S>, &cfg);
+        if (e != cudaSuccess) {
+            cudaGetLastError();                              // not this launch's error: the form is not offered
+            n = 0;
+        }
+        known[dev] = n + 1;
+    }
+    return known[dev] - 1;
 }
 
 template <int WPR>
@@ -690,8 +783,30 @@ extern "C" int frt_b200_gemm_int8_nt(const void* A, const void* W, void* D, int 
         if (M <= 64) return i8::launch_lane<64>(A, W, p, K, splits, st);
         return i8::launch_lane<128>(A, W, p, K, splits, st);
     }
-    // 256 columns unless narrower tiles save more of the last wave than their operand traffic costs
-    const long long pairs = device_sm_count() / 2, mt = (M + 255) / 256;
-    const long long wide = (mt * ((N + 255) / 256) + pairs - 1) / pairs * 2, narrow = (mt * ((N + 127) / 128) + pairs - 1) / pairs;
-    return narrow * 1.1 < wide ? i8::launch_pair<128>(A, W, p, K, st) : i8::launch_pair<256>(A, W, p, K, st);
+    // The cheapest of: tiles of 256 or 128 columns in whole waves of CTA pairs, or, where the device holds them all at once, tiles whose K
+    // two or four pairs share.  A k-block takes 0.30 us on 256 columns and 0.235 on 128 (operands from L2 bound it), an exchange of
+    // partials 5.  817 x 2048 x 16384 30.0 us on 64 pairs of 128 columns, 26.7 with two pairs a tile; 256 x 2048 x 8192 on 16 pairs 18.9,
+    // with four pairs a tile 14.5; 300 x 2048 x 2048 7.2 unshared, 22.7 shared.
+    const long long pairs = device_sm_count() / 2, mt = (M + 255) / 256, wide = mt * ((N + 255) / 256), narrow = mt * ((N + 127) / 128);
+    auto waves = [&](long long tiles) { return (double)((tiles + pairs - 1) / pairs); };
+    double best = waves(wide) * p.kb * 0.30;
+    int form = 0;
+    if (waves(narrow) * p.kb * 0.235 < best) {
+        best = waves(narrow) * p.kb * 0.235;
+        form = 1;
+    }
+    auto shared = [&](int f, long long tiles, int S, double per_kb, long long (*clusters)()) {
+        const double cost = (p.kb + S - 1) / S * per_kb + 5.0;
+        if (cost < best && p.kb >= 4 * S && tiles <= clusters()) { best = cost; form = f; }
+    };
+    shared(2, wide, 2, 0.30, i8::pair_clusters<256, 2>);
+    shared(3, wide, 4, 0.30, i8::pair_clusters<256, 4>);
+    shared(4, narrow, 2, 0.235, i8::pair_clusters<128, 2>);
+    switch (form) {
+        case 1: return i8::launch_pair<128, 1>(A, W, p, K, st);
+        case 2: return i8::launch_pair<256, 2>(A, W, p, K, st);
+        case 3: return i8::launch_pair<256, 4>(A, W, p, K, st);
+        case 4: return i8::launch_pair<128, 2>(A, W, p, K, st);
+        default: return i8::launch_pair<256, 1>(A, W, p, K, st);
+    }
 }

@@ -190,9 +190,21 @@ __device__ __forceinline__ float inverse_sum(float l) { return l > 0.0f ? __frcp
 __device__ __forceinline__ int query_exponent(float top) {
     return top > 1e-30f && top < INFINITY ? min((int)((__float_as_uint(top) >> 23) & 255) - 126, 126) : 0;
 }
-// tanh through the hardware's exp2 and reciprocal: 2^-22 absolute, where tanh.approx has 2^-11
-__device__ __forceinline__ float soft_cap(float s, float cap, float inv_cap2) {
-    return cap * (1.0f - 2.0f * rcp(1.0f + ex2(s * inv_cap2)));
+// cap * tanh(s / cap).  Through the hardware's exp2 and reciprocal: 2^-22 of the cap, where tanh.approx has 2^-11.  For |s| <= cap / 2,
+// which scores seldom leave, the first seven terms of the series (the next is below 10^-7 of the value): the exponential unit has
+// the softmax's own to do.
+__device__ __forceinline__ float soft_cap(float s, float cap, float inv_cap) {
+    constexpr float LOG2E2 = 2.8853900817779268f;
+    return cap * (1.0f - 2.0f * rcp(1.0f + ex2(s * inv_cap * LOG2E2)));
+}
+__device__ __forceinline__ float soft_cap_low(float s, float inv_cap) {
+    const float x = s * inv_cap, y = x * x;
+    float q = fmaf(y, 21844.0f / 6081075.0f, -1382.0f / 155925.0f);
+    q = fmaf(q, y, 62.0f / 2835.0f);
+    q = fmaf(q, y, -17.0f / 315.0f);
+    q = fmaf(q, y, 2.0f / 15.0f);
+    q = fmaf(q, y, -1.0f / 3.0f);
+    return fmaf(s * y, q, s);
 }
 
 // The line cut into `grid` stretches whose lengths differ by one at most.
@@ -441,7 +453,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
     const int group = warp >> 2, part_w = warp & 3;
     int turn = 0;
     const bool capped = p.cap > 0.0f;
-    const float inv_cap2 = capped ? 2.0f * LOG2E / p.cap : 0.0f;
+    const float inv_cap = capped ? 1.0f / p.cap : 0.0f;
 
     for (long long at = w0; at < w1;) {
         if (at != w0) next_segment();
@@ -588,12 +600,23 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
                     for (int x = 0; x < 4; ++x) sc[st][nt][x] = fmaf(sc[st][nt][x], f[x & 1], capped ? 0.0f : lv[st]);
                 }
             if (capped) {
+                float far = 0.0f;
 #pragma unroll
                 for (int st = 0; st < ST; ++st)
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                        for (int x = 0; x < 4; ++x) sc[st][nt][x] = fmaf(soft_cap(sc[st][nt][x], p.cap, inv_cap2), LOG2E, lv[st]);
+                        for (int x = 0; x < 4; ++x) far = fmaxf(far, fabsf(sc[st][nt][x]));
+                const bool low = __all_sync(0xffffffffu, far <= 0.5f * p.cap);
+#pragma unroll
+                for (int st = 0; st < ST; ++st)
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                        for (int x = 0; x < 4; ++x) {
+                            const float s = sc[st][nt][x];
+                            sc[st][nt][x] = fmaf(low ? soft_cap_low(s, inv_cap) : soft_cap(s, p.cap, inv_cap), LOG2E, lv[st]);
+                        }
             }
             if (!open) {
                 // values outside the item's keys may be anything, and 0 x NaN is NaN: zero their rows, 16 bytes a lane

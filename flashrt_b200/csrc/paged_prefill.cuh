@@ -365,7 +365,7 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
             const uint32_t lane_off = (uint32_t)((warp & 3) * 32) << 16;
             const uint32_t tmem_O = tmem + Cfg::O_COL + t * D + lane_off;
             const bool capped = p.cap > 0.0f;
-            const float inv_cap2 = capped ? 2.0f * LOG2E / p.cap : 0.0f;
+            const float inv_cap = capped ? 1.0f / p.cap : 0.0f;
             // keys that every row of the warp sees
             const int w_hi = (int)__reduce_min_sync(0xffffffffu, (unsigned)hi), w_lo = (int)__reduce_max_sync(0xffffffffu, (unsigned)lo);
             const bool idle = t * 128 + (warp & 3) * 32 >= rows;    // a warp behind the last row only signs
@@ -395,13 +395,19 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
                         tc::tmem_ld32(tmem_S + k, v);
                         const float2 s0 = *reinterpret_cast<const float2*>(&sc[k / 16]), s1 = *reinterpret_cast<const float2*>(&sc[k / 16 + 1]);
                         tc::tmem_ld_wait();
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) v[e] = __float_as_uint(__uint_as_float(v[e]) * (rf * (e < 16 ? s0.x : s1.x)));
                         if (capped) {
+                            float far = 0.0f;
 #pragma unroll
-                            for (int e = 0; e < 32; ++e)
-                                v[e] = __float_as_uint(soft_cap(__uint_as_float(v[e]) * (rf * (e < 16 ? s0.x : s1.x)), p.cap, inv_cap2) * LOG2E);
-                        } else {
+                            for (int e = 0; e < 32; ++e) far = fmaxf(far, fabsf(__uint_as_float(v[e])));
+                            if (__all_sync(0xffffffffu, far <= 0.5f * p.cap)) {
 #pragma unroll
-                            for (int e = 0; e < 32; ++e) v[e] = __float_as_uint(__uint_as_float(v[e]) * (rf * (e < 16 ? s0.x : s1.x)));
+                                for (int e = 0; e < 32; ++e) v[e] = __float_as_uint(soft_cap_low(__uint_as_float(v[e]), inv_cap) * LOG2E);
+                            } else {
+#pragma unroll
+                                for (int e = 0; e < 32; ++e) v[e] = __float_as_uint(soft_cap(__uint_as_float(v[e]), p.cap, inv_cap) * LOG2E);
+                            }
                         }
                         const int from = lo - key0 - k, to = hi - key0 - k;
 #pragma unroll

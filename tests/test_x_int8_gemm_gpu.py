@@ -119,6 +119,14 @@ def test_longest_sums(m):
     check(m, 160, 131056, bias=False)
 
 
+@pytest.mark.parametrize("m,n,k", [(817, 2048, 16384), (300, 2048, 2048), (129, 256, 8192), (256, 4096, 4096), (513, 1000, 10000), (400, 333, 16384),
+                                   (200, 8192, 1024), (1024, 1024, 1040)])
+def test_shared_sums(m, n, k):
+    """Few tiles and a long K: two or four pairs share a tile's sum."""
+    check(m, n, k, bias=False)
+    check(m, n, k)
+
+
 def test_many_tiles():
     check(4096, 8192, 256, bias=False)
     check(96, 32768, 2048, bias=False, pdl=True)
