@@ -421,6 +421,112 @@ def test_attention_captured():
         close(o, None, want)
 
 
+# ---------------------------------------------------------------- chunks of prompts: the tensor-memory kernel
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("block", [16, 32, 64, 128])
+def test_chunk_blocks(d, block):
+    _run_attend(8, 2, d, block, [70, 33, 1], [390, 33, 200], seed=d + block)
+
+
+@pytest.mark.parametrize("hq,hkv", [(3, 1), (5, 1), (7, 1), (16, 1), (4, 4), (12, 2)])
+def test_chunk_groups(hq, hkv):
+    """Groups that do not divide 128 rows: a token's heads lie in two tiles."""
+    _run_attend(hq, hkv, 128, 32, [45, 100], [45, 350], seed=hq)
+
+
+@pytest.mark.parametrize("kw", [dict(), dict(window=70), dict(window=1), dict(cap=0.3), dict(cap=20.0), dict(causal=False), dict(cap=0.3, window=130),
+                                dict(causal=False, cap=20.0)])
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_chunk_masks(kw, d):
+    _run_attend(4, 1, d, 32, [150, 65], [700, 65], seed=d + 3, tail=2, **kw)
+
+
+def test_chunk_one_row_tile_and_key_splits():
+    """One sequence of few rows and a long context: the keys are split over CTAs and the pieces joined."""
+    for d, block in ((128, 64), (64, 16), (256, 128)):
+        _run_attend(4, 1, d, block, [9], [2600], seed=d)
+        _run_attend(8, 1, d, block, [40], [1900], seed=d + 1, window=300)
+    _run_attend(2, 1, 128, 16, [20], [3], seed=5)                  # more splits than tiles, rows without keys
+
+
+def test_chunk_many_sequences():
+    """More sequences than threads of a block, all of them with more rows than the other kernel takes, or mixed."""
+    n = 560
+    _run_attend(4, 1, 64, 16, [7] * n, [7 + i % 12 for i in range(n)], seed=6)
+    _run_attend(8, 2, 64, 16, [(1, 7, 2, 40)[i % 4] for i in range(40)], [45 + i for i in range(40)], seed=7)
+
+
+def test_chunk_absent_pages_and_what_lies_around():
+    hq, hkv, d, block = 4, 1, 128, 16
+    lens, cu = [170], [0, 60]
+    pool = Pool(14, hkv, block, d, 5)
+    table = torch.tensor([[0, 1, -1, 2, 3, 99, 4, 5, 6, 7, 8, 9, 9]], dtype=torch.int32)
+    q = torch.randn(60, hq * d, generator=torch.Generator().manual_seed(1)).to(BF16)
+    c, s = pool.host()
+    for kw in (dict(), dict(window=40)):
+        want = R.attention(q.view(-1, hq, d), c["k"], c["v"], s["k"], s["v"], table, cu, lens, 0.1, **kw)
+        for n in "kv":
+            pool.c[n][8, :, 170 % block:] = 0x7F                  # behind the sequence's end (block 10 of it)
+            for page in (10, 11, 12, 13):
+                pool.c[n][page], pool.s[n][page] = 0xFF, math.inf
+        if kw:
+            table = table.clone()
+            table[0, :4] = torch.tensor([12, 99, 13, -1], dtype=torch.int32)      # in front of every window (keys below 71)
+            want = R.attention(q.view(-1, hq, d), c["k"], c["v"], s["k"], s["v"], table, cu, lens, 0.1, **kw)
+        close(*attend(pool, q.cuda(), table, cu, lens, hq, hkv, d, scale=0.1, **kw), want)
+
+
+@pytest.mark.parametrize("new", [[1, 1, 1], [3, 1, 2], [40, 3, 100]])
+def test_attention_strides_streams_and_captures(new):
+    """Rows of Q and O inside wider ones, no lse, a larger max_new, another stream, a captured launch replayed: the same bits."""
+    from flashrt_b200 import flash_rt_fa2 as fa2
+    hq, hkv, d, block = 8, 2, 128, 32
+    ctx = [n + 200 * i for i, n in enumerate(new)]
+    pool, table, cu, q, o, lse = _run_attend(hq, hkv, d, block, new, ctx, seed=2)
+    wide_q = torch.zeros(cu[-1], hq * d + 40, dtype=BF16, device="cuda")
+    wide_q[:, :hq * d] = q.cuda()
+    wide_o = torch.full((cu[-1], hq * d + 24), -7.0, dtype=BF16, device="cuda")
+    n = fa2.paged_workspace_bytes(cu[-1], len(ctx), max(new), hq, hkv, d)
+    work = torch.zeros(n, dtype=torch.uint8, device="cuda")
+    dev = lambda y: torch.tensor(y, dtype=torch.int32).cuda()  # noqa: E731
+    cu_d, lens_d, table_d = dev(cu), dev(ctx), table.cuda()
+
+    def call(stream):
+        fa2.paged_fwd_fp8(wide_q.data_ptr(), wide_o.data_ptr(), 0, pool.c["k"].data_ptr(), pool.c["v"].data_ptr(), pool.s["k"].data_ptr(),
+                          pool.s["v"].data_ptr(), table_d.data_ptr(), table.shape[1], cu_d.data_ptr(), lens_d.data_ptr(), cu[-1], len(ctx),
+                          max(new), pool.num_blocks, block, hq, hkv, d, d ** -0.5, work.data_ptr(), n, stream, q_stride=hq * d + 40,
+                          o_stride=hq * d + 24)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    call(side.cuda_stream)
+    side.synchronize()
+    assert torch.equal(wide_o[:, :hq * d], o) and (wide_o[:, hq * d:] == -7).all()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        call(_stream())
+    for _ in range(3):
+        wide_o.fill_(-7.0)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(wide_o[:, :hq * d], o) and (wide_o[:, hq * d:] == -7).all()
+    o2, lse2 = attend(pool, q.cuda(), table, cu, ctx, hq, hkv, d, max_new=max(new) + 200)
+    c, s = pool.host()
+    close(o2, lse2, R.attention(q.view(-1, hq, d), c["k"], c["v"], s["k"], s["v"], table, cu, ctx, d ** -0.5))
+
+
+def test_attention_workspace_too_small_is_refused():
+    from flashrt_b200 import flash_rt_fa2 as fa2
+    from flashrt_b200._lib import KernelError
+    hq, hkv, d = 8, 2, 128
+    t = torch.zeros(4096, dtype=torch.int32, device="cuda")
+    for new in (1, 300):
+        n = fa2.paged_workspace_bytes(new, 1, new, hq, hkv, d)
+        with pytest.raises(KernelError, match="-1"):
+            fa2.paged_fwd_fp8(*[t.data_ptr()] * 8, 1, t.data_ptr(), t.data_ptr(), new, 1, new, 4, 16, hq, hkv, d, 0.1, t.data_ptr(), n - 16, _stream())
+    torch.cuda.synchronize()
+
+
 def test_attention_offsets_beyond_32_bits():
     """A pool of more than 4 GB: blocks at its far end."""
     hq, hkv, d, block = 8, 8, 256, 128
