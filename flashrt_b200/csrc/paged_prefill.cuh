@@ -371,6 +371,17 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
             const bool idle = t * 128 + (warp & 3) * 32 >= rows;    // a warp behind the last row only signs
             float m = -INFINITY, l = 0.0f;
             bool alive = true;
+            // A parity tells a phase of o_done from its neighbours only.  While a warp has not signed tile i, the products of tile i - 2 are
+            // through (its scores stood behind them) and that of tile i is not, so it may wait for tile i - 1's; once it has signed, it may
+            // find itself two behind, or two ahead of warps that have not.  Hence the last product but one is waited for before the
+            // last tile is signed, and the last one after it.
+            auto last_but_one = [&](int i) {
+                if (i == 0 || i != nt - 1) return true;
+                const bool ok = tc::mbar_wait_until(&o_done[t], (uint32_t)((i - 1) & 1), deadline, &abort_s);
+                alive = __all_sync(0xffffffffu, ok) != 0;
+                if (!alive) gave_up(5);
+                return alive;
+            };
             for (int i = 0; i < nt; ++i) {
                 const int sb = 2 * t + (i & 1);
                 const uint32_t par = (uint32_t)((i >> 1) & 1), tmem_S = tmem + sb * BKV + lane_off;
@@ -381,6 +392,7 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
                 if (!__all_sync(0xffffffffu, ok)) { gave_up(4); alive = false; break; }
                 tc::tc_fence_after_sync();
                 if (idle) {
+                    if (!last_but_one(i)) break;
                     tc::tc_fence_before_sync();
                     tc::mbar_arrive(&p_half[sb]);
                     tc::mbar_arrive(&p_ready[sb]);
@@ -489,6 +501,7 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
                     }
                 }
                 tc::tmem_st_wait();
+                if (!last_but_one(i)) break;
                 tc::tc_fence_before_sync();
                 tc::mbar_arrive(&p_ready[sb]);
             }

@@ -449,6 +449,16 @@ def test_chunk_one_row_tile_and_key_splits():
     _run_attend(2, 1, 128, 16, [20], [3], seed=5)                  # more splits than tiles, rows without keys
 
 
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_chunk_warps_that_run_ahead(d):
+    """Second row tiles with warps without rows, whose neighbours in the first finish tiles before the others: a row is through only when
+    its last product is, and the same call gives the same bits."""
+    pool, table, cu, q, o, lse = _run_attend(8, 1, d, 16, [24, 25, 36, 23], [903, 1210, 640, 1100], seed=d, cap=30.0)
+    for _ in range(3):
+        again, l2 = attend(pool, q.cuda(), table, cu, [903, 1210, 640, 1100], 8, 1, d, cap=30.0)
+        assert torch.equal(o, again) and torch.equal(lse, l2)
+
+
 def test_chunk_many_sequences():
     """More sequences than threads of a block, all of them with more rows than the other kernel takes, or mixed."""
     n = 560
