@@ -37,7 +37,9 @@
 
 namespace frt {
 
-constexpr int PA_MAX_GRID = 512, PA_HEAD_BYTES = 4096;      // arrival counters at the head of the workspace
+// The head of a workspace: arrival counters of this kernel's CTAs, then of the other kernel's items.  At places of their own, whatever the
+// shapes: every launch leaves them at zero, and no partial is written over them.
+constexpr int PA_MAX_GRID = 512, PA_HEAD_BYTES = 4096;
 
 struct PagedAttnParams {
     const __nv_bfloat16* q;
@@ -1053,7 +1055,8 @@ extern "C" int frt_b200_paged_attention_fp8(const void* Q, long long q_stride, v
     const long long pool_rows = (long long)num_blocks * num_heads_kv * block_size;
     if (pool_rows > 0x7fffffffLL) return FRT_ERR_UNSUPPORTED;
     p.pool_rows = (int)pool_rows;
-    p.status = attention_status_device_ptr();
+    static PerDevicePointer status;
+    p.status = status.get(attention_status_device_ptr);
     if (!p.status) return FRT_ERR_UNSUPPORTED;
     // Sequences of few rows and of many go to different kernels; a batch whose sequences all bring max_new tokens needs one of them.
     const int few = paged_few(head_dim);
@@ -1071,5 +1074,5 @@ extern "C" int frt_b200_paged_attention_fp8(const void* Q, long long q_stride, v
             return r;
         });
     if (rc || !many) return rc;
-    return prefill_dispatch(head_dim, rows, [&](auto D, auto T) { return launch_prefill<D(), T()>(p, max_new, work, workspace_bytes, stream_of); });
+    return prefill_dispatch(head_dim, rows, [&](auto D, auto T) { return launch_prefill<D(), T()>(p, max_new, static_cast<unsigned*>(workspace) + PA_MAX_GRID, work, workspace_bytes, stream_of); });
 }

@@ -24,7 +24,7 @@ struct PrefillCfg {
     static constexpr int RAWS = BKV == 64 && D <= 128 ? 6 : 4, OPS = BKV == 64 && D <= 128 ? 6 : 3;
     static constexpr int OFF_OP = T * Q_BYTES, OFF_RAW = OFF_OP + OPS * KV_BYTES;
     static constexpr int SMEM_BYTES = OFF_RAW + RAWS * RAW_BYTES + 1024;
-    static_assert(SMEM_BYTES <= 232448 - (D == 256 ? 2048 : 3072), "dynamic and static shared memory of a CTA");
+    static_assert(SMEM_BYTES <= 232448 - (D == 256 ? 2 : 3) * 1024, "dynamic and static shared memory of a CTA");
     static constexpr int O_COL = T * 2 * BKV;             // accumulators behind the S
     static_assert(O_COL + T * D <= 512, "tensor memory");
     static constexpr int THREADS = 512;
@@ -37,7 +37,7 @@ struct PrefillCfg {
 struct PrefillParams {
     PagedAttnParams a;
     int splits;                  // along the keys; pieces joined by the CTA that arrives last at an item
-    unsigned* counters;          // one per item
+    unsigned* counters;          // one per item: at most SMs / 2 where the keys are split
     float* part_o;               // [item][split][tile][D][128]
     float2* part_ml;             // [item][split][tile][128]
 };
@@ -610,15 +610,16 @@ static int prefill_splits(long long items, int sms) {
     const long long s = sms / (items < 1 ? 1 : items);
     return s < 1 ? 1 : s > 8 ? 8 : (int)s;
 }
+// Pieces of all items; their arrival counters are in the workspace's head, where no partial ever lies.
 template <int D, int T>
 static long long prefill_workspace(long long tokens, long long batch, long long max_new, int group, int hkv) {
     const long long items = prefill_tiles(tokens, batch, max_new, group, 128 * T) * hkv;
     const int splits = prefill_splits(items, device_sm_count());
-    return splits == 1 ? 0 : (items * 4 + 15) / 16 * 16 + items * splits * T * 128 * (8 + 4 * D);
+    return splits == 1 ? 0 : items * splits * T * 128 * (8 + 4 * D);
 }
 
 template <int D, int T>
-static int launch_prefill(const PagedAttnParams& a, int max_new, void* work, long long work_bytes, cudaStream_t stream) {
+static int launch_prefill(const PagedAttnParams& a, int max_new, unsigned* counters, void* work, long long work_bytes, cudaStream_t stream) {
     using Cfg = PrefillCfg<D, T>;
     static PerDeviceOnce attr_once;
     int attr_dev = 0;
@@ -633,11 +634,9 @@ static int launch_prefill(const PagedAttnParams& a, int max_new, void* work, lon
     PrefillParams pp = {};
     pp.a = a;
     pp.splits = prefill_splits(items, device_sm_count());
-    uint8_t* w = static_cast<uint8_t*>(work);
-    pp.counters = reinterpret_cast<unsigned*>(w);
-    w += (items * 4 + 15) / 16 * 16;
-    pp.part_ml = reinterpret_cast<float2*>(w);
-    pp.part_o = reinterpret_cast<float*>(w + items * pp.splits * T * 128 * 8);
+    pp.counters = counters;
+    pp.part_ml = static_cast<float2*>(work);
+    pp.part_o = reinterpret_cast<float*>(static_cast<uint8_t*>(work) + items * pp.splits * T * 128 * 8);
     CUtensorMap tmK, tmV;
     const int box = Cfg::BKV < a.block_size ? Cfg::BKV : a.block_size;
     int rc = paged_map(&tmK, a.k, a.pool_rows, D, box, false);

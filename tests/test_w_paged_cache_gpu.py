@@ -525,6 +525,24 @@ def test_attention_strides_streams_and_captures(new):
     close(o2, lse2, R.attention(q.view(-1, hq, d), c["k"], c["v"], s["k"], s["v"], table, cu, ctx, d ** -0.5))
 
 
+def test_attention_one_workspace_for_all_shapes():
+    """A workspace that fits the largest serves every shape in any order: no launch leaves its partials where another one counts."""
+    from flashrt_b200 import flash_rt_fa2 as fa2
+    shapes = [(8, 1, 256, 16, [1, 1], [1500, 40]), (4, 1, 128, 32, [9], [2000]), (8, 2, 64, 64, [1], [3000]), (4, 1, 256, 128, [40], [900]),
+              (6, 2, 128, 16, [7, 1, 30], [400, 900, 1100]), (32, 1, 128, 64, [1], [2500]), (4, 1, 64, 16, [70], [1300])]
+    size = max(fa2.paged_workspace_bytes(sum(new), len(new), max(new), hq, hkv, d) for hq, hkv, d, _, new, _ in shapes)
+    work = torch.zeros(size, dtype=torch.uint8, device="cuda")
+    runs = []
+    for i, (hq, hkv, d, block, new, ctx) in enumerate(shapes):
+        pool, table, cu, q, o, lse = _run_attend(hq, hkv, d, block, new, ctx, seed=i)
+        runs.append((pool, q.cuda(), table, cu, ctx, hq, hkv, d, o, lse))
+    order = torch.randperm(3 * len(runs), generator=torch.Generator().manual_seed(0)) % len(runs)
+    for i in order.tolist():
+        pool, q, table, cu, ctx, hq, hkv, d, o, lse = runs[i]
+        again, l2 = attend(pool, q, table, cu, ctx, hq, hkv, d, work=work)
+        assert torch.equal(o, again) and torch.equal(lse, l2), i
+
+
 def test_attention_workspace_too_small_is_refused():
     from flashrt_b200 import flash_rt_fa2 as fa2
     from flashrt_b200._lib import KernelError
