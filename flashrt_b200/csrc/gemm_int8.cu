@@ -755,7 +755,7 @@ extern "C" int frt_b200_gemm_int8_nt(const void* A, const void* W, void* D, int 
                                      const float* channel_scale, const void* bias, int flags, void* stream) {
     using namespace frt;
     if (M < 0 || N < 0 || K < 1) return FRT_ERR_INVALID;
-    if (K % 16 || K >= 131072) return FRT_ERR_UNSUPPORTED;              // 2^17 products of 2^14 leave 32 bits
+    if (K % 16 || K >= 131072 || M > 1 << 30 || N > 1 << 30) return FRT_ERR_UNSUPPORTED;      // 2^17 products of 2^14 leave 32 bits
     if (M == 0 || N == 0) return FRT_OK;
     if (!A || !W || !D || !token_scale || !channel_scale) return FRT_ERR_INVALID;
     if (misaligned(A, 16) || misaligned(W, 16) || misaligned(D, 16) || misaligned(token_scale, 4) || misaligned(channel_scale, 4) ||
@@ -766,7 +766,8 @@ extern "C" int frt_b200_gemm_int8_nt(const void* A, const void* W, void* D, int 
     p.token_scale = token_scale;
     p.channel_scale = channel_scale;
     p.bias = static_cast<const __nv_bfloat16*>(bias);
-    p.status = gemm_status_device_ptr();
+    static PerDevicePointer status;
+    p.status = status.get(gemm_status_device_ptr);
     if (!p.status) return FRT_ERR_UNSUPPORTED;
     p.M = M;
     p.N = N;

@@ -292,7 +292,7 @@ static int launch_append(PagedAppendParams p, cudaStream_t stream) {
     const long long kv_blocks = (items * GROUP + APPEND_THREADS - 1) / APPEND_THREADS;
     const long long q_items = p.q ? (long long)p.tokens * ((p.hq + p.q_heads - 1) / p.q_heads) * (p.d / 16) : 0;
     const long long blocks = kv_blocks + (q_items + APPEND_THREADS - 1) / APPEND_THREADS;
-    if (blocks > 0x7fffffffLL) return FRT_ERR_UNSUPPORTED;
+    if (blocks > 0x7fffffffLL || items > 0xffffffffLL) return FRT_ERR_UNSUPPORTED;
     p.kv_items = (unsigned)items;
     p.kv_blocks = (unsigned)kv_blocks;
     cudaLaunchConfig_t cfg = {};

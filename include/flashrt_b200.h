@@ -524,7 +524,7 @@ int frt_b200_expert_loop_status(int reset);
  *     s = max(s_old if the block holds earlier tokens, max |finite y| / 448, 1e-12);  code = e4m3(clamp(y * (1 / s), +-448));
  *     codes that the block holds already, if s has grown: e4m3(c * (s_old / s)).  y: the rotated key in fp32, the value.
  *   Infinite values are clamped, NaN becomes -448 (as in frt_b200_quantize_fp8_static).  A block that is written belongs to one
- *   sequence; what a block holds behind its sequence's tokens is left as it was.  Left out, neither rotated nor stored: tokens
+ *   place of one sequence's table; what a block holds behind its sequence's tokens is left as it was.  Left out, neither rotated nor stored: tokens
  *   with a negative position (seq_lens 0: an idle slot) or one without a table row.  Keys and values whose page is no block of the
  *   pool (a negative entry), or lies outside the table, are not stored.
  *   flags bit 1: pairs are (i, i + head_dim / 2) instead of (2 i, 2 i + 1). */
@@ -562,7 +562,7 @@ int frt_b200_quantize_int8_rows(const void* in_bf16, long long in_stride, void* 
                                 int flags, void* stream);
 /* D(M,N) bf16 = (sum_k A[m][k] W[n][k]) * token_scale[m] * channel_scale[n] + bias[n] (no counterpart in the reference): A (M, K) and
  *   W (N, K) int8, K contiguous, 16-byte aligned; token_scale (M), channel_scale (N) fp32; bias (N) bf16 or NULL.  The sums are
- *   32-bit integers and exact: K % 16 == 0, K < 131072; any M, any N.  flags bit 0: the weights are settled and may be read
+ *   32-bit integers and exact: K % 16 == 0, K < 131072; any M and N up to 2^30.  flags bit 0: the weights are settled and may be read
  *   before the kernel in front has ended.  A wait that gave up shows in frt_b200_gemm_status. */
 int frt_b200_gemm_int8_nt(const void* A, const void* W, void* D, int M, int N, int K, const float* token_scale,
                           const float* channel_scale, const void* bias, int flags, void* stream);
