@@ -37,8 +37,8 @@
 
 namespace frt {
 
-// The head of a workspace: arrival counters of this kernel's CTAs, then of the other kernel's items.  At places of their own, whatever the
-// shapes: every launch leaves them at zero, and no partial is written over them.
+// The head of a workspace: arrival counters of the CTAs.  A place of their own, whatever the shapes: every launch leaves them at zero, and no
+// partial is written over them.
 constexpr int PA_MAX_GRID = 512, PA_HEAD_BYTES = 4096;
 
 struct PagedAttnParams {
@@ -994,10 +994,7 @@ extern "C" int frt_b200_paged_attention_workspace_bytes(int tokens, int batch, i
     const int group = num_heads_q / num_heads_kv, few = paged_few(head_dim);
     const long long rows = (long long)max_new * group;
     *out_bytes = paged_dispatch(head_dim, paged_nt(rows < few ? rows : few), [](auto D, auto NT) { return paged_workspace<D(), NT()>(); });
-    if (rows > few)
-        *out_bytes += prefill_dispatch(head_dim, rows, [&](auto D, auto T) {
-            return prefill_workspace<D(), T()>(tokens, batch, max_new, group, num_heads_kv);
-        });
+    if (rows > few) *out_bytes += prefill_workspace(head_dim);
     return FRT_OK;
 }
 
@@ -1074,5 +1071,5 @@ extern "C" int frt_b200_paged_attention_fp8(const void* Q, long long q_stride, v
             return r;
         });
     if (rc || !many) return rc;
-    return prefill_dispatch(head_dim, rows, [&](auto D, auto T) { return launch_prefill<D(), T()>(p, max_new, static_cast<unsigned*>(workspace) + PA_MAX_GRID, work, workspace_bytes, stream_of); });
+    return prefill_dispatch(head_dim, rows, [&](auto D, auto T) { return launch_prefill<D(), T()>(p, max_new, work, workspace_bytes, stream_of); });
 }

@@ -36,8 +36,9 @@ struct PrefillCfg {
 
 struct PrefillParams {
     PagedAttnParams a;
-    int splits;                  // along the keys; pieces joined by the CTA that arrives last at an item
-    unsigned* counters;          // one per item: at most SMs / 2 where the keys are split
+    int splits;                  // along the keys, at most: an item's pieces have two tiles or more; paged_join_kernel joins them
+    int tiles;                   // row tiles of all sequences, at most: items of one head
+    int4* items;                 // [item] first token, first row, rows, pieces
     float* part_o;               // [item][split][tile][D][128]
     float2* part_ml;             // [item][split][tile][128]
 };
@@ -56,7 +57,6 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
     __shared__ float rf_s[T * 128];
     __shared__ int warp_s[16], item_s[2];
     __shared__ uint32_t tmem_slot;
-    __shared__ unsigned last_s;
     __shared__ volatile int abort_s;
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -125,9 +125,10 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
         item_s[0] = b;
     }
     __syncthreads();
-    const int b = item_s[0];
+    const int b = item_s[0], item = (int)(blockIdx.y * gridDim.x + blockIdx.x);
     const uint32_t tmem = tmem_slot;
     if (b < 0) {                                            // fewer items than the grid's bound
+        if (pp.splits > 1 && blockIdx.z == 0 && tid == 0) pp.items[item] = make_int4(0, 0, 0, 0);
         if (warp == 12) tc::tmem_dealloc(tmem, 512);
         return;
     }
@@ -139,8 +140,13 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
     const int key_lo = p.window > 0 ? max(0, p0 - p.window + 1) : 0;
     const int key_hi = p.causal ? min(len, p1 + 1) : len;
     const int jl = key_lo / BKV, jn = max(key_hi > 0 ? (key_hi + BKV - 1) / BKV - jl : 0, 0);
-    const int split = (int)blockIdx.z;
-    const int j0 = jl + (int)((long long)jn * split / pp.splits), j1 = jl + (int)((long long)jn * (split + 1) / pp.splits);
+    const int split = (int)blockIdx.z, pieces = max(min(pp.splits, (jn + 1) / 2), 1);
+    if (pp.splits > 1 && split == 0 && tid == 0) pp.items[item] = make_int4(start, row0, rows, pieces);
+    if (split >= pieces) {
+        if (warp == 12) tc::tmem_dealloc(tmem, 512);
+        return;
+    }
+    const int j0 = jl + (int)((long long)jn * split / pieces), j1 = jl + (int)((long long)jn * (split + 1) / pieces);
     const int nt = j1 - j0;
     const int* table = p.table + (size_t)b * p.table_stride;
     const uint32_t sm = tc::smem_u32(smem);
@@ -511,7 +517,6 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
                 if (!alive) gave_up(6);
                 tc::tc_fence_after_sync();
             }
-            const int item = (int)(blockIdx.y * gridDim.x + blockIdx.x);
             const size_t part = (size_t)(item * pp.splits + split) * T + t;
             if (alive) {
                 const float inv = inverse_sum(l);
@@ -527,7 +532,7 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
                         for (int e = 0; e < 32; ++e) v[e] = 0u;
                     }
                     if (!real) continue;
-                    if (pp.splits > 1) {
+                    if (pieces > 1) {
 #pragma unroll
                         for (int e = 0; e < 32; ++e) __stcg(pp.part_o + (part * D + k + e) * 128 + row, __uint_as_float(v[e]));
                     } else {
@@ -541,50 +546,8 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
                     }
                 }
                 if (real) {
-                    if (pp.splits > 1) __stcg(pp.part_ml + part * 128 + row, make_float2(m, l));
+                    if (pieces > 1) __stcg(pp.part_ml + part * 128 + row, make_float2(m, l));
                     else if (p.lse) p.lse[(size_t)hh * p.tokens + token] = l == 0.0f ? -INFINITY : 0.6931471805599453f * (m - Cfg::OFFSET + log2f(l));
-                }
-            }
-            if (pp.splits > 1) {
-                sync_threads(128 * T);
-                if (tid == 0) {
-                    __threadfence();                            // the whole CTA's stores (its softmax warps met at the barrier)
-                    last_s = atomicInc(pp.counters + item, (unsigned)(pp.splits - 1)) == (unsigned)(pp.splits - 1);
-                    __threadfence();
-                }
-                sync_threads(128 * T);
-                if (last_s && real) {
-                    const size_t p_first = (size_t)item * pp.splits * T + t;
-                    float mm = -INFINITY, ll = 0.0f;
-                    for (int z = 0; z < pp.splits; ++z) mm = fmaxf(mm, __ldcg(pp.part_ml + (p_first + (size_t)z * T) * 128 + row).x);
-                    const float safe = mm == -INFINITY ? 0.0f : mm;
-                    for (int z = 0; z < pp.splits; ++z) {
-                        const float2 ml = __ldcg(pp.part_ml + (p_first + (size_t)z * T) * 128 + row);
-                        ll = fmaf(ml.y, ex2(ml.x - safe), ll);
-                    }
-                    const float inv = inverse_sum(ll);
-#pragma unroll 1
-                    for (int k = 0; k < D; k += 16) {
-                        float sum[16];
-#pragma unroll
-                        for (int e = 0; e < 16; ++e) sum[e] = 0.0f;
-#pragma unroll 1
-                        for (int z = 0; z < pp.splits; ++z) {
-                            const size_t at = p_first + (size_t)z * T;
-                            const float f = ex2(__ldcg(pp.part_ml + at * 128 + row).x - safe);
-                            float v[16];
-#pragma unroll
-                            for (int e = 0; e < 16; ++e) v[e] = __ldcg(pp.part_o + (at * D + k + e) * 128 + row);
-#pragma unroll
-                            for (int e = 0; e < 16; ++e) sum[e] = fmaf(v[e], f, sum[e]);
-                        }
-                        __nv_bfloat16* dst = p.o + (size_t)token * p.o_stride + (size_t)hh * D + k;
-#pragma unroll
-                        for (int e = 0; e < 16; e += 8)
-                            st_global_v4(dst + e, make_uint4(pack_bf16x2(sum[e] * inv, sum[e + 1] * inv), pack_bf16x2(sum[e + 2] * inv, sum[e + 3] * inv),
-                                                             pack_bf16x2(sum[e + 4] * inv, sum[e + 5] * inv), pack_bf16x2(sum[e + 6] * inv, sum[e + 7] * inv)));
-                    }
-                    if (p.lse) p.lse[(size_t)hh * p.tokens + token] = ll == 0.0f ? -INFINITY : 0.6931471805599453f * (mm - Cfg::OFFSET + log2f(ll));
                 }
             }
         }
@@ -600,26 +563,79 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
     if (warp == 12) tc::tmem_dealloc(tmem, 512);
 }
 
+// Joins an item's pieces: row r has o = sum_z 2^(m_z - m) o_z / sum_z 2^(m_z - m) l_z, m = max_z m_z, in the order of z.  A block takes 32
+// rows (lanes) x 32 columns (4 a warp), so that an item of 8 pieces of 128 x 256 sums, a megabyte, is read by 32 SMs.  One CTA of the kernel
+// above, the last to arrive, took 26 us for it: 64 rows on 300 keys (heads of 256) 64 -> 18 us,
+// on 16384 107 -> 35, now that an item may have more than 8 pieces.
+template <int D>
+__global__ void __launch_bounds__(256) paged_join_kernel(const PrefillParams pp, int row_tiles) {
+    const PagedAttnParams& p = pp.a;
+    pdl_launch_dependents();
+    pdl_wait();
+    const int item = (int)blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int4 it = __ldcg(pp.items + item);
+    const int row = (int)blockIdx.y * 32 + lane, col = (int)blockIdx.z * 32 + warp * 4;
+    if (it.w <= 1 || row >= it.z) return;
+    const size_t step = (size_t)row_tiles * 128, first = (size_t)item * pp.splits * step + row;      // of (m, l): [piece][tile][row]
+    const float2* ml = pp.part_ml + first;
+    const float* o = pp.part_o + (first - (row & 127)) * D + (size_t)col * 128 + (row & 127);
+    float m = -INFINITY, l = 0.0f, sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 1
+    for (int z0 = 0; z0 < it.w; z0 += 8) {                  // all loads of 8 pieces in front of their sums
+        float2 part[8];
+        float v[8][4];
+#pragma unroll
+        for (int z = 0; z < 8; ++z) {
+            const bool there = z0 + z < it.w;
+            part[z] = there ? __ldcg(ml + (z0 + z) * step) : make_float2(-INFINITY, 0.0f);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[z][e] = there ? __ldcg(o + (z0 + z) * step * D + e * 128) : 0.0f;
+        }
+        float now = m;
+#pragma unroll
+        for (int z = 0; z < 8; ++z) now = fmaxf(now, part[z].x);
+        const float safe = now == -INFINITY ? 0.0f : now, keep = ex2(m - safe);
+        m = now;
+        l *= keep;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sum[e] *= keep;
+#pragma unroll
+        for (int z = 0; z < 8; ++z) {
+            const float f = ex2(part[z].x - safe);
+            l = fmaf(part[z].y, f, l);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) sum[e] = fmaf(v[z][e], f, sum[e]);
+        }
+    }
+    const float inv = inverse_sum(l);
+    const int at = it.y + row, token = it.x + at / p.group, hh = (item / pp.tiles) * p.group + at % p.group;
+    st_global_v2(p.o + (size_t)token * p.o_stride + (size_t)hh * D + col,
+                 make_uint2(pack_bf16x2(sum[0] * inv, sum[1] * inv), pack_bf16x2(sum[2] * inv, sum[3] * inv)));
+    if (p.lse && col == 0)
+        p.lse[(size_t)hh * p.tokens + token] = l == 0.0f ? -INFINITY : 0.6931471805599453f * (m - PrefillCfg<D, 1>::OFFSET + log2f(l));
+}
+
 // Row tiles of all sequences, at most: a sequence adds less than one to its rows' share, and has no more than max_new tokens.
 static long long prefill_tiles(long long tokens, long long batch, long long max_new, int group, int tile_rows) {
     const long long by_rows = tokens * group / tile_rows + batch, by_sequence = batch * ((max_new * group + tile_rows - 1) / tile_rows);
     return by_rows < by_sequence ? by_rows : by_sequence;
 }
-// Splits of the keys where the items leave SMs idle; at most 8, since a CTA joins them.
-static int prefill_splits(long long items, int sms) {
-    const long long s = sms / (items < 1 ? 1 : items);
-    return s < 1 ? 1 : s > 8 ? 8 : (int)s;
+// Splits of the keys where the items leave SMs idle; `tiles`: of keys that a table has room for.  Beyond 64 pieces the join takes longer
+// than the tiles that it saves.
+static int prefill_splits(long long items, long long tiles, int sms) {
+    long long s = sms / (items < 1 ? 1 : items);
+    s = s < 64 ? s : 64;
+    s = s < (tiles + 1) / 2 ? s : (tiles + 1) / 2;
+    return s < 1 ? 1 : (int)s;
 }
-// Pieces of all items; their arrival counters are in the workspace's head, where no partial ever lies.
-template <int D, int T>
-static long long prefill_workspace(long long tokens, long long batch, long long max_new, int group, int hkv) {
-    const long long items = prefill_tiles(tokens, batch, max_new, group, 128 * T) * hkv;
-    const int splits = prefill_splits(items, device_sm_count());
-    return splits == 1 ? 0 : items * splits * T * 128 * (8 + 4 * D);
+// Pieces of all items where the keys are split (no more than SMs), at the larger of the row tiles: a workspace for many rows serves fewer,
+// which may be split more.
+static long long prefill_workspace(int d) {
+    return (long long)device_sm_count() * (16 + (d == 256 ? 1 : 2) * 128 * (8 + 4 * d));
 }
 
 template <int D, int T>
-static int launch_prefill(const PagedAttnParams& a, int max_new, unsigned* counters, void* work, long long work_bytes, cudaStream_t stream) {
+static int launch_prefill(const PagedAttnParams& a, int max_new, void* work, long long work_bytes, cudaStream_t stream) {
     using Cfg = PrefillCfg<D, T>;
     static PerDeviceOnce attr_once;
     int attr_dev = 0;
@@ -628,15 +644,17 @@ static int launch_prefill(const PagedAttnParams& a, int max_new, unsigned* count
         if (e != cudaSuccess) return FRT_CUDA_ERR(e);
         attr_once.set(attr_dev);
     }
-    if (work_bytes < prefill_workspace<D, T>(a.tokens, a.batch, max_new, a.group, a.hkv)) return FRT_ERR_INVALID;
+    if (work_bytes < prefill_workspace(D)) return FRT_ERR_INVALID;
     const long long tiles = prefill_tiles(a.tokens, a.batch, max_new, a.group, 128 * T), items = tiles * a.hkv;
     if (items > 0x7fffffffLL) return FRT_ERR_UNSUPPORTED;
     PrefillParams pp = {};
     pp.a = a;
-    pp.splits = prefill_splits(items, device_sm_count());
-    pp.counters = counters;
-    pp.part_ml = static_cast<float2*>(work);
-    pp.part_o = reinterpret_cast<float*>(static_cast<uint8_t*>(work) + items * pp.splits * T * 128 * 8);
+    const long long room = (long long)a.table_stride * a.block_size;
+    pp.splits = prefill_splits(items, (room + Cfg::BKV - 1) / Cfg::BKV, device_sm_count());
+    pp.tiles = (int)tiles;
+    pp.items = static_cast<int4*>(work);
+    pp.part_ml = reinterpret_cast<float2*>(pp.items + items);
+    pp.part_o = reinterpret_cast<float*>(pp.part_ml + items * pp.splits * T * 128);
     CUtensorMap tmK, tmV;
     const int box = Cfg::BKV < a.block_size ? Cfg::BKV : a.block_size;
     int rc = paged_map(&tmK, a.k, a.pool_rows, D, box, false);
@@ -652,6 +670,11 @@ static int launch_prefill(const PagedAttnParams& a, int max_new, unsigned* count
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, paged_prefill_kernel<D, T>, tmK, tmV, pp);
+    cudaError_t e = cudaLaunchKernelEx(&cfg, paged_prefill_kernel<D, T>, tmK, tmV, pp);
+    if (e != cudaSuccess || pp.splits == 1) return e == cudaSuccess ? FRT_OK : FRT_CUDA_ERR(e);
+    cfg.gridDim = dim3((unsigned)items, T * 4, D / 32);
+    cfg.blockDim = dim3(256);
+    cfg.dynamicSmemBytes = 0;
+    e = cudaLaunchKernelEx(&cfg, paged_join_kernel<D>, pp, T);
     return e == cudaSuccess ? FRT_OK : FRT_CUDA_ERR(e);
 }

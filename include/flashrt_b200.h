@@ -535,14 +535,16 @@ int frt_b200_paged_kv_append_fp8(const void* qkv, long long qkv_stride, const fl
                                  void* stream);
 /* Attention of the new tokens over that cache (no counterpart in the reference): O = softmax(cap(softmax_scale Q K^T)) V, query
  *   head hh on key/value head hh / (hq / hkv).  Q, O (tokens, hq * head_dim) bf16, rows q_stride / o_stride elements apart;
- *   lse (hq, tokens) fp32 or NULL; softmax_scale > 0.  A token sees the positions up to its own, with window > 0 the last `window` of them, with
- *   flags bit 1 (no window then) all seq_lens.  softcap > 0: scores become softcap * tanh(s / softcap).  Keys whose page is no
- *   block of the pool are absent.  A row that sees no key is zero, its lse -infinity.  Codes and scales are finite, scales
- *   positive, as the append leaves them; nothing is read behind a sequence's end or in front of its window.
+ *   lse (hq, tokens) fp32 or NULL; softmax_scale > 0.  A token sees the positions up to its own, with window > 0 the last
+ *   `window` of them, with flags bit 1 (no window then) all seq_lens.  softcap > 0: scores become softcap * tanh(s / softcap).
+ *   Keys whose page is no block of the pool are absent.  A row that sees no key is zero, its lse -infinity.  Codes and scales are
+ *   finite, scales positive, as the append leaves them; what lies behind a sequence's end or in front of its window has no
+ *   influence, whatever it holds.
  *   max_new: new tokens of the longest sequence, or more: by it the kernels are chosen, whose results agree to rounding, and their
  *   grid; rows of a sequence with more may be left out.
- *   workspace: frt_b200_paged_attention_workspace_bytes bytes for the same figures, 16-byte aligned, zeroed once; every launch
- *   leaves it ready for the next, of any shape that it is large enough for.  Launches that share one must not overlap. */
+ *   workspace: frt_b200_paged_attention_workspace_bytes bytes, 16-byte aligned, zeroed once; one for the largest tokens, batch and
+ *   max_new serves smaller ones of the same heads, and every launch leaves it ready for the next.  Launches that share one must
+ *   not overlap. */
 int frt_b200_paged_attention_fp8(const void* Q, long long q_stride, void* O, long long o_stride, float* lse,
                                  const void* k_cache, const void* v_cache, const float* k_scale, const float* v_scale,
                                  const int* block_table, int table_stride, const int* cu_seqlens, const int* seq_lens, int tokens,

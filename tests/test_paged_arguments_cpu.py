@@ -65,5 +65,7 @@ def test_workspace():
         assert rc == 0 and few > 0 and few % 16 == 0
         rc, more = size(64, 4, 16, 32, 8, d)
         assert rc == 0 and more >= few
+        at_most = size(8192, 16, 8192, 32, 8, d)[1]            # one for the largest figures serves all smaller ones
+        assert all(size(b * n, b, n, 32, 8, d)[1] <= at_most for b in (1, 4, 16) for n in (1, 2, 4, 5, 6, 30, 200, 8192 // b))
     assert size(4, 4, 1, 32, 8, 96)[0] == -2 and size(4, 4, 1, 30, 8, 128)[0] == -2 and size(-1, 4, 1, 32, 8, 128)[0] == -1
     assert _lib.call_status("frt_b200_paged_attention_workspace_bytes", 4, 4, 1, 32, 8, 128, None) == -1
