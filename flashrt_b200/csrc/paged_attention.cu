@@ -184,6 +184,12 @@ __device__ __forceinline__ void st_shared_v4(uint32_t a, uint32_t x, uint32_t y,
     asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(a), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
 }
 __device__ __forceinline__ void st_shared_zero(uint32_t a) { asm volatile("st.shared.v4.u32 [%0], {%1,%1,%1,%1};" ::"r"(a), "r"(0) : "memory"); }
+// atomicInc between the fences that a hand-over wants, without two full ones around it: 1700 clocks for 3400
+__device__ __forceinline__ unsigned arrive_inc(unsigned* a, unsigned limit) {
+    unsigned old;
+    asm volatile("atom.acq_rel.gpu.global.inc.u32 %0, [%1], %2;" : "=r"(old) : "l"(a), "r"(limit) : "memory");
+    return old;
+}
 // the warps that compute meet without those that copy
 __device__ __forceinline__ void sync_threads(int n) { asm volatile("bar.sync 1, %0;" ::"r"(n) : "memory"); }
 
@@ -315,7 +321,10 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
         if (w < warp) before += warp_s[w];
         total += warp_s[w];
     }
-    const int grid = (int)max(1LL, min((long long)gridDim.x, (total + Cfg::GROUPS - 1) / Cfg::GROUPS));   // a unit for every group
+    // A unit for every CTA, which then meets one item: 16 rows of 64 on 300 keys 13.8 us with a unit for every group, 8.1 so.  Items of more
+    // than 16 units (that many pieces' loads are in flight together at a join) keep every group busy: on 4000 keys 9.5 and 10.8.
+    const int dense = total > 16LL * p.batch * p.hkv ? Cfg::GROUPS : 1;
+    const int grid = (int)max(1LL, min((long long)gridDim.x, (total + dense - 1) / dense));
     const int cta = blockIdx.x;
     if (cta >= grid || total == 0) return;
     const PagedShare share(total, grid);
@@ -462,20 +471,23 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
         const int rows = cur.rows, row0 = cur.row0, h = cur.h;
 
         // queries -> fp16 operand fragments, at most 1 in magnitude: one warp per row
+        constexpr int PL = D / 32, RW = ROWS / NW;                           // dimensions of a lane, rows of a warp
+        uint32_t raw[RW][PL / 2];
+#pragma unroll
+        for (int k = 0; k < RW; ++k) {
+            const int at_row = row0 + min(warp + k * NW, rows - 1), hh = h * p.group + at_row % p.group;
+            const uint32_t* src = reinterpret_cast<const uint32_t*>(p.q + (size_t)(cur.start + at_row / p.group) * p.q_stride + (size_t)hh * D + lane * PL);
+#pragma unroll
+            for (int j = 0; j < PL / 2; ++j) raw[k][j] = src[j];
+        }
         sync_threads(32 * NW);                                               // the item before is through with shared memory
-        for (int r = warp; r < ROWS; r += NW) {
-            constexpr int PL = D / 32;                                       // dimensions of a lane
+#pragma unroll
+        for (int k = 0; k < RW; ++k) {
+            const int r = warp + k * NW;
             float x[PL];
             float top = 0.0f;
-            if (r < rows) {
-                const int i = (row0 + r) / p.group, hh = h * p.group + (row0 + r) % p.group;
-                const uint32_t* src = reinterpret_cast<const uint32_t*>(p.q + (size_t)(cur.start + i) * p.q_stride + (size_t)hh * D + lane * PL);
 #pragma unroll
-                for (int j = 0; j < PL / 2; ++j) unpack_bf16x2(src[j], x[2 * j], x[2 * j + 1]);
-            } else {
-#pragma unroll
-                for (int j = 0; j < PL; ++j) x[j] = 0.0f;
-            }
+            for (int j = 0; j < PL / 2; ++j) unpack_bf16x2(r < rows ? raw[k][j] : 0u, x[2 * j], x[2 * j + 1]);
 #pragma unroll
             for (int j = 0; j < PL; ++j) top = fmaxf(top, fabsf(x[j]));
             top = warp_max_butterfly(top);
@@ -828,52 +840,47 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
             const int c0 = share.owner(first), c1 = share.owner(last_unit);
             sync_threads(32 * NW);
             if (tid == 0) {
-                __threadfence();                                             // the whole CTA's stores (it met at the barrier)
-                last_s = atomicInc(p.counters + c0, (unsigned)(c1 - c0)) == (unsigned)(c1 - c0);
-                __threadfence();
+                // releases the whole CTA's stores (it met at the barrier), acquires the others'
+                last_s = arrive_inc(p.counters + c0, (unsigned)(c1 - c0)) == (unsigned)(c1 - c0);
             }
             sync_threads(32 * NW);
             if (last_s) {
                 const int slot0 = share.begin(c0) < first;                   // the first CTA had another item in front
                 const int pieces = c1 - c0 + 1;
                 const size_t part0 = (size_t)c0 * 2 + slot0;                 // the others' are at 2 (c0 + q)
-                // a warp per row: maximum, weights of the pieces (in the accumulators' space), sum
-                float* weight_s = acc_s;
-                constexpr int CAP = Cfg::ACC_BYTES / 4 / ROWS;               // pieces whose weights fit; the others' are formed again
                 auto part_of = [&](int q) { return (q ? ((size_t)c0 + q) * 2 : part0) * ROWS; };
-                for (int r = warp; r < rows; r += NW) {
-                    float mm = -INFINITY, ll = 0.0f;
-                    for (int q = lane; q < pieces; q += 32) mm = fmaxf(mm, __ldcg(p.part_ml + part_of(q) + r).x);
-                    mm = warp_max_butterfly(mm);
-                    const float safe = mm == -INFINITY ? 0.0f : mm;
-                    for (int q = lane; q < pieces; q += 32) {
-                        const float2 ml = __ldcg(p.part_ml + part_of(q) + r);
-                        const float f = ex2(ml.x - safe);
-                        if (q < CAP) weight_s[r * CAP + q] = f;
-                        ll = fmaf(ml.y, f, ll);
-                    }
-                    ll = warp_sum_butterfly(ll);
-                    if (lane == 0) ml_s[0][r] = make_float2(mm, ll);
-                }
-                sync_threads(32 * NW);
                 for (int x = tid; x < rows * (D / 4); x += 32 * NW) {
                     const int r = x / (D / 4), d4 = x % (D / 4);
-                    const float safe = ml_s[0][r].x == -INFINITY ? 0.0f : ml_s[0][r].x;
+                    float mm = -INFINITY, ll = 0.0f;
                     float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                    for (int q = 0; q < pieces; q += 8) {                    // eight loads in flight
-                        float4 v[8];
+                    constexpr int B = 16;                                    // pieces whose loads are in flight together
+#pragma unroll 1
+                    for (int q0 = 0; q0 < pieces; q0 += B) {
+                        float2 ml[B];
+                        float4 v[B];
 #pragma unroll
-                        for (int i = 0; i < 8; ++i)
-                            if (q + i < pieces) v[i] = __ldcg(reinterpret_cast<const float4*>(p.part_o + (part_of(q + i) + r) * D + d4 * 4));
+                        for (int q = 0; q < B; ++q) {
+                            const bool there = q0 + q < pieces;
+                            ml[q] = there ? __ldcg(p.part_ml + part_of(q0 + q) + r) : make_float2(-INFINITY, 0.0f);
+                            v[q] = there ? __ldcg(reinterpret_cast<const float4*>(p.part_o + (part_of(q0 + q) + r) * D + d4 * 4))
+                                         : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                        }
+                        float now = mm;
 #pragma unroll
-                        for (int i = 0; i < 8; ++i)
-                            if (q + i < pieces) {
-                                const float f = q + i < CAP ? weight_s[r * CAP + q + i] : ex2(__ldcg(p.part_ml + part_of(q + i) + r).x - safe);
-                                sum.x = fmaf(v[i].x, f, sum.x); sum.y = fmaf(v[i].y, f, sum.y);
-                                sum.z = fmaf(v[i].z, f, sum.z); sum.w = fmaf(v[i].w, f, sum.w);
-                            }
+                        for (int q = 0; q < B; ++q) now = fmaxf(now, ml[q].x);
+                        const float safe = now == -INFINITY ? 0.0f : now, keep = ex2(mm - safe);
+                        mm = now;
+                        ll *= keep;
+                        sum.x *= keep; sum.y *= keep; sum.z *= keep; sum.w *= keep;
+#pragma unroll
+                        for (int q = 0; q < B; ++q) {
+                            const float f = ex2(ml[q].x - safe);
+                            ll = fmaf(ml[q].y, f, ll);
+                            sum.x = fmaf(v[q].x, f, sum.x); sum.y = fmaf(v[q].y, f, sum.y);
+                            sum.z = fmaf(v[q].z, f, sum.z); sum.w = fmaf(v[q].w, f, sum.w);
+                        }
                     }
-                    finish(r, d4, sum, ml_s[0][r].x, ml_s[0][r].y);
+                    finish(r, d4, sum, mm, ll);
                 }
             }
         }
@@ -956,9 +963,10 @@ static int launch_paged_attention(PagedAttnParams p, void* work, cudaStream_t st
 // Row tiles of 8 NT rows, no wider than the rows need (at most paged_few of them).
 static int paged_nt(long long rows) { return rows > 16 ? 3 : rows > 8 ? 2 : 1; }
 // Query rows of a sequence up to which the kernel for few rows takes it.  16 sequences x 4 key/value heads on 4000 keys, this kernel and the
-// other: heads of 128, 16 rows 28 and 45 us, 24 rows 40 and 45, 32 rows 66 and 42; of 64, 24 rows 27 and 34, 32 rows 36 and 33; of 256,
-// 16 rows 54 and 75, 24 rows 108 and 76.
-static int paged_few(int d) { return d == 256 ? 16 : 24; }
+// other: heads of 128, 16 rows 25 and 38 us, 24 rows 32 and 38, 32 rows 66 and 42; of 64, 24 rows 23 and 31, 32 rows 36 and 33; of 256,
+// 16 rows 41 and 63, 24 rows 108 and 64.  Heads of 256 in few sequences (one: 33 and 19, four: 31 and 26): a join of two row tiles by one
+// CTA takes longer than the other kernel's launch for it.
+static int paged_few(int d, long long items) { return d < 256 ? 24 : items > 16 ? 16 : 8; }
 // f(head dim, row tiles of a CTA)
 template <typename F>
 static auto prefill_dispatch(int d, long long rows, F f) {
@@ -991,10 +999,10 @@ extern "C" int frt_b200_paged_attention_workspace_bytes(int tokens, int batch, i
     if (!out_bytes || tokens < 0 || batch < 0 || max_new < 0 || num_heads_q < 1 || num_heads_kv < 1) return FRT_ERR_INVALID;
     if (num_heads_q % num_heads_kv) return FRT_ERR_UNSUPPORTED;
     if (head_dim != 64 && head_dim != 128 && head_dim != 256) return FRT_ERR_UNSUPPORTED;
-    const int group = num_heads_q / num_heads_kv, few = paged_few(head_dim);
+    const int group = num_heads_q / num_heads_kv, few = paged_few(head_dim, LLONG_MAX);
     const long long rows = (long long)max_new * group;
     *out_bytes = paged_dispatch(head_dim, paged_nt(rows < few ? rows : few), [](auto D, auto NT) { return paged_workspace<D(), NT()>(); });
-    if (rows > few) *out_bytes += prefill_workspace(head_dim);
+    if (rows > paged_few(head_dim, 0)) *out_bytes += prefill_workspace(head_dim);        // fewer sequences may go there sooner
     return FRT_OK;
 }
 
@@ -1056,7 +1064,7 @@ extern "C" int frt_b200_paged_attention_fp8(const void* Q, long long q_stride, v
     p.status = status.get(attention_status_device_ptr);
     if (!p.status) return FRT_ERR_UNSUPPORTED;
     // Sequences of few rows and of many go to different kernels; a batch whose sequences all bring max_new tokens needs one of them.
-    const int few = paged_few(head_dim);
+    const int few = paged_few(head_dim, (long long)batch * num_heads_kv);
     const long long rows = (long long)max_new * p.group;
     const bool many = rows > few, some_few = !many || (long long)batch * max_new != tokens;
     p.few_rows = many ? few : INT_MAX;

@@ -525,6 +525,20 @@ def test_attention_strides_streams_and_captures(new):
     close(o2, lse2, R.attention(q.view(-1, hq, d), c["k"], c["v"], s["k"], s["v"], table, cu, ctx, d ** -0.5))
 
 
+@pytest.mark.parametrize("d,hq,new", [(64, 4, 1), (64, 8, 3), (128, 8, 1), (128, 8, 2), (256, 8, 1), (256, 4, 2), (256, 8, 9)])
+def test_attention_many_pieces(d, hq, new):
+    """One key/value head on a long context: an item in more pieces than a join has in flight."""
+    _run_attend(hq, 1, d, 64, [new], [9001], seed=d + new)
+
+
+@pytest.mark.parametrize("hq,hkv,new", [(8, 1, 2), (6, 3, 5), (16, 4, 4), (12, 1, 1)])
+def test_attention_heads_of_256_many_sequences_of_few_rows(hq, hkv, new):
+    """9 to 16 rows a sequence: with many sequences the kernel for few rows, with few the other one."""
+    ctx = [new + (37 * i) % 211 for i in range(21)]
+    _run_attend(hq, hkv, 256, 16, [new] * 21, ctx, seed=hq)
+    _run_attend(hq, hkv, 256, 16, [new] * 2, ctx[:2], seed=hq)
+
+
 def test_attention_one_workspace_for_all_shapes():
     """A workspace that fits the largest serves every shape in any order: no launch leaves its partials where another one counts."""
     from flashrt_b200 import flash_rt_fa2 as fa2
