@@ -356,12 +356,6 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
     int stage = 0;
     uint32_t phase = 0;
 
-    auto next_segment = [&] {                                                // a stretch that does not end the work ends its item
-        const long long at = cur.end;
-        cur.first = at;
-        ++cur.item;
-        paged_segment<UK, ROWS>(p, cur, at, w1);
-    };
     if (warp >= NW) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Cfg::REGS_COPY));
         if (warp >= NW + Cfg::COPIERS) return;
@@ -376,6 +370,12 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
         const float* my_scale = lane & 1 ? p.v_scale : p.k_scale;
         const CUtensorMap* map = lane & 1 ? &tmV : &tmK;
         const uint64_t once = tc::l2_policy_evict_first();
+        auto next_segment = [&] {                                            // a stretch that does not end the work ends its item
+            const long long at = cur.end;
+            cur.first = at;
+            ++cur.item;
+            paged_segment<UK, ROWS>(p, cur, at, w1);
+        };
         struct Unit {
             int page[PER_LANE];      // table entry; INT_MIN: no key of the item there
             int h, k0;               // key/value head, first key
@@ -466,20 +466,23 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
     const bool capped = p.cap > 0.0f;
     const float inv_cap = capped ? 1.0f / p.cap : 0.0f;
 
-    for (long long at = w0; at < w1;) {
-        if (at != w0) next_segment();
-        const int rows = cur.rows, row0 = cur.row0, h = cur.h;
-
-        // queries -> fp16 operand fragments, at most 1 in magnitude: one warp per row
-        constexpr int PL = D / 32, RW = ROWS / NW;                           // dimensions of a lane, rows of a warp
-        uint32_t raw[RW][PL / 2];
+    // a warp's query rows of a stretch, asked for while the stretch before is joined
+    constexpr int PL = D / 32, RW = ROWS / NW;                               // dimensions of a lane, rows of a warp
+    uint32_t raw[RW][PL / 2];
+    auto ask_queries = [&](const PagedSegment& s) {
 #pragma unroll
         for (int k = 0; k < RW; ++k) {
-            const int at_row = row0 + min(warp + k * NW, rows - 1), hh = h * p.group + at_row % p.group;
-            const uint32_t* src = reinterpret_cast<const uint32_t*>(p.q + (size_t)(cur.start + at_row / p.group) * p.q_stride + (size_t)hh * D + lane * PL);
+            const int at_row = s.row0 + min(warp + k * NW, s.rows - 1), hh = s.h * p.group + at_row % p.group;
+            const uint32_t* src = reinterpret_cast<const uint32_t*>(p.q + (size_t)(s.start + at_row / p.group) * p.q_stride + (size_t)hh * D + lane * PL);
 #pragma unroll
             for (int j = 0; j < PL / 2; ++j) raw[k][j] = src[j];
         }
+    };
+    ask_queries(cur);
+    for (long long at = w0; at < w1;) {
+        const int rows = cur.rows, row0 = cur.row0, h = cur.h;
+
+        // queries -> fp16 operand fragments, at most 1 in magnitude: one warp per row
         sync_threads(32 * NW);                                               // the item before is through with shared memory
 #pragma unroll
         for (int k = 0; k < RW; ++k) {
@@ -769,6 +772,13 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
                     for (int i = 0; i < MT / 2; ++i)
                         *place(w, nt, x, i) = make_float4(acc[nt][2 * i][x], acc[nt][2 * i][2 + x], acc[nt][2 * i + 1][x], acc[nt][2 * i + 1][2 + x]);
         };
+        PagedSegment after = cur;
+        if (cur.end < w1) {                                                  // a stretch that does not end the work ends its item
+            after.first = cur.end;
+            ++after.item;
+            paged_segment<UK, ROWS>(p, after, cur.end, w1);
+            ask_queries(after);
+        }
         // four warps at a time hand theirs to the four below, until four are left
         constexpr int BUFS = Cfg::BUFS;
 #pragma unroll 1
@@ -885,6 +895,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
             }
         }
         at = cur.end;
+        cur = after;
     }
     if (abort_s) {                       // a wait gave up: copies may be in flight, a bounded time for them to land
         const uint64_t until = tc::global_timer_ns() + 1000000ull;
