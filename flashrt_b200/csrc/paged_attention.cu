@@ -93,6 +93,9 @@ struct PagedCfg {
     static constexpr int RING_BYTES = STAGES * STAGE_BYTES;
     static constexpr int SMEM_BYTES = 1024 + RING_BYTES + Q_BYTES + ACC_BYTES;
     static constexpr bool Q_REGS = NT == 1;           // query fragments stay in registers
+    // The next stretch's queries are asked for in front of this one's join.  More rows have no registers for it: 16 sequences x 16 rows of
+    // 256 on 4000 keys 41 us without, 44 with.
+    static constexpr bool EARLY = NT == 1;
 };
 
 // One sequence's share of the work line.
@@ -356,6 +359,12 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
     int stage = 0;
     uint32_t phase = 0;
 
+    auto next_segment = [&](PagedSegment& s) {                               // a stretch that does not end the work ends its item
+        const long long at = s.end;
+        s.first = at;
+        ++s.item;
+        paged_segment<UK, ROWS>(p, s, at, w1);
+    };
     if (warp >= NW) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Cfg::REGS_COPY));
         if (warp >= NW + Cfg::COPIERS) return;
@@ -370,12 +379,6 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
         const float* my_scale = lane & 1 ? p.v_scale : p.k_scale;
         const CUtensorMap* map = lane & 1 ? &tmV : &tmK;
         const uint64_t once = tc::l2_policy_evict_first();
-        auto next_segment = [&] {                                            // a stretch that does not end the work ends its item
-            const long long at = cur.end;
-            cur.first = at;
-            ++cur.item;
-            paged_segment<UK, ROWS>(p, cur, at, w1);
-        };
         struct Unit {
             int page[PER_LANE];      // table entry; INT_MIN: no key of the item there
             int h, k0;               // key/value head, first key
@@ -389,7 +392,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
                 if (skip < left) break;
                 skip -= left;
                 if (cur.end >= w1) { u = cur.unit_hi; return; }
-                next_segment();
+                next_segment(cur);
                 u = cur.unit_lo;
             }
             u += skip;
@@ -478,8 +481,12 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
             for (int j = 0; j < PL / 2; ++j) raw[k][j] = src[j];
         }
     };
-    ask_queries(cur);
+    if constexpr (Cfg::EARLY) ask_queries(cur);
     for (long long at = w0; at < w1;) {
+        if constexpr (!Cfg::EARLY) {
+            if (at != w0) next_segment(cur);
+            ask_queries(cur);
+        }
         const int rows = cur.rows, row0 = cur.row0, h = cur.h;
 
         // queries -> fp16 operand fragments, at most 1 in magnitude: one warp per row
@@ -773,11 +780,11 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
                         *place(w, nt, x, i) = make_float4(acc[nt][2 * i][x], acc[nt][2 * i][2 + x], acc[nt][2 * i + 1][x], acc[nt][2 * i + 1][2 + x]);
         };
         PagedSegment after = cur;
-        if (cur.end < w1) {                                                  // a stretch that does not end the work ends its item
-            after.first = cur.end;
-            ++after.item;
-            paged_segment<UK, ROWS>(p, after, cur.end, w1);
-            ask_queries(after);
+        if constexpr (Cfg::EARLY) {
+            if (cur.end < w1) {
+                next_segment(after);
+                ask_queries(after);
+            }
         }
         // four warps at a time hand theirs to the four below, until four are left
         constexpr int BUFS = Cfg::BUFS;
@@ -895,7 +902,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
             }
         }
         at = cur.end;
-        cur = after;
+        if constexpr (Cfg::EARLY) cur = after;
     }
     if (abort_s) {                       // a wait gave up: copies may be in flight, a bounded time for them to land
         const uint64_t until = tc::global_timer_ns() + 1000000ull;
