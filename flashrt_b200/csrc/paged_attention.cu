@@ -13,7 +13,7 @@
 //
 // What bounds it: a decode step reads every key and value once and does 4 x group flops per byte, so memory does, and the kernel is
 // built to keep copies in flight.  Up to four warps copy -- a lane per block, by TMA, into a ring of stages, across the items of the CTA's
-// work, so that neither the join of an item's warps nor the set-up of the next lets the memory wait -- and two or three groups of four
+// work, so that neither the join of an item's warps nor the set-up of the next lets the memory wait -- and one or two groups of four
 // take the stages in turn, a warp KT keys.
 // Codes go from shared memory to the tensor cores as fp16: keys are the M rows of K . Q^T and dimensions the M rows of V^T . P^T
 // (mma.sync m16n8k16), so a group of up to eight query rows fills the N side and no tensor work is wasted.  Which dimension a k index
@@ -176,7 +176,7 @@ __device__ __forceinline__ float ld_shared_f(uint32_t a) {
     asm volatile("ld.shared.f32 %0, [%1];" : "=f"(r) : "r"(a) : "memory");
     return r;
 }
-// a box that nobody reads again soon: with the default policy a cache larger than L2 pushes itself through it (96.6 us for 90.4, above)
+// a box that nobody reads again soon: with the default policy a cache larger than L2 pushes itself through it (64 sequences of 1500 .. 6000 tokens 96.6 us for 90.4)
 __device__ __forceinline__ void tma_load_once(uint32_t dst, const CUtensorMap* m, uint32_t bar, int x, int y, uint64_t policy) {
     asm volatile(
         "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1, {%3, %4}], [%2], %5;"

@@ -524,9 +524,9 @@ int frt_b200_expert_loop_status(int reset);
  *     s = max(s_old if the block holds earlier tokens, max |finite y| / 448, 1e-12);  code = e4m3(clamp(y * (1 / s), +-448));
  *     codes that the block holds already, if s has grown: e4m3(c * (s_old / s)).  y: the rotated key in fp32, the value.
  *   Infinite values are clamped, NaN becomes -448 (as in frt_b200_quantize_fp8_static).  A block that is written belongs to one
- *   place of one sequence's table; what a block holds behind its sequence's tokens is left as it was.  Left out, neither rotated nor stored: tokens
- *   with a negative position (seq_lens 0: an idle slot) or one without a table row.  Keys and values whose page is no block of the
- *   pool (a negative entry), or lies outside the table, are not stored.
+ *   place of one sequence's table; what a block holds behind its sequence's tokens is left as it was.  Left out, neither rotated
+ *   nor stored: tokens with a negative position (seq_lens 0: an idle slot) or one without a table row.  Keys and values whose page
+ *   is no block of the pool (a negative entry), or lies outside the table, are not stored.
  *   flags bit 1: pairs are (i, i + head_dim / 2) instead of (2 i, 2 i + 1). */
 int frt_b200_paged_kv_append_fp8(const void* qkv, long long qkv_stride, const float* rope, int rope_rows, void* Q,
                                  void* k_cache, void* v_cache, float* k_scale, float* v_scale, const int* block_table,
