@@ -525,8 +525,8 @@ int frt_b200_expert_loop_status(int reset);
  *     codes that the block holds already, if s has grown: e4m3(c * (s_old / s)).  y: the rotated key in fp32, the value.
  *   Infinite values are clamped, NaN becomes -448 (as in frt_b200_quantize_fp8_static).  A block that is written belongs to one
  *   place of one sequence's table; what a block holds behind its sequence's tokens is left as it was.  Left out, neither rotated
- *   nor stored: tokens with a negative position (seq_lens 0: an idle slot) or one without a table row.  Keys and values whose page
- *   is no block of the pool (a negative entry), or lies outside the table, are not stored.
+ *   nor stored: tokens with a negative position (seq_lens 0: an idle slot) or with one that `rope` has no row for.  Keys and values
+ *   whose page is no block of the pool (a negative entry), or whose block lies behind the table's last entry, are not stored.
  *   flags bit 1: pairs are (i, i + head_dim / 2) instead of (2 i, 2 i + 1). */
 int frt_b200_paged_kv_append_fp8(const void* qkv, long long qkv_stride, const float* rope, int rope_rows, void* Q,
                                  void* k_cache, void* v_cache, float* k_scale, float* v_scale, const int* block_table,
@@ -537,9 +537,9 @@ int frt_b200_paged_kv_append_fp8(const void* qkv, long long qkv_stride, const fl
  *   head hh on key/value head hh / (hq / hkv).  Q, O (tokens, hq * head_dim) bf16, rows q_stride / o_stride elements apart;
  *   lse (hq, tokens) fp32 or NULL; softmax_scale > 0.  A token sees the positions up to its own, with window > 0 the last
  *   `window` of them, with flags bit 1 (no window then) all seq_lens.  softcap > 0: scores become softcap * tanh(s / softcap).
- *   Keys whose page is no block of the pool are absent.  A row that sees no key is zero, its lse -infinity.  Codes and scales are
- *   finite, scales positive, as the append leaves them; what lies behind a sequence's end or in front of its window has no
- *   influence, whatever it holds.
+ *   Keys whose page is no block of the pool, or behind the table's last entry, are absent.  A row that sees no key is zero, its
+ *   lse -infinity.  Codes and scales are finite, scales positive, as the append leaves them; what lies behind a sequence's end or
+ *   in front of its window has no influence, whatever it holds.
  *   max_new: new tokens of the longest sequence, or more: by it the kernels are chosen, whose results agree to rounding, and their
  *   grid; rows of a sequence with more may be left out.
  *   workspace: frt_b200_paged_attention_workspace_bytes bytes, 16-byte aligned, zeroed once; one for the largest tokens, batch and

@@ -539,6 +539,21 @@ def test_attention_heads_of_256_many_sequences_of_few_rows(hq, hkv, new):
     _run_attend(hq, hkv, 256, 16, [new] * 2, ctx[:2], seed=hq)
 
 
+@pytest.mark.parametrize("d,new", [(128, [1, 1, 1]), (64, [3, 1, 2]), (256, [1, 1, 1]), (128, [40, 9, 33])])
+@pytest.mark.parametrize("window,causal", [(0, True), (150, True), (20, True), (0, False)])
+def test_attention_of_sequences_longer_than_their_table(d, new, window, causal):
+    """Keys behind the table's last entry are absent; positions, masks and windows are those of the whole sequence."""
+    ctx, block, width, hq, hkv = [300, 176, 40], 16, 11, 8, 2          # room for 176 keys
+    pool = Pool(60, hkv, block, d, 3)
+    table = R.pages(ctx, block, 60, 3, width=19)
+    table[:, width:] = -1
+    cu = [0, new[0], new[0] + new[1], sum(new)]
+    q = torch.randn(cu[-1], hq * d, generator=torch.Generator().manual_seed(4)).to(BF16)
+    c, s = pool.host()
+    o, lse = attend(pool, q.cuda(), table[:, :width].contiguous(), cu, ctx, hq, hkv, d, window=window, causal=causal)
+    close(o, lse, R.attention(q.view(-1, hq, d), c["k"], c["v"], s["k"], s["v"], table, cu, ctx, d ** -0.5, window=window, causal=causal))
+
+
 def test_attention_one_workspace_for_all_shapes():
     """A workspace that fits the largest serves every shape in any order: no launch leaves its partials where another one counts."""
     from flashrt_b200 import flash_rt_fa2 as fa2
