@@ -366,13 +366,13 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
                 }
                 tc::fence_proxy_async_smem();
                 __syncwarp();
-                rf = rf_s[r] * p.scale * (p.cap > 0.0f ? 1.0f : LOG2E);
+                rf = rf_s[r] * p.scale * LOG2E;
                 tc::mbar_arrive(&q_full);
             }
             const uint32_t lane_off = (uint32_t)((warp & 3) * 32) << 16;
             const uint32_t tmem_O = tmem + Cfg::O_COL + t * D + lane_off;
             const bool capped = p.cap > 0.0f;
-            const float inv_cap = capped ? 1.0f / p.cap : 0.0f;
+            const float cap2 = p.cap * LOG2E, inv_cap2 = capped ? 1.0f / cap2 : 0.0f;       // of base-2 logits
             // keys that every row of the warp sees
             const int w_hi = (int)__reduce_min_sync(0xffffffffu, (unsigned)hi), w_lo = (int)__reduce_max_sync(0xffffffffu, (unsigned)lo);
             const bool idle = t * 128 + (warp & 3) * 32 >= rows;    // a warp behind the last row only signs
@@ -394,7 +394,7 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
                 const uint32_t par = (uint32_t)((i >> 1) & 1), tmem_S = tmem + sb * BKV + lane_off;
                 const int key0 = (j0 + i) * BKV;
                 const float4* sc = scale_s[i % Cfg::RING];
-                const bool plain = !capped && key0 >= w_lo && key0 + BKV <= w_hi;     // warp-uniform
+                const bool open = key0 >= w_lo && key0 + BKV <= w_hi, plain = !capped && open;     // warp-uniform
                 const bool ok = tc::mbar_wait_until(&s_full[sb], par, deadline, &abort_s);
                 if (!__all_sync(0xffffffffu, ok)) { gave_up(4); alive = false; break; }
                 tc::tc_fence_after_sync();
@@ -406,6 +406,8 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
                     continue;
                 }
                 if (!plain) {
+                    // Capped tiles that no mask cuts leave the comparisons out, and the cap works on base-2 logits: 16 x 5 drafted tokens under a
+                    // window and a cap 48.6 -> 42.8 us, capped chunks of 2048 on 4096 keys 506 -> 417.
                     // the base-2 logits themselves, masked, over S; factor 1 and addend 0 from here on.  In a loop of 32 columns: written out
                     // over a row of registers this was 40 KB of instructions, fetched anew for every tile
 #pragma unroll 1
@@ -420,18 +422,23 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
                             float far = 0.0f;
 #pragma unroll
                             for (int e = 0; e < 32; ++e) far = fmaxf(far, fabsf(__uint_as_float(v[e])));
-                            if (__all_sync(0xffffffffu, far <= 0.5f * p.cap)) {
+                            if (__all_sync(0xffffffffu, far <= 0.5f * cap2)) {
 #pragma unroll
-                                for (int e = 0; e < 32; ++e) v[e] = __float_as_uint(soft_cap_low(__uint_as_float(v[e]), inv_cap) * LOG2E);
+                                for (int e = 0; e < 32; ++e) v[e] = __float_as_uint(soft_cap_low(__uint_as_float(v[e]), inv_cap2));
                             } else {
 #pragma unroll
-                                for (int e = 0; e < 32; ++e) v[e] = __float_as_uint(soft_cap(__uint_as_float(v[e]), p.cap, inv_cap) * LOG2E);
+                                for (int e = 0; e < 32; ++e) v[e] = __float_as_uint(soft_cap(__uint_as_float(v[e]), cap2, inv_cap2));
                             }
                         }
-                        const int from = lo - key0 - k, to = hi - key0 - k;
+                        if (open) {
 #pragma unroll
-                        for (int e = 0; e < 32; ++e)
-                            v[e] = __float_as_uint(e >= from && e < to ? __uint_as_float(v[e]) + (e < 16 ? s0.y : s1.y) : -INFINITY);
+                            for (int e = 0; e < 32; ++e) v[e] = __float_as_uint(__uint_as_float(v[e]) + (e < 16 ? s0.y : s1.y));
+                        } else {
+                            const int from = lo - key0 - k, to = hi - key0 - k;
+#pragma unroll
+                            for (int e = 0; e < 32; ++e)
+                                v[e] = __float_as_uint(e >= from && e < to ? __uint_as_float(v[e]) + (e < 16 ? s0.y : s1.y) : -INFINITY);
+                        }
                         tc::tmem_st32(tmem_S + k, v);
                     }
                     tc::tmem_st_wait();
