@@ -8,7 +8,8 @@
 //   O += P . V     P fp16 from tensor memory, written over S
 // The block's scales stay out of the operands: a column of S has the factor softmax_scale * log2(e) * ks of its 16 keys and the addend
 // log2(vs), which replace the one factor that a softmax has anyway; the sum takes 1 / vs per 16 keys.
-// Every row tile has two S: the next scores are issued in front of this tile's P . V and stand when the softmax is through.  O is rescaled only when a row's maximum grows by more than 2^8: weights are 2^(u - m + 7) with the stale m, at most 2^15.
+// Every row tile has two S: the next scores are issued in front of this tile's P . V and stand when the softmax is through.  O is rescaled
+// only when a row's maximum grows by more than 2^8: weights are 2^(u - m + 7) with the stale m, at most 2^15.
 // Warps: 0-3 and 4-7 softmax (thread = row), 8-11 turn E4M3 bytes into swizzled fp16 operands, 12 and 14 issue a row tile's MMAs, 13 the copies.
 // Heads of 256 (an O of 256 columns) and calls of at most 128 rows have one tile.
 // Bound by: the tensor pipe (4 x 128 x 128 x 128 products a key tile and pair: some 2050 clocks) and, close to it, the exponentials
