@@ -1088,11 +1088,12 @@ extern "C" int frt_b200_paged_attention_fp8(const void* Q, long long q_stride, v
     static PerDevicePointer status;
     p.status = status.get(attention_status_device_ptr);
     if (!p.status) return FRT_ERR_UNSUPPORTED;
-    // Sequences of few rows and of many go to different kernels; a batch whose sequences all bring max_new tokens needs one of them.
+    // Sequences of few rows and of many go to different kernels.  A batch with room for max_new tokens of every sequence most likely has
+    // them: the kernel for many rows takes all of it, whatever a padded batch holds in the end.
     const int few = paged_few(head_dim, (long long)batch * num_heads_kv);
     const long long rows = (long long)max_new * p.group;
     const bool many = rows > few, some_few = !many || (long long)batch * max_new != tokens;
-    p.few_rows = many ? few : INT_MAX;
+    p.few_rows = !many ? INT_MAX : some_few ? few : 0;
     uint8_t* work = static_cast<uint8_t*>(workspace);
     int rc = FRT_OK;
     rc = paged_dispatch(head_dim, paged_nt(rows < few ? rows : few), [&](auto D, auto NT) {

@@ -539,6 +539,13 @@ def test_attention_heads_of_256_many_sequences_of_few_rows(hq, hkv, new):
     _run_attend(hq, hkv, 256, 16, [new] * 2, ctx[:2], seed=hq)
 
 
+@pytest.mark.parametrize("d,hq", [(64, 4), (128, 4), (256, 2)])
+@pytest.mark.parametrize("new,ctx", [([40, 5], [90, 70]), ([40, 0, 1], [40, 33, 300]), ([3, 40, 2], [3, 40, 150])])
+def test_attention_padded_to_the_longest(d, hq, new, ctx):
+    """Room for max_new tokens of every sequence, some of which bring few: all are answered, the rows behind them left alone."""
+    _run_attend(hq, 1, d, 16, new, ctx, seed=d, tail=len(new) * max(new) - sum(new))
+
+
 @pytest.mark.parametrize("d,new", [(128, [1, 1, 1]), (64, [3, 1, 2]), (256, [1, 1, 1]), (128, [40, 9, 33])])
 @pytest.mark.parametrize("window,causal", [(0, True), (150, True), (20, True), (0, False)])
 def test_attention_of_sequences_longer_than_their_table(d, new, window, causal):
