@@ -28,8 +28,8 @@
 // order, so results do not depend on the order of arrival.  No host knowledge of lengths: a captured graph serves every step.
 //
 // Measured (times of a replayed graph): 64 sequences of 1500 .. 6000 tokens, 32 query and 8 key heads of 128, 87 us, 5.7 TB/s; two of 48000
-// and 131071 tokens 81 us, 5.7 TB/s; one token on 819 keys, heads of 256, 10.9 us, of which the chain of dependent trips to memory is
-// nearly all: lengths 2.1, queries 0.8, keys 0.8, products 1.0, joins of warps 1.4, arrival 1.2, join of CTAs 2.3.
+// and 131071 tokens 81 us, 5.7 TB/s; one token on 819 keys, heads of 256, 10.7 us, of which the chain of dependent trips to memory is
+// nearly all: lengths 1.9, queries 0.8, keys 0.8, products 1.0, joins of warps 1.4, arrival 1.2, join of CTAs 2.3.
 #include "common.cuh"
 #include "tc05.cuh"
 #include "flashrt_b200.h"
@@ -260,7 +260,10 @@ __device__ __forceinline__ void paged_segment(const PagedAttnParams& p, PagedSeg
         s = paged_seq<UK, ROWS>(p, g.b);
     }
     g.items = s.row_tiles * p.hkv;
-    g.h = g.item / s.row_tiles;
+    // one new token: no divisions, some 100 clocks each of a chain that nothing hides (one token on 819 keys 10.9 -> 10.7 us).  With more rows
+    // a sequence the short cuts cost registers: 24 rows 80 -> 85 us
+    const bool one = ROWS == 8 && s.n == 1;
+    g.h = ROWS == 8 && s.row_tiles == 1 ? g.item : g.item / s.row_tiles;
     g.row0 = (g.item - g.h * s.row_tiles) * ROWS;
     g.rows = min(ROWS, s.n * p.group - g.row0);
     g.tiles = s.tiles;
@@ -268,7 +271,7 @@ __device__ __forceinline__ void paged_segment(const PagedAttnParams& p, PagedSeg
     g.n = s.n;
     g.start = s.start;
     g.end = min(g.first + s.tiles, w1);
-    const int p0 = s.len - s.n + g.row0 / p.group, p1 = s.len - s.n + (g.row0 + g.rows - 1) / p.group;
+    const int p0 = s.len - s.n + (one ? 0 : g.row0 / p.group), p1 = s.len - s.n + (one ? 0 : (g.row0 + g.rows - 1) / p.group);
     g.key_lo = p.window > 0 ? max(0, p0 - p.window + 1) : 0;
     g.key_hi = min(p.causal ? p1 + 1 : s.len, p.room);
     g.unit_lo = max(s.t0 + (int)(at - g.first), g.key_lo / UK);
@@ -332,8 +335,8 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
     }
     // A unit for every CTA, which then meets one item: 16 rows of 64 on 300 keys 13.8 us with a unit for every group, 8.1 so.  Items of more
     // than 16 units (that many pieces' loads are in flight together at a join) keep every group busy: on 4000 keys 9.5 and 10.8.
-    const int dense = total > 16LL * p.batch * p.hkv ? Cfg::GROUPS : 1;
-    const int grid = (int)max(1LL, min((long long)gridDim.x, (total + dense - 1) / dense));
+    const bool dense = Cfg::GROUPS == 2 && total > 16LL * p.batch * p.hkv;
+    const int grid = (int)max(1LL, min((long long)gridDim.x, dense ? (total + 1) >> 1 : total));
     const int cta = blockIdx.x;
     if (cta >= grid || total == 0) return;
     const PagedShare share(total, grid);
@@ -481,8 +484,8 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
     auto ask_queries = [&](const PagedSegment& s) {
 #pragma unroll
         for (int k = 0; k < RW; ++k) {
-            const int at_row = s.row0 + min(warp + k * NW, s.rows - 1), hh = s.h * p.group + at_row % p.group;
-            const uint32_t* src = reinterpret_cast<const uint32_t*>(p.q + (size_t)(s.start + at_row / p.group) * p.q_stride + (size_t)hh * D + lane * PL);
+            const int at_row = s.row0 + min(warp + k * NW, s.rows - 1), i = NT == 1 && s.n == 1 ? 0 : at_row / p.group, hh = s.h * p.group + at_row - i * p.group;
+            const uint32_t* src = reinterpret_cast<const uint32_t*>(p.q + (size_t)(s.start + i) * p.q_stride + (size_t)hh * D + lane * PL);
 #pragma unroll
             for (int j = 0; j < PL / 2; ++j) raw[k][j] = src[j];
         }
@@ -529,11 +532,12 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
             for (int x = 0; x < 2; ++x) {
                 const int r = nt * 8 + 2 * c + x;
                 rf[nt][x] = rf_s[r] * p.scale * (capped ? 1.0f : LOG2E);
-                const int pos = cur.len - cur.n + (row0 + min(r, rows - 1)) / p.group;
+                const int pos = cur.len - cur.n + (NT == 1 && cur.n == 1 ? 0 : (row0 + min(r, rows - 1)) / p.group);
                 row_hi[nt][x] = min(p.causal ? pos + 1 : cur.len, cur.key_hi);
                 row_lo[nt][x] = p.window > 0 ? max(0, pos - p.window + 1) : 0;
             }
-        const int p0 = cur.len - cur.n + row0 / p.group, p1 = cur.len - cur.n + (row0 + rows - 1) / p.group;
+        const bool one = NT == 1 && cur.n == 1;
+        const int p0 = cur.len - cur.n + (one ? 0 : row0 / p.group), p1 = cur.len - cur.n + (one ? 0 : (row0 + rows - 1) / p.group);
         const int all_hi = min(p.causal ? p0 + 1 : cur.len, cur.key_hi);      // keys that every row sees
         const int all_lo = p.window > 0 ? max(0, p1 - p.window + 1) : 0;
         uint2 q_r[Cfg::Q_REGS ? MT : 1];
@@ -825,7 +829,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
         const int slot = at == w0 ? 0 : 1;
         const size_t part = (size_t)cta * 2 + slot;
         auto finish = [&](int r, int d4, float4 sum, float mm, float ll) {
-            const int i = (row0 + r) / p.group, hh = h * p.group + (row0 + r) % p.group;
+            const int i = NT == 1 && cur.n == 1 ? 0 : (row0 + r) / p.group, hh = h * p.group + row0 + r - i * p.group;
             const float inv = inverse_sum(ll);
             uint2 out;
             out.x = pack_bf16x2(sum.x * inv, sum.y * inv);
