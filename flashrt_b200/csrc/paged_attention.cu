@@ -104,6 +104,12 @@ struct PagedCfg {
     static constexpr bool EARLY = NT == 1;
 };
 
+// First position that a token at `pos` sees.  A sequence with more new tokens than positions has negative ones, and a window may be any
+// positive number: compared first, so that nothing leaves 32 bits.
+__device__ __forceinline__ int window_from(const PagedAttnParams& p, int pos) {
+    return p.window > 0 && pos >= p.window ? pos - p.window + 1 : 0;
+}
+
 // One sequence's share of the work line.
 struct PagedSeq { int start, n, len, row_tiles, t0, tiles; };
 
@@ -116,8 +122,7 @@ __device__ __forceinline__ PagedSeq paged_seq(const PagedAttnParams& p, int b) {
     if ((long long)s.n * p.group > p.few_rows) s.n = 0;
     s.len = min(max(p.lens[b], 0), 0x7fffff00);
     s.row_tiles = (int)(((long long)s.n * p.group + ROWS - 1) / ROWS);
-    const int lo = p.window > 0 ? max(0, s.len - s.n - p.window + 1) : 0;
-    s.t0 = lo / UK;
+    s.t0 = window_from(p, s.len - s.n) / UK;
     s.tiles = max(1, (min(s.len, p.room) + UK - 1) / UK - s.t0);             // an item without keys still writes its rows
     return s;
 }
@@ -272,7 +277,7 @@ __device__ __forceinline__ void paged_segment(const PagedAttnParams& p, PagedSeg
     g.start = s.start;
     g.end = min(g.first + s.tiles, w1);
     const int p0 = s.len - s.n + (one ? 0 : g.row0 / p.group), p1 = s.len - s.n + (one ? 0 : (g.row0 + g.rows - 1) / p.group);
-    g.key_lo = p.window > 0 ? max(0, p0 - p.window + 1) : 0;
+    g.key_lo = window_from(p, p0);
     g.key_hi = min(p.causal ? p1 + 1 : s.len, p.room);
     g.unit_lo = max(s.t0 + (int)(at - g.first), g.key_lo / UK);
     g.unit_hi = min(s.t0 + (int)(g.end - g.first), g.key_hi > 0 ? (g.key_hi + UK - 1) / UK : 0);
@@ -534,12 +539,12 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
                 rf[nt][x] = rf_s[r] * p.scale * (capped ? 1.0f : LOG2E);
                 const int pos = cur.len - cur.n + (NT == 1 && cur.n == 1 ? 0 : (row0 + min(r, rows - 1)) / p.group);
                 row_hi[nt][x] = min(p.causal ? pos + 1 : cur.len, cur.key_hi);
-                row_lo[nt][x] = p.window > 0 ? max(0, pos - p.window + 1) : 0;
+                row_lo[nt][x] = window_from(p, pos);
             }
         const bool one = NT == 1 && cur.n == 1;
         const int p0 = cur.len - cur.n + (one ? 0 : row0 / p.group), p1 = cur.len - cur.n + (one ? 0 : (row0 + rows - 1) / p.group);
         const int all_hi = min(p.causal ? p0 + 1 : cur.len, cur.key_hi);      // keys that every row sees
-        const int all_lo = p.window > 0 ? max(0, p1 - p.window + 1) : 0;
+        const int all_lo = window_from(p, p1);
         uint2 q_r[Cfg::Q_REGS ? MT : 1];
         if constexpr (Cfg::Q_REGS) {
 #pragma unroll

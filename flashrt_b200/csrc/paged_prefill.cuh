@@ -139,7 +139,7 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
     const int rows = (int)min((long long)128 * T, (long long)n_new * p.group - row0);
     const int len = min(max(p.lens[b], 0), 0x7fffff00);
     const int p0 = len - n_new + row0 / p.group, p1 = len - n_new + (row0 + rows - 1) / p.group;
-    const int key_lo = p.window > 0 ? max(0, p0 - p.window + 1) : 0;
+    const int key_lo = window_from(p, p0);
     const int key_hi = min(p.causal ? p1 + 1 : len, p.room);
     const int jl = key_lo / BKV, jn = max(key_hi > 0 ? (key_hi + BKV - 1) / BKV - jl : 0, 0);
     const int split = (int)blockIdx.z, pieces = max(min(pp.splits, (jn + 1) / 2), 1);
@@ -329,7 +329,7 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
             const int at_row = row0 + min(r, rows - 1);             // rows behind the last go along with it
             const int i_tok = at_row / p.group, hh = h * p.group + at_row % p.group, token = start + i_tok;
             const int pos = len - n_new + i_tok;
-            const int hi = max(0, min(p.causal ? pos + 1 : len, key_hi)), lo = p.window > 0 ? max(0, pos - p.window + 1) : 0;
+            const int hi = max(0, min(p.causal ? pos + 1 : len, key_hi)), lo = window_from(p, pos);
             // the warp's 32 queries, 16 bytes a lane: fp16 at most 1 in magnitude, 16-byte chunks at chunk xor row % 8
             float rf;
             {
