@@ -58,10 +58,11 @@ __device__ __forceinline__ TokenPlace place_of(const int* cu, const int* lens, i
 }
 
 // x c + y s, the rounding error of y s given back (Kahan): half a unit in the last place or little more, where the plain fma has two and
-// more when the products nearly cancel.  Codes near the middle of two go the right way more often.
+// more when the products nearly cancel.  Codes near the middle of two go the right way more often.  An infinite y s has no error to give
+// back (infinity minus itself would make the element NaN): the plain sum stands, infinite, or NaN where x c is the other infinity.
 __device__ __forceinline__ float two_products(float x, float c, float y, float s) {
-    const float w = __fmul_rn(y, s), e = __fmaf_rn(y, s, -w);
-    return __fadd_rn(__fmaf_rn(x, c, w), e);
+    const float w = __fmul_rn(y, s), e = __fmaf_rn(y, s, -w), plain = __fmaf_rn(x, c, w), sum = __fadd_rn(plain, e);
+    return sum == sum ? sum : plain;
 }
 // 16 values of one head: 16 neighbours, or (HALVES) 8 of the first half and their partners of the second.
 template <bool HALVES>

@@ -25,3 +25,35 @@ def test_window_without_end_where_tokens_have_no_position(window, d):
     assert (o[:3] == 0).all() and lse[:, :3].isneginf().all() and lse[:, 3:].isfinite().all()
     _, _, _, _, o, lse = W._run_attend(4, 1, d, 16, [40, 70], [17, 90], seed=3, window=window)
     assert (o[:23] == 0).all() and lse[:, :23].isneginf().all() and lse[:, 23:].isfinite().all()
+
+
+@pytest.mark.parametrize("halves", [False, True])
+@pytest.mark.parametrize("d,block,tokens", [(64, 16, 9), (128, 32, 7), (64, 64, 200), (256, 64, 70)])
+def test_append_infinities_under_the_rotation(halves, d, block, tokens):
+    """Infinite elements of a key turn as the formula says: infinite where one term is or both agree (clamped), NaN where they differ
+    (-448).  The queries of the row show the same.  Angles of all four quadrants; no sine or cosine is zero."""
+    hq = hkv = 1
+    g = torch.Generator().manual_seed(tokens)
+    x = torch.randn(tokens, 3 * d, generator=g).to(BF16)
+    kind = torch.randint(0, 12, (tokens, d), generator=g)               # a sixth of all elements
+    x[:, d:2 * d] = torch.where(kind == 0, math.inf, torch.where(kind == 1, -math.inf, x[:, d:2 * d].float())).to(BF16)
+    x[:, :d] = x[:, d:2 * d]
+    angle = torch.arange(4)[torch.randint(0, 4, (tokens, d // 2), generator=g)] * (math.pi / 2) + 0.1 + 1.3 * torch.rand(tokens, d // 2, generator=g)
+    rope = torch.stack([angle.cos(), angle.sin()], -1).reshape(tokens, d).float()
+    table = R.pages([tokens], block, 8, 1)
+    pool = W.Pool(8, hkv, block, d, 1)
+    q = W.append(pool, x.cuda(), rope.cuda(), table.cuda(), _dev([0, tokens]), _dev([tokens]), hq, hkv, d, halves).cpu().double()
+    c, s = pool.host()
+    y = R.rotate(x.double().view(tokens, 3, d)[:, :2], rope, halves)
+    yq, yk = y[:, 0], y[:, 1]
+    assert yk.isnan().any() and (yk == math.inf).any() and (yk == -math.inf).any()
+    assert torch.equal(q.isnan(), yq.isnan()) and torch.equal(q == math.inf, yq == math.inf) and torch.equal(q == -math.inf, yq == -math.inf)
+    for j in range((tokens + block - 1) // block):
+        rows, page = yk[j * block:(j + 1) * block], int(table[0, j])
+        fin = rows.isfinite()
+        now = torch.where(fin, rows.abs(), 0.0).max() / 448
+        assert (s["k"][page, 0].double() - now).abs() <= now * 2.0 ** -20
+        code = R.codes(c["k"][page, 0, :len(rows)])
+        want = torch.where(rows.isnan(), -448.0, (rows / now).clamp(-448, 448))
+        bar = (want.abs() * 2.0 ** -4 * (1 + 2.0 ** -12)).clamp_min(2.0 ** -10 * (1 + 2.0 ** -12)) + 2.0 ** -12
+        assert ((code - want).abs() <= torch.where(fin, bar, 0.0)).all()
