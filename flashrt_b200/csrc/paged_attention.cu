@@ -214,8 +214,9 @@ __device__ __forceinline__ int query_exponent(float top) {
 }
 // cap * tanh(s / cap).  Through the hardware's exp2 and reciprocal: 2^-22 of the cap, where tanh.approx has 2^-11.  For |s| <= cap / 2,
 // which scores seldom leave, the first seven terms of the series (the next is below 10^-7 of the value): the exponential unit has
-// the softmax's own to do.
-__device__ __forceinline__ float soft_cap(float s, float cap, float inv_cap) {
+// the softmax's own to do.  A score takes the form of its own size: were it the tile's largest that chose, keys that a row does not see --
+// tokens after it, what a block holds behind its sequence -- would reach the row's last bits.
+__device__ __forceinline__ float soft_cap_far(float s, float cap, float inv_cap) {
     constexpr float LOG2E2 = 2.8853900817779268f;
     return cap * (1.0f - 2.0f * rcp(1.0f + ex2(s * inv_cap * LOG2E2)));
 }
@@ -227,6 +228,10 @@ __device__ __forceinline__ float soft_cap_low(float s, float inv_cap) {
     q = fmaf(q, y, 2.0f / 15.0f);
     q = fmaf(q, y, -1.0f / 3.0f);
     return fmaf(s * y, q, s);
+}
+__device__ __forceinline__ float soft_cap(float s, float cap, float inv_cap) {
+    const float far = soft_cap_far(s, cap, inv_cap), low = soft_cap_low(s, inv_cap);
+    return fabsf(s) <= 0.5f * cap ? low : far;
 }
 
 // The line cut into `grid` stretches whose lengths differ by one at most.

@@ -57,3 +57,37 @@ def test_append_infinities_under_the_rotation(halves, d, block, tokens):
         want = torch.where(rows.isnan(), -448.0, (rows / now).clamp(-448, 448))
         bar = (want.abs() * 2.0 ** -4 * (1 + 2.0 ** -12)).clamp_min(2.0 ** -10 * (1 + 2.0 ** -12)) + 2.0 ** -12
         assert ((code - want).abs() <= torch.where(fin, bar, 0.0)).all()
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("hq,hkv,new,ctx", [(8, 2, [1, 3], [70, 100]), (4, 2, [1, 1], [70, 100]), (4, 1, [60], [62])])
+def test_capped_scores_beside_hidden_keys(d, hq, hkv, new, ctx):
+    """Finite codes that a row does not see -- behind its sequence's end, or of tokens after it -- change no bit of it, under a cap
+    of which the hidden scores pass half and the seen ones stay far below."""
+    cap, block = 30.0, 16
+    pool = W.Pool(20, hkv, block, d, d)
+    pool.s["k"] *= 3.0
+    table = R.pages(ctx, block, 20, 1)
+    cu = [0] + torch.tensor(new).cumsum(0).tolist()
+    q = torch.randn(cu[-1], hq * d, generator=torch.Generator().manual_seed(2)).abs().to(BF16)
+    hidden = q.double().view(-1, hq, d).sum(-1).min() * 448 * float(pool.s["k"].min()) * d ** -0.5
+    assert hidden > cap / 2                               # where the form of tanh changes
+    run = lambda: W.attend(pool, q.cuda(), table, cu, ctx, hq, hkv, d, cap=cap)  # noqa: E731
+    last = [(int(table[b, (n - 1) // block]), n % block) for b, n in enumerate(ctx)]
+    seen = []
+    for code in (0x00, 0x7E, 0xFE):
+        for page, used in last:
+            if used:
+                pool.c["k"][page, :, used:] = code
+        seen.append(run())
+    assert all(torch.equal(seen[0][i], s[i]) for s in seen for i in (0, 1))
+    if new[-1] == 1:
+        return
+    seen = []
+    for code in (0x00, 0x7E, 0xFE):                        # the key of the last token
+        pool.c["k"][last[-1][0], :, (ctx[-1] - 1) % block] = code
+        seen.append(run())
+    assert all(torch.equal(seen[0][0][:-1], o[:-1]) and torch.equal(seen[0][1][:, :-1], lse[:, :-1]) for o, lse in seen)
+    assert not torch.equal(seen[0][0][-1], seen[1][0][-1])
+    c, s = pool.host()
+    W.close(*seen[-1], R.attention(q.view(-1, hq, d), c["k"], c["v"], s["k"], s["v"], table, cu, ctx, d ** -0.5, cap=cap))
