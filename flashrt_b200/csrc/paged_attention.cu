@@ -1053,8 +1053,8 @@ extern "C" int frt_b200_paged_attention_fp8(const void* Q, long long q_stride, v
     using namespace frt;
     auto off = [](const void* a, uintptr_t n) { return (reinterpret_cast<uintptr_t>(a) & (n - 1)) != 0; };
     if (tokens < 0 || batch < 0 || max_new < 0 || num_blocks < 0 || table_stride < 0 || num_heads_q < 1 || num_heads_kv < 1 ||
-        window < 0 || !(softcap >= 0.0f) || softcap > 1e30f || !(softmax_scale > 0.0f && softmax_scale < 1e30f))
-        return FRT_ERR_INVALID;
+        window < 0 || !(softcap == 0.0f || (softcap >= 1e-30f && softcap <= 1e30f)) || !(softmax_scale > 0.0f && softmax_scale < 1e30f))
+        return FRT_ERR_INVALID;                              // a cap's reciprocal is a number too
     if (head_dim != 64 && head_dim != 128 && head_dim != 256) return FRT_ERR_UNSUPPORTED;
     if (block_size < 16 || block_size > 128 || (block_size & (block_size - 1))) return FRT_ERR_UNSUPPORTED;
     if (num_heads_q > 1024 || num_heads_q % num_heads_kv) return FRT_ERR_UNSUPPORTED;

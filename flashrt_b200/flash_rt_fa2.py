@@ -116,7 +116,7 @@ def paged_fwd_fp8(Q, O, softmax_lse, k_cache, v_cache, k_scale, v_scale, block_t
     """Attention of packed new tokens over the cache of ``flash_rt_kernels.paged_kv_append_fp8``: one token per sequence, a few, or
     a chunk of a prompt.  ``Q``, ``O`` (tokens, hq * head_dim) bf16 (strides in elements, 0: packed), ``softmax_lse`` (hq, tokens)
     fp32 or 0; ``max_new``: new tokens of the longest sequence, or more.  ``window`` > 0: a token sees the last ``window``
-    positions up to its own; ``causal=False``: all of its sequence.  ``softcap`` > 0: softcap * tanh(score / softcap)."""
+    positions up to its own; ``causal=False``: all of its sequence.  ``softcap`` from 1e-30 to 1e30: softcap * tanh(score / softcap)."""
     width = num_heads_q * head_dim
     call("frt_b200_paged_attention_fp8", Q, q_stride or width, O, o_stride or width, softmax_lse or None, k_cache, v_cache, k_scale,
          v_scale, block_table, table_stride, cu_seqlens or None, seq_lens, tokens, batch, max_new, num_blocks, block_size,

@@ -536,7 +536,8 @@ int frt_b200_paged_kv_append_fp8(const void* qkv, long long qkv_stride, const fl
 /* Attention of the new tokens over that cache (no counterpart in the reference): O = softmax(cap(softmax_scale Q K^T)) V, query
  *   head hh on key/value head hh / (hq / hkv).  Q, O (tokens, hq * head_dim) bf16, rows q_stride / o_stride elements apart;
  *   lse (hq, tokens) fp32 or NULL; softmax_scale > 0.  A token sees the positions up to its own, with window > 0 the last
- *   `window` of them, with flags bit 1 (no window then) all seq_lens.  softcap > 0: scores become softcap * tanh(s / softcap).
+ *   `window` of them, with flags bit 1 (no window then) all seq_lens.  softcap from 1e-30 to 1e30: scores become
+ *   softcap * tanh(s / softcap); 0: they do not.
  *   Keys whose page is no block of the pool, or behind the table's last entry, are absent.  A row that sees no key is zero, its
  *   lse -infinity.  Codes and scales are finite, scales positive, as the append leaves them; what lies behind a sequence's end or
  *   in front of its window has no influence, whatever it holds.
