@@ -523,6 +523,9 @@ int frt_b200_expert_loop_status(int reset);
  *   Q (tokens, hq * head_dim) bf16 or NULL.  Per block, head and tensor, over the new tokens of this call:
  *     s = max(s_old if the block holds earlier tokens, max |finite y| / 448, 1e-12);  code = e4m3(clamp(y * (1 / s), +-448));
  *     codes that the block holds already, if s has grown: e4m3(c * (s_old / s)).  y: the rotated key in fp32, the value.
+ *   So a value is rounded when it is stored and again whenever its block's scale grows.  After g growths it is off by at most
+ *   ((1 + 2^-4)^(g+1) - 1) * (|y| + 2^-6 s), s the scale of now: 6 % for a block that is filled at once, 13 % after one growth, 20 %
+ *   after two.  A block that normal values fill token by token sees two to five, and its rms error is 3.5 to 3.9 % instead of 2.6.
  *   Infinite values are clamped, NaN becomes -448 (as in frt_b200_quantize_fp8_static).  A block that is written belongs to one
  *   place of one sequence's table; what a block holds behind its sequence's tokens is left as it was.  Left out, neither rotated
  *   nor stored: tokens with a negative position (seq_lens 0: an idle slot) or with one that `rope` has no row for.  Keys and values

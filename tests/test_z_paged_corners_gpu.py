@@ -7,6 +7,7 @@ import torch
 
 import paged_ref as R
 import test_w_paged_cache_gpu as W
+import test_y_int8_block_gpu as Y
 
 pytestmark = pytest.mark.gpu
 BF16, F32, F64 = torch.bfloat16, torch.float32, torch.float64
@@ -91,3 +92,84 @@ def test_capped_scores_beside_hidden_keys(d, hq, hkv, new, ctx):
     assert not torch.equal(seen[0][0][-1], seen[1][0][-1])
     c, s = pool.host()
     W.close(*seen[-1], R.attention(q.view(-1, hq, d), c["k"], c["v"], s["k"], s["v"], table, cu, ctx, d ** -0.5, cap=cap))
+
+
+def lost(y, s, growths):
+    """Largest error of a stored value after its block's scale has grown `growths` times, s the scale of now: each rounding is off by
+    2^-4 of what it rounds or by 2^-10 of the scale, and rounds what the one before has left, so
+    e_g <= e_{g-1} (1 + 2^-4) + 2^-4 |y| + 2^-10 s.  The fp32 operations in front of it by 2^-22: 2^-10 of a rounding is plenty."""
+    r = 2.0 ** -4 * (1 + 2.0 ** -10)
+    return ((1 + r) ** (growths + 1) - 1) * (y.abs() + 2.0 ** -6 * s)
+
+
+@pytest.mark.parametrize("block", [16, 32])
+@pytest.mark.parametrize("growth", [1.0, 1.07, 1.3])
+def test_what_a_block_loses_while_its_scale_grows(block, growth):
+    """A block filled token by token against the bound that the header gives; one filled at once is held to a single rounding."""
+    hkv, d, n = 2, 64, 2 * block + 5
+    x = (torch.randn(n, 3 * hkv * d, generator=torch.Generator().manual_seed(block)) * growth ** torch.arange(n)[:, None]).to(BF16)
+    table = R.pages([n], block, 4, 1)
+    for step in (1, 3, n):
+        pool = W.Pool(4, hkv, block, d, 2)
+        before = {m: torch.zeros(4, hkv) for m in "kv"}
+        grown, records = ({m: torch.zeros(n, hkv) for m in "kv"} for _ in range(2))
+        for a in range(0, n, step):
+            e = min(a + step, n)
+            W.append(pool, x[a:e].cuda(), None, table.cuda(), _dev([0, e - a]), _dev([e]), hkv, hkv, d)
+            c, s = pool.host()
+            for m, first in (("k", hkv), ("v", 2 * hkv)):
+                # a scale grows when a call brings the block's largest magnitude so far
+                size = x[:, first * d:(first + hkv) * d].float().abs().view(n, hkv, d).amax(2)
+                for i in range(a):
+                    lo, hi = i // block * block, min(i // block * block + block, e)
+                    if hi > a:
+                        records[m][i] += size[a:hi].amax(0) > size[lo:a].amax(0)
+                for i in range(a):
+                    grown[m][i] += s[m][table[0, i // block]] != before[m][table[0, i // block]]
+                before[m] = s[m]
+                for i in range(e):
+                    page = int(table[0, i // block])
+                    y = x[i, first * d:(first + hkv) * d].to(F64).view(hkv, d)
+                    now = s[m][page].to(F64)[:, None]
+                    assert ((R.codes(c[m][page, :, i % block]) * now - y).abs() <= lost(y, now, grown[m][i].to(F64)[:, None])).all()
+                assert torch.equal(grown[m], records[m])
+        assert (max(int(grown[m].max()) for m in "kv") > 0) == (step < n)
+
+
+@pytest.mark.parametrize("hq,hkv,d,block", [(8, 2, 128, 32), (6, 2, 64, 64)])
+def test_cache_of_the_block_holds_each_token_to_its_own_roundings(hq, hkv, d, block):
+    """The attention block from prompts to tokens: a value just written is off by one rounding, an older one by one more for each time its
+    block's scale has really grown."""
+    batch, width = 3, 256 // block
+    b = Y.Block(512, hq, hkv, d, block, 3 * width, batch, width, 128, seed=d)
+    b.table.copy_(torch.randperm(3 * width, generator=torch.Generator().manual_seed(1)).view(batch, width))
+    table, rope = b.table.cpu(), b.rope.cpu()
+    g = torch.Generator().manual_seed(2)
+    lens, tokens, before = [0] * batch, [], None
+    for new in [[60, 1, 0], [25, 50, 30], [1, 1, 1], [1, 1, 1], [3, 1, 40], [1, 1, 1], [1, 2, 0]]:
+        lens = [a + n for a, n in zip(lens, new)]
+        cu = [0] + torch.tensor(new).cumsum(0).tolist()
+        T = cu[-1]
+        b.x[:T] = torch.randn(T, 512, generator=g).to(BF16)
+        b.cu.copy_(torch.tensor(cu, dtype=torch.int32))
+        b.lens.copy_(torch.tensor(lens, dtype=torch.int32))
+        b.step(T, max(new), new != [1] * batch)
+        torch.cuda.synchronize()
+        now = {"k": b.ks.cpu(), "v": b.vs.cpu()}
+        codes = {"k": b.k.cpu(), "v": b.v.cpu()}
+        for t in tokens:
+            t["growths"] += now[t["of"]][t["page"]] != before[t["of"]][t["page"]]
+        before = now
+        qkv = b.qkv[:T].cpu().to(F64).view(T, hq + 2 * hkv, d)
+        for s in range(batch):
+            rows = qkv[cu[s]:cu[s + 1]]
+            k = R.rotate(rows[:, hq:hq + hkv], rope[lens[s] - new[s]:lens[s]], True)
+            for i in range(new[s]):
+                at = lens[s] - new[s] + i
+                for of, y in (("k", k[i]), ("v", rows[i, hq + hkv:])):
+                    tokens.append({"of": of, "y": y, "page": int(table[s, at // block]), "slot": at % block, "growths": torch.zeros(hkv)})
+        for t in tokens:
+            scale = now[t["of"]][t["page"]].to(F64)[:, None]
+            got = R.codes(codes[t["of"]][t["page"], :, t["slot"]]) * scale
+            assert ((got - t["y"]).abs() <= lost(t["y"], scale, t["growths"].to(F64)[:, None])).all()
+    assert max(int(t["growths"].max()) for t in tokens) >= 1
