@@ -1,5 +1,6 @@
 """Corners of the paged cache and of the attention over it: windows without end, infinite keys under the rotation, capped scores beside
-hidden keys, what a block loses while its scale grows, batches of single tokens and chunks."""
+hidden keys, what a block loses while its scale grows, single tokens beside chunks, calls at once and over one workspace, groups wider than
+a tile, rows that are no numbers, shared blocks."""
 import math
 
 import pytest
@@ -173,3 +174,115 @@ def test_cache_of_the_block_holds_each_token_to_its_own_roundings(hq, hkv, d, bl
             got = R.codes(codes[t["of"]][t["page"], :, t["slot"]]) * scale
             assert ((got - t["y"]).abs() <= lost(t["y"], scale, t["growths"].to(F64)[:, None])).all()
     assert max(int(t["growths"].max()) for t in tokens) >= 1
+
+
+@pytest.mark.parametrize("kw", [dict(), dict(window=700), dict(cap=20.0)])
+@pytest.mark.parametrize("d,hq,hkv", [(64, 8, 2), (128, 8, 1), (256, 4, 1)])
+def test_single_tokens_and_a_chunk_in_one_call(d, hq, hkv, kw):
+    """Decoding sequences, drafted tokens and a chunk of a prompt, each on a context of thousands; rows behind them left alone."""
+    W._run_attend(hq, hkv, d, 32, [1, 1, 33, 1, 4, 1, 0], [2900, 17, 1700, 1, 900, 3001, 40], seed=d, tail=5, **kw)
+
+
+def _call(pool, q, table, cu, ctx, hq, hkv, d, work, stream, o, lse):
+    """A call over tensors that it keeps alive."""
+    from flashrt_b200 import flash_rt_fa2 as fa2
+    new = max(b - a for a, b in zip(cu, cu[1:]))
+    q, cu_d, lens_d, table_d = q.cuda(), _dev(cu), _dev(ctx), table.cuda()
+    return lambda: fa2.paged_fwd_fp8(
+        q.data_ptr(), o.data_ptr(), lse.data_ptr(), pool.c["k"].data_ptr(), pool.c["v"].data_ptr(), pool.s["k"].data_ptr(),
+        pool.s["v"].data_ptr(), table_d.data_ptr(), table.shape[1], cu_d.data_ptr(), lens_d.data_ptr(), q.shape[0], len(ctx), new,
+        pool.num_blocks, pool.block, hq, hkv, d, d ** -0.5, work.data_ptr(), work.numel(), stream.cuda_stream)
+
+
+def _work(shapes):
+    from flashrt_b200 import flash_rt_fa2 as fa2
+    size = max(fa2.paged_workspace_bytes(sum(n), len(n), max(n), hq, hkv, d) for hq, hkv, d, n, _ in shapes)
+    return torch.zeros(size, dtype=torch.uint8, device="cuda")
+
+
+def test_two_calls_at_once():
+    """A decode batch and chunks on two streams, each with its workspace: the bits of the calls one behind the other."""
+    calls, want, got = [], [], []
+    for i, (hq, hkv, d, new, ctx) in enumerate([(8, 2, 128, [1, 1, 1, 1], [3000, 1200, 2500, 77]), (8, 2, 128, [50, 90], [1500, 2100])]):
+        pool, table, cu, q, o, lse = W._run_attend(hq, hkv, d, 32, new, ctx, seed=i)
+        want.append((o, lse))
+        got.append((torch.zeros_like(o), torch.zeros_like(lse)))
+        calls.append(_call(pool, q, table, cu, ctx, hq, hkv, d, _work([(hq, hkv, d, new, ctx)]), torch.cuda.Stream(), *got[-1]))
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for call in calls:
+            call()
+    torch.cuda.synchronize()
+    for a, b in zip(want, got):
+        assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+
+
+def test_calls_behind_one_another_in_one_graph_share_a_workspace():
+    """Layers of a model: captured calls of both kernels over one workspace, replayed."""
+    shapes = [(8, 2, 128, [1, 1, 1], [900, 1200, 77]), (8, 2, 128, [50, 9], [1500, 700]), (8, 2, 128, [1, 40, 3], [2000, 300, 1100])]
+    work, stream, calls, want, got = _work(shapes), torch.cuda.Stream(), [], [], []
+    for i, (hq, hkv, d, new, ctx) in enumerate(shapes):
+        pool, table, cu, q, o, lse = W._run_attend(hq, hkv, d, 32, new, ctx, seed=i)
+        want.append((o, lse))
+        got.append((torch.zeros_like(o), torch.zeros_like(lse)))
+        calls.append(_call(pool, q, table, cu, ctx, hq, hkv, d, work, stream, *got[-1]))
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        for _ in range(3):
+            for call in calls:
+                call()
+    for _ in range(3):
+        for o, lse in got:
+            o.fill_(-7.0)
+            lse.fill_(-7.0)
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(want, got):
+            assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+
+
+@pytest.mark.parametrize("hq,hkv,new", [(64, 1, [1, 1]), (200, 1, [1, 1, 1]), (300, 1, [2, 1, 3]), (96, 2, [5, 1, 0])])
+def test_one_key_head_for_many_query_heads(hq, hkv, new):
+    """More heads of a group than a row tile has rows: the rows of one token fill several."""
+    W._run_attend(hq, hkv, 64, 16, new, [n + 61 * i + 40 for i, n in enumerate(new)], seed=hq)
+    W._run_attend(hq // 4 * hkv, hkv, 128, 32, new, [n + 61 * i + 40 for i, n in enumerate(new)], seed=hq, window=50)
+
+
+@pytest.mark.parametrize("max_new", [1, 40])
+def test_no_sequence_brings_a_token(max_new):
+    pool = W.Pool(4, 2, 16, 128, 1)
+    q = torch.randn(5, 8 * 128, device="cuda").to(BF16)
+    o, lse = W.attend(pool, q, R.pages([20, 3], 16, 4, 1), [0, 0, 0], [20, 3], 8, 2, 128, max_new=max_new)
+    assert (o == -7).all() and (lse == -7).all()
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("new,ctx", [([1, 2], [300, 90]), ([40, 30], [300, 90])])
+def test_a_row_that_is_no_number_spoils_no_other(d, new, ctx):
+    """NaN or infinite queries of one token and head: that row shows it, every other one keeps its bits."""
+    hq, hkv = 8, 2
+    pool, table, cu, q, o, lse = W._run_attend(hq, hkv, d, 16, new, ctx, seed=d, cap=20.0)
+    token, head = cu[-1] - 1, 5
+    others = torch.ones(cu[-1], hq, dtype=torch.bool, device="cuda")
+    others[token, head] = False
+    for bad in (math.nan, math.inf):
+        q2 = q.clone().view(-1, hq, d)
+        q2[token, head, ::2] = bad
+        o2, lse2 = W.attend(pool, q2.view(-1, hq * d).cuda(), table, cu, ctx, hq, hkv, d, cap=20.0)
+        assert torch.equal(o.view(-1, hq, d)[others], o2.view(-1, hq, d)[others]) and torch.equal(lse.T[others], lse2.T[others])
+        if bad != bad:
+            assert o2.view(-1, hq, d)[token, head].isnan().all() and lse2[head, token].isnan()
+
+
+def test_sequences_share_the_blocks_of_a_prefix():
+    """Blocks that are only read may stand in several tables, and twice in one."""
+    hq, hkv, d, block = 8, 2, 128, 16
+    pool = W.Pool(9, hkv, block, d, 3)
+    table = torch.tensor([[0, 1, 2, 3, -1], [0, 1, 2, 4, 5], [0, 1, 0, 1, 6]], dtype=torch.int32)
+    for new, ctx in (([1, 1, 1], [60, 77, 70]), ([12, 29, 6], [60, 77, 70])):
+        cu = [0] + torch.tensor(new).cumsum(0).tolist()
+        q = torch.randn(cu[-1], hq * d, generator=torch.Generator().manual_seed(4)).to(BF16)
+        c, s = pool.host()
+        want = R.attention(q.view(-1, hq, d), c["k"], c["v"], s["k"], s["v"], table, cu, ctx, d ** -0.5)
+        W.close(*W.attend(pool, q.cuda(), table, cu, ctx, hq, hkv, d), want)
