@@ -1109,15 +1109,14 @@ extern "C" int frt_b200_paged_attention_fp8(const void* Q, long long q_stride, v
     const bool many = rows > few, some_few = !many || (long long)batch * max_new != tokens;
     p.few_rows = !many ? INT_MAX : some_few ? few : 0;
     uint8_t* work = static_cast<uint8_t*>(workspace);
-    int rc = FRT_OK;
-    rc = paged_dispatch(head_dim, paged_nt(rows < few ? rows : few), [&](auto D, auto NT) {
-            const long long need = paged_workspace<D(), NT()>();
-            if (workspace_bytes < need) return (int)FRT_ERR_INVALID;
-            const int r = some_few ? launch_paged_attention<D(), NT()>(p, work, stream_of) : FRT_OK;
-            work += need;
-            workspace_bytes -= need;
-            return r;
-        });
+    int rc = paged_dispatch(head_dim, paged_nt(rows < few ? rows : few), [&](auto D, auto NT) {
+        const long long need = paged_workspace<D(), NT()>();
+        // of both kernels, in front of the first launch: a call that is refused has written nothing
+        if (workspace_bytes < need + (many ? prefill_workspace(D()) : 0)) return (int)FRT_ERR_INVALID;
+        const int r = some_few ? launch_paged_attention<D(), NT()>(p, work, stream_of) : FRT_OK;
+        work += need;
+        return r;
+    });
     if (rc || !many) return rc;
-    return prefill_dispatch(head_dim, rows, [&](auto D, auto T) { return launch_prefill<D(), T()>(p, max_new, work, workspace_bytes, stream_of); });
+    return prefill_dispatch(head_dim, rows, [&](auto D, auto T) { return launch_prefill<D(), T()>(p, max_new, work, stream_of); });
 }

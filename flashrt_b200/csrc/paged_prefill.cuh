@@ -644,7 +644,7 @@ static long long prefill_workspace(int d) {
 }
 
 template <int D, int T>
-static int launch_prefill(const PagedAttnParams& a, int max_new, void* work, long long work_bytes, cudaStream_t stream) {
+static int launch_prefill(const PagedAttnParams& a, int max_new, void* work, cudaStream_t stream) {
     using Cfg = PrefillCfg<D, T>;
     static PerDeviceOnce attr_once;
     int attr_dev = 0;
@@ -653,7 +653,6 @@ static int launch_prefill(const PagedAttnParams& a, int max_new, void* work, lon
         if (e != cudaSuccess) return FRT_CUDA_ERR(e);
         attr_once.set(attr_dev);
     }
-    if (work_bytes < prefill_workspace(D)) return FRT_ERR_INVALID;
     const long long tiles = prefill_tiles(a.tokens, a.batch, max_new, a.group, 128 * T), items = tiles * a.hkv;
     if (items > 0x7fffffffLL) return FRT_ERR_UNSUPPORTED;
     PrefillParams pp = {};

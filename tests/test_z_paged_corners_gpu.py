@@ -286,3 +286,23 @@ def test_sequences_share_the_blocks_of_a_prefix():
         c, s = pool.host()
         want = R.attention(q.view(-1, hq, d), c["k"], c["v"], s["k"], s["v"], table, cu, ctx, d ** -0.5)
         W.close(*W.attend(pool, q.cuda(), table, cu, ctx, hq, hkv, d), want)
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_refused_workspace_leaves_the_outputs_alone(d):
+    """Single tokens and chunks: a workspace that is too small for one of the two kernels is refused in front of both."""
+    from flashrt_b200._lib import KernelError
+    hq, hkv, new, ctx = 8, 2, [1, 40, 2], [90, 50, 30]
+    pool = W.Pool(16, hkv, 16, d, 1)
+    q = torch.randn(43, hq * d, device="cuda").to(BF16)
+    o, lse = torch.full((43, hq * d), -7.0, dtype=BF16, device="cuda"), torch.full((hq, 43), -7.0, device="cuda")
+    work = _work([(hq, hkv, d, new, ctx)])
+    args = (pool, q, R.pages(ctx, 16, 16, 1), [0, 1, 41, 43], ctx, hq, hkv, d)
+    for size in (4096, work.numel() // 2):                 # too small for either, enough for single tokens alone
+        with pytest.raises(KernelError, match="-1"):
+            _call(*args, work[:size], torch.cuda.current_stream(), o, lse)()
+    torch.cuda.synchronize()
+    assert (o == -7).all() and (lse == -7).all()
+    _call(*args, work, torch.cuda.current_stream(), o, lse)()
+    torch.cuda.synchronize()
+    assert (o != -7).any(1).all()
