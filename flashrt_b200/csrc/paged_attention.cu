@@ -7,9 +7,9 @@
 //   u_ij = t_ij + log2(vs_p),  m_i = max_j u_ij,  w_ij = 2^(u_ij - m_i + 15)
 //   o_i = (sum_j w_ij c_j) / l_i,  l_i = sum_j w_ij / vs_p,  lse_i = ln 2 (m_i - 15 + log2 l_i)
 // The values' scale goes into the exponent, so a weight that meets the codes is at most 2^15 whatever the scales are: it is rounded to
-// fp16 (2^-12 relative down to 2^-29 of the largest; bf16 weights would give up four bits) while every sum stays in fp32.  E4M3 codes
-// are fp16 values exactly; queries are brought to at most 1 by a power of two per row, which is exact too (elements under 2^-24 of
-// the row's largest lose bits).
+// fp16 (2^-11 relative down to 2^-29 of the largest; bf16 weights, 2^-8, would give up three bits) while every sum stays in fp32.  E4M3
+// codes are fp16 values exactly; queries are brought below 1 by a power of two per row, which is exact as well as long as the eight bits
+// of an element lie above fp16's last one, 2^-24: elements under 2^-16 of the row's largest may lose bits, those under 2^-25 vanish.
 //
 // What bounds it: a decode step reads every key and value once and does 4 x group flops per byte, so memory does, and the kernel is
 // built to keep copies in flight.  Up to four warps copy -- a lane per block, by TMA, into a ring of stages, across the items of the CTA's
@@ -27,8 +27,8 @@
 // whose range ends inside an item leaves fp32 partials in the workspace; the CTA that arrives last at the item adds them in
 // order, so results do not depend on the order of arrival.  No host knowledge of lengths: a captured graph serves every step.
 //
-// Measured (times of a replayed graph): 64 sequences of 1500 .. 6000 tokens, 32 query and 8 key heads of 128, 87 us, 5.7 TB/s; two of 48000
-// and 131071 tokens 81 us, 5.7 TB/s; one token on 819 keys, heads of 256, 10.7 us, of which the chain of dependent trips to memory is
+// Measured (times of a replayed graph): 64 sequences of 1500 .. 6000 tokens, 32 query and 8 key heads of 128, 87 to 90 us, 5.6 TB/s; two of 48000
+// and 131071 tokens 81 to 82 us, 5.6 TB/s; one token on 819 keys, heads of 256, 10.7 us, of which the chain of dependent trips to memory is
 // nearly all: lengths 1.9, queries 0.8, keys 0.8, products 1.0, joins of warps 1.4, arrival 1.2, join of CTAs 2.3.
 #include "common.cuh"
 #include "tc05.cuh"

@@ -12,9 +12,12 @@
 // only when a row's maximum grows by more than 2^8: weights are 2^(u - m + 7) with the stale m, at most 2^15.
 // Warps: 0-3 and 4-7 softmax (thread = row), 8-11 turn E4M3 bytes into swizzled fp16 operands, 12 and 14 issue a row tile's MMAs, 13 the copies.
 // Heads of 256 (an O of 256 columns) and calls of at most 128 rows have one tile.
-// Bound by: the tensor pipe (4 x 128 x 128 x 128 products a key tile and pair: some 2050 clocks) and, close to it, the exponentials
-// (2 x 128 x 128 at 16 a clock: 2048).
-// Measured: two chunks of up to 2048 tokens on up to 8191 keys, 32 query and 8 key heads of 128, 466 us, 0.83 PFLOP/s.
+// Two row tiles with heads of 128 need 4 x 128 x 64 x 128 products for a tile of 64 keys, 1024 clocks of the tensor pipe, and
+// 2 x 128 x 64 exponentials at 16 a clock, 1024 as well; a tile takes some 2400.
+// Bound by: neither unit alone, each is active for 44 % of the time.  A row tile's softmax, a chain of dependent steps of one thread a row,
+// hides behind the other's products only in part; and items are whole: of 472 on 148 SMs the last SM ends after 364 key tiles where the mean is
+// 316 (longest first: 366).
+// Measured: two chunks of up to 2048 tokens on up to 8191 keys, 32 query and 8 key heads of 128, 468 us, 0.83 PFLOP/s.
 template <int D, int T>
 struct PrefillCfg {
     static_assert(T == 1 || D <= 128, "tensor memory: two tiles of S and O");
@@ -408,7 +411,8 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
                 }
                 if (!plain) {
                     // Capped tiles that no mask cuts leave the comparisons out, and the cap works on base-2 logits: 16 x 5 drafted tokens under a
-                    // window and a cap 48.6 -> 42.8 us, capped chunks of 2048 on 4096 keys 506 -> 417.
+                    // window and a cap 48.6 -> 42.8 us, capped chunks of 2048 on 4096 keys 506 -> 417 (42.9 and 420 with the form of tanh
+                    // chosen score by score where a warp's columns need both; 545 where most scores pass half of the cap).
                     // the base-2 logits themselves, masked, over S; factor 1 and addend 0 from here on.  In a loop of 32 columns: written out
                     // over a row of registers this was 40 KB of instructions, fetched anew for every tile
 #pragma unroll 1
