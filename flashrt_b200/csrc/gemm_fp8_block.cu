@@ -1,0 +1,831 @@
+// E4M3 products with a scale for each row and 128 of K of the activations and for each 128 x 128 block of the weights, and the quantiser
+// of the activations.
+//
+// Stands beside the FP8 products with one scale per tensor (GemmRunner::fp8_nt_dev of the reference, csrc/gemm/gemm_runner.cu:67-76) and
+// the int8 ones of gemm_int8.cu; no counterpart in the reference.
+//
+//   D(M,N) = sum_kb a_scale[kb][m] * w_scale[n / 128][kb] * (sum_{k in block kb} A[m,k] W[n,k]) + bias[n]
+//
+// tcgen05.mma kind::f8f6f4 sums one k-block of 128 into a buffer of tensor memory; the epilogue warps take it out, multiply by the block's
+// scales and add it to the tile's sums, which they keep in registers (fp32).  The buffers go round, so that the next block's products run
+// meanwhile: 256 x 256 x 128 on a CTA pair are 512 cycles of the tensor pipe, and the same block is 256 cycles of tcgen05.ld and 256 of fma
+// for the epilogue.
+//
+// More than 64 rows: the tokens are the rows of a tile (a thread of the epilogue owns a row, its scale is one register), on CTA pairs or
+// single CTAs; up to 64 rows: the weights are the 128 lanes and the tokens the columns, because nothing is left but streaming the weights.
+#include "common.cuh"
+#include "tc05.cuh"
+#include "flashrt_b200.h"
+
+namespace frt {
+
+int make_tmap_2d_u8(CUtensorMap* out, const void* base, uint64_t rows, uint64_t row_bytes, uint64_t pitch_bytes, uint32_t box_rows);
+
+namespace f8b {
+
+// ------------------------------------------------------------------------------------------------ quantise groups of 128
+//   t = max(max |finite x|, 448e-12),  s = t / 448,  code = e4m3(clamp(x 448 / t, +-448)); infinities are clamped, NaN becomes -448.
+// The quotient is the correctly rounded one (Markstein, IBM J. Res. Dev. 34, 1990: the product with the rounded reciprocal, its exact
+// remainder, one correction): bf16 values and the largest of them are short enough for quotients that lie exactly between two codes, one
+// in some hundred, and a product with 1 / s puts those on either side.
+// 16 lanes have a group, eight values each.
+struct Quotient {
+    float t, r;                                              // t / 1024 and its reciprocal: both normal numbers for every bf16 t
+    __device__ __forceinline__ explicit Quotient(float top) {
+        t = __fmul_rn(top, 9.765625e-4f);
+        r = __fdiv_rn(1.0f, t);
+    }
+    __device__ __forceinline__ float operator()(float x) const {
+        const float a = __fmul_rn(x, 0.4375f);               // 448 / 1024: three bits, exact
+        const float q = fminf(clamp448(__fmul_rn(a, r)), 448.0f);
+        return clamp448(__fmaf_rn(__fmaf_rn(-q, t, a), r, q));
+    }
+};
+
+template <int U>
+__global__ void __launch_bounds__(256)
+quantize_groups_kernel(const __nv_bfloat16* x, long long x_stride, uint8_t* out, float* scale, long long scale_stride, int rows, int dim,
+                       int groups, unsigned items) {
+    pdl_launch_dependents();
+    pdl_wait();
+    const int lane16 = threadIdx.x & 15;
+    const unsigned first = (blockIdx.x * 16u + (threadIdx.x >> 4)) * U;      // (row, group), group fastest
+    uint4 v[U];
+    int row[U], grp[U];
+    bool in[U];
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+        const unsigned item = first + i;
+        row[i] = (int)(item / (unsigned)groups);
+        grp[i] = (int)(item - (unsigned)row[i] * (unsigned)groups);
+        in[i] = item < items && grp[i] * 128 + lane16 * 8 < dim;
+        v[i] = in[i] ? ld_stream_v4(x + row[i] * x_stride + grp[i] * 128 + lane16 * 8) : make_uint4(0, 0, 0, 0);
+    }
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+        float f[8], top = 0.0f;
+        const uint32_t* w = &v[i].x;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) unpack_bf16x2(w[j], f[2 * j], f[2 * j + 1]);
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            if (fabsf(f[j]) < INFINITY) top = fmaxf(top, fabsf(f[j]));
+#pragma unroll
+        for (int d = 8; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+        top = fmaxf(top, 448e-12f);
+        const Quotient q(top);
+        if (in[i])
+            st_global_v2(out + (size_t)row[i] * dim + grp[i] * 128 + lane16 * 8,
+                         make_uint2(f32x4_to_e4m3x4(q(f[0]), q(f[1]), q(f[2]), q(f[3])), f32x4_to_e4m3x4(q(f[4]), q(f[5]), q(f[6]), q(f[7]))));
+        if (lane16 == 0 && first + i < items) scale[grp[i] * scale_stride + row[i]] = __fdiv_rn(top, 448.0f);
+    }
+}
+
+// ------------------------------------------------------------------------------------------------ products
+struct Params {
+    void* out;
+    const float* a_scale;        // (kb, a_stride)
+    long long a_stride;
+    const float* w_scale;        // (ceil(N / 128), kb)
+    const __nv_bfloat16* bias;
+    int* status;
+    int M, N, kb;                // kb: k-blocks of 128
+    int early;                   // the weights may be read before the kernel in front has ended
+    int gm;                      // tile kernel: m-tiles of a group
+    int f32;                     // out is fp32
+};
+enum { ERR_PRODUCER = 1, ERR_MMA = 2, ERR_EPILOGUE = 3 };
+
+template <int CG>
+__device__ __forceinline__ void mma(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+    if constexpr (CG == 1) {
+        tc::mma_f8(tmem_d, adesc, bdesc, idesc, accumulate);
+    } else {
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "setp.ne.b32 p, %4, 0;\n\t"
+            "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}"
+            ::"r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+            : "memory");
+    }
+}
+template <int CG>
+__device__ __forceinline__ void tmem_take(uint32_t* slot, uint32_t ncols) {
+    if constexpr (CG == 1) {
+        tc::tmem_alloc(slot, ncols);
+        tc::tmem_relinquish();
+    } else {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tc::smem_u32(slot)), "r"(ncols) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    }
+}
+template <int CG>
+__device__ __forceinline__ void tmem_give(uint32_t taddr, uint32_t ncols) {
+    if constexpr (CG == 1) tc::tmem_dealloc(taddr, ncols);
+    else asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(ncols) : "memory");
+}
+template <int CG>
+__device__ __forceinline__ void load(uint32_t dst, const CUtensorMap* m, uint32_t bar, int x, int y) {
+    if constexpr (CG == 1) {
+        tc::tma_load_2d(dst, m, bar, x, y);
+    } else {
+        asm volatile(
+            "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
+            ::"r"(dst), "l"(m), "r"(bar), "r"(x), "r"(y)
+            : "memory");
+    }
+}
+template <int CG>
+__device__ __forceinline__ void commit(uint32_t bar, uint32_t leader) {
+    if constexpr (CG == 1)
+        tc::mma_commit(bar);
+    else
+        asm volatile(
+            "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
+            "h"((uint16_t)(3u << leader))
+            : "memory");
+}
+__device__ __forceinline__ void gave_up(int* status, volatile int* abort_flag, int code) {
+    if (!*abort_flag) atomicCAS(status, 0, code | (blockIdx.x << 8));
+    *abort_flag = 1;
+}
+// A CTA that gave up may have copies in flight: a bounded time for them before its shared memory goes to another.
+__device__ __forceinline__ void let_copies_land() {
+    const uint64_t until = tc::global_timer_ns() + 1000000ull;
+    while (tc::global_timer_ns() < until) {}
+}
+__device__ __forceinline__ void sts_v4(uint32_t a, float x, float y, float z, float w) {
+    asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(a), "f"(x), "f"(y), "f"(z), "f"(w) : "memory");
+}
+__device__ __forceinline__ float4 lds_v4(uint32_t a) {
+    float4 v;
+    asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(a) : "memory");
+    return v;
+}
+__device__ __forceinline__ void store_one(const Params& p, size_t at, float v) {
+    if (p.f32) static_cast<float*>(p.out)[at] = v;
+    else static_cast<__nv_bfloat16*>(p.out)[at] = __float2bfloat16_rn(v);
+}
+
+// ---------------------------------------------------------------- up to 64 rows: weights on the lanes, tokens on the columns
+template <int BN>
+struct LaneCfg {
+    static constexpr int A_BYTES = 128 * 128, B_BYTES = BN * 128, STAGE_BYTES = A_BYTES + B_BYTES;
+    static constexpr int STAGES = BN <= 32 ? 5 : 4;                          // about 100 KB: two CTAs per SM
+    static constexpr int BUFS = BN == 64 ? 4 : 8;                            // accumulators: k-blocks under way
+    static constexpr int RED_BYTES = 128 * BN * 4;                           // a rank's partial, where the ring was
+    static_assert(RED_BYTES <= STAGES * STAGE_BYTES, "partials in the ring");
+    static constexpr int SCALE_BYTES = 4 * 2 * BN * 4;                       // of each epilogue warp, two k-blocks
+    static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + 1024 + 256 + SCALE_BYTES;
+    static constexpr int TMEM_COLS = BUFS * BN;
+};
+
+// S = 1: grid of as many CTAs as there is room for, each walks over n tiles.  S > 1: grid (n tiles, S), cluster (1, S), rank r takes the
+// k-blocks [kb r / S, kb (r + 1) / S); the ranks then lay their partials into shared memory and each finishes every S-th four tokens.
+template <int BN>
+__global__ void __launch_bounds__(192, 2)
+gemm_fp8_block_lane_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmW, Params p) {
+    using Cfg = LaneCfg<BN>;
+    constexpr int STAGES = Cfg::STAGES, BUFS = Cfg::BUFS;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+    uint64_t* full = reinterpret_cast<uint64_t*>(smem + STAGES * Cfg::STAGE_BYTES);
+    uint64_t* empty = full + STAGES;
+    uint64_t* acc_full = empty + STAGES;       // [BUFS]
+    uint64_t* acc_empty = acc_full + BUFS;     // [BUFS]
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + BUFS);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+    static_assert((2 * STAGES + 2 * BUFS) * 8 + 8 <= 256, "barriers");
+    uint8_t* scales = smem + STAGES * Cfg::STAGE_BYTES + 256;
+    const uint64_t deadline = tc::global_timer_ns() + FRT_KERNEL_DEADLINE_NS;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int S = (int)gridDim.y, rank = (int)blockIdx.y, tiles = (p.N + 127) / 128;
+    const int kb0 = (int)((long long)p.kb * rank / S), kb1 = (int)((long long)p.kb * (rank + 1) / S);
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < STAGES; ++s) {
+            tc::mbar_init(&full[s], 1);
+            tc::mbar_init(&empty[s], 1);
+        }
+        for (int i = 0; i < BUFS; ++i) {
+            tc::mbar_init(&acc_full[i], 1);
+            tc::mbar_init(&acc_empty[i], 4);
+        }
+        *abort_flag = 0;
+        tc::mbar_fence_init();
+        tc::tma_prefetch_desc(&tmA);
+        tc::tma_prefetch_desc(&tmW);
+    }
+    if (warp == 1) tmem_take<1>(tmem_slot, Cfg::TMEM_COLS);
+    tc::tc_fence_before_sync();
+    __syncthreads();
+    tc::tc_fence_after_sync();
+    const uint32_t tmem = *tmem_slot;
+    pdl_launch_dependents();
+
+    if (warp == 0) {
+        // ---------------- producer (whole warp); settled weights: the first ring of them before the wait
+        const uint32_t ring = tc::smem_u32(smem), full_a = tc::smem_u32(full), empty_a = tc::smem_u32(empty);
+        const int ahead = p.early && (int)blockIdx.x < tiles ? min(STAGES, kb1 - kb0) : 0;
+        if (tc::elect_one())
+            for (int s = 0; s < ahead; ++s) {
+                tc::mbar_arrive_expect_tx(full_a + 8 * s, Cfg::STAGE_BYTES);
+                tc::tma_load_2d(ring + s * Cfg::STAGE_BYTES, &tmW, full_a + 8 * s, (kb0 + s) * 128, (int)blockIdx.x * 128);
+            }
+        __syncwarp();
+        pdl_wait();
+        if (tc::elect_one())
+            for (int s = 0; s < ahead; ++s)
+                tc::tma_load_2d(ring + s * Cfg::STAGE_BYTES + Cfg::A_BYTES, &tmA, full_a + 8 * s, (kb0 + s) * 128, 0);
+        __syncwarp();
+        int s = ahead % STAGES, skip = ahead;
+        uint32_t ph = ahead < STAGES;
+        for (int t = (int)blockIdx.x; t < tiles; t += (int)gridDim.x) {
+            for (int kb = kb0 + skip; kb < kb1; ++kb) {
+                if (!tc::warp_wait(empty_a + 8 * s, ph, false, deadline, abort_flag)) {
+                    if (lane == 0) gave_up(p.status, abort_flag, ERR_PRODUCER);
+                    t = tiles;
+                    break;
+                }
+                if (tc::elect_one()) {
+                    const uint32_t dst = ring + s * Cfg::STAGE_BYTES, bar = full_a + 8 * s;
+                    tc::mbar_arrive_expect_tx(bar, Cfg::STAGE_BYTES);
+                    tc::tma_load_2d(dst, &tmW, bar, kb * 128, t * 128);
+                    tc::tma_load_2d(dst + Cfg::A_BYTES, &tmA, bar, kb * 128, 0);
+                }
+                __syncwarp();
+                if (++s == STAGES) { s = 0; ph ^= 1; }
+            }
+            skip = 0;
+        }
+    } else if (warp == 1) {
+        // ---------------- MMA issuer (whole warp): a k-block, a buffer
+        constexpr uint32_t idesc = tc::make_idesc(0, 0, 0, 0, 128, BN);
+        const uint32_t full_a = tc::smem_u32(full), empty_a = tc::smem_u32(empty);
+        const uint32_t accF_a = tc::smem_u32(acc_full), accE_a = tc::smem_u32(acc_empty);
+        const uint64_t dA0 = tc::make_desc_kmajor_sw128(tc::smem_u32(smem));
+        const uint64_t dB0 = tc::make_desc_kmajor_sw128(tc::smem_u32(smem + Cfg::A_BYTES));
+        int s = 0, buf = 0;
+        uint32_t ph = 0, bph = 1;                              // the first round of the buffers is empty
+        for (int t = (int)blockIdx.x; t < tiles; t += (int)gridDim.x)
+            for (int kb = kb0; kb < kb1; ++kb) {
+                if (!tc::warp_wait(accE_a + 8 * buf, bph, false, deadline, abort_flag) ||
+                    !tc::warp_wait(full_a + 8 * s, ph, false, deadline, abort_flag)) {
+                    if (lane == 0) gave_up(p.status, abort_flag, ERR_MMA);
+                    t = tiles;
+                    break;
+                }
+                tc::tc_fence_after_sync();
+                if (tc::elect_one()) {
+                    const uint64_t so = (uint64_t)(s * (Cfg::STAGE_BYTES >> 4));
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) tc::mma_f8(tmem + buf * BN, dA0 + so + 2 * k, dB0 + so + 2 * k, idesc, k > 0 ? 1u : 0u);
+                    tc::mma_commit(empty_a + 8 * s);
+                    tc::mma_commit(accF_a + 8 * buf);
+                }
+                __syncwarp();
+                if (++s == STAGES) { s = 0; ph ^= 1; }
+                if (++buf == BUFS) { buf = 0; bph ^= 1; }
+            }
+    } else {
+        // ---------------- epilogue: warps 2..5, lane quadrant = warp % 4; a thread's lane is one output channel
+        pdl_wait();
+        const int q = warp & 3;
+        const uint32_t t_src = tmem + ((uint32_t)(q * 32) << 16);
+        const uint32_t sc = tc::smem_u32(scales) + (warp - 2) * (2 * BN * 4);
+        constexpr int PER = (BN + 31) / 32;                    // scales of a lane
+        int buf = 0;
+        uint32_t bph = 0;
+        bool ok = true;
+        for (int t = (int)blockIdx.x; t < tiles && ok; t += (int)gridDim.x) {
+            const int n = t * 128 + q * 32 + lane;
+            const bool in = n < p.N;
+            float acc[BN];
+#pragma unroll
+            for (int j = 0; j < BN; ++j) acc[j] = 0.0f;
+            // scales of a k-block are asked for two blocks ahead and lie in the warp's own shared memory, token by token
+            auto ask = [&](int kb, float (&r)[PER]) {
+                const float w = kb < kb1 ? p.w_scale[(size_t)t * p.kb + kb] : 0.0f;
+#pragma unroll
+                for (int i = 0; i < PER; ++i) {
+                    const int m = lane + 32 * i;
+                    r[i] = kb < kb1 && m < p.M ? __fmul_rn(p.a_scale[kb * p.a_stride + m], w) : 0.0f;
+                }
+            };
+            float next[PER], later[PER];
+            ask(kb0, next);
+            ask(kb0 + 1, later);
+            for (int kb = kb0; kb < kb1; ++kb) {
+                const uint32_t slot = sc + (kb & 1) * (BN * 4);
+#pragma unroll
+                for (int i = 0; i < PER; ++i)
+                    if (BN >= 32 || lane < BN)
+                        asm volatile("st.shared.f32 [%0], %1;" ::"r"(slot + (lane + 32 * i) * 4), "f"(next[i]) : "memory");
+#pragma unroll
+                for (int i = 0; i < PER; ++i) next[i] = later[i];
+                ask(kb + 2, later);
+                ok = tc::warp_wait(tc::smem_u32(&acc_full[buf]), bph, false, deadline, abort_flag);
+                if (!ok) {
+                    if (lane == 0) gave_up(p.status, abort_flag, ERR_EPILOGUE);
+                    break;
+                }
+                tc::tc_fence_after_sync();
+#pragma unroll
+                for (int c = 0; c < BN; c += 16) {
+                    if (c >= p.M) break;
+                    uint32_t v[16];
+                    __syncwarp();
+                    tc::tmem_ld16(t_src + buf * BN + c, v);
+                    tc::tmem_ld_wait();
+#pragma unroll
+                    for (int j = 0; j < 16; j += 4) {
+                        const float4 f = lds_v4(slot + (c + j) * 4);
+                        acc[c + j] = __fmaf_rn(__uint_as_float(v[j]), f.x, acc[c + j]);
+                        acc[c + j + 1] = __fmaf_rn(__uint_as_float(v[j + 1]), f.y, acc[c + j + 1]);
+                        acc[c + j + 2] = __fmaf_rn(__uint_as_float(v[j + 2]), f.z, acc[c + j + 2]);
+                        acc[c + j + 3] = __fmaf_rn(__uint_as_float(v[j + 3]), f.w, acc[c + j + 3]);
+                    }
+                }
+                tc::tc_fence_before_sync();
+                __syncwarp();
+                if (lane == 0) tc::mbar_arrive(&acc_empty[buf]);
+                if (++buf == BUFS) { buf = 0; bph ^= 1; }
+            }
+            if (!ok) break;
+            if (S > 1) {                                       // [four tokens][channel]: a warp's store is 512 contiguous bytes
+                const uint32_t red = tc::smem_u32(smem) + (uint32_t)(q * 32 + lane) * 16;
+#pragma unroll
+                for (int j = 0; j < BN; j += 4)
+                    if (j < p.M) sts_v4(red + j * 512, acc[j], acc[j + 1], acc[j + 2], acc[j + 3]);
+            } else if (in) {
+                const float bias = p.bias ? __bfloat162float(p.bias[n]) : 0.0f;
+#pragma unroll
+                for (int j = 0; j < BN; ++j)
+                    if (j < p.M) store_one(p, (size_t)j * p.N + n, p.bias ? __fadd_rn(acc[j], bias) : acc[j]);
+            }
+        }
+    }
+    if (S > 1) {
+        __syncwarp();
+        tc::cluster_sync_all();                              // all partials are there
+        if (warp >= 2 && !*abort_flag) {
+            const int q = warp & 3, n = (int)blockIdx.x * 128 + q * 32 + lane;
+            const bool in = n < p.N;
+            const float bias = in && p.bias ? __bfloat162float(p.bias[n]) : 0.0f;
+            const uint32_t red = tc::smem_u32(smem) + (uint32_t)(q * 32 + lane) * 16;
+            for (int g = rank; 4 * g < p.M; g += S) {        // four tokens; the ranks' partials are all on their way before the first is added
+                float4 w[8];
+#pragma unroll
+                for (int r = 0; r < 8; ++r)
+                    if (r < S) w[r] = tc::dsmem_ld_f32x4(tc::dsmem_map(red + (uint32_t)g * 2048, (uint32_t)r));
+                float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int r = 0; r < 8; ++r)
+                    if (r < S) {                             // in the order of K
+                        sum[0] = __fadd_rn(sum[0], w[r].x);
+                        sum[1] = __fadd_rn(sum[1], w[r].y);
+                        sum[2] = __fadd_rn(sum[2], w[r].z);
+                        sum[3] = __fadd_rn(sum[3], w[r].w);
+                    }
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int m = 4 * g + e;
+                    if (in && m < p.M) store_one(p, (size_t)m * p.N + n, p.bias ? __fadd_rn(sum[e], bias) : sum[e]);
+                }
+            }
+        }
+        __syncwarp();
+        tc::cluster_sync_all();                              // nobody leaves while its partial is read
+    }
+    if (*abort_flag && threadIdx.x == 0) let_copies_land();
+    tc::tc_fence_before_sync();
+    __syncthreads();
+    tc::tc_fence_after_sync();
+    if (warp == 1) tmem_give<1>(tmem, Cfg::TMEM_COLS);
+}
+
+// ---------------------------------------------------------------- more rows: tokens on the rows, tiles of 128 CG x BN
+template <int CG, int BN>
+struct TileCfg {
+    static constexpr int A_BYTES = 128 * 128, B_BYTES = BN / CG * 128, STAGE_BYTES = A_BYTES + B_BYTES;  // per CTA
+    static constexpr int EPI_BYTES = 8 * 32 * 128;           // 32 rows x 32 fp32 columns of each epilogue warp
+    static constexpr int STAGES = (227 * 1024 - 1024 - 256 - EPI_BYTES) / STAGE_BYTES > 8 ? 8 : (227 * 1024 - 1024 - 256 - EPI_BYTES) / STAGE_BYTES;
+    static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + 1024 + 256 + EPI_BYTES;
+    static constexpr int BUFS = 512 / BN;                    // accumulators: k-blocks under way
+};
+
+// Tiles in groups of gm m-tiles, m fastest inside a group: the CTAs of a wave then share operand rows in L2.
+__device__ __forceinline__ void tile_at(int t, int gm, int m_tiles, int n_tiles, int& m, int& n) {
+    const int per = gm * n_tiles, g = t / per, r = t - g * per, h = min(m_tiles - g * gm, gm);
+    n = r / h;
+    m = g * gm + (r - n * h);
+}
+
+// 32 rows x 32 columns of a tile, a thread holds a row: through shared memory (16-byte chunks of a 128-byte row, chunk index xor row % 8) to
+// threads that own four columns of four rows at a time, so that a store covers whole sectors of a row.
+__device__ __forceinline__ void store_block(const Params& p, const float* f, int m_base, int nb, uint8_t* stg, bool vec) {
+    const int lane = threadIdx.x & 31, ch = lane & 7, r0 = lane >> 3, n = nb + ch * 4;
+    const uint32_t base = tc::smem_u32(stg), sw = (uint32_t)(lane & 7) << 4;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) sts_v4(base + lane * 128 + (((uint32_t)k << 4) ^ sw), f[4 * k], f[4 * k + 1], f[4 * k + 2], f[4 * k + 3]);
+    if (!vec) {
+        // rows that start anywhere: a lane takes a column, a store two to three sectors of one row
+        const int col = nb + lane;
+        const float bias = p.bias && col < p.N ? __bfloat162float(p.bias[col]) : 0.0f;
+        __syncwarp();
+        const int rows = min(32, p.M - m_base);
+#pragma unroll 8
+        for (int r = 0; r < 32; ++r) {
+            float v;
+            asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(base + r * 128 + ((uint32_t)((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4) : "memory");
+            if (p.bias) v = __fadd_rn(v, bias);
+            if (r < rows && col < p.N) store_one(p, (size_t)(m_base + r) * p.N + col, v);
+        }
+        __syncwarp();
+        return;
+    }
+    float bias[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (p.bias && n < p.N)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) bias[e] = __bfloat162float(p.bias[n + e]);
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const int r = 4 * i + r0, m = m_base + r;
+        float4 v = lds_v4(base + r * 128 + ((uint32_t)(ch ^ (r & 7)) << 4));
+        if (p.bias) {
+            v.x = __fadd_rn(v.x, bias[0]);
+            v.y = __fadd_rn(v.y, bias[1]);
+            v.z = __fadd_rn(v.z, bias[2]);
+            v.w = __fadd_rn(v.w, bias[3]);
+        }
+        if (m < p.M && n < p.N) {                            // N % 4 == 0: all four
+            const size_t at = (size_t)m * p.N + n;
+            if (p.f32) *reinterpret_cast<float4*>(static_cast<float*>(p.out) + at) = v;
+            else st_global_v2(static_cast<__nv_bfloat16*>(p.out) + at, make_uint2(pack_bf16x2(v.x, v.y), pack_bf16x2(v.z, v.w)));
+        }
+    }
+    __syncwarp();
+}
+
+// CG = 2: a CTA pair has a tile of 256 rows, each CTA stages its 128 rows of A and half of the weight rows.  S > 1: a cluster of S such
+// takes one tile, unit s the k-blocks [kb s / S, kb (s + 1) / S); they then lay their partials into shared memory, where their rings were,
+// and each finishes BN / S of the columns.
+template <int CG, int BN, int S>
+__global__ void __launch_bounds__(320, 1)
+gemm_fp8_block_tile_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmW, Params p) {
+    using Cfg = TileCfg<CG, BN>;
+    constexpr int STAGES = Cfg::STAGES, BUFS = Cfg::BUFS, W2 = BN / 2;
+    static_assert(S == 1 || (BN / S >= 64 && 128 * BN * 4 <= STAGES * Cfg::STAGE_BYTES), "columns of a half of the warps, partials in the ring");
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+    uint64_t* full = reinterpret_cast<uint64_t*>(smem + STAGES * Cfg::STAGE_BYTES);   // the leader's count both CTAs' bytes
+    uint64_t* empty = full + STAGES;
+    uint64_t* acc_full = empty + STAGES;       // [BUFS]
+    uint64_t* acc_empty = acc_full + BUFS;     // [BUFS] the leader's
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + BUFS);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+    static_assert((2 * STAGES + 2 * BUFS) * 8 + 8 <= 256, "barriers");
+    const uint64_t deadline = tc::global_timer_ns() + FRT_KERNEL_DEADLINE_NS;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t cluster_rank = CG * S > 1 ? tc::cluster_ctarank() : 0u, rank = cluster_rank % CG, leader = cluster_rank - rank;
+    const int split = (int)cluster_rank / CG;
+    const int unit = (int)blockIdx.x / (CG * S), units = (int)gridDim.x / (CG * S);     // S > 1: as many as tiles
+    const int kb0 = S == 1 ? 0 : (int)((long long)p.kb * split / S), kb1 = S == 1 ? p.kb : (int)((long long)p.kb * (split + 1) / S);
+    const int m_tiles = (p.M + 128 * CG - 1) / (128 * CG), n_tiles = (p.N + BN - 1) / BN, total = m_tiles * n_tiles;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < STAGES; ++s) {
+            tc::mbar_init(&full[s], 1);
+            tc::mbar_init(&empty[s], 1);
+        }
+        for (int i = 0; i < BUFS; ++i) {
+            tc::mbar_init(&acc_full[i], 1);
+            tc::mbar_init(&acc_empty[i], CG * 8);
+        }
+        *abort_flag = 0;
+        tc::mbar_fence_init();
+        tc::tma_prefetch_desc(&tmA);
+        tc::tma_prefetch_desc(&tmW);
+    }
+    if (warp == 1) tmem_take<CG>(tmem_slot, 512);
+    tc::tc_fence_before_sync();
+    if constexpr (CG * S > 1) tc::cluster_sync_all();        // the CTAs' barriers exist before anything signals across
+    else __syncthreads();
+    tc::tc_fence_after_sync();
+    const uint32_t tmem = *tmem_slot;
+    pdl_launch_dependents();
+
+    if (warp == 0) {
+        // ---------------- producer of this CTA's rows, bytes counted at the leader
+        const uint32_t ring = tc::smem_u32(smem), empty_a = tc::smem_u32(empty), full_a = tc::smem_u32(full);
+        const uint32_t lead_full = CG == 1 ? full_a : tc::dsmem_map(full_a, leader);
+        pdl_wait();
+        int s = 0;
+        uint32_t ph = 1;
+        bool ready = true;
+        for (int t = unit; t < total; t += units) {
+            int mt, nt;
+            tile_at(t, p.gm, m_tiles, n_tiles, mt, nt);
+            const int m0 = (mt * CG + (int)rank) * 128, n0 = nt * BN + (int)rank * (BN / CG);
+            for (int kb = kb0; kb < kb1; ++kb) {
+                if (!tc::warp_wait(empty_a + 8 * s, ph, ready, deadline, abort_flag)) {
+                    if (lane == 0) gave_up(p.status, abort_flag, ERR_PRODUCER);
+                    t = total;
+                    break;
+                }
+                const uint32_t dst = ring + s * Cfg::STAGE_BYTES, bar = lead_full + 8 * s, own = full_a + 8 * s;
+                if (++s == STAGES) { s = 0; ph ^= 1; }
+                ready = tc::mbar_test(empty_a + 8 * s, ph);
+                if (tc::elect_one()) {
+                    if (rank == 0) tc::mbar_arrive_expect_tx(own, CG * Cfg::STAGE_BYTES);
+                    load<CG>(dst, &tmA, bar, kb * 128, m0);
+                    load<CG>(dst + Cfg::A_BYTES, &tmW, bar, kb * 128, n0);
+                }
+            }
+        }
+    } else if (warp == 1 && rank == 0) {
+        // ---------------- MMA issuer for the tile: a k-block, a buffer
+        constexpr uint32_t idesc = tc::make_idesc(0, 0, 0, 0, 128 * CG, BN);
+        const uint64_t dA0 = tc::make_desc_kmajor_sw128(tc::smem_u32(smem));
+        const uint64_t dB0 = tc::make_desc_kmajor_sw128(tc::smem_u32(smem + Cfg::A_BYTES));
+        const uint32_t full_a = tc::smem_u32(full), empty_a = tc::smem_u32(empty);
+        const uint32_t accF_a = tc::smem_u32(acc_full), accE_a = tc::smem_u32(acc_empty);
+        int s = 0, buf = 0;
+        uint32_t ph = 0, bph = 1;                            // the first round of the buffers is empty
+        bool ready = false;
+        for (int t = unit; t < total; t += units)
+            for (int kb = kb0; kb < kb1; ++kb) {
+                if (!tc::warp_wait(accE_a + 8 * buf, bph, false, deadline, abort_flag) ||
+                    !tc::warp_wait(full_a + 8 * s, ph, ready, deadline, abort_flag)) {
+                    if (lane == 0) gave_up(p.status, abort_flag, ERR_MMA);
+                    t = total;
+                    break;
+                }
+                tc::tc_fence_after_sync();
+                const uint64_t so = (uint64_t)(s * (Cfg::STAGE_BYTES >> 4));
+                const uint32_t done = empty_a + 8 * s, d_tm = tmem + buf * BN, there = accF_a + 8 * buf;
+                if (++s == STAGES) { s = 0; ph ^= 1; }
+                if (++buf == BUFS) { buf = 0; bph ^= 1; }
+                ready = tc::mbar_test(full_a + 8 * s, ph);
+                if (tc::elect_one()) {
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) mma<CG>(d_tm, dA0 + so + 2 * k, dB0 + so + 2 * k, idesc, k > 0 ? 1u : 0u);
+                    commit<CG>(done, leader);
+                    commit<CG>(there, leader);
+                }
+            }
+    } else if (warp >= 2) {
+        // ---------------- epilogue: this CTA's 128 rows; a warp's lane quadrant and half of the columns
+        pdl_wait();
+        const int q = warp & 3, half = (warp - 2) >> 2;
+        const uint32_t t_src = tmem + ((uint32_t)(q * 32) << 16) + half * W2;
+        const bool vec = (p.N & 3) == 0;
+        uint8_t* stg = smem + STAGES * Cfg::STAGE_BYTES + 256 + (warp - 2) * (32 * 128);
+        const uint32_t accF_a = tc::smem_u32(acc_full), accE_a = tc::smem_u32(acc_empty);
+        const uint32_t accE_lead = CG == 1 ? accE_a : tc::dsmem_map(accE_a, leader);
+        const int n_blocks = (p.N + 127) / 128;
+        int buf = 0;
+        uint32_t bph = 0;
+        for (int t = unit; t < total; t += units) {
+            int mt, nt;
+            tile_at(t, p.gm, m_tiles, n_tiles, mt, nt);
+            const int m_base = (mt * CG + (int)rank) * 128 + q * 32, n_base = nt * BN + half * W2;
+            const bool in = m_base + lane < p.M;
+            const float* ws = p.w_scale + (size_t)min(n_base / 128, n_blocks - 1) * p.kb;
+            const float* as = p.a_scale + (in ? m_base + lane : 0);
+            auto ask = [&](int kb) { return in && kb < kb1 ? __fmul_rn(as[kb * p.a_stride], ws[kb]) : 0.0f; };
+            float acc[W2], now = ask(kb0), next = ask(kb0 + 1);
+#pragma unroll
+            for (int j = 0; j < W2; ++j) acc[j] = 0.0f;
+            bool ok = true;
+            for (int kb = kb0; kb < kb1; ++kb) {
+                const float s = now;
+                now = next;
+                next = ask(kb + 2);
+                ok = tc::warp_wait(accF_a + 8 * buf, bph, false, deadline, abort_flag);
+                if (!ok) {
+                    if (lane == 0) gave_up(p.status, abort_flag, ERR_EPILOGUE);
+                    break;
+                }
+                tc::tc_fence_after_sync();
+                const uint64_t s2 = f32x2(s, s);
+#pragma unroll
+                for (int c = 0; c < W2; c += 16) {
+                    uint32_t v[16];
+                    tc::tmem_ld16(t_src + buf * BN + c, v);
+                    tc::tmem_ld_wait();
+#pragma unroll
+                    for (int j = 0; j < 16; j += 2) {
+                        const uint64_t r = fma_f32x2(f32x2(__uint_as_float(v[j]), __uint_as_float(v[j + 1])), s2, f32x2(acc[c + j], acc[c + j + 1]));
+                        f32x2_parts(r, acc[c + j], acc[c + j + 1]);
+                    }
+                }
+                tc::tc_fence_before_sync();
+                __syncwarp();
+                if (lane == 0) {
+                    if constexpr (CG == 1) tc::mbar_arrive(&acc_empty[buf]);
+                    else tc::mbar_arrive_cluster(accE_lead + 8 * buf);
+                }
+                if (++buf == BUFS) { buf = 0; bph ^= 1; }
+            }
+            if (!ok) break;
+            if constexpr (S > 1) {                           // [four columns][row]: a warp's store is 512 contiguous bytes
+                const uint32_t red = tc::smem_u32(smem) + (half * (W2 / 4) * 128 + q * 32 + lane) * 16;
+#pragma unroll
+                for (int j = 0; j < W2; j += 4) sts_v4(red + j * 512, acc[j], acc[j + 1], acc[j + 2], acc[j + 3]);
+                break;
+            } else {
+#pragma unroll
+                for (int c = 0; c < W2; c += 32)
+                    if (m_base < p.M && n_base + c < p.N) store_block(p, acc + c, m_base, n_base + c, stg, vec);
+            }
+        }
+    }
+    if constexpr (S > 1) {
+        __syncwarp();
+        tc::cluster_sync_all();                // all partials are there
+        if (warp >= 2 && !*abort_flag) {
+            constexpr int W = BN / S / 2;      // columns of this warp
+            const int q = warp & 3, half = (warp - 2) >> 2, col = split * (BN / S) + half * W;
+            int mt, nt;
+            tile_at(unit, p.gm, m_tiles, n_tiles, mt, nt);
+            const int m_base = (mt * CG + (int)rank) * 128 + q * 32, n_base = nt * BN + col;
+            uint8_t* stg = smem + STAGES * Cfg::STAGE_BYTES + 256 + (warp - 2) * (32 * 128);
+            const uint32_t red = tc::smem_u32(smem) + (uint32_t)(col / 4 * 128 + q * 32 + lane) * 16;
+#pragma unroll 1
+            for (int c = 0; c < W; c += 32) {
+                float v[32];
+#pragma unroll
+                for (int j = 0; j < 32; ++j) v[j] = 0.0f;
+#pragma unroll
+                for (int s = 0; s < S; ++s) {                // in the order of K
+                    const uint32_t from = tc::dsmem_map(red + (uint32_t)c * 512, (uint32_t)(CG * s) + rank);
+                    float4 w[8];
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) w[j] = tc::dsmem_ld_f32x4(from + (uint32_t)j * 2048);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        v[4 * j] = __fadd_rn(v[4 * j], w[j].x);
+                        v[4 * j + 1] = __fadd_rn(v[4 * j + 1], w[j].y);
+                        v[4 * j + 2] = __fadd_rn(v[4 * j + 2], w[j].z);
+                        v[4 * j + 3] = __fadd_rn(v[4 * j + 3], w[j].w);
+                    }
+                }
+                if (m_base < p.M && n_base + c < p.N) store_block(p, v, m_base, n_base + c, stg, (p.N & 3) == 0);
+            }
+        }
+    }
+    if (*abort_flag && threadIdx.x == 0) let_copies_land();
+    __syncwarp();
+    tc::tc_fence_before_sync();
+    if constexpr (CG * S > 1) tc::cluster_sync_all();        // the leader's MMAs read the peer's shared memory until the end
+    else __syncthreads();
+    tc::tc_fence_after_sync();
+    if (warp == 1) tmem_give<CG>(tmem, 512);
+}
+
+// ------------------------------------------------------------------------------------------------ host
+static void set_attrs(cudaLaunchConfig_t& cfg, cudaLaunchAttribute (&attr)[2], unsigned cx, unsigned cy, cudaStream_t stream) {
+    cfg.stream = stream;
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = cx;
+    attr[0].val.clusterDim.y = cy;
+    attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+}
+
+template <int BN>
+static int launch_lane(const void* A, const void* W, Params p, int K, int splits, cudaStream_t stream) {
+    using Cfg = LaneCfg<BN>;
+    static PerDeviceOnce once;
+    CUtensorMap tmA, tmW;
+    int dev = 0;
+    if (once.need(dev)) {
+        const cudaError_t e = cudaFuncSetAttribute(gemm_fp8_block_lane_kernel<BN>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::SMEM_BYTES);
+        if (e != cudaSuccess) return FRT_CUDA_ERR(e);
+        once.set(dev);
+    }
+    int rc = make_tmap_2d_u8(&tmA, A, (uint64_t)p.M, (uint64_t)K, (uint64_t)K, BN);
+    if (!rc) rc = make_tmap_2d_u8(&tmW, W, (uint64_t)p.N, (uint64_t)K, (uint64_t)K, 128);
+    if (rc) return rc;
+    const int tiles = (p.N + 127) / 128, room = 2 * device_sm_count();
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[2];
+    cfg.gridDim = dim3(splits > 1 || tiles < room ? tiles : room, splits);
+    cfg.blockDim = dim3(192);
+    cfg.dynamicSmemBytes = Cfg::SMEM_BYTES;
+    set_attrs(cfg, attr, 1, (unsigned)splits, stream);
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, gemm_fp8_block_lane_kernel<BN>, tmA, tmW, p);
+    return e == cudaSuccess ? FRT_OK : FRT_CUDA_ERR(e);
+}
+
+template <int CG, int BN, int S>
+static int launch_tile(const void* A, const void* W, Params p, int K, cudaStream_t stream) {
+    using Cfg = TileCfg<CG, BN>;
+    static PerDeviceOnce once;
+    CUtensorMap tmA, tmW;
+    int dev = 0;
+    if (once.need(dev)) {
+        const cudaError_t e = cudaFuncSetAttribute(gemm_fp8_block_tile_kernel<CG, BN, S>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::SMEM_BYTES);
+        if (e != cudaSuccess) return FRT_CUDA_ERR(e);
+        once.set(dev);
+    }
+    int rc = make_tmap_2d_u8(&tmA, A, (uint64_t)p.M, (uint64_t)K, (uint64_t)K, 128);
+    if (!rc) rc = make_tmap_2d_u8(&tmW, W, (uint64_t)p.N, (uint64_t)K, (uint64_t)K, BN / CG);
+    if (rc) return rc;
+    const int m_tiles = (p.M + 128 * CG - 1) / (128 * CG), n_tiles = (p.N + BN - 1) / BN, workers = device_sm_count() / CG;
+    const long long total = (long long)m_tiles * n_tiles;
+    if (total > 1 << 30) return FRT_ERR_UNSUPPORTED;
+    // rows of A and of W that a wave reads: 128 CG gm and BN workers / gm, fewest when they are alike
+    p.gm = 1;
+    if (total <= workers) p.gm = m_tiles;
+    else
+        while (p.gm < m_tiles && (long long)(p.gm + 1) * (p.gm + 1) * 128 * CG <= (long long)BN * workers) ++p.gm;
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[2];
+    cfg.gridDim = dim3(CG * (S > 1 ? S * (unsigned)total : (unsigned)(total < workers ? total : workers)));
+    cfg.blockDim = dim3(320);
+    cfg.dynamicSmemBytes = Cfg::SMEM_BYTES;
+    set_attrs(cfg, attr, CG * S, 1, stream);
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, gemm_fp8_block_tile_kernel<CG, BN, S>, tmA, tmW, p);
+    return e == cudaSuccess ? FRT_OK : FRT_CUDA_ERR(e);
+}
+
+template <int U>
+static int launch_quantize(const void* x, long long stride, void* out, float* scale, long long scale_stride, int rows, int dim, cudaStream_t stream) {
+    const int groups = (dim + 127) / 128;
+    const unsigned items = (unsigned)((long long)rows * groups);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((items + 16 * U - 1) / (16 * U));
+    cfg.blockDim = dim3(256);
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, quantize_groups_kernel<U>, static_cast<const __nv_bfloat16*>(x), stride,
+                                             static_cast<uint8_t*>(out), scale, scale_stride, rows, dim, groups, items);
+    return e == cudaSuccess ? FRT_OK : FRT_CUDA_ERR(e);
+}
+
+}  // namespace f8b
+}  // namespace frt
+
+static bool misaligned(const void* a, uintptr_t n) { return (reinterpret_cast<uintptr_t>(a) & (n - 1)) != 0; }
+
+extern "C" int frt_b200_quantize_fp8_groups(const void* in_bf16, long long in_stride, void* out8, float* group_scale, long long scale_stride,
+                                            int rows, int dim, int flags, void* stream) {
+    using namespace frt;
+    (void)flags;
+    if (rows < 0 || dim < 0 || in_stride < dim || in_stride % 8 || scale_stride < rows) return FRT_ERR_INVALID;
+    if (dim % 16 || (long long)rows * ((dim + 127) / 128) > 1 << 30) return FRT_ERR_UNSUPPORTED;
+    if (rows == 0 || dim == 0) return FRT_OK;
+    if (!in_bf16 || !out8 || !group_scale) return FRT_ERR_INVALID;
+    if (misaligned(in_bf16, 16) || misaligned(out8, 16) || misaligned(group_scale, 4)) return FRT_ERR_INVALID;
+    const cudaStream_t st = static_cast<cudaStream_t>(stream);
+    const bool few = (long long)rows * ((dim + 127) / 128) < 64ll * device_sm_count();
+    if (few) return f8b::launch_quantize<1>(in_bf16, in_stride, out8, group_scale, scale_stride, rows, dim, st);
+    return f8b::launch_quantize<4>(in_bf16, in_stride, out8, group_scale, scale_stride, rows, dim, st);
+}
+
+extern "C" int frt_b200_gemm_fp8_block_nt(const void* A, const void* W, void* D, int M, int N, int K, const float* a_scale,
+                                          long long a_scale_stride, const float* w_scale, const void* bias, int flags, void* stream) {
+    using namespace frt;
+    if (M < 0 || N < 0 || K < 1 || a_scale_stride < M) return FRT_ERR_INVALID;
+    if (K % 16 || K > 1 << 20 || M > 1 << 30 || N > 1 << 30) return FRT_ERR_UNSUPPORTED;
+    if (M == 0 || N == 0) return FRT_OK;
+    if (!A || !W || !D || !a_scale || !w_scale) return FRT_ERR_INVALID;
+    if (misaligned(A, 16) || misaligned(W, 16) || misaligned(D, 16) || misaligned(a_scale, 4) || misaligned(w_scale, 4) || misaligned(bias, 2))
+        return FRT_ERR_INVALID;
+    f8b::Params p = {};
+    p.out = D;
+    p.a_scale = a_scale;
+    p.a_stride = a_scale_stride;
+    p.w_scale = w_scale;
+    p.bias = static_cast<const __nv_bfloat16*>(bias);
+    static PerDevicePointer status;
+    p.status = status.get(gemm_status_device_ptr);
+    if (!p.status) return FRT_ERR_UNSUPPORTED;
+    p.M = M;
+    p.N = N;
+    p.kb = (K + 127) / 128;
+    p.early = flags & 1;
+    p.f32 = flags & 2;
+    const cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (M <= 64) {
+        // K splits (a cluster) while the tiles alone leave SMs idle and every rank keeps two k-blocks
+        const int tiles = (N + 127) / 128;
+        int splits = 1;
+        while (splits < 8 && tiles * splits * 2 <= 2 * device_sm_count() && p.kb / (splits * 2) >= 2) splits *= 2;
+        if (M <= 16) return f8b::launch_lane<16>(A, W, p, K, splits, st);
+        if (M <= 32) return f8b::launch_lane<32>(A, W, p, K, splits, st);
+        return f8b::launch_lane<64>(A, W, p, K, splits, st);
+    }
+    if (M <= 128) return f8b::launch_tile<1, 256, 1>(A, W, p, K, st);
+    return f8b::launch_tile<2, 256, 1>(A, W, p, K, st);
+}

@@ -261,6 +261,12 @@ def quantize_int8_rows(input, output, row_scale, rows, dim, stream=0, *, in_stri
     call("frt_b200_quantize_int8_rows", input, in_stride or dim, output, row_scale, rows, dim, 0, stream)
 
 
+def quantize_fp8_groups(input, output, group_scale, rows, dim, stream=0, *, in_stride=0, scale_stride=0):  # noqa: A002
+    """(rows, dim) bf16 -> E4M3 with one fp32 scale per row and group of 128, max |x| / 448 (no counterpart in the reference).
+    ``group_scale`` (ceil(dim / 128), ``scale_stride`` or rows).  The activations of :meth:`GemmRunner.fp8_block_nt`."""
+    call("frt_b200_quantize_fp8_groups", input, in_stride or dim, output, group_scale, scale_stride or rows, rows, dim, 0, stream)
+
+
 def fp8_accumulate_scale_max(src_scale, dst_scale, stream=0):
     call("frt_b200_fp8_accumulate_scale_max", src_scale, dst_scale, stream)
 
@@ -309,6 +315,13 @@ class GemmRunner:
         """D(M,N) bf16 = (A(M,K) . B(N,K)^T) * token_scale[m] * channel_scale[n] + bias[n] of int8 matrices, exact integer sums
         (no counterpart in the reference).  K % 16 == 0; any M and N."""
         call("frt_b200_gemm_int8_nt", A, B, D, M, N, K, token_scale, channel_scale, bias or None, _f(pdl), stream)
+
+    def fp8_block_nt(self, A, B, D, M, N, K, a_scale, b_scale, stream=0, *, bias=0, a_scale_stride=0, d_f32=False, pdl=False):
+        """D(M,N) = A(M,K) . B(N,K)^T (+ bias) of E4M3 matrices with a scale for each row and 128 of K of A (``quantize_fp8_groups``) and
+        for each 128 x 128 block of B, (ceil(N / 128), ceil(K / 128)) (no counterpart in the reference).  D bf16, ``d_f32``: fp32.
+        K % 16 == 0; any M and N."""
+        call("frt_b200_gemm_fp8_block_nt", A, B, D, M, N, K, a_scale, a_scale_stride or M, b_scale, bias or None,
+             _f(pdl) | (2 if d_f32 else 0), stream)
 
     # -- the decoder's projections with the norm kernel between them folded in ------------------------------
     def fp8_nt_dev_gate_residual(self, A, B, M, N, K, d_scale_a, d_scale_b, residual, gate, stats_out, stream=0, *,
@@ -423,6 +436,39 @@ class GemmRunner:
 
     def autotune_fp8_nt_dev(self, *a, **k):
         return 0
+
+
+# ------------------------------------------------------------------ steps of a language model (no counterpart in the reference)
+def softmax_rows(input, output, rows, vocab, stream=0, *, temperature=0, in_f32=False, in_stride=0, out_stride=0):  # noqa: A002
+    """Logits (rows, vocab) bf16 (``in_f32``: fp32) -> probabilities fp32; ``temperature`` (rows) fp32, 0: 1 everywhere.  A row whose
+    temperature is not above zero has one at the first of its largest."""
+    call("frt_b200_softmax_rows", input, in_stride or vocab, output, out_stride or vocab, temperature or None, rows, vocab,
+         2 if in_f32 else 0, stream)
+
+
+def verify_drafts(target_probs, draft_probs, tokens, cu_seqlens, seq_lens, u_accept, u_sample, out_tokens, accepted, kept_lens,
+                  n_tokens, batch, vocab, stream=0, *, p_stride=0, q_stride=0):
+    """Drafted tokens against the target's probabilities: row t of a sequence answers with token t + 1, which stands if
+    u_accept[t] * q < p; behind the last that stands comes one from what p has left, chosen by u_sample (batch).  ``draft_probs`` 0:
+    the draft was sure.  ``out_tokens`` (n_tokens): tokens that stand, the new one, -1; ``accepted`` (batch); ``kept_lens`` (batch) or
+    0: seq_lens less what does not stand, for :func:`paged_release` and :func:`paged_plan`."""
+    call("frt_b200_verify_drafts", target_probs, p_stride or vocab, draft_probs or None, q_stride or vocab, tokens, cu_seqlens,
+         seq_lens or None, u_accept, u_sample, out_tokens, accepted, kept_lens or None, n_tokens, batch, vocab, 0, stream)
+
+
+def paged_plan(kept_lens, new_lens, block_table, table_stride, free_list, free_in, free_out, cu_seqlens, seq_lens, positions, slots,
+               refused, tokens, batch, num_blocks, block_size, stream=0):
+    """The next step of a batch over the paged cache: blocks from the free list for ``new_lens`` tokens behind ``kept_lens``, written
+    into the block table; ``cu_seqlens`` and ``seq_lens`` as :func:`paged_kv_append_fp8` and ``paged_fwd_fp8`` read them; ``positions``
+    (tokens) int32, ``slots`` (tokens) int64, ``refused`` int32, each 0 where not wanted."""
+    call("frt_b200_paged_plan", kept_lens, new_lens, block_table, table_stride, free_list, free_in, free_out, cu_seqlens, seq_lens,
+         positions or None, slots or None, refused or None, tokens, batch, num_blocks, block_size, 0, stream)
+
+
+def paged_release(kept_lens, seq_lens, block_table, table_stride, free_list, free_in, free_out, batch, num_blocks, block_size, stream=0):
+    """Blocks behind the tokens that stay go back to the free list; ``kept_lens`` 0 ends a sequence."""
+    call("frt_b200_paged_release", kept_lens, seq_lens, block_table, table_stride, free_list, free_in, free_out, batch, num_blocks,
+         block_size, 0, stream)
 
 
 # ------------------------------------------------------------------ capability probes (csrc/bindings.cpp:2424-2459)

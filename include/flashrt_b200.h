@@ -573,6 +573,70 @@ int frt_b200_quantize_int8_rows(const void* in_bf16, long long in_stride, void* 
 int frt_b200_gemm_int8_nt(const void* A, const void* W, void* D, int M, int N, int K, const float* token_scale,
                           const float* channel_scale, const void* bias, int flags, void* stream);
 
+/* ---------------------------------------------------------------- E4M3 products with a scale for each block of 128
+ * No counterpart in the reference (its FP8 products have one scale per tensor: csrc/gemm/gemm_runner.cu:67-76).
+ * Rows of activations to E4M3, a scale for each row and group of 128 values (the last group may be shorter): t = max(max |finite x| of the
+ *   group, 448e-12), s = t / 448, code = e4m3(clamp(x * 448 / t, +-448)), the quotient rounded once, so that values exactly between two
+ *   codes go to the even one; infinities are clamped, NaN becomes -448.  in (rows, dim) bf16, rows in_stride elements apart; out
+ *   (rows, dim) E4M3; group_scale (ceil(dim / 128), scale_stride >= rows) fp32: the scales of a group lie row by row.
+ *   dim % 16 == 0, in_stride % 8 == 0, in and out 16-byte aligned, at most 2^30 groups. */
+int frt_b200_quantize_fp8_groups(const void* in_bf16, long long in_stride, void* out_fp8, float* group_scale, long long scale_stride,
+                                 int rows, int dim, int flags, void* stream);
+/* D(M,N) = sum_j a_scale[j][m] * w_scale[n / 128][j] * (sum_{k in block j} A[m][k] W[n][k]) + bias[n], blocks j of 128 along K
+ *   (no counterpart in the reference): A (M, K) and W (N, K) E4M3, K contiguous, 16-byte aligned; a_scale (ceil(K / 128), a_scale_stride >= M)
+ *   as the quantiser leaves it, w_scale (ceil(N / 128), ceil(K / 128)) fp32; bias (N) bf16 or NULL; D bf16, with flags bit 1 fp32 (logits).
+ *   Sums are fp32, over a block of 128 in the tensor core, then block by block, each scaled; the order of the blocks is that of K, where K
+ *   is split over CTAs (few rows, few tiles) that of the parts.  K % 16 == 0, K <= 2^20; any M and N up to 2^30.  flags bit 0: the weights
+ *   are settled and may be read before the kernel in front has ended.  A wait that gave up shows in frt_b200_gemm_status. */
+int frt_b200_gemm_fp8_block_nt(const void* A, const void* W, void* D, int M, int N, int K, const float* a_scale,
+                               long long a_scale_stride, const float* w_scale, const void* bias, int flags, void* stream);
+
+/* ---------------------------------------------------------------- probabilities, drafted tokens
+ * Softmax of rows (no counterpart in the reference): out = exp((x - max) / T) / sum, fp32.  in (rows, vocab) bf16, with flags bit 1 fp32, rows
+ *   in_stride elements apart; out (rows, vocab) fp32, rows out_stride elements apart; temperature (rows) fp32 or NULL: 1.  A temperature
+ *   that is not above zero (0, negative, NaN): one at the first of the row's largest, zero elsewhere.  NaN counts as -infinity; a row of
+ *   nothing else is zero; infinite entries share the whole.  Not in place.  vocab <= 2^30. */
+int frt_b200_softmax_rows(const void* in, long long in_stride, float* out, long long out_stride, const float* temperature, int rows,
+                          int vocab, int flags, void* stream);
+/* Drafted tokens against the target's probabilities, from given random numbers (no counterpart in the reference).  Sequence b has the rows
+ *   cu_seqlens[b] .. cu_seqlens[b + 1] - 1 of this step: a token that stands already and the drafted ones behind it; row t answers with
+ *   token t + 1.  tokens (n_tokens) int32; target_probs, draft_probs (n_tokens, vocab) fp32, not negative, finite, rows p_stride / q_stride
+ *   elements apart (a sequence's last row of draft_probs is not read; NULL: all of the draft's probability lay on its token).
+ *   Drafted token d of row t stands if those in front do and u_accept[t] * q[t][d] < p[t][d], in 64 bits; a token outside the vocabulary
+ *   does not.  Behind the last that stands comes a token from max(p - q, 0) of the first row whose token does not (without draft_probs: p
+ *   without that token; where nothing is left: p), or from p of the sequence's last row: the first entry whose running sum is above
+ *   u_sample[b] * sum, in 64 bits (u_sample is taken into [0, 1); -1 if all is zero).
+ *   out_tokens (n_tokens), not `tokens` itself: the tokens that stand, the new one, then -1 up to the sequence's end; rows behind the last
+ *   sequence are left as they were.  accepted (batch): drafted tokens that stand.  kept_lens (batch) or NULL: seq_lens less the drafted
+ *   tokens that do not; may be seq_lens itself.  A sequence without rows, or whose rows leave [0, n_tokens): accepted 0, kept_lens =
+ *   seq_lens, nothing else. */
+int frt_b200_verify_drafts(const float* target_probs, long long p_stride, const float* draft_probs, long long q_stride,
+                           const int* tokens, const int* cu_seqlens, const int* seq_lens, const float* u_accept,
+                           const float* u_sample, int* out_tokens, int* accepted, int* kept_lens, int n_tokens, int batch,
+                           int vocab, int flags, void* stream);
+
+/* ---------------------------------------------------------------- blocks of the paged cache between two steps
+ * No counterpart in the reference.  All arrays are device memory that is read when the launch runs.  free_list (num_blocks) int32: the first
+ * *free_in entries are free blocks.  block_table, block_size as for the cache above; batch <= 8192, batch * table_stride <= 2^30.
+ *
+ * The next step (no counterpart in the reference): sequence b keeps kept_lens[b] tokens, whose blocks its row of the table holds, and brings
+ *   new_lens[b].  Written: cu_seqlens (batch + 1), seq_lens = kept + new, the table's entries of blocks that are begun now, taken from the
+ *   list's end in the order of sequences and positions; *free_out; positions (tokens) int32 and slots (tokens) int64 = block * block_size +
+ *   offset, -1 for rows behind the last sequence and for pages that are no block of the pool (either may be NULL); *refused (or NULL).
+ *   A sequence with a negative length, or with more blocks than its row has entries, brings nothing (its seq_lens is max(kept, 0)); from the
+ *   first one on for which the list or `tokens` rows do not suffice, none brings anything.  *refused counts them all.
+ *   Other entries of the table stay as they were.  free_out is not free_in, seq_lens neither kept_lens nor new_lens. */
+int frt_b200_paged_plan(const int* kept_lens, const int* new_lens, int* block_table, int table_stride, const int* free_list,
+                        const int* free_in, int* free_out, int* cu_seqlens, int* seq_lens, int* positions, long long* slots,
+                        int* refused, int tokens, int batch, int num_blocks, int block_size, int flags, void* stream);
+/* Tokens are dropped (no counterpart in the reference): drafted ones that do not stand (kept_lens of frt_b200_verify_drafts), or a whole
+ *   sequence (0).  The table's entries of blocks behind ceil(kept_lens / block_size), up to ceil(seq_lens / block_size), become -1; those
+ *   that are blocks of the pool go on the list, a sequence's last one and the last sequence's first, so that a plan that takes as many finds
+ *   them in their old places.  *free_out = *free_in + their number, at most num_blocks; not free_in itself.  Blocks carry no count of
+ *   their users: one that two rows share is put on the list by each that drops it. */
+int frt_b200_paged_release(const int* kept_lens, const int* seq_lens, int* block_table, int table_stride, int* free_list,
+                           const int* free_in, int* free_out, int batch, int num_blocks, int block_size, int flags, void* stream);
+
 /* number of SMs of the current device (grid sizing) */
 int frt_b200_device_sm_count(void);
 
