@@ -46,184 +46,269 @@ __device__ __forceinline__ float warp_max(float x) {
 
 // ------------------------------------------------------------------------------------------------ softmax
 //   p = exp((x - max) / T) / sum;  T not above zero: one on the first of the largest;  nothing but -infinity and NaN: zeros.
-// A CTA's part: exponentials against its own maximum, then one exchange of (maximum, sum) in the cluster, and a factor that takes them to
-// the row's.  NV vectors a thread; HELD false: what is behind them is read twice.
+// Weights are exponentials against the warp's own maximum; the (maximum, sum) of warps meet in shared memory, those of the cluster's CTAs
+// by st.async (a cluster barrier waits for every store in front of it: 384 rows of 131072 in fp32 103 us with two a row), and a factor
+// takes a warp's weights to the row's probabilities.  NV vectors a thread.  FORM 0: a row a cluster; 1: what is behind NV vectors is read
+// twice; 2: clusters stay and go from row to row, the next row's part is copied to shared memory meanwhile.
 struct SoftmaxParams {
     const void* x;
     float* p;
     const float* temperature;
     long long in_stride, out_stride;
-    int vocab, ctas;             // ctas: of a row
+    int rows, vocab, ctas;       // ctas: of a row
+    int* status;
 };
+constexpr int ONE_ROW = 0, READ_TWICE = 1, STAY = 2;
+enum { ERR_MAIL = 1, ERR_ROW = 2 };
 
-template <int THREADS, int NV, bool F32, bool HELD>
+struct Yes { static constexpr bool value = true; };
+struct No { static constexpr bool value = false; };
+
+template <int THREADS, int NV, bool F32, int FORM>
 __global__ void __launch_bounds__(THREADS, NV * (F32 ? 4 : 8) > 32 ? 1 : 1024 / THREADS)
 softmax_rows_kernel(SoftmaxParams p) {
-    constexpr int VE = F32 ? 4 : 8, WARPS = THREADS / 32;    // values of 16 bytes
-    __shared__ float part[WARPS], part2[WARPS];
-    __shared__ int part3[WARPS];
-    __shared__ uint4 mine;                                   // maximum, sum, index of the first of the largest
+    constexpr int VE = F32 ? 4 : 8, ES = F32 ? 4 : 2, WARPS = THREADS / 32;      // values of 16 bytes, bytes of a value
+    constexpr bool HELD = FORM != READ_TWICE, STAGED = FORM == STAY;
+    extern __shared__ uint4 stage[];                         // STAY: the next row's part
+    __shared__ float part[2][WARPS], part2[2][WARPS];        // of each warp: maximum, sum
+    __shared__ int part3[2][WARPS];                          // first of its largest
+    __shared__ uint4 box[2][8];                              // the same of each CTA of the cluster
+    __shared__ uint64_t mail[2], there;
     pdl_launch_dependents();
-    pdl_wait();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int ctas = p.ctas, rank = (int)(blockIdx.x % (unsigned)ctas);
-    const long long row = blockIdx.x / (unsigned)ctas;
-    const uint8_t* x = static_cast<const uint8_t*>(p.x) + row * p.in_stride * (F32 ? 4 : 2);
-    float* out = p.p + row * p.out_stride;
-    // vector j has the entries VE j - skew ..: rows start anywhere, vectors at 16 bytes
-    const int skew = (int)(reinterpret_cast<uintptr_t>(x) & 15) / (F32 ? 4 : 2), vectors = (p.vocab + skew + VE - 1) / VE;
-    const bool wide = ((reinterpret_cast<uintptr_t>(out) - 4 * (uintptr_t)skew) & 15) == 0;
-    const int j0 = (int)((long long)vectors * rank / ctas), j1 = (int)((long long)vectors * (rank + 1) / ctas);
-    const float T = p.temperature ? p.temperature[row] : 1.0f;
-    const bool hot = !(T > 0.0f);
-    const float c = hot ? 0.0f : __fdiv_rn(1.4426950408889634f, T);
-    const int ja = max(j0, skew ? 1 : 0), jb = min(j1, (p.vocab + skew) / VE);       // whole vectors of this CTA; one may lie at each end
-    constexpr uint32_t MASKED = F32 ? 0xff800000u : 0xff80ff80u;
-    auto raw = [&](int j) { return ld_v4_if(x + ((long long)j * VE - skew) * (F32 ? 4 : 2), j >= ja && j < jb, MASKED); };
-    auto values = [&](const uint4& w, int j, float* v) {     // masked: -infinity, as NaN is
-        if (F32) {
-            v[0] = __uint_as_float(w.x);
-            v[1] = __uint_as_float(w.y);
-            v[2] = __uint_as_float(w.z);
-            v[3] = __uint_as_float(w.w);
-        } else {
-            unpack_bf16x2(w.x, v[0], v[1]);
-            unpack_bf16x2(w.y, v[2], v[3]);
-            unpack_bf16x2(w.z, v[VE - 4], v[VE - 3]);
-            unpack_bf16x2(w.w, v[VE - 2], v[VE - 1]);
-        }
-        if (j < j1 && (j < ja || j >= jb)) {
-            const int e = j * VE - skew;
-#pragma unroll
-            for (int k = 0; k < VE; ++k)
-                if (e + k >= 0 && e + k < p.vocab)
-                    v[k] = F32 ? reinterpret_cast<const float*>(x)[e + k] : __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(x)[e + k]);
-        }
-#pragma unroll
-        for (int k = 0; k < VE; ++k) v[k] = v[k] == v[k] ? v[k] : -INFINITY;
-    };
-    float v[NV * VE], top = -INFINITY;
-    {
-        uint4 w[NV];
-#pragma unroll
-        for (int i = 0; i < NV; ++i) w[i] = raw(j0 + tid + i * THREADS);
-#pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            values(w[i], j0 + tid + i * THREADS, v + i * VE);
-#pragma unroll
-            for (int k = 0; k < VE; ++k) top = fmaxf(top, v[i * VE + k]);
-        }
+    const int ctas = p.ctas, rank = (int)(blockIdx.x % (unsigned)ctas), step = (int)(gridDim.x / (unsigned)ctas);
+    const uint64_t deadline = tc::global_timer_ns() + FRT_KERNEL_DEADLINE_NS;
+    int no_flag = 0;
+    if (tid == 0 && (STAGED || ctas > 1)) {
+        tc::mbar_init(&mail[0], 1);
+        tc::mbar_init(&mail[1], 1);
+        tc::mbar_init(&there, 1);
+        tc::mbar_fence_init();
     }
-    auto rest = [&](auto f) {                                // what this thread does not hold
-        if (!HELD)
-            for (int j = j0 + tid + NV * THREADS; j < j1; j += THREADS) {
-                float w[VE];
-                values(raw(j), j, w);
-                f(j, w);
-            }
+    if (ctas > 1) tc::cluster_arrive();                      // waited for in front of the first message
+    if (STAGED) __syncthreads();
+    pdl_wait();
+    // A row's part: vector j has the entries VE j - skew .., since rows start anywhere and vectors at 16 bytes; whole vectors [ja, jb) of
+    // this CTA's [j0, j1), one may lie at each end of the row.
+    struct Place { const uint8_t* base; int skew, j0, j1, ja, jb; };
+    auto place = [&](int row) {
+        Place w;
+        const uint8_t* x = static_cast<const uint8_t*>(p.x) + row * p.in_stride * ES;
+        w.skew = (int)(reinterpret_cast<uintptr_t>(x) & 15) / ES;
+        w.base = x - w.skew * ES;
+        const int vectors = (p.vocab + w.skew + VE - 1) / VE;
+        w.j0 = (int)((long long)vectors * rank / ctas);
+        w.j1 = (int)((long long)vectors * (rank + 1) / ctas);
+        w.ja = max(w.j0, w.skew ? 1 : 0);
+        w.jb = min(w.j1, (p.vocab + w.skew) / VE);
+        return w;
     };
-    rest([&](int, const float* w) {
-#pragma unroll
-        for (int k = 0; k < VE; ++k) top = fmaxf(top, w[k]);
-    });
-    top = warp_max(top);
-    if (lane == 0) part[warp] = top;
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < WARPS; ++w) top = fmaxf(top, part[w]);
-    // against this CTA's maximum; where that is infinite, the infinite ones share the mass
-    auto weight = [&](float y) { return y == top ? 1.0f : exp2_approx(fmaxf(__fmul_rn(__fsub_rn(y, top), c), -3.0e38f)); };
-    float sum = 0.0f;
-    int first = 0x7fffffff;
-    if (hot) {
-        auto look = [&](int j, const float* w) {
+    auto fetch = [&](int row) {                              // one thread
+        if (row >= p.rows) return;
+        const Place w = place(row);
+        tc::mbar_arrive_expect_tx(&there, (uint32_t)max(w.jb - w.ja, 0) * 16u);
+        for (int j = w.ja; j < w.jb; j += 1024)
+            tc::bulk_load(&stage[j - w.j0], w.base + (size_t)j * 16, (uint32_t)min(w.jb - j, 1024) * 16u, &there);
+    };
+    int row = (int)(blockIdx.x / (unsigned)ctas);
+    if (STAGED && tid == 0) fetch(row);
+    for (int turn = 0; row < p.rows; row += step, ++turn) {
+        const Place at = place(row);
+        const int odd = turn & 1, me = at.j0 + tid;
+        float* out = p.p + row * p.out_stride;
+        const float* xf = reinterpret_cast<const float*>(at.base) + at.skew;
+        const __nv_bfloat16* xh = reinterpret_cast<const __nv_bfloat16*>(at.base) + at.skew;
+        const bool edges = at.ja > at.j0 || at.jb < at.j1, wide = ((reinterpret_cast<uintptr_t>(out) - 4 * (uintptr_t)at.skew) & 15) == 0;
+        const bool wide32 = ((reinterpret_cast<uintptr_t>(out) - 4 * (uintptr_t)at.skew) & 31) == 0;
+        const float T = p.temperature ? p.temperature[row] : 1.0f;
+        const bool hot = !(T > 0.0f);
+        const float c = hot ? 0.0f : __fdiv_rn(1.4426950408889634f, T);
+        constexpr uint32_t MASKED = F32 ? 0xff800000u : 0xff80ff80u;
+        auto unpack = [&](const uint4& w, float* v) {
+            if (F32) {
+                v[0] = __uint_as_float(w.x);
+                v[1] = __uint_as_float(w.y);
+                v[2] = __uint_as_float(w.z);
+                v[3] = __uint_as_float(w.w);
+            } else {
+                unpack_bf16x2(w.x, v[0], v[1]);
+                unpack_bf16x2(w.y, v[2], v[3]);
+                unpack_bf16x2(w.z, v[VE - 4], v[VE - 3]);
+                unpack_bf16x2(w.w, v[VE - 2], v[VE - 1]);
+            }
+        };
+        auto at_edge = [&](int j) { return j < at.j1 && (j < at.ja || j >= at.jb); };
+        auto edge = [&](int j, float* v) {                   // value by value
+            const int e = j * VE - at.skew;
 #pragma unroll
             for (int k = 0; k < VE; ++k) {
-                const int e = j * VE - skew + k;
-                if (j < j1 && e >= 0 && e < p.vocab && w[k] == top) first = min(first, e);
+                v[k] = -INFINITY;
+                if (e + k >= 0 && e + k < p.vocab) v[k] = F32 ? xf[e + k] : __bfloat162float(xh[e + k]);
+            }
+        };
+        // NaN: fmaxf leaves it out, here and in a weight's argument, which it puts at the lower end
+        float v[NV * VE], top = -INFINITY;
+        if (STAGED && !tc::mbar_wait_until(&there, (uint32_t)odd, deadline, &no_flag) && tid == 0) atomicCAS(p.status, 0, ERR_ROW);
+        {
+            uint4 w[NV];
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                const int j = me + i * THREADS;
+                const bool in = j >= at.ja && j < at.jb;
+                if (STAGED) w[i] = in ? stage[j - at.j0] : make_uint4(MASKED, MASKED, MASKED, MASKED);
+                else w[i] = ld_v4_if(at.base + (size_t)(unsigned)j * 16, in, MASKED);
+            }
+#pragma unroll
+            for (int i = 0; i < NV; ++i) unpack(w[i], v + i * VE);
+        }
+        if (edges)
+#pragma unroll
+            for (int i = 0; i < NV; ++i)
+                if (at_edge(me + i * THREADS)) edge(me + i * THREADS, v + i * VE);
+#pragma unroll
+        for (int i = 0; i < NV * VE; ++i) top = fmaxf(top, v[i]);
+        auto rest = [&](auto f) {                            // what this thread does not hold
+            if (!HELD)
+                for (int j = me + NV * THREADS; j < at.j1; j += THREADS) {
+                    float w[VE];
+                    if (at_edge(j)) edge(j, w);
+                    else unpack(ld_v4_if(at.base + (size_t)(unsigned)j * 16, true, MASKED), w);
+                    f(j, w);
+                }
+        };
+        rest([&](int, float* w) {
+#pragma unroll
+            for (int k = 0; k < VE; ++k) top = fmaxf(top, w[k]);
+        });
+        top = warp_max(top);
+        // weights two at a time; where the maximum is infinite (the infinite ones share the mass), or the temperature so small that its
+        // reciprocal is, the largest are one by comparison, since 0 times infinity would stand there
+        const bool plain = fabsf(top) < INFINITY && c < INFINITY;
+        const uint64_t minus_top = f32x2(-top, -top), c2 = f32x2(c, c);
+        auto weigh = [&](float* w, auto slow) {
+            if (!decltype(slow)::value) {
+#pragma unroll
+                for (int k = 0; k < VE; k += 2) {
+                    float a, b;
+                    f32x2_parts(mul_f32x2(add_f32x2(f32x2(w[k], w[k + 1]), minus_top), c2), a, b);
+                    w[k] = exp2_approx(fmaxf(a, -3.0e38f));
+                    w[k + 1] = exp2_approx(fmaxf(b, -3.0e38f));
+                }
+            } else {
+#pragma unroll
+                for (int k = 0; k < VE; ++k) w[k] = w[k] == top ? 1.0f : exp2_approx(fmaxf(__fmul_rn(__fsub_rn(w[k], top), c), -3.0e38f));
+            }
+        };
+        const bool nothing = top == -INFINITY;               // this warp's entries are all masked: zeros
+        uint64_t sum2 = 0;
+        int first = 0x7fffffff;
+        auto look = [&](int j, float* w) {
+#pragma unroll
+            for (int k = 0; k < VE; ++k) {
+                const int e = j * VE - at.skew + k;
+                if (j < at.j1 && e >= 0 && e < p.vocab && w[k] == top) first = min(first, e);
+            }
+        };
+        auto add = [&](float* w) {
+#pragma unroll
+            for (int k = 0; k < VE; k += 2) sum2 = add_f32x2(sum2, f32x2(w[k], w[k + 1]));
+        };
+        if (hot) {
+#pragma unroll
+            for (int i = 0; i < NV; ++i) look(me + i * THREADS, v + i * VE);
+            rest(look);
+            first = __reduce_min_sync(0xffffffffu, first);
+        } else if (plain) {
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                weigh(v + i * VE, No());
+                add(v + i * VE);
+            }
+            rest([&](int, float* w) {
+                weigh(w, No());
+                add(w);
+            });
+        } else if (!nothing) {
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                weigh(v + i * VE, Yes());
+                add(v + i * VE);
+            }
+            rest([&](int, float* w) {
+                weigh(w, Yes());
+                add(w);
+            });
+        }
+        float sum, sum_odd;
+        f32x2_parts(sum2, sum, sum_odd);
+        sum = warp_sum_butterfly(__fadd_rn(sum, sum_odd));
+        if (lane == 0) {
+            part[odd][warp] = top;
+            part2[odd][warp] = sum;
+            part3[odd][warp] = first;
+        }
+        __syncthreads();
+        if (STAGED && tid == 0) fetch(row + step);           // everyone has taken this row's part
+        // lane w of every warp has warp w's, later CTA w's
+        auto join = [&](float& m, float& s, int& f) {
+            const float its = m;
+            m = warp_max(its);
+            const float w = its == m ? 1.0f : exp2_approx(fmaxf(__fmul_rn(__fsub_rn(its, m), c), -3.0e38f));
+            s = warp_sum_butterfly(__fmul_rn(s, w));
+            f = __reduce_min_sync(0xffffffffu, its == m ? f : 0x7fffffff);
+        };
+        float m = lane < WARPS ? part[odd][lane] : -INFINITY, total = lane < WARPS ? part2[odd][lane] : 0.0f;
+        int f = lane < WARPS ? part3[odd][lane] : 0x7fffffff;
+        if (ctas == 1 || warp == 0) join(m, total, f);
+        if (ctas > 1) {
+            if (turn == 0) tc::cluster_wait();               // the peers' barriers exist
+            if (tid == 0) tc::mbar_arrive_expect_tx(&mail[odd], (uint32_t)ctas * 16u);
+            if (warp == 0 && lane < ctas)
+                tc::st_async_v4(tc::dsmem_map(tc::smem_u32(&box[odd][rank]), (uint32_t)lane), tc::dsmem_map(tc::smem_u32(&mail[odd]), (uint32_t)lane),
+                                __float_as_uint(m), __float_as_uint(total), (uint32_t)f, 0u);
+            // a box is written again two rows on, when every CTA has sent the row between, and so has read this one
+            if (!tc::mbar_wait_until(&mail[odd], (uint32_t)(turn >> 1) & 1u, deadline, &no_flag) && tid == 0) atomicCAS(p.status, 0, ERR_MAIL);
+            const uint4 its = lane < ctas ? box[odd][lane] : make_uint4(0xff800000u, 0u, 0x7fffffffu, 0u);
+            m = __uint_as_float(its.x);
+            total = __uint_as_float(its.y);
+            f = (int)its.z;
+            join(m, total, f);
+        }
+        if (m == -INFINITY) f = -1;
+        const float factor = __fdiv_rn(top == m ? 1.0f : exp2_approx(fmaxf(__fmul_rn(__fsub_rn(top, m), c), -3.0e38f)), total);
+        const uint64_t factor2 = f32x2(factor, factor);
+        auto store = [&](int j, float* w) {
+            const int e = j * VE - at.skew;
+            if (hot || nothing) {
+#pragma unroll
+                for (int k = 0; k < VE; ++k) w[k] = hot && e + k == f ? 1.0f : 0.0f;
+            } else {
+#pragma unroll
+                for (int k = 0; k < VE; k += 2) f32x2_parts(mul_f32x2(f32x2(w[k], w[k + 1]), factor2), w[k], w[k + 1]);
+            }
+            if (!F32 && wide32 && j >= at.ja && j < at.jb) {
+                uint32_t r[8];
+#pragma unroll
+                for (int k = 0; k < 8; ++k) r[k] = __float_as_uint(w[k % VE]);
+                st_global_32(out + e, true, true, r);
+            } else if (wide && j >= at.ja && j < at.jb) {
+#pragma unroll
+                for (int k = 0; k < VE; k += 4) *reinterpret_cast<float4*>(out + e + k) = make_float4(w[k], w[k + 1], w[k + 2], w[k + 3]);
+            } else if (j < at.j1) {
+#pragma unroll
+                for (int k = 0; k < VE; ++k)
+                    if (e + k >= 0 && e + k < p.vocab) out[e + k] = w[k];
             }
         };
 #pragma unroll
-        for (int i = 0; i < NV; ++i) look(j0 + tid + i * THREADS, v + i * VE);
-        rest(look);
-    } else if (top != -INFINITY) {                           // otherwise every weight stays 0 through the factor
-#pragma unroll
-        for (int i = 0; i < NV * VE; ++i) {
-            v[i] = weight(v[i]);
-            sum += v[i];
-        }
-        rest([&](int, const float* w) {
-#pragma unroll
-            for (int k = 0; k < VE; ++k) sum += weight(w[k]);
-        });
-    }
-    first = __reduce_min_sync(0xffffffffu, first);
-    sum = warp_sum_butterfly(sum);
-    if (lane == 0) {
-        part2[warp] = sum;
-        part3[warp] = first;
-    }
-    __syncthreads();
-    sum = 0.0f;
-#pragma unroll
-    for (int w = 0; w < WARPS; ++w) {
-        sum += part2[w];
-        first = min(first, part3[w]);
-    }
-    float factor;
-    bool nothing = top == -INFINITY;                         // this CTA's entries are all masked: zeros
-    if (ctas > 1) {
-        if (tid == 0) mine = make_uint4(__float_as_uint(top), __float_as_uint(sum), (uint32_t)first, 0);
-        tc::cluster_sync_all();
-        uint4 all[8];
-#pragma unroll
-        for (int r = 0; r < 8; ++r)
-            if (r < ctas) all[r] = dsmem_ld_u32x4(tc::dsmem_map(tc::smem_u32(&mine), (uint32_t)r));
-        tc::cluster_arrive();
-        float m = -INFINITY, total = 0.0f;
-#pragma unroll
-        for (int r = 0; r < 8; ++r)
-            if (r < ctas) m = fmaxf(m, __uint_as_float(all[r].x));
-        int f = 0x7fffffff;
-#pragma unroll
-        for (int r = 0; r < 8; ++r)
-            if (r < ctas) {
-                const float x_r = __uint_as_float(all[r].x);
-                const float w = x_r == m ? 1.0f : exp2_approx(fmaxf(__fmul_rn(__fsub_rn(x_r, m), c), -3.0e38f));
-                total = __fmaf_rn(__uint_as_float(all[r].y), w, total);
-                if (x_r == m) f = min(f, (int)all[r].z);
-            }
-        first = m == -INFINITY ? -1 : f;
-        factor = __fdiv_rn(top == m ? 1.0f : exp2_approx(fmaxf(__fmul_rn(__fsub_rn(top, m), c), -3.0e38f)), total);
-    } else {
-        if (nothing) first = -1;
-        factor = __fdiv_rn(1.0f, sum);
-    }
-    auto store = [&](int j, float* w) {
-        const int e = j * VE - skew;
-        if (j >= j1) return;
-#pragma unroll
-        for (int k = 0; k < VE; ++k) w[k] = hot ? (e + k == first ? 1.0f : 0.0f) : nothing ? 0.0f : __fmul_rn(w[k], factor);
-        if (wide && j >= ja && j < jb) {
-#pragma unroll
-            for (int k = 0; k < VE; k += 4) *reinterpret_cast<float4*>(out + e + k) = make_float4(w[k], w[k + 1], w[k + 2], w[k + 3]);
-        } else {
-#pragma unroll
-            for (int k = 0; k < VE; ++k)
-                if (e + k >= 0 && e + k < p.vocab) out[e + k] = w[k];
-        }
-    };
-#pragma unroll
-    for (int i = 0; i < NV; ++i) store(j0 + tid + i * THREADS, v + i * VE);
-    if (!HELD)
-        for (int j = j0 + tid + NV * THREADS; j < j1; j += THREADS) {
-            float w[VE];
-            values(raw(j), j, w);
-#pragma unroll
-            for (int k = 0; k < VE; ++k) w[k] = hot || nothing ? 0.0f : weight(w[k]);
+        for (int i = 0; i < NV; ++i) store(me + i * THREADS, v + i * VE);
+        rest([&](int j, float* w) {
+            if (plain) weigh(w, No());
+            else if (!hot && !nothing) weigh(w, Yes());
             store(j, w);
-        }
-    if (ctas > 1) tc::cluster_wait();                        // nobody leaves while its numbers are read
+        });
+        if (!STAGED) break;                                  // a cluster for each row
+    }
 }
 
 // ------------------------------------------------------------------------------------------------ verification
@@ -457,6 +542,11 @@ verify_drafts_kernel(VerifyParams a) {
     if (ctas > 1) tc::cluster_wait();                        // nobody leaves while its sum is read
 }
 
+static int* status_word() {
+    static PerDevicePointer status;
+    return status.get(gemm_status_device_ptr);
+}
+
 template <typename P>
 static int launch(void (*kernel)(P), const P& p, unsigned ctas, unsigned rows, unsigned threads, cudaStream_t stream) {
     cudaLaunchConfig_t cfg = {};
@@ -476,6 +566,42 @@ static int launch(void (*kernel)(P), const P& p, unsigned ctas, unsigned rows, u
     return e == cudaSuccess ? FRT_OK : FRT_CUDA_ERR(e);
 }
 
+// Form 2.  Clusters that the device holds at once: asked once per device and cluster size.
+template <int NV, bool F32>
+static int launch_staying(SoftmaxParams p, int rows, cudaStream_t st) {
+    constexpr int THREADS = 512, SMEM = THREADS * NV * 16;
+    static int known[64][4] = {};
+    const int c = p.ctas == 8 ? 3 : p.ctas / 2;
+    auto kernel = softmax_rows_kernel<THREADS, NV, F32, STAY>;
+    cudaLaunchConfig_t cfg = {};
+    cfg.blockDim = dim3(THREADS);
+    cfg.dynamicSmemBytes = SMEM;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = p.ctas;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return FRT_ERR_UNSUPPORTED;
+    if (!known[dev][c]) {
+        int n = 0;
+        cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
+        cfg.gridDim = dim3(p.ctas);
+        cfg.numAttrs = 1;
+        if (e == cudaSuccess) e = cudaOccupancyMaxActiveClusters(&n, kernel, &cfg);
+        if (e != cudaSuccess) return FRT_CUDA_ERR(e);
+        known[dev][c] = n > 0 ? n : 1;
+    }
+    cfg.gridDim = dim3(p.ctas * (unsigned)(rows < known[dev][c] ? rows : known[dev][c]));
+    cfg.numAttrs = 2;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, p);
+    return e == cudaSuccess ? FRT_OK : FRT_CUDA_ERR(e);
+}
+
 template <bool F32>
 static int launch_softmax(SoftmaxParams p, int rows, cudaStream_t st) {
     constexpr int N16 = F32 ? 4 : 2, VE = F32 ? 4 : 8;       // vectors of 16 values; values of a vector
@@ -485,11 +611,18 @@ static int launch_softmax(SoftmaxParams p, int rows, cudaStream_t st) {
     p.ctas = ctas;
     const bool aligned = ((reinterpret_cast<uintptr_t>(p.x) | (uintptr_t)(p.in_stride * (16 / VE))) & 15) == 0;
     const int vectors = (p.vocab + (aligned ? 0 : VE - 1) + VE - 1) / VE, each = (vectors + ctas - 1) / ctas;
-    if (each <= N16 * 128) return launch(softmax_rows_kernel<128, N16, F32, true>, p, ctas, rows, 128, st);
-    if (each <= N16 * 512) return launch(softmax_rows_kernel<512, N16, F32, true>, p, ctas, rows, 512, st);
-    if (each <= 2 * N16 * 512) return launch(softmax_rows_kernel<512, 2 * N16, F32, true>, p, ctas, rows, 512, st);
-    if (each <= 4 * N16 * 512) return launch(softmax_rows_kernel<512, 4 * N16, F32, true>, p, ctas, rows, 512, st);
-    return launch(softmax_rows_kernel<512, 2 * N16, F32, false>, p, ctas, rows, 512, st);
+    const bool few = (long long)rows * ctas <= 2 * device_sm_count();
+    if (few && each <= N16 * 512) return launch(softmax_rows_kernel<512, N16, F32, ONE_ROW>, p, ctas, rows, 512, st);
+    if (each <= 2 * N16 * 64) return launch(softmax_rows_kernel<64, 2 * N16, F32, ONE_ROW>, p, ctas, rows, 64, st);
+    if (each <= 2 * N16 * 128) return launch(softmax_rows_kernel<128, 2 * N16, F32, ONE_ROW>, p, ctas, rows, 128, st);
+    if (each <= 2 * N16 * 256) return launch(softmax_rows_kernel<256, 2 * N16, F32, ONE_ROW>, p, ctas, rows, 256, st);
+    if (each <= 2 * N16 * 512) {
+        if (few || ctas == 1) return launch(softmax_rows_kernel<512, 2 * N16, F32, ONE_ROW>, p, ctas, rows, 512, st);
+        return launch_staying<2 * N16, F32>(p, rows, st);
+    }
+    // a little more (a row that starts inside a vector has one more of them) is read twice rather than held by half as many CTAs
+    if (each > 2 * N16 * 640 && each <= 4 * N16 * 512) return launch_staying<4 * N16, F32>(p, rows, st);
+    return launch(softmax_rows_kernel<512, 2 * N16, F32, READ_TWICE>, p, ctas, rows, 512, st);
 }
 
 }  // namespace smp
@@ -505,7 +638,8 @@ extern "C" int frt_b200_softmax_rows(const void* in, long long in_stride, float*
     if (rows == 0 || vocab == 0) return FRT_OK;
     const bool f32 = flags & 2;
     if (!in || !out || misaligned(in, f32 ? 4 : 2) || misaligned(out, 4) || misaligned(temperature, 4)) return FRT_ERR_INVALID;
-    const smp::SoftmaxParams p = {in, out, temperature, in_stride, out_stride, vocab, 1};
+    smp::SoftmaxParams p = {in, out, temperature, in_stride, out_stride, rows, vocab, 1, smp::status_word()};
+    if (!p.status) return FRT_ERR_UNSUPPORTED;
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
     return f32 ? smp::launch_softmax<true>(p, rows, st) : smp::launch_softmax<false>(p, rows, st);
 }
