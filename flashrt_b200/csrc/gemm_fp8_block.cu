@@ -93,6 +93,7 @@ struct Params {
     int early;                   // the weights may be read before the kernel in front has ended
     int gm;                      // tile kernel: m-tiles of a group
     int f32;                     // out is fp32
+    int tma;                     // tile kernel: rows of D start at 16 bytes
 };
 enum { ERR_PRODUCER = 1, ERR_MMA = 2, ERR_EPILOGUE = 3 };
 
@@ -162,12 +163,25 @@ __device__ __forceinline__ float4 lds_v4(uint32_t a) {
     asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(a) : "memory");
     return v;
 }
+// four bytes from global to shared memory without a register between: nothing waits for them but cp.async.wait_group; absent ones are zero
+__device__ __forceinline__ void copy_4(uint32_t dst, const float* src, bool in) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(in ? 4 : 0) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+// 8 columns of this thread's TMEM lane
+__device__ __forceinline__ void tmem_ld8(uint32_t taddr, uint32_t* v) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]) : "r"(taddr) : "memory");
+}
 __device__ __forceinline__ void store_one(const Params& p, size_t at, float v) {
     if (p.f32) static_cast<float*>(p.out)[at] = v;
     else static_cast<__nv_bfloat16*>(p.out)[at] = __float2bfloat16_rn(v);
 }
 
 // ---------------------------------------------------------------- up to 64 rows: weights on the lanes, tokens on the columns
+constexpr int LANE_SCALES = 4;
 template <int BN>
 struct LaneCfg {
     static constexpr int A_BYTES = 128 * 128, B_BYTES = BN * 128, STAGE_BYTES = A_BYTES + B_BYTES;
@@ -175,7 +189,8 @@ struct LaneCfg {
     static constexpr int BUFS = BN == 64 ? 4 : 8;                            // accumulators: k-blocks under way
     static constexpr int RED_BYTES = 128 * BN * 4;                           // a rank's partial, where the ring was
     static_assert(RED_BYTES <= STAGES * STAGE_BYTES, "partials in the ring");
-    static constexpr int SCALE_BYTES = 4 * 2 * BN * 4;                       // of each epilogue warp, two k-blocks
+    static constexpr int SLOT_BYTES = BN * 4 + 16;                            // a k-block's scales: tokens, weights
+    static constexpr int SCALE_BYTES = 4 * LANE_SCALES * SLOT_BYTES;         // of each epilogue warp
     static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + 1024 + 256 + SCALE_BYTES;
     static constexpr int TMEM_COLS = BUFS * BN;
 };
@@ -292,7 +307,7 @@ gemm_fp8_block_lane_kernel(const __grid_constant__ CUtensorMap tmA, const __grid
         pdl_wait();
         const int q = warp & 3;
         const uint32_t t_src = tmem + ((uint32_t)(q * 32) << 16);
-        const uint32_t sc = tc::smem_u32(scales) + (warp - 2) * (2 * BN * 4);
+        const uint32_t sc = tc::smem_u32(scales) + (warp - 2) * (LANE_SCALES * Cfg::SLOT_BYTES);
         constexpr int PER = (BN + 31) / 32;                    // scales of a lane
         int buf = 0;
         uint32_t bph = 0;
@@ -303,27 +318,27 @@ gemm_fp8_block_lane_kernel(const __grid_constant__ CUtensorMap tmA, const __grid
             float acc[BN];
 #pragma unroll
             for (int j = 0; j < BN; ++j) acc[j] = 0.0f;
-            // scales of a k-block are asked for two blocks ahead and lie in the warp's own shared memory, token by token
-            auto ask = [&](int kb, float (&r)[PER]) {
-                const float w = kb < kb1 ? p.w_scale[(size_t)t * p.kb + kb] : 0.0f;
+            // scales of a k-block come LANE_SCALES - 1 blocks ahead into the warp's own shared memory, token by token, the weights' behind them
+            auto ask = [&](int kb) {
+                if (kb < kb1) {
+                    const uint32_t to = sc + (kb % LANE_SCALES) * Cfg::SLOT_BYTES;
 #pragma unroll
-                for (int i = 0; i < PER; ++i) {
-                    const int m = lane + 32 * i;
-                    r[i] = kb < kb1 && m < p.M ? __fmul_rn(p.a_scale[kb * p.a_stride + m], w) : 0.0f;
+                    for (int i = 0; i < PER; ++i) {
+                        const int m = lane + 32 * i;
+                        if (BN >= 32 || lane < BN) copy_4(to + m * 4, p.a_scale + (m < p.M ? kb * p.a_stride + m : 0), m < p.M);
+                    }
+                    if (lane == 0) copy_4(to + BN * 4, p.w_scale + (size_t)t * p.kb + kb, true);
                 }
+                copy_commit();
             };
-            float next[PER], later[PER];
-            ask(kb0, next);
-            ask(kb0 + 1, later);
+            for (int i = 0; i < LANE_SCALES - 1; ++i) ask(kb0 + i);
             for (int kb = kb0; kb < kb1; ++kb) {
-                const uint32_t slot = sc + (kb & 1) * (BN * 4);
-#pragma unroll
-                for (int i = 0; i < PER; ++i)
-                    if (BN >= 32 || lane < BN)
-                        asm volatile("st.shared.f32 [%0], %1;" ::"r"(slot + (lane + 32 * i) * 4), "f"(next[i]) : "memory");
-#pragma unroll
-                for (int i = 0; i < PER; ++i) next[i] = later[i];
-                ask(kb + 2, later);
+                const uint32_t slot = sc + (kb % LANE_SCALES) * Cfg::SLOT_BYTES;
+                ask(kb + LANE_SCALES - 1);
+                copy_wait<LANE_SCALES - 1>();
+                __syncwarp();
+                float w_s;
+                asm volatile("ld.shared.f32 %0, [%1];" : "=f"(w_s) : "r"(slot + BN * 4) : "memory");
                 ok = tc::warp_wait(tc::smem_u32(&acc_full[buf]), bph, false, deadline, abort_flag);
                 if (!ok) {
                     if (lane == 0) gave_up(p.status, abort_flag, ERR_EPILOGUE);
@@ -340,10 +355,10 @@ gemm_fp8_block_lane_kernel(const __grid_constant__ CUtensorMap tmA, const __grid
 #pragma unroll
                     for (int j = 0; j < 16; j += 4) {
                         const float4 f = lds_v4(slot + (c + j) * 4);
-                        acc[c + j] = __fmaf_rn(__uint_as_float(v[j]), f.x, acc[c + j]);
-                        acc[c + j + 1] = __fmaf_rn(__uint_as_float(v[j + 1]), f.y, acc[c + j + 1]);
-                        acc[c + j + 2] = __fmaf_rn(__uint_as_float(v[j + 2]), f.z, acc[c + j + 2]);
-                        acc[c + j + 3] = __fmaf_rn(__uint_as_float(v[j + 3]), f.w, acc[c + j + 3]);
+                        acc[c + j] = __fmaf_rn(__uint_as_float(v[j]), __fmul_rn(f.x, w_s), acc[c + j]);
+                        acc[c + j + 1] = __fmaf_rn(__uint_as_float(v[j + 1]), __fmul_rn(f.y, w_s), acc[c + j + 1]);
+                        acc[c + j + 2] = __fmaf_rn(__uint_as_float(v[j + 2]), __fmul_rn(f.z, w_s), acc[c + j + 2]);
+                        acc[c + j + 3] = __fmaf_rn(__uint_as_float(v[j + 3]), __fmul_rn(f.w, w_s), acc[c + j + 3]);
                     }
                 }
                 tc::tc_fence_before_sync();
@@ -351,6 +366,8 @@ gemm_fp8_block_lane_kernel(const __grid_constant__ CUtensorMap tmA, const __grid
                 if (lane == 0) tc::mbar_arrive(&acc_empty[buf]);
                 if (++buf == BUFS) { buf = 0; bph ^= 1; }
             }
+            copy_wait<0>();
+            __syncwarp();                                      // the next tile's scales go to the same place
             if (!ok) break;
             if (S > 1) {                                       // [four tokens][channel]: a warp's store is 512 contiguous bytes
                 const uint32_t red = tc::smem_u32(smem) + (uint32_t)(q * 32 + lane) * 16;
@@ -405,13 +422,15 @@ gemm_fp8_block_lane_kernel(const __grid_constant__ CUtensorMap tmA, const __grid
 }
 
 // ---------------------------------------------------------------- more rows: tokens on the rows, tiles of 128 CG x BN
+constexpr int SCALE_SLOT = 520;       // a buffer's scales: 128 rows, two blocks of weights
 template <int CG, int BN>
 struct TileCfg {
     static constexpr int A_BYTES = 128 * 128, B_BYTES = BN / CG * 128, STAGE_BYTES = A_BYTES + B_BYTES;  // per CTA
-    static constexpr int EPI_BYTES = 8 * 32 * 128;           // 32 rows x 32 fp32 columns of each epilogue warp
-    static constexpr int STAGES = (227 * 1024 - 1024 - 256 - EPI_BYTES) / STAGE_BYTES > 8 ? 8 : (227 * 1024 - 1024 - 256 - EPI_BYTES) / STAGE_BYTES;
-    static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + 1024 + 256 + EPI_BYTES;
+    static constexpr int OUT_BYTES = 32 * BN;                // of each epilogue warp: 32 rows of its half of the columns in bf16
     static constexpr int BUFS = 512 / BN;                    // accumulators: k-blocks under way
+    static constexpr int REST = 1024 + 256 + 8 * OUT_BYTES + BUFS * SCALE_SLOT;
+    static constexpr int STAGES = (227 * 1024 - REST) / STAGE_BYTES > 8 ? 8 : (227 * 1024 - REST) / STAGE_BYTES;
+    static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + REST;
 };
 
 // Tiles in groups of gm m-tiles, m fastest inside a group: the CTAs of a wave then share operand rows in L2.
@@ -419,6 +438,63 @@ __device__ __forceinline__ void tile_at(int t, int gm, int m_tiles, int n_tiles,
     const int per = gm * n_tiles, g = t / per, r = t - g * per, h = min(m_tiles - g * gm, gm);
     n = r / h;
     m = g * gm + (r - n * h);
+}
+
+// 128 bytes x 32 rows of shared memory (128-byte swizzle) to the output, what lies outside it is left out; x in bytes
+__device__ __forceinline__ void store_box(const CUtensorMap* m, uint32_t src, int x, int y) {
+    asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];" ::"l"(m), "r"(src), "r"(x), "r"(y) : "memory");
+}
+// A warp's 32 rows of W columns from registers, a thread holds a row: through its own shared memory to the output by TMA, which goes on while
+// the next tile is summed (all SMs reach the ends of their tiles together, and with the stores in the way of the sums 8192 x 8192 x 8192 took
+// 4 us a tile more).
+template <int W>
+__device__ __forceinline__ void store_rows(const Params& p, const CUtensorMap* tmD, const float* acc, int m_base, int nb, uint32_t stg) {
+    const int lane = threadIdx.x & 31;
+    const uint32_t row = stg + lane * 128, sw = (uint32_t)(lane & 7) << 4;
+    const bool wide = p.f32 != 0;
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {                   // fp32: W / 2 columns fill the warp's place, bf16: at the end
+        if (half == 0 || wide) {
+            if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+            __syncwarp();
+        }
+#pragma unroll
+        for (int c = half * (W / 2); c < (half + 1) * (W / 2); c += 8) {
+            float f[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) f[j] = acc[c + j];
+            if (p.bias) {
+                uint4 b = make_uint4(0, 0, 0, 0);
+                if (nb + c < p.N) b = ld_global_v4(p.bias + nb + c);         // N % 8 == 0
+                const uint32_t* w = &b.x;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    float x, y;
+                    unpack_bf16x2(w[j], x, y);
+                    f[2 * j] = __fadd_rn(f[2 * j], x);
+                    f[2 * j + 1] = __fadd_rn(f[2 * j + 1], y);
+                }
+            }
+            if (wide) {
+                const uint32_t at = row + (c - half * (W / 2)) / 32 * 4096, k = (uint32_t)(c % 32) * 4;
+                sts_v4(at + (k ^ sw), f[0], f[1], f[2], f[3]);
+                sts_v4(at + ((k + 16) ^ sw), f[4], f[5], f[6], f[7]);
+            } else {
+                asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(row + c / 64 * 4096 + (((uint32_t)(c % 64) * 2) ^ sw)), "r"(pack_bf16x2(f[0], f[1])),
+                             "r"(pack_bf16x2(f[2], f[3])), "r"(pack_bf16x2(f[4], f[5])), "r"(pack_bf16x2(f[6], f[7])) : "memory");
+            }
+        }
+        if (half == 1 || wide) {
+            tc::fence_proxy_async_smem();
+            __syncwarp();
+            const int n0 = wide ? nb + half * (W / 2) : nb, per = wide ? 32 : 64, boxes = (wide ? W / 2 : W) / per;
+            if (lane == 0 && m_base < p.M) {
+                for (int i = 0; i < boxes; ++i)
+                    if (n0 + i * per < p.N) store_box(tmD, stg + i * 4096, (n0 + i * per) * (wide ? 4 : 2), m_base);
+                asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+            }
+        }
+    }
 }
 
 // 32 rows x 32 columns of a tile, a thread holds a row: through shared memory (16-byte chunks of a 128-byte row, chunk index xor row % 8) to
@@ -471,21 +547,25 @@ __device__ __forceinline__ void store_block(const Params& p, const float* f, int
 // CG = 2: a CTA pair has a tile of 256 rows, each CTA stages its 128 rows of A and half of the weight rows.  S > 1: a cluster of S such
 // takes one tile, unit s the k-blocks [kb s / S, kb (s + 1) / S); they then lay their partials into shared memory, where their rings were,
 // and each finishes BN / S of the columns.
+constexpr int TILE_THREADS = 384;     // producer, issuer, scales, an idle warp; eight for the epilogue
 template <int CG, int BN, int S>
-__global__ void __launch_bounds__(320, 1)
-gemm_fp8_block_tile_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmW, Params p) {
+__global__ void __launch_bounds__(TILE_THREADS, 1)
+gemm_fp8_block_tile_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmD, Params p) {
     using Cfg = TileCfg<CG, BN>;
     constexpr int STAGES = Cfg::STAGES, BUFS = Cfg::BUFS, W2 = BN / 2;
     static_assert(S == 1 || (BN / S >= 64 && 128 * BN * 4 <= STAGES * Cfg::STAGE_BYTES), "columns of a half of the warps, partials in the ring");
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-    uint64_t* full = reinterpret_cast<uint64_t*>(smem + STAGES * Cfg::STAGE_BYTES);   // the leader's count both CTAs' bytes
+    uint8_t* outs = smem + STAGES * Cfg::STAGE_BYTES;        // 1024-byte boundaries, for the swizzle of the stores
+    uint64_t* full = reinterpret_cast<uint64_t*>(outs + 8 * Cfg::OUT_BYTES);   // the leader's count both CTAs' bytes
     uint64_t* empty = full + STAGES;
     uint64_t* acc_full = empty + STAGES;       // [BUFS]
     uint64_t* acc_empty = acc_full + BUFS;     // [BUFS] the leader's
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + BUFS);
+    uint64_t* scale_empty = acc_empty + BUFS;  // [BUFS]
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(scale_empty + BUFS);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-    static_assert((2 * STAGES + 2 * BUFS) * 8 + 8 <= 256, "barriers");
+    static_assert((2 * STAGES + 3 * BUFS) * 8 + 8 <= 256, "barriers");
+    const uint32_t scale_a = tc::smem_u32(outs + 8 * Cfg::OUT_BYTES + 256);
     const uint64_t deadline = tc::global_timer_ns() + FRT_KERNEL_DEADLINE_NS;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t cluster_rank = CG * S > 1 ? tc::cluster_ctarank() : 0u, rank = cluster_rank % CG, leader = cluster_rank - rank;
@@ -500,7 +580,8 @@ gemm_fp8_block_tile_kernel(const __grid_constant__ CUtensorMap tmA, const __grid
             tc::mbar_init(&empty[s], 1);
         }
         for (int i = 0; i < BUFS; ++i) {
-            tc::mbar_init(&acc_full[i], 1);
+            tc::mbar_init(&acc_full[i], 2);                  // the products, the scales
+            tc::mbar_init(&scale_empty[i], 8);
             tc::mbar_init(&acc_empty[i], CG * 8);
         }
         *abort_flag = 0;
@@ -553,79 +634,132 @@ gemm_fp8_block_tile_kernel(const __grid_constant__ CUtensorMap tmA, const __grid
         const uint32_t accF_a = tc::smem_u32(acc_full), accE_a = tc::smem_u32(acc_empty);
         int s = 0, buf = 0;
         uint32_t ph = 0, bph = 1;                            // the first round of the buffers is empty
-        bool ready = false;
-        for (int t = unit; t < total; t += units)
+        bool ready = false, failed = false;
+        for (int t = unit; t < total && !failed; t += units)
             for (int kb = kb0; kb < kb1; ++kb) {
-                if (!tc::warp_wait(accE_a + 8 * buf, bph, false, deadline, abort_flag) ||
-                    !tc::warp_wait(full_a + 8 * s, ph, ready, deadline, abort_flag)) {
+                if (!tc::warp_wait(full_a + 8 * s, ph, ready, deadline, abort_flag)) {
                     if (lane == 0) gave_up(p.status, abort_flag, ERR_MMA);
-                    t = total;
+                    failed = true;
+                    break;
+                }
+                const uint64_t so = (uint64_t)(s * (Cfg::STAGE_BYTES >> 4));
+                const uint32_t done = empty_a + 8 * s;
+                if (++s == STAGES) { s = 0; ph ^= 1; }
+                if (!tc::warp_wait(accE_a + 8 * buf, bph, false, deadline, abort_flag)) {
+                    if (lane == 0) gave_up(p.status, abort_flag, ERR_MMA);
+                    failed = true;
                     break;
                 }
                 tc::tc_fence_after_sync();
-                const uint64_t so = (uint64_t)(s * (Cfg::STAGE_BYTES >> 4));
-                const uint32_t done = empty_a + 8 * s, d_tm = tmem + buf * BN, there = accF_a + 8 * buf;
-                if (++s == STAGES) { s = 0; ph ^= 1; }
+                const uint32_t d_tm = tmem + buf * BN, there = accF_a + 8 * buf;
                 if (++buf == BUFS) { buf = 0; bph ^= 1; }
                 ready = tc::mbar_test(full_a + 8 * s, ph);
                 if (tc::elect_one()) {
 #pragma unroll
                     for (int k = 0; k < 4; ++k) mma<CG>(d_tm, dA0 + so + 2 * k, dB0 + so + 2 * k, idesc, k > 0 ? 1u : 0u);
-                    commit<CG>(done, leader);
                     commit<CG>(there, leader);
+                    commit<CG>(done, leader);
                 }
             }
-    } else if (warp >= 2) {
-        // ---------------- epilogue: this CTA's 128 rows; a warp's lane quadrant and half of the columns
+    } else if (warp == 2) {
+        // ---------------- scales of this CTA's rows and of the tile's two blocks of weights, a buffer's beside it.  Loads of the block after
+        // next are under way while one is handed over; whoever takes them from a register that a loop moves on waits for them a block earlier.
         pdl_wait();
-        const int q = warp & 3, half = (warp - 2) >> 2;
-        const uint32_t t_src = tmem + ((uint32_t)(q * 32) << 16) + half * W2;
-        const bool vec = (p.N & 3) == 0;
-        uint8_t* stg = smem + STAGES * Cfg::STAGE_BYTES + 256 + (warp - 2) * (32 * 128);
+        struct Scales { float a[4], w; };
+        int buf = 0;
+        uint32_t bph = 1;
+        bool ok = true;
+        for (int t = unit; t < total && ok; t += units) {
+            int mt, nt;
+            tile_at(t, p.gm, m_tiles, n_tiles, mt, nt);
+            const int m_base = (mt * CG + (int)rank) * 128 + lane;
+            const float* ws = p.w_scale + (size_t)(min(nt * BN + (lane & 1) * W2, p.N - 1) / 128) * p.kb;
+            auto ask = [&](int kb, Scales& r) {
+                if (kb >= kb1) return;
+                r.w = ws[kb];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) r.a[i] = m_base + 32 * i < p.M ? p.a_scale[kb * p.a_stride + m_base + 32 * i] : 0.0f;
+            };
+            auto give = [&](const Scales& r) {
+                ok = tc::warp_wait(tc::smem_u32(&scale_empty[buf]), bph, false, deadline, abort_flag);
+                if (!ok) {
+                    if (lane == 0) gave_up(p.status, abort_flag, ERR_EPILOGUE);
+                    return;
+                }
+                const uint32_t to = scale_a + buf * SCALE_SLOT;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) asm volatile("st.shared.f32 [%0], %1;" ::"r"(to + (lane + 32 * i) * 4), "f"(r.a[i]) : "memory");
+                if (lane < 2) asm volatile("st.shared.f32 [%0], %1;" ::"r"(to + 512 + lane * 4), "f"(r.w) : "memory");
+                __syncwarp();
+                if (lane == 0) tc::mbar_arrive(&acc_full[buf]);
+                if (++buf == BUFS) { buf = 0; bph ^= 1; }
+            };
+            Scales r[4] = {};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) ask(kb0 + i, r[i]);
+            for (int kb = kb0; kb < kb1 && ok; kb += 4)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (kb + i < kb1 && ok) {
+                        give(r[i]);
+                        ask(kb + i + 4, r[i]);
+                    }
+        }
+    } else if (warp >= 4) {
+        // ---------------- epilogue: this CTA's 128 rows; a warp's lane quadrant and half of the columns
+        
+        pdl_wait();
+        const int q = warp & 3, half = (warp - 4) >> 2;
+        const uint32_t t_src = tmem + ((uint32_t)(q * 32) << 16);
+        uint8_t* stg = outs + (warp - 4) * Cfg::OUT_BYTES;
         const uint32_t accF_a = tc::smem_u32(acc_full), accE_a = tc::smem_u32(acc_empty);
         const uint32_t accE_lead = CG == 1 ? accE_a : tc::dsmem_map(accE_a, leader);
-        const int n_blocks = (p.N + 127) / 128;
-        int buf = 0;
+                int buf = 0;
         uint32_t bph = 0;
         for (int t = unit; t < total; t += units) {
             int mt, nt;
             tile_at(t, p.gm, m_tiles, n_tiles, mt, nt);
             const int m_base = (mt * CG + (int)rank) * 128 + q * 32, n_base = nt * BN + half * W2;
-            const bool in = m_base + lane < p.M;
-            const float* ws = p.w_scale + (size_t)min(n_base / 128, n_blocks - 1) * p.kb;
-            const float* as = p.a_scale + (in ? m_base + lane : 0);
-            auto ask = [&](int kb) { return in && kb < kb1 ? __fmul_rn(as[kb * p.a_stride], ws[kb]) : 0.0f; };
-            float acc[W2], now = ask(kb0), next = ask(kb0 + 1);
+            float acc[W2];
 #pragma unroll
             for (int j = 0; j < W2; ++j) acc[j] = 0.0f;
             bool ok = true;
             for (int kb = kb0; kb < kb1; ++kb) {
-                const float s = now;
-                now = next;
-                next = ask(kb + 2);
                 ok = tc::warp_wait(accF_a + 8 * buf, bph, false, deadline, abort_flag);
                 if (!ok) {
                     if (lane == 0) gave_up(p.status, abort_flag, ERR_EPILOGUE);
                     break;
                 }
                 tc::tc_fence_after_sync();
+                // 32 columns on their way from tensor memory while the 32 in front are added
+                float a, w_s;
+                asm volatile("ld.shared.f32 %0, [%1];" : "=f"(a) : "r"(scale_a + buf * SCALE_SLOT + (q * 32 + lane) * 4) : "memory");
+                asm volatile("ld.shared.f32 %0, [%1];" : "=f"(w_s) : "r"(scale_a + buf * SCALE_SLOT + 512 + half * 4) : "memory");
+                const float s = __fmul_rn(a, w_s);
                 const uint64_t s2 = f32x2(s, s);
+                const uint32_t src = t_src + buf * BN + half * W2;
+                uint32_t v[2][8];
+                tmem_ld8(src, v[0]);
 #pragma unroll
-                for (int c = 0; c < W2; c += 16) {
-                    uint32_t v[16];
-                    tc::tmem_ld16(t_src + buf * BN + c, v);
+                for (int c = 0; c < W2; c += 8) {
                     tc::tmem_ld_wait();
+                    if (c + 8 < W2) {
+                        tmem_ld8(src + c + 8, v[(c / 8 + 1) & 1]);
+                    } else {                                 // all is taken: the buffer may be filled again
+                        tc::tc_fence_before_sync();
+                        __syncwarp();
+                        if (lane == 0) {
+                            if constexpr (CG == 1) tc::mbar_arrive(&acc_empty[buf]);
+                            else tc::mbar_arrive_cluster(accE_lead + 8 * buf);
+                            tc::mbar_arrive(&scale_empty[buf]);
+                        }
+                    }
+                    const uint32_t* w = v[(c / 8) & 1];
 #pragma unroll
-                    for (int j = 0; j < 16; j += 2) {
-                        const uint64_t r = fma_f32x2(f32x2(__uint_as_float(v[j]), __uint_as_float(v[j + 1])), s2, f32x2(acc[c + j], acc[c + j + 1]));
+                    for (int j = 0; j < 8; j += 2) {
+                        const uint64_t r = fma_f32x2(f32x2(__uint_as_float(w[j]), __uint_as_float(w[j + 1])), s2, f32x2(acc[c + j], acc[c + j + 1]));
                         f32x2_parts(r, acc[c + j], acc[c + j + 1]);
                     }
-                }
-                tc::tc_fence_before_sync();
-                __syncwarp();
-                if (lane == 0) {
-                    if constexpr (CG == 1) tc::mbar_arrive(&acc_empty[buf]);
-                    else tc::mbar_arrive_cluster(accE_lead + 8 * buf);
                 }
                 if (++buf == BUFS) { buf = 0; bph ^= 1; }
             }
@@ -636,22 +770,24 @@ gemm_fp8_block_tile_kernel(const __grid_constant__ CUtensorMap tmA, const __grid
                 for (int j = 0; j < W2; j += 4) sts_v4(red + j * 512, acc[j], acc[j + 1], acc[j + 2], acc[j + 3]);
                 break;
             } else {
+                if (p.tma) store_rows<W2>(p, &tmD, acc, m_base, n_base, tc::smem_u32(stg));
+                else
 #pragma unroll
-                for (int c = 0; c < W2; c += 32)
-                    if (m_base < p.M && n_base + c < p.N) store_block(p, acc + c, m_base, n_base + c, stg, vec);
+                    for (int c = 0; c < W2; c += 32)
+                        if (m_base < p.M && n_base + c < p.N) store_block(p, acc + c, m_base, n_base + c, stg, false);
             }
         }
     }
     if constexpr (S > 1) {
         __syncwarp();
         tc::cluster_sync_all();                // all partials are there
-        if (warp >= 2 && !*abort_flag) {
+        if (warp >= 4 && !*abort_flag) {
             constexpr int W = BN / S / 2;      // columns of this warp
-            const int q = warp & 3, half = (warp - 2) >> 2, col = split * (BN / S) + half * W;
+            const int q = warp & 3, half = (warp - 4) >> 2, col = split * (BN / S) + half * W;
             int mt, nt;
             tile_at(unit, p.gm, m_tiles, n_tiles, mt, nt);
             const int m_base = (mt * CG + (int)rank) * 128 + q * 32, n_base = nt * BN + col;
-            uint8_t* stg = smem + STAGES * Cfg::STAGE_BYTES + 256 + (warp - 2) * (32 * 128);
+            uint8_t* stg = outs + (warp - 4) * Cfg::OUT_BYTES;
             const uint32_t red = tc::smem_u32(smem) + (uint32_t)(col / 4 * 128 + q * 32 + lane) * 16;
 #pragma unroll 1
             for (int c = 0; c < W; c += 32) {
@@ -677,6 +813,7 @@ gemm_fp8_block_tile_kernel(const __grid_constant__ CUtensorMap tmA, const __grid
         }
     }
     if (*abort_flag && threadIdx.x == 0) let_copies_land();
+    if (warp >= 4 && lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
     __syncwarp();
     tc::tc_fence_before_sync();
     if constexpr (CG * S > 1) tc::cluster_sync_all();        // the leader's MMAs read the peer's shared memory until the end
@@ -727,7 +864,7 @@ template <int CG, int BN, int S>
 static int launch_tile(const void* A, const void* W, Params p, int K, cudaStream_t stream) {
     using Cfg = TileCfg<CG, BN>;
     static PerDeviceOnce once;
-    CUtensorMap tmA, tmW;
+    CUtensorMap tmA, tmW, tmD;
     int dev = 0;
     if (once.need(dev)) {
         const cudaError_t e = cudaFuncSetAttribute(gemm_fp8_block_tile_kernel<CG, BN, S>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::SMEM_BYTES);
@@ -736,6 +873,10 @@ static int launch_tile(const void* A, const void* W, Params p, int K, cudaStream
     }
     int rc = make_tmap_2d_u8(&tmA, A, (uint64_t)p.M, (uint64_t)K, (uint64_t)K, 128);
     if (!rc) rc = make_tmap_2d_u8(&tmW, W, (uint64_t)p.N, (uint64_t)K, (uint64_t)K, BN / CG);
+    const uint64_t out_row = (uint64_t)p.N * (p.f32 ? 4 : 2);
+    p.tma = p.N % 8 == 0 && (reinterpret_cast<uintptr_t>(p.bias) & 15) == 0;
+    if (!rc && p.tma) rc = make_tmap_2d_u8(&tmD, p.out, (uint64_t)p.M, out_row, out_row, 32);
+    if (!p.tma) tmD = tmA;
     if (rc) return rc;
     const int m_tiles = (p.M + 128 * CG - 1) / (128 * CG), n_tiles = (p.N + BN - 1) / BN, workers = device_sm_count() / CG;
     const long long total = (long long)m_tiles * n_tiles;
@@ -748,10 +889,10 @@ static int launch_tile(const void* A, const void* W, Params p, int K, cudaStream
     cudaLaunchConfig_t cfg = {};
     cudaLaunchAttribute attr[2];
     cfg.gridDim = dim3(CG * (S > 1 ? S * (unsigned)total : (unsigned)(total < workers ? total : workers)));
-    cfg.blockDim = dim3(320);
+    cfg.blockDim = dim3(TILE_THREADS);
     cfg.dynamicSmemBytes = Cfg::SMEM_BYTES;
     set_attrs(cfg, attr, CG * S, 1, stream);
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, gemm_fp8_block_tile_kernel<CG, BN, S>, tmA, tmW, p);
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, gemm_fp8_block_tile_kernel<CG, BN, S>, tmA, tmW, tmD, p);
     return e == cudaSuccess ? FRT_OK : FRT_CUDA_ERR(e);
 }
 
