@@ -175,6 +175,12 @@ __device__ __forceinline__ void tmem_ld8(uint32_t taddr, uint32_t* v) {
     asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
                  : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]) : "r"(taddr) : "memory");
 }
+template <int N>
+__device__ __forceinline__ void tmem_ld(uint32_t taddr, uint32_t* v) {
+    if constexpr (N == 8) tmem_ld8(taddr, v);
+    else if constexpr (N == 16) tc::tmem_ld16(taddr, v);
+    else tc::tmem_ld32(taddr, v);
+}
 __device__ __forceinline__ void store_one(const Params& p, size_t at, float v) {
     if (p.f32) static_cast<float*>(p.out)[at] = v;
     else static_cast<__nv_bfloat16*>(p.out)[at] = __float2bfloat16_rn(v);
@@ -272,6 +278,11 @@ gemm_fp8_block_lane_kernel(const __grid_constant__ CUtensorMap tmA, const __grid
                 if (++s == STAGES) { s = 0; ph ^= 1; }
             }
             skip = 0;
+        }
+        // the last stages' returns arrive in this CTA's shared memory too: not after it has gone to another
+        for (int i = 0; i < STAGES; ++i) {
+            if (!tc::warp_wait(empty_a + 8 * s, ph, false, deadline, abort_flag)) break;
+            if (++s == STAGES) { s = 0; ph ^= 1; }
         }
     } else if (warp == 1) {
         // ---------------- MMA issuer (whole warp): a k-block, a buffer
@@ -422,14 +433,19 @@ gemm_fp8_block_lane_kernel(const __grid_constant__ CUtensorMap tmA, const __grid
 }
 
 // ---------------------------------------------------------------- more rows: tokens on the rows, tiles of 128 CG x BN
-constexpr int SCALE_SLOT = 520;       // a buffer's scales: 128 rows, two blocks of weights
+constexpr int SCALE_SLOT = 528;       // a buffer's scales: 128 rows, two blocks of weights
 template <int CG, int BN>
 struct TileCfg {
     static constexpr int A_BYTES = 128 * 128, B_BYTES = BN / CG * 128, STAGE_BYTES = A_BYTES + B_BYTES;  // per CTA
     static constexpr int OUT_BYTES = 32 * BN;                // of each epilogue warp: 32 rows of its half of the columns in bf16
     static constexpr int BUFS = 512 / BN;                    // accumulators: k-blocks under way
     static constexpr int REST = 1024 + 256 + 8 * OUT_BYTES + BUFS * SCALE_SLOT;
-    static constexpr int STAGES = (227 * 1024 - REST) / STAGE_BYTES > 8 ? 8 : (227 * 1024 - REST) / STAGE_BYTES;
+    static constexpr int FIT = (227 * 1024 - REST) / STAGE_BYTES > 8 ? 8 : (227 * 1024 - REST) / STAGE_BYTES;
+    // With 128 columns the waits, four products and two commits of a k-block take a warp longer than the products: two issue, every other
+    // block each, with stages and buffers of their own -- of one that both wait for, who is a round ahead would take the phase before for its own.
+    static constexpr int ISSUERS = BN == 128 ? 2 : 1;
+    static constexpr int STAGES = FIT / ISSUERS * ISSUERS;
+    static_assert(BUFS % ISSUERS == 0, "buffers of an issuer");
     static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + REST;
 };
 
@@ -552,7 +568,7 @@ template <int CG, int BN, int S>
 __global__ void __launch_bounds__(TILE_THREADS, 1)
 gemm_fp8_block_tile_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmD, Params p) {
     using Cfg = TileCfg<CG, BN>;
-    constexpr int STAGES = Cfg::STAGES, BUFS = Cfg::BUFS, W2 = BN / 2;
+    constexpr int STAGES = Cfg::STAGES, BUFS = Cfg::BUFS, ISSUERS = Cfg::ISSUERS, W2 = BN / 2, LW = BN == 256 ? 8 : 16;
     static_assert(S == 1 || (BN / S >= 64 && 128 * BN * 4 <= STAGES * Cfg::STAGE_BYTES), "columns of a half of the warps, partials in the ring");
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
@@ -625,70 +641,71 @@ gemm_fp8_block_tile_kernel(const __grid_constant__ CUtensorMap tmA, const __grid
                 }
             }
         }
-    } else if (warp == 1 && rank == 0) {
-        // ---------------- MMA issuer for the tile: a k-block, a buffer
+        // the last stages' returns arrive in this CTA's shared memory too: not after it has gone to another
+        for (int i = 0; i < STAGES; ++i) {
+            if (!tc::warp_wait(empty_a + 8 * s, ph, false, deadline, abort_flag)) break;
+            if (++s == STAGES) { s = 0; ph ^= 1; }
+        }
+    } else if ((warp & 1) && warp < 2 * ISSUERS && rank == 0) {
+        // ---------------- MMA issuers for the tiles, warps 1 and (two issuers) 3: a k-block, a buffer
         constexpr uint32_t idesc = tc::make_idesc(0, 0, 0, 0, 128 * CG, BN);
         const uint64_t dA0 = tc::make_desc_kmajor_sw128(tc::smem_u32(smem));
         const uint64_t dB0 = tc::make_desc_kmajor_sw128(tc::smem_u32(smem + Cfg::A_BYTES));
         const uint32_t full_a = tc::smem_u32(full), empty_a = tc::smem_u32(empty);
         const uint32_t accF_a = tc::smem_u32(acc_full), accE_a = tc::smem_u32(acc_empty);
-        int s = 0, buf = 0;
+        const int mine = unit < total ? ((total - 1 - unit) / units + 1) * (kb1 - kb0) : 0;       // k-blocks of this unit's tiles
+        int s = warp >> 1, buf = warp >> 1;
         uint32_t ph = 0, bph = 1;                            // the first round of the buffers is empty
-        bool ready = false, failed = false;
-        for (int t = unit; t < total && !failed; t += units)
-            for (int kb = kb0; kb < kb1; ++kb) {
-                if (!tc::warp_wait(full_a + 8 * s, ph, ready, deadline, abort_flag)) {
-                    if (lane == 0) gave_up(p.status, abort_flag, ERR_MMA);
-                    failed = true;
-                    break;
-                }
-                const uint64_t so = (uint64_t)(s * (Cfg::STAGE_BYTES >> 4));
-                const uint32_t done = empty_a + 8 * s;
-                if (++s == STAGES) { s = 0; ph ^= 1; }
-                if (!tc::warp_wait(accE_a + 8 * buf, bph, false, deadline, abort_flag)) {
-                    if (lane == 0) gave_up(p.status, abort_flag, ERR_MMA);
-                    failed = true;
-                    break;
-                }
-                tc::tc_fence_after_sync();
-                const uint32_t d_tm = tmem + buf * BN, there = accF_a + 8 * buf;
-                if (++buf == BUFS) { buf = 0; bph ^= 1; }
-                ready = tc::mbar_test(full_a + 8 * s, ph);
-                if (tc::elect_one()) {
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) mma<CG>(d_tm, dA0 + so + 2 * k, dB0 + so + 2 * k, idesc, k > 0 ? 1u : 0u);
-                    commit<CG>(there, leader);
-                    commit<CG>(done, leader);
-                }
+        bool ready = false;
+        for (int i = warp >> 1; i < mine; i += ISSUERS) {
+            if (!tc::warp_wait(full_a + 8 * s, ph, ready, deadline, abort_flag) ||
+                !tc::warp_wait(accE_a + 8 * buf, bph, false, deadline, abort_flag)) {
+                if (lane == 0) gave_up(p.status, abort_flag, ERR_MMA);
+                break;
             }
+            tc::tc_fence_after_sync();
+            const uint64_t so = (uint64_t)(s * (Cfg::STAGE_BYTES >> 4));
+            const uint32_t done = empty_a + 8 * s, there = accF_a + 8 * buf, d_tm = tmem + buf * BN;
+            s += ISSUERS;
+            if (s >= STAGES) { s -= STAGES; ph ^= 1; }
+            buf += ISSUERS;
+            if (buf >= BUFS) { buf -= BUFS; bph ^= 1; }
+            ready = tc::mbar_test(full_a + 8 * s, ph);
+            if (tc::elect_one()) {
+#pragma unroll
+                for (int k = 0; k < 4; ++k) mma<CG>(d_tm, dA0 + so + 2 * k, dB0 + so + 2 * k, idesc, k > 0 ? 1u : 0u);
+                commit<CG>(done, leader);
+                commit<CG>(there, leader);
+            }
+        }
     } else if (warp == 2) {
-        // ---------------- scales of this CTA's rows and of the tile's two blocks of weights, a buffer's beside it.  Loads of the block after
-        // next are under way while one is handed over; whoever takes them from a register that a loop moves on waits for them a block earlier.
+        // ---------------- scales of this CTA's rows and of the tile's two blocks of weights, a buffer's beside it: a lane has four rows.  Four
+        // blocks' loads are under way; whoever takes them from a register that a loop moves on waits for them a block earlier.  Rows behind the
+        // last have its scale: what they make of it is not stored.
         pdl_wait();
         struct Scales { float a[4], w; };
         int buf = 0;
         uint32_t bph = 1;
-        bool ok = true;
-        for (int t = unit; t < total && ok; t += units) {
+        for (int t = unit; t < total; t += units) {
             int mt, nt;
             tile_at(t, p.gm, m_tiles, n_tiles, mt, nt);
-            const int m_base = (mt * CG + (int)rank) * 128 + lane;
-            const float* ws = p.w_scale + (size_t)(min(nt * BN + (lane & 1) * W2, p.N - 1) / 128) * p.kb;
-            auto ask = [&](int kb, Scales& r) {
-                if (kb >= kb1) return;
-                r.w = ws[kb];
+            const int m0 = (mt * CG + (int)rank) * 128 + 4 * lane;
+            int row[4];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) r.a[i] = m_base + 32 * i < p.M ? p.a_scale[kb * p.a_stride + m_base + 32 * i] : 0.0f;
+            for (int i = 0; i < 4; ++i) row[i] = min(m0 + i, p.M - 1);
+            const float* ws = p.w_scale + (size_t)(min(nt * BN + (lane & 1) * W2, p.N - 1) / 128) * p.kb + kb0;
+            const float* as = p.a_scale + kb0 * p.a_stride;
+            auto ask = [&](int kb, Scales& r) {              // block after block
+                if (kb >= kb1) return;
+                r.w = *ws++;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) r.a[i] = as[row[i]];
+                as += p.a_stride;
             };
             auto give = [&](const Scales& r) {
-                ok = tc::warp_wait(tc::smem_u32(&scale_empty[buf]), bph, false, deadline, abort_flag);
-                if (!ok) {
-                    if (lane == 0) gave_up(p.status, abort_flag, ERR_EPILOGUE);
-                    return;
-                }
+                if (!tc::mbar_wait_until(tc::smem_u32(&scale_empty[buf]), bph, deadline, abort_flag)) gave_up(p.status, abort_flag, ERR_EPILOGUE);
                 const uint32_t to = scale_a + buf * SCALE_SLOT;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) asm volatile("st.shared.f32 [%0], %1;" ::"r"(to + (lane + 32 * i) * 4), "f"(r.a[i]) : "memory");
+                sts_v4(to + lane * 16, r.a[0], r.a[1], r.a[2], r.a[3]);
                 if (lane < 2) asm volatile("st.shared.f32 [%0], %1;" ::"r"(to + 512 + lane * 4), "f"(r.w) : "memory");
                 __syncwarp();
                 if (lane == 0) tc::mbar_arrive(&acc_full[buf]);
@@ -697,13 +714,14 @@ gemm_fp8_block_tile_kernel(const __grid_constant__ CUtensorMap tmA, const __grid
             Scales r[4] = {};
 #pragma unroll
             for (int i = 0; i < 4; ++i) ask(kb0 + i, r[i]);
-            for (int kb = kb0; kb < kb1 && ok; kb += 4)
+            for (int kb = kb0; kb < kb1; kb += 4)
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
-                    if (kb + i < kb1 && ok) {
+                    if (kb + i < kb1) {
                         give(r[i]);
                         ask(kb + i + 4, r[i]);
                     }
+            if (__any_sync(0xffffffffu, *abort_flag != 0)) break;
         }
     } else if (warp >= 4) {
         // ---------------- epilogue: this CTA's 128 rows; a warp's lane quadrant and half of the columns
@@ -738,13 +756,13 @@ gemm_fp8_block_tile_kernel(const __grid_constant__ CUtensorMap tmA, const __grid
                 const float s = __fmul_rn(a, w_s);
                 const uint64_t s2 = f32x2(s, s);
                 const uint32_t src = t_src + buf * BN + half * W2;
-                uint32_t v[2][8];
-                tmem_ld8(src, v[0]);
+                uint32_t v[2][LW];
+                tmem_ld<LW>(src, v[0]);
 #pragma unroll
-                for (int c = 0; c < W2; c += 8) {
+                for (int c = 0; c < W2; c += LW) {
                     tc::tmem_ld_wait();
-                    if (c + 8 < W2) {
-                        tmem_ld8(src + c + 8, v[(c / 8 + 1) & 1]);
+                    if (c + LW < W2) {
+                        tmem_ld<LW>(src + c + LW, v[(c / LW + 1) & 1]);
                     } else {                                 // all is taken: the buffer may be filled again
                         tc::tc_fence_before_sync();
                         __syncwarp();
@@ -754,9 +772,9 @@ gemm_fp8_block_tile_kernel(const __grid_constant__ CUtensorMap tmA, const __grid
                             tc::mbar_arrive(&scale_empty[buf]);
                         }
                     }
-                    const uint32_t* w = v[(c / 8) & 1];
+                    const uint32_t* w = v[(c / LW) & 1];
 #pragma unroll
-                    for (int j = 0; j < 8; j += 2) {
+                    for (int j = 0; j < LW; j += 2) {
                         const uint64_t r = fma_f32x2(f32x2(__uint_as_float(w[j]), __uint_as_float(w[j + 1])), s2, f32x2(acc[c + j], acc[c + j + 1]));
                         f32x2_parts(r, acc[c + j], acc[c + j + 1]);
                     }
