@@ -28,7 +28,8 @@ namespace f8b {
 // The quotient is the correctly rounded one (Markstein, IBM J. Res. Dev. 34, 1990: the product with the rounded reciprocal, its exact
 // remainder, one correction): bf16 values and the largest of them are short enough for quotients that lie exactly between two codes, one
 // in some hundred, and a product with 1 / s puts those on either side.
-// 16 lanes have a group, eight values each.
+// Eight lanes have a group, 16 values each; U groups a lane, whose loads are all under way at once.  What a row of groups costs beside its
+// bytes is the scale: one of four bytes in a line of its own.
 struct Quotient {
     float t, r;                                              // t / 1024 and its reciprocal: both normal numbers for every bf16 t
     __device__ __forceinline__ explicit Quotient(float top) {
@@ -48,36 +49,51 @@ quantize_groups_kernel(const __nv_bfloat16* x, long long x_stride, uint8_t* out,
                        int groups, unsigned items) {
     pdl_launch_dependents();
     pdl_wait();
-    const int lane16 = threadIdx.x & 15;
-    const unsigned first = (blockIdx.x * 16u + (threadIdx.x >> 4)) * U;      // (row, group), group fastest
-    uint4 v[U];
+    const int me = threadIdx.x & 7;
+    const unsigned first = blockIdx.x * (32u * U) + (threadIdx.x >> 3);      // (row, group), group fastest; a lane's are 32 apart
+    uint32_t v[U][8];
     int row[U], grp[U];
     bool in[U];
 #pragma unroll
     for (int i = 0; i < U; ++i) {
-        const unsigned item = first + i;
+        const unsigned item = first + 32u * i;
         row[i] = (int)(item / (unsigned)groups);
         grp[i] = (int)(item - (unsigned)row[i] * (unsigned)groups);
-        in[i] = item < items && grp[i] * 128 + lane16 * 8 < dim;
-        v[i] = in[i] ? ld_stream_v4(x + row[i] * x_stride + grp[i] * 128 + lane16 * 8) : make_uint4(0, 0, 0, 0);
+        in[i] = item < items && grp[i] * 128 + me * 16 < dim;
+        const __nv_bfloat16* src = x + (in[i] ? row[i] * x_stride + grp[i] * 128 + me * 16 : 0);
+        const uint4 a = ld_stream_v4(src), b = ld_stream_v4(src + 8);
+        v[i][0] = a.x; v[i][1] = a.y; v[i][2] = a.z; v[i][3] = a.w;
+        v[i][4] = b.x; v[i][5] = b.y; v[i][6] = b.z; v[i][7] = b.w;
     }
 #pragma unroll
     for (int i = 0; i < U; ++i) {
-        float f[8], top = 0.0f;
-        const uint32_t* w = &v[i].x;
+        float f[16], top = 0.0f;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) unpack_bf16x2(w[j], f[2 * j], f[2 * j + 1]);
+        for (int j = 0; j < 8; ++j) unpack_bf16x2(in[i] ? v[i][j] : 0u, f[2 * j], f[2 * j + 1]);
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
-            if (fabsf(f[j]) < INFINITY) top = fmaxf(top, fabsf(f[j]));
+        for (int j = 0; j < 16; ++j) top = fmaxf(top, fabsf(f[j]));
 #pragma unroll
-        for (int d = 8; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+        for (int d = 4; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+        if (top == INFINITY) {                               // the group's lanes agree; the finite ones count
+            top = 0.0f;
+#pragma unroll
+            for (int j = 0; j < 16; ++j)
+                if (fabsf(f[j]) < INFINITY) top = fmaxf(top, fabsf(f[j]));
+            const unsigned group = 0xffu << (threadIdx.x & 24);
+#pragma unroll
+            for (int d = 4; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(group, top, d));
+        }
         top = fmaxf(top, 448e-12f);
         const Quotient q(top);
-        if (in[i])
-            st_global_v2(out + (size_t)row[i] * dim + grp[i] * 128 + lane16 * 8,
-                         make_uint2(f32x4_to_e4m3x4(q(f[0]), q(f[1]), q(f[2]), q(f[3])), f32x4_to_e4m3x4(q(f[4]), q(f[5]), q(f[6]), q(f[7]))));
-        if (lane16 == 0 && first + i < items) scale[grp[i] * scale_stride + row[i]] = __fdiv_rn(top, 448.0f);
+        if (in[i]) {
+            uint4 o;
+            uint32_t* w = &o.x;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) w[j] = f32x4_to_e4m3x4(q(f[4 * j]), q(f[4 * j + 1]), q(f[4 * j + 2]), q(f[4 * j + 3]));
+            st_global_v4(out + (size_t)row[i] * dim + grp[i] * 128 + me * 16, o);
+        }
+        if (me == 0 && first + 32u * i < items) scale[grp[i] * scale_stride + row[i]] = __fdiv_rn(top, 448.0f);
+        __syncwarp();
     }
 }
 
@@ -437,7 +453,10 @@ constexpr int SCALE_SLOT = 528;       // a buffer's scales: 128 rows, two blocks
 template <int CG, int BN>
 struct TileCfg {
     static constexpr int A_BYTES = 128 * 128, B_BYTES = BN / CG * 128, STAGE_BYTES = A_BYTES + B_BYTES;  // per CTA
-    static constexpr int OUT_BYTES = 32 * BN;                // of each epilogue warp: 32 rows of its half of the columns in bf16
+    // a warp's place for stores: 32 rows of its half of the columns in bf16 (half of it, and a stage more where that makes one, waits for the
+    // first half's copy in every tile: 8191 x 4096 x 4096 on single CTAs 138 us instead of 129)
+    static constexpr int OUT_BYTES = 32 * BN;
+    static_assert(OUT_BYTES >= 32 * 32 * 4, "a block of store_block");
     static constexpr int BUFS = 512 / BN;                    // accumulators: k-blocks under way
     static constexpr int REST = 1024 + 256 + 8 * OUT_BYTES + BUFS * SCALE_SLOT;
     static constexpr int FIT = (227 * 1024 - REST) / STAGE_BYTES > 8 ? 8 : (227 * 1024 - REST) / STAGE_BYTES;
@@ -466,16 +485,17 @@ __device__ __forceinline__ void store_box(const CUtensorMap* m, uint32_t src, in
 template <int W>
 __device__ __forceinline__ void store_rows(const Params& p, const CUtensorMap* tmD, const float* acc, int m_base, int nb, uint32_t stg) {
     const int lane = threadIdx.x & 31;
+    constexpr int BOX = 32 * 128;
     const uint32_t row = stg + lane * 128, sw = (uint32_t)(lane & 7) << 4;
     const bool wide = p.f32 != 0;
 #pragma unroll
-    for (int half = 0; half < 2; ++half) {                   // fp32: W / 2 columns fill the warp's place, bf16: at the end
-        if (half == 0 || wide) {
-            if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
-            __syncwarp();
-        }
+    for (int half = 0; half < 2; ++half) {                   // fp32: W / 2 columns fill the warp's place
+        if (half == 1 && !wide) continue;
+        if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+        __syncwarp();
 #pragma unroll
-        for (int c = half * (W / 2); c < (half + 1) * (W / 2); c += 8) {
+        for (int c = half * (W / 2); c < W; c += 8) {
+            if (half == 0 && c >= W / 2 && wide) continue;
             float f[8];
 #pragma unroll
             for (int j = 0; j < 8; ++j) f[j] = acc[c + j];
@@ -492,23 +512,21 @@ __device__ __forceinline__ void store_rows(const Params& p, const CUtensorMap* t
                 }
             }
             if (wide) {
-                const uint32_t at = row + (c - half * (W / 2)) / 32 * 4096, k = (uint32_t)(c % 32) * 4;
+                const uint32_t at = row + (c - half * (W / 2)) / 32 * BOX, k = (uint32_t)(c % 32) * 4;
                 sts_v4(at + (k ^ sw), f[0], f[1], f[2], f[3]);
                 sts_v4(at + ((k + 16) ^ sw), f[4], f[5], f[6], f[7]);
             } else {
-                asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(row + c / 64 * 4096 + (((uint32_t)(c % 64) * 2) ^ sw)), "r"(pack_bf16x2(f[0], f[1])),
+                asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(row + c / 64 * BOX + (((uint32_t)(c % 64) * 2) ^ sw)), "r"(pack_bf16x2(f[0], f[1])),
                              "r"(pack_bf16x2(f[2], f[3])), "r"(pack_bf16x2(f[4], f[5])), "r"(pack_bf16x2(f[6], f[7])) : "memory");
             }
         }
-        if (half == 1 || wide) {
-            tc::fence_proxy_async_smem();
-            __syncwarp();
-            const int n0 = wide ? nb + half * (W / 2) : nb, per = wide ? 32 : 64, boxes = (wide ? W / 2 : W) / per;
-            if (lane == 0 && m_base < p.M) {
-                for (int i = 0; i < boxes; ++i)
-                    if (n0 + i * per < p.N) store_box(tmD, stg + i * 4096, (n0 + i * per) * (wide ? 4 : 2), m_base);
-                asm volatile("cp.async.bulk.commit_group;" ::: "memory");
-            }
+        tc::fence_proxy_async_smem();
+        __syncwarp();
+        const int n0 = nb + half * (W / 2), per = wide ? 32 : 64, boxes = (wide ? W / 2 : W) / per;
+        if (lane == 0 && m_base < p.M) {
+            for (int i = 0; i < boxes; ++i)
+                if (n0 + i * per < p.N) store_box(tmD, stg + i * BOX, (n0 + i * per) * (wide ? 4 : 2), m_base);
+            asm volatile("cp.async.bulk.commit_group;" ::: "memory");
         }
     }
 }
@@ -914,12 +932,43 @@ static int launch_tile(const void* A, const void* W, Params p, int K, cudaStream
     return e == cudaSuccess ? FRT_OK : FRT_CUDA_ERR(e);
 }
 
+// Clusters of a sharing form that the device holds at once (a cluster lies in one GPC, whose SMs its size need not divide): asked once.
+template <int CG, int BN, int S>
+static long long tile_clusters() {
+    using Cfg = TileCfg<CG, BN>;
+    static int known[64] = {0};
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 0;
+    if (!known[dev]) {
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3(CG * S);
+        cfg.blockDim = dim3(TILE_THREADS);
+        cfg.dynamicSmemBytes = Cfg::SMEM_BYTES;
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = CG * S;
+        attr[0].val.clusterDim.y = 1;
+        attr[0].val.clusterDim.z = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = 1;
+        int n = 0;
+        cudaError_t e = cudaFuncSetAttribute(gemm_fp8_block_tile_kernel<CG, BN, S>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::SMEM_BYTES);
+        if (e == cudaSuccess) e = cudaOccupancyMaxActiveClusters(&n, gemm_fp8_block_tile_kernel<CG, BN, S>, &cfg);
+        if (e != cudaSuccess) {
+            cudaGetLastError();                              // not this launch's error: the form is not offered
+            n = 0;
+        }
+        known[dev] = n + 1;
+    }
+    return known[dev] - 1;
+}
+
 template <int U>
 static int launch_quantize(const void* x, long long stride, void* out, float* scale, long long scale_stride, int rows, int dim, cudaStream_t stream) {
     const int groups = (dim + 127) / 128;
     const unsigned items = (unsigned)((long long)rows * groups);
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((items + 16 * U - 1) / (16 * U));
+    cfg.gridDim = dim3((items + 32 * U - 1) / (32 * U));
     cfg.blockDim = dim3(256);
     cfg.stream = stream;
     cudaLaunchAttribute attr[1];
@@ -947,7 +996,7 @@ extern "C" int frt_b200_quantize_fp8_groups(const void* in_bf16, long long in_st
     if (!in_bf16 || !out8 || !group_scale) return FRT_ERR_INVALID;
     if (misaligned(in_bf16, 16) || misaligned(out8, 16) || misaligned(group_scale, 4)) return FRT_ERR_INVALID;
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
-    const bool few = (long long)rows * ((dim + 127) / 128) < 64ll * device_sm_count();
+    const bool few = (long long)rows * ((dim + 127) / 128) < 256ll * device_sm_count();
     if (few) return f8b::launch_quantize<1>(in_bf16, in_stride, out8, group_scale, scale_stride, rows, dim, st);
     return f8b::launch_quantize<4>(in_bf16, in_stride, out8, group_scale, scale_stride, rows, dim, st);
 }
@@ -976,15 +1025,44 @@ extern "C" int frt_b200_gemm_fp8_block_nt(const void* A, const void* W, void* D,
     p.early = flags & 1;
     p.f32 = flags & 2;
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
-    if (M <= 64) {
+    const int sms = device_sm_count(), n128 = (N + 127) / 128, n256 = (N + 255) / 256;
+    // 33 to 64 rows of wide weights: as rows of tiles the tokens are staged half as often (64 x 32768 x 2048 16.6 us against 18.1)
+    if (M <= 32 || (M <= 64 && 4 * n256 < 3 * sms)) {
         // K splits (a cluster) while the tiles alone leave SMs idle and every rank keeps two k-blocks
-        const int tiles = (N + 127) / 128;
         int splits = 1;
-        while (splits < 8 && tiles * splits * 2 <= 2 * device_sm_count() && p.kb / (splits * 2) >= 2) splits *= 2;
+        while (splits < 8 && n128 * splits * 2 <= 2 * sms && p.kb / (splits * 2) >= 2) splits *= 2;
         if (M <= 16) return f8b::launch_lane<16>(A, W, p, K, splits, st);
         if (M <= 32) return f8b::launch_lane<32>(A, W, p, K, splits, st);
         return f8b::launch_lane<64>(A, W, p, K, splits, st);
     }
-    if (M <= 128) return f8b::launch_tile<1, 256, 1>(A, W, p, K, st);
-    return f8b::launch_tile<2, 256, 1>(A, W, p, K, st);
+    // The cheapest of the forms: whole waves of tiles, k-blocks of a tile, the microseconds of one and of what a tile takes besides; where K is
+    // shared, the exchange, and only if the device holds all clusters at once.  Measured at 128 x 4096 x 4096 (12 us in 128-column tiles, 10 with
+    // K shared by two, 18 in 256-column ones), 256 x 2048 x 8192 (20 on pairs of 128 columns, 13 with K shared by two), 817 x 2048 x 16384 (66 in
+    // 256-column tiles, 40 with K shared by two), 8191 x 4096 x 4096 (125 on pairs of 256 columns, 129 on single CTAs, 162 on pairs of 128).
+    const long long m128 = (M + 127) / 128, m256 = (M + 255) / 256;
+    double best = 1e30;
+    int form = 0;
+    auto offer = [&](int f, long long tiles, int ctas, int S, double per_kb, double exchange, long long (*clusters)()) {
+        const long long room = sms / ctas, waves = S == 1 ? (tiles + room - 1) / room : 1;
+        const double cost = (double)waves * ((p.kb + S - 1) / S * per_kb + 2.0) + exchange;
+        if (cost < best && (S == 1 || (p.kb >= 4 * S && tiles <= clusters()))) { best = cost; form = f; }
+    };
+    offer(0, m256 * n256, 2, 1, 0.47, 0.0, nullptr);
+    offer(1, m128 * n256, 1, 1, 0.50, 0.0, nullptr);
+    offer(2, m256 * n128, 2, 1, 0.30, 0.0, nullptr);
+    offer(3, m128 * n128, 1, 1, 0.345, 0.0, nullptr);
+    offer(4, m128 * n128, 1, 2, 0.345, 2.5, f8b::tile_clusters<1, 128, 2>);
+    offer(5, m256 * n128, 2, 2, 0.30, 3.8, f8b::tile_clusters<2, 128, 2>);
+    offer(6, m128 * n256, 1, 2, 0.50, 5.0, f8b::tile_clusters<1, 256, 2>);
+    offer(7, m128 * n256, 1, 4, 0.50, 7.0, f8b::tile_clusters<1, 256, 4>);
+    switch (form) {
+        case 1: return f8b::launch_tile<1, 256, 1>(A, W, p, K, st);
+        case 2: return f8b::launch_tile<2, 128, 1>(A, W, p, K, st);
+        case 3: return f8b::launch_tile<1, 128, 1>(A, W, p, K, st);
+        case 4: return f8b::launch_tile<1, 128, 2>(A, W, p, K, st);
+        case 5: return f8b::launch_tile<2, 128, 2>(A, W, p, K, st);
+        case 6: return f8b::launch_tile<1, 256, 2>(A, W, p, K, st);
+        case 7: return f8b::launch_tile<1, 256, 4>(A, W, p, K, st);
+        default: return f8b::launch_tile<2, 256, 1>(A, W, p, K, st);
+    }
 }
