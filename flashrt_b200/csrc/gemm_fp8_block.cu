@@ -31,15 +31,22 @@ namespace f8b {
 // Eight lanes have a group, 16 values each; U groups a lane, whose loads are all under way at once.  What a row of groups costs beside its
 // bytes is the scale: one of four bytes in a line of its own.
 struct Quotient {
-    float t, r;                                              // t / 1024 and its reciprocal: both normal numbers for every bf16 t
+    uint64_t t, r;                                           // -t / 1024 and its reciprocal, twice: normal numbers for every bf16 t
     __device__ __forceinline__ explicit Quotient(float top) {
-        t = __fmul_rn(top, 9.765625e-4f);
-        r = __fdiv_rn(1.0f, t);
+        const float s = __fmul_rn(top, 9.765625e-4f), inv = __fdiv_rn(1.0f, s);
+        t = f32x2(-s, -s);
+        r = f32x2(inv, inv);
     }
-    __device__ __forceinline__ float operator()(float x) const {
-        const float a = __fmul_rn(x, 0.4375f);               // 448 / 1024: three bits, exact
-        const float q = fminf(clamp448(__fmul_rn(a, r)), 448.0f);
-        return clamp448(__fmaf_rn(__fmaf_rn(-q, t, a), r, q));
+    // codes of four values, none infinite
+    __device__ __forceinline__ uint32_t operator()(const float* x) const {
+        float q[4];
+#pragma unroll
+        for (int i = 0; i < 4; i += 2) {
+            const uint64_t a = mul_f32x2(f32x2(x[i], x[i + 1]), f32x2(0.4375f, 0.4375f));      // 448 / 1024: three bits, exact
+            const uint64_t y = mul_f32x2(a, r);
+            f32x2_parts(fma_f32x2(fma_f32x2(y, t, a), r, y), q[i], q[i + 1]);
+        }
+        return f32x4_to_e4m3x4(clamp448(q[0]), clamp448(q[1]), clamp448(q[2]), clamp448(q[3]));
     }
 };
 
@@ -51,6 +58,7 @@ quantize_groups_kernel(const __nv_bfloat16* x, long long x_stride, uint8_t* out,
     pdl_wait();
     const int me = threadIdx.x & 7;
     const unsigned first = blockIdx.x * (32u * U) + (threadIdx.x >> 3);      // (row, group), group fastest; a lane's are 32 apart
+    const bool wide = ((reinterpret_cast<uintptr_t>(x) | (uintptr_t)(x_stride * 2)) & 31) == 0;
     uint32_t v[U][8];
     int row[U], grp[U];
     bool in[U];
@@ -61,9 +69,7 @@ quantize_groups_kernel(const __nv_bfloat16* x, long long x_stride, uint8_t* out,
         grp[i] = (int)(item - (unsigned)row[i] * (unsigned)groups);
         in[i] = item < items && grp[i] * 128 + me * 16 < dim;
         const __nv_bfloat16* src = x + (in[i] ? row[i] * x_stride + grp[i] * 128 + me * 16 : 0);
-        const uint4 a = ld_stream_v4(src), b = ld_stream_v4(src + 8);
-        v[i][0] = a.x; v[i][1] = a.y; v[i][2] = a.z; v[i][3] = a.w;
-        v[i][4] = b.x; v[i][5] = b.y; v[i][6] = b.z; v[i][7] = b.w;
+        ld_stream_32(src, wide, true, v[i]);
     }
 #pragma unroll
     for (int i = 0; i < U; ++i) {
@@ -82,6 +88,10 @@ quantize_groups_kernel(const __nv_bfloat16* x, long long x_stride, uint8_t* out,
             const unsigned group = 0xffu << (threadIdx.x & 24);
 #pragma unroll
             for (int d = 4; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(group, top, d));
+            top = fmaxf(top, 448e-12f);
+#pragma unroll
+            for (int j = 0; j < 16; ++j)                     // clamped: the quotient of the largest
+                if (fabsf(f[j]) == INFINITY) f[j] = copysignf(top, f[j]);
         }
         top = fmaxf(top, 448e-12f);
         const Quotient q(top);
@@ -89,7 +99,7 @@ quantize_groups_kernel(const __nv_bfloat16* x, long long x_stride, uint8_t* out,
             uint4 o;
             uint32_t* w = &o.x;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) w[j] = f32x4_to_e4m3x4(q(f[4 * j]), q(f[4 * j + 1]), q(f[4 * j + 2]), q(f[4 * j + 3]));
+            for (int j = 0; j < 4; ++j) w[j] = q(f + 4 * j);
             st_global_v4(out + (size_t)row[i] * dim + grp[i] * 128 + me * 16, o);
         }
         if (me == 0 && first + 32u * i < items) scale[grp[i] * scale_stride + row[i]] = __fdiv_rn(top, 448.0f);
