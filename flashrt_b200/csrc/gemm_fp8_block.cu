@@ -53,21 +53,24 @@ struct Quotient {
 template <int U>
 __global__ void __launch_bounds__(256)
 quantize_groups_kernel(const __nv_bfloat16* x, long long x_stride, uint8_t* out, float* scale, long long scale_stride, int rows, int dim,
-                       int groups, unsigned items) {
+                       int groups, unsigned items, int down) {
     pdl_launch_dependents();
     pdl_wait();
     const int me = threadIdx.x & 7;
-    const unsigned first = blockIdx.x * (32u * U) + (threadIdx.x >> 3);      // (row, group), group fastest; a lane's are 32 apart
+    const unsigned slot = threadIdx.x >> 3, first = blockIdx.x * (32u * U) + slot;
+    // down: a block has 32 rows of U neighbouring groups, so that its scales fill lines; otherwise (row, group) in one row, group fastest
+    const unsigned across = (unsigned)(groups + U - 1) / U, row0 = down ? blockIdx.x / across * 32u + slot : 0, grp0 = down ? blockIdx.x % across * U : 0;
     const bool wide = ((reinterpret_cast<uintptr_t>(x) | (uintptr_t)(x_stride * 2)) & 31) == 0;
     uint32_t v[U][8];
     int row[U], grp[U];
-    bool in[U];
+    bool in[U], there[U];
 #pragma unroll
     for (int i = 0; i < U; ++i) {
         const unsigned item = first + 32u * i;
-        row[i] = (int)(item / (unsigned)groups);
-        grp[i] = (int)(item - (unsigned)row[i] * (unsigned)groups);
-        in[i] = item < items && grp[i] * 128 + me * 16 < dim;
+        row[i] = down ? (int)row0 : (int)(item / (unsigned)groups);
+        grp[i] = down ? (int)(grp0 + i) : (int)(item - (unsigned)row[i] * (unsigned)groups);
+        there[i] = row[i] < rows && grp[i] < groups;
+        in[i] = there[i] && grp[i] * 128 + me * 16 < dim;
         const __nv_bfloat16* src = x + (in[i] ? row[i] * x_stride + grp[i] * 128 + me * 16 : 0);
         ld_stream_32(src, wide, true, v[i]);
     }
@@ -102,7 +105,7 @@ quantize_groups_kernel(const __nv_bfloat16* x, long long x_stride, uint8_t* out,
             for (int j = 0; j < 4; ++j) w[j] = q(f + 4 * j);
             st_global_v4(out + (size_t)row[i] * dim + grp[i] * 128 + me * 16, o);
         }
-        if (me == 0 && first + 32u * i < items) scale[grp[i] * scale_stride + row[i]] = __fdiv_rn(top, 448.0f);
+        if (me == 0 && there[i]) scale[grp[i] * scale_stride + row[i]] = __fdiv_rn(top, 448.0f);
         __syncwarp();
     }
 }
@@ -978,7 +981,8 @@ static int launch_quantize(const void* x, long long stride, void* out, float* sc
     const int groups = (dim + 127) / 128;
     const unsigned items = (unsigned)((long long)rows * groups);
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((items + 32 * U - 1) / (32 * U));
+    const int down = rows >= 32 * U;
+    cfg.gridDim = dim3(down ? (unsigned)((rows + 31) / 32) * (unsigned)((groups + U - 1) / U) : (items + 32 * U - 1) / (32 * U));
     cfg.blockDim = dim3(256);
     cfg.stream = stream;
     cudaLaunchAttribute attr[1];
@@ -987,7 +991,7 @@ static int launch_quantize(const void* x, long long stride, void* out, float* sc
     cfg.attrs = attr;
     cfg.numAttrs = 1;
     const cudaError_t e = cudaLaunchKernelEx(&cfg, quantize_groups_kernel<U>, static_cast<const __nv_bfloat16*>(x), stride,
-                                             static_cast<uint8_t*>(out), scale, scale_stride, rows, dim, groups, items);
+                                             static_cast<uint8_t*>(out), scale, scale_stride, rows, dim, groups, items, down);
     return e == cudaSuccess ? FRT_OK : FRT_CUDA_ERR(e);
 }
 
