@@ -12,16 +12,6 @@
 namespace frt {
 namespace smp {
 
-__device__ __forceinline__ uint64_t dsmem_ld_u64(uint32_t cluster_addr) {
-    uint64_t v;
-    asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(cluster_addr) : "memory");
-    return v;
-}
-__device__ __forceinline__ uint4 dsmem_ld_u32x4(uint32_t cluster_addr) {
-    uint4 v;
-    asm volatile("ld.shared::cluster.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(cluster_addr) : "memory");
-    return v;
-}
 // 16 bytes, or four times `other` and no access: no branch, so that the loads of an unrolled loop are all under way at once
 __device__ __forceinline__ uint4 ld_v4_if(const void* p, bool in, uint32_t other) {
     uint4 v;
@@ -326,6 +316,7 @@ struct VerifyParams {
     const float *u, *v;
     int *out, *accepted, *kept;
     int n_tokens, batch, vocab, ctas;
+    int* status;
 };
 
 __device__ __forceinline__ double warp_scan(double x) {
@@ -347,10 +338,23 @@ __global__ void __launch_bounds__(VERIFY_THREADS, 2)
 verify_drafts_kernel(VerifyParams a) {
     constexpr int WARPS = VERIFY_WARPS;
     __shared__ double sums[WARPS];
-    __shared__ double mine;
+    __shared__ uint4 box[2][8];                              // sums of the cluster's CTAs, of what is left and of p
+    __shared__ uint64_t mail[2];
     pdl_launch_dependents();
-    pdl_wait();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const uint64_t deadline = tc::global_timer_ns() + FRT_KERNEL_DEADLINE_NS;
+    int no_flag = 0;
+    if (a.ctas > 1) {
+        if (tid == 0) {
+            for (int i = 0; i < 2; ++i) {
+                tc::mbar_init(&mail[i], 1);
+                tc::mbar_arrive_expect_tx(&mail[i], (uint32_t)a.ctas * 16u);
+            }
+            tc::mbar_fence_init();
+        }
+        tc::cluster_arrive();                                // waited for in front of the first message
+    }
+    pdl_wait();
     const int ctas = a.ctas, rank = (int)(blockIdx.x % (unsigned)ctas), b = (int)(blockIdx.x / (unsigned)ctas);
     const int first = a.cu[b], end = a.cu[b + 1];
     const int len = a.lens ? a.lens[b] : 0;
@@ -385,7 +389,10 @@ verify_drafts_kernel(VerifyParams a) {
             for (int i = tid; i <= drafts; i += VERIFY_THREADS)
                 if (i != stood) a.out[first + i] = i < stood ? a.tokens[first + i + 1] : -1;
     }
-    if (idle) return;                                        // all CTAs of the cluster
+    if (idle) {                                              // all CTAs of the cluster
+        if (ctas > 1) tc::cluster_wait();
+        return;
+    }
     const int t = first + stood;
     const bool rejected = stood < drafts;
     const float* p = a.p + t * a.p_stride;
@@ -420,34 +427,63 @@ verify_drafts_kernel(VerifyParams a) {
         }
     };
     const float4 zero4 = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    const int at_gone = gone >= 0 ? (gone + skew) / 4 : -1;
+    // Whole vectors weigh alike; those at the row's ends and the one with the token that is gone are left out there and added by a lane.
+    const bool easy = !q || q_wide;
     double slot[SLOTS], start = 0.0, total = 0.0, target = 0.0;
     bool from_p = false;
     int owner = -1;
-    for (;; from_p = true) {
+    for (int turn = 0;; ++turn, from_p = true) {
 #pragma unroll
         for (int k = 0; k < SLOTS; ++k) slot[k] = 0.0;
+        const bool minus = q && !from_p;
         for (int i = lane; i < stretch; i += 32) {
 #pragma unroll
             for (int k0 = 0; k0 < SLOTS; k0 += 4) {
                 uint4 x[4], y[4];
 #pragma unroll
-                for (int k = 0; k < 4; ++k) x[k] = raw(p, true, j0 + (k0 + k) * stretch + i, j1);
+                for (int k = 0; k < 4; ++k) x[k] = raw(p, !easy || j0 + (k0 + k) * stretch + i != at_gone, j0 + (k0 + k) * stretch + i, j1);
 #pragma unroll
-                for (int k = 0; k < 4; ++k) y[k] = raw(q, q_wide && !from_p, j0 + (k0 + k) * stretch + i, j1);
+                for (int k = 0; k < 4; ++k) y[k] = raw(q, q_wide && minus, j0 + (k0 + k) * stretch + i, j1);
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
-                    const int j = j0 + (k0 + k) * stretch + i;
-                    double w[4];
-                    weigh(values(x[k], p, true, j, j1), q && !from_p ? values(y[k], q, q_wide, j, j1) : zero4, j, from_p, w);
-                    slot[k0 + k] += (w[0] + w[1]) + (w[2] + w[3]);
+                    if (easy) {                              // larger of both less q: two conversions, no selection
+                        const float xs[4] = {__uint_as_float(x[k].x), __uint_as_float(x[k].y), __uint_as_float(x[k].z), __uint_as_float(x[k].w)};
+                        const float ys[4] = {__uint_as_float(y[k].x), __uint_as_float(y[k].y), __uint_as_float(y[k].z), __uint_as_float(y[k].w)};
+                        double w[4];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) w[e] = (double)fmaxf(xs[e], ys[e]) - (double)ys[e];
+                        slot[k0 + k] += (w[0] + w[1]) + (w[2] + w[3]);
+                    } else {
+                        const int j = j0 + (k0 + k) * stretch + i;
+                        double w[4];
+                        weigh(values(x[k], p, true, j, j1), minus ? values(y[k], q, q_wide, j, j1) : zero4, j, from_p, w);
+                        slot[k0 + k] += (w[0] + w[1]) + (w[2] + w[3]);
+                    }
                 }
             }
+        }
+        if (easy && lane == 0) {
+            auto add = [&](int j) {
+                const uint4 zero = make_uint4(0, 0, 0, 0);
+                const bool whole = j >= ja && j < jb;        // the one whose token is gone
+                double w[4];
+                weigh(values(whole ? raw(p, true, j, j1) : zero, p, true, j, j1), minus ? values(zero, q, true, j, j1) : zero4, j, from_p, w);
+                const double sum = (w[0] + w[1]) + (w[2] + w[3]);
+#pragma unroll
+                for (int k = 0; k < SLOTS; ++k)
+                    if (j >= j0 + k * stretch && j < j0 + (k + 1) * stretch) slot[k] += sum;
+            };
+            const bool head = ja > j0, tail = jb < j1 && !(head && j1 == 1);
+            if (head) add(0);
+            if (tail) add(j1 - 1);
+            if (at_gone >= j0 && at_gone < j1 && !(head && at_gone == 0) && !(tail && at_gone == j1 - 1)) add(at_gone);
         }
         double s = 0.0;
 #pragma unroll
         for (int k = 0; k < SLOTS; ++k) s += slot[k];
         s = warp_sum(s);
-        __syncthreads();                                     // `sums` of a pass before are read
+        if (turn) __syncthreads();                           // `sums` of the turn before are read
         if (lane == 0) sums[warp] = s;
         __syncthreads();
         double cta = 0.0;
@@ -455,12 +491,20 @@ verify_drafts_kernel(VerifyParams a) {
         for (int w = 0; w < WARPS; ++w) cta += sums[w];
         double all[8];
         if (ctas > 1) {
-            if (tid == 0) mine = cta;
-            tc::cluster_sync_all();
+            if (turn == 0) tc::cluster_wait();
+            if (warp == 0 && lane < ctas) {
+                const unsigned long long bits = (unsigned long long)__double_as_longlong(cta);
+                tc::st_async_v4(tc::dsmem_map(tc::smem_u32(&box[turn][rank]), (uint32_t)lane), tc::dsmem_map(tc::smem_u32(&mail[turn]), (uint32_t)lane),
+                                (uint32_t)bits, (uint32_t)(bits >> 32), 0u, 0u);
+            }
+            if (!tc::mbar_wait_until(&mail[turn], 0, deadline, &no_flag) && tid == 0) atomicCAS(a.status, 0, ERR_MAIL);
+            __syncwarp();
 #pragma unroll
             for (int r = 0; r < 8; ++r)
-                if (r < ctas) all[r] = __longlong_as_double((long long)dsmem_ld_u64(tc::dsmem_map(tc::smem_u32(&mine), (uint32_t)r)));
-            tc::cluster_arrive();
+                if (r < ctas) {
+                    const uint4 w = box[turn][r];
+                    all[r] = __longlong_as_double((long long)((unsigned long long)w.x | (unsigned long long)w.y << 32));
+                }
         } else {
             all[0] = cta;
         }
@@ -482,7 +526,6 @@ verify_drafts_kernel(VerifyParams a) {
                 at += all[r];
             }
         if (total > 0.0 || from_p) break;
-        if (ctas > 1) tc::cluster_wait();                    // everyone has read: `mine` may change
     }
     if (owner < 0 && rank == 0 && tid == 0) a.out[t] = -1;   // no probability anywhere, or an infinite one
     if (owner == rank) {
@@ -539,7 +582,6 @@ verify_drafts_kernel(VerifyParams a) {
             if (lane == 0) a.out[t] = token >= 0 ? token : last;     // roundings left the target behind the last one: that one
         }
     }
-    if (ctas > 1) tc::cluster_wait();                        // nobody leaves while its sum is read
 }
 
 static int* status_word() {
@@ -660,7 +702,8 @@ extern "C" int frt_b200_verify_drafts(const float* target_probs, long long p_str
         misaligned(u_accept, 4) || misaligned(u_sample, 4) || misaligned(out_tokens, 4) || misaligned(accepted, 4) || misaligned(kept_lens, 4))
         return FRT_ERR_INVALID;
     smp::VerifyParams p = {target_probs, draft_probs, p_stride, q_stride, tokens, cu_seqlens, seq_lens, u_accept, u_sample,
-                           out_tokens, accepted, kept_lens, n_tokens, batch, vocab, 1};
+                           out_tokens, accepted, kept_lens, n_tokens, batch, vocab, 1, smp::status_word()};
+    if (!p.status) return FRT_ERR_UNSUPPORTED;
     int ctas = 1;
     while (ctas < 8 && ctas * 8 * smp::VERIFY_THREADS <= vocab && (long long)batch * ctas * 2 <= 2ll * device_sm_count()) ctas *= 2;
     p.ctas = ctas;
