@@ -68,9 +68,9 @@ struct PlanParams {
 
 __global__ void __launch_bounds__(PLAN_THREADS)
 paged_plan_kernel(PlanParams p) {
-    extern __shared__ int start[];                           // (batch + 1) first token, (batch + 1) first new block of each sequence
+    extern __shared__ int start[];                           // (batch + 1) first token, (batch + 1) first new block of each sequence, tokens it keeps
     __shared__ int part[2 * PLAN_THREADS / 32];
-    int* first = start + p.batch + 1;
+    int *first = start + p.batch + 1, *stay = first + p.batch + 1;
     pdl_launch_dependents();
     pdl_wait();
     const int tid = threadIdx.x, per = (p.batch + PLAN_THREADS - 1) / PLAN_THREADS;
@@ -105,7 +105,8 @@ paged_plan_kernel(PlanParams p) {
         const bool served = t <= p.tokens && k <= room;
         if (served) { last_t = t; last_k = k; }
         refused += !(fits && served);
-        if (blockIdx.x == 0) p.lens[b] = fits && served ? p.kept[b] + n : max(p.kept[b], 0);
+        stay[b] = p.kept[b];
+        if (blockIdx.x == 0) p.lens[b] = fits && served ? stay[b] + n : max(stay[b], 0);
     }
     const int total_t = __reduce_max_sync(0xffffffffu, last_t), total_k = __reduce_max_sync(0xffffffffu, last_k);
     const int warp_refused = __reduce_add_sync(0xffffffffu, refused);
@@ -142,15 +143,15 @@ paged_plan_kernel(PlanParams p) {
     const int gsize = gridDim.x * PLAN_THREADS, gid = blockIdx.x * PLAN_THREADS + tid;
     for (int i = gid; i < blocks; i += gsize) {
         const int b = last_not_above(first, p.batch, i);
-        p.table[(size_t)b * p.table_stride + blocks_of(p.kept[b], p.shift) + (i - first[b])] = p.free_list[room - 1 - i];
+        p.table[(size_t)b * p.table_stride + blocks_of(stay[b], p.shift) + (i - first[b])] = p.free_list[room - 1 - i];
     }
     if (!p.positions && !p.slots) return;
     for (long long i = gid; i < p.tokens; i += gsize) {
         int pos = -1;
         long long slot = -1;
         if (i < tokens) {
-            const int b = last_not_above(start, p.batch, (int)i), have = blocks_of(p.kept[b], p.shift);
-            pos = p.kept[b] + ((int)i - start[b]);
+            const int b = last_not_above(start, p.batch, (int)i), have = blocks_of(stay[b], p.shift);
+            pos = stay[b] + ((int)i - start[b]);
             const int j = pos >> p.shift;
             const int page = j < have ? p.table[(size_t)b * p.table_stride + j] : p.free_list[room - 1 - (first[b] + j - have)];
             if (page >= 0 && page < p.num_blocks) slot = ((long long)page << p.shift) + (pos & ((1 << p.shift) - 1));
@@ -173,9 +174,10 @@ struct ReleaseParams {
 // that takes as many finds them in the order in which they were.
 __global__ void __launch_bounds__(RELEASE_THREADS)
 paged_release_kernel(ReleaseParams p) {
-    extern __shared__ int first[];                           // (batch + 1) first item of each sequence
+    extern __shared__ int first[];                           // first item of each sequence; blocks that it keeps
     __shared__ int part[2 * RELEASE_THREADS / 32];
     __shared__ int mine;
+    int* stay = first + p.batch;
     pdl_launch_dependents();
     pdl_wait();
     const int tid = threadIdx.x, per = (p.batch + RELEASE_THREADS - 1) / RELEASE_THREADS;
@@ -192,15 +194,19 @@ paged_release_kernel(ReleaseParams p) {
     for (int b = b0; b < b1; ++b) {
         first[b] = at;
         at = sat_add(at, drops(b, from));
+        stay[b] = from;
     }
     __syncthreads();
     auto entry = [&](int i) {
         const int b = last_not_above(first, p.batch, i);
-        return p.table + (size_t)b * p.table_stride + blocks_of(p.kept[b], p.shift) + (i - first[b]);
+        return p.table + (size_t)b * p.table_stride + stay[b] + (i - first[b]);
     };
-    const int i0 = (int)((long long)items * rank / ctas), i1 = (int)((long long)items * (rank + 1) / ctas);
+    // few items (the tables are large, but a step drops little): the first CTA's alone, and nobody waits for a count
+    const bool alone = items <= RELEASE_THREADS;
+    if (alone && rank > 0) return;
+    const int i0 = alone ? 0 : (int)((long long)items * rank / ctas), i1 = alone ? items : (int)((long long)items * (rank + 1) / ctas);
     int before = 0, total = 0;                               // blocks of the pool in front of this CTA's items, and in all
-    if (i1 - i0 > RELEASE_THREADS || ctas > 1) {
+    if (!alone) {
         int n = 0, unused = 0, all, none2;
         for (int i = i0 + tid; i < i1; i += RELEASE_THREADS) n += (unsigned)*entry(i) < (unsigned)p.num_blocks;
         block_scan2<RELEASE_THREADS>(n, unused, part, all, none2);
@@ -219,15 +225,14 @@ paged_release_kernel(ReleaseParams p) {
             total = all;
         }
     }
-    const bool counted = i1 - i0 > RELEASE_THREADS || ctas > 1;
-    for (int base = i0; base < i1 || (!counted && base == i0); base += RELEASE_THREADS) {
+    for (int base = i0; base < i1 || (alone && base == i0); base += RELEASE_THREADS) {
         const int i = base + tid;
         int* e = i < i1 ? entry(i) : nullptr;
         const int page = e ? *e : -1;
         int n = (unsigned)page < (unsigned)p.num_blocks, unused = 0, all, none2;
         const bool valid = n;
         block_scan2<RELEASE_THREADS>(n, unused, part, all, none2);
-        if (!counted) total = all;
+        if (alone) total = all;
         if (valid) {
             const int to = room + total - 1 - (before + n);
             if (to >= 0 && to < p.num_blocks) p.free_list[to] = page;
@@ -238,7 +243,7 @@ paged_release_kernel(ReleaseParams p) {
     if (rank == 0 && tid == 0) *p.free_out = min(room + total, p.num_blocks);
 }
 
-constexpr int PLAN_SMEM = 2 * (MAX_BATCH + 1) * 4;
+constexpr int PLAN_SMEM = 3 * (MAX_BATCH + 1) * 4;
 
 static int launch_plan(const PlanParams& p, cudaStream_t stream) {
     static PerDeviceOnce once;
@@ -254,7 +259,7 @@ static int launch_plan(const PlanParams& p, cudaStream_t stream) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(want < 1 ? 1 : want < most ? want : most));
     cfg.blockDim = dim3(PLAN_THREADS);
-    cfg.dynamicSmemBytes = 2 * (size_t)(p.batch + 1) * 4;
+    cfg.dynamicSmemBytes = 3 * (size_t)(p.batch + 1) * 4;
     cfg.stream = stream;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -266,21 +271,28 @@ static int launch_plan(const PlanParams& p, cudaStream_t stream) {
 }
 
 static int launch_release(const ReleaseParams& p, cudaStream_t stream) {
+    static PerDeviceOnce once;
+    int dev = 0;
+    if (once.need(dev)) {
+        const cudaError_t e = cudaFuncSetAttribute(paged_release_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, PLAN_SMEM);
+        if (e != cudaSuccess) return FRT_CUDA_ERR(e);
+        once.set(dev);
+    }
     cudaLaunchConfig_t cfg = {};
     const unsigned ctas = (long long)p.batch * p.table_stride > 16 * RELEASE_THREADS ? 8 : 1;
     cfg.gridDim = dim3(ctas);
     cfg.blockDim = dim3(RELEASE_THREADS);
-    cfg.dynamicSmemBytes = (size_t)(p.batch + 1) * 4;
+    cfg.dynamicSmemBytes = 2 * (size_t)p.batch * 4;
     cfg.stream = stream;
     cudaLaunchAttribute attr[2];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = ctas;
-    attr[0].val.clusterDim.y = 1;
-    attr[0].val.clusterDim.z = 1;
-    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = ctas;
+    attr[1].val.clusterDim.y = 1;
+    attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = 2;
+    cfg.numAttrs = ctas > 1 ? 2 : 1;
     const cudaError_t e = cudaLaunchKernelEx(&cfg, paged_release_kernel, p);
     return e == cudaSuccess ? FRT_OK : FRT_CUDA_ERR(e);
 }
