@@ -7,9 +7,11 @@
 //   D(M,N) = sum_kb a_scale[kb][m] * w_scale[n / 128][kb] * (sum_{k in block kb} A[m,k] W[n,k]) + bias[n]
 //
 // tcgen05.mma kind::f8f6f4 sums one k-block of 128 into a buffer of tensor memory; the epilogue warps take it out, multiply by the block's
-// scales and add it to the tile's sums, which they keep in registers (fp32).  The buffers go round, so that the next block's products run
-// meanwhile: 256 x 256 x 128 on a CTA pair are 512 cycles of the tensor pipe, and the same block is 256 cycles of tcgen05.ld and 256 of fma
-// for the epilogue.
+// scales and add it to the tile's sums, which they keep in registers (fp32: the block's scales differ, so tensor memory cannot hold them).
+// The buffers go round, so that the next block's products run meanwhile.  That taking out is what bounds many rows: 256 x 256 x 128 on a CTA
+// pair are 512 cycles of products, and a warp's 128 columns come out of tensor memory in 370 cycles when it is idle but in 850 beside the
+// products, which go there for their sums too; with the signals between the warps a k-block takes 0.47 us, 2.2 PFLOP/s, where the products
+// with one scale per tensor, taken out once a tile, reach 2.9.
 //
 // More than 64 rows: the tokens are the rows of a tile (a thread of the epilogue owns a row, its scale is one register), on CTA pairs or
 // single CTAs; up to 64 rows: the weights are the 128 lanes and the tokens the columns, because nothing is left but streaming the weights.
@@ -207,8 +209,7 @@ __device__ __forceinline__ void tmem_ld8(uint32_t taddr, uint32_t* v) {
 template <int N>
 __device__ __forceinline__ void tmem_ld(uint32_t taddr, uint32_t* v) {
     if constexpr (N == 8) tmem_ld8(taddr, v);
-    else if constexpr (N == 16) tc::tmem_ld16(taddr, v);
-    else tc::tmem_ld32(taddr, v);
+    else tc::tmem_ld16(taddr, v);
 }
 __device__ __forceinline__ void store_one(const Params& p, size_t at, float v) {
     if (p.f32) static_cast<float*>(p.out)[at] = v;
@@ -594,7 +595,7 @@ __device__ __forceinline__ void store_block(const Params& p, const float* f, int
 // CG = 2: a CTA pair has a tile of 256 rows, each CTA stages its 128 rows of A and half of the weight rows.  S > 1: a cluster of S such
 // takes one tile, unit s the k-blocks [kb s / S, kb (s + 1) / S); they then lay their partials into shared memory, where their rings were,
 // and each finishes BN / S of the columns.
-constexpr int TILE_THREADS = 384;     // producer, issuer, scales, an idle warp; eight for the epilogue
+constexpr int TILE_THREADS = 384;     // producer, issuer, scales, second issuer or none; eight warps of the epilogue
 template <int CG, int BN, int S>
 __global__ void __launch_bounds__(TILE_THREADS, 1)
 gemm_fp8_block_tile_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmD, Params p) {
@@ -756,14 +757,13 @@ gemm_fp8_block_tile_kernel(const __grid_constant__ CUtensorMap tmA, const __grid
         }
     } else if (warp >= 4) {
         // ---------------- epilogue: this CTA's 128 rows; a warp's lane quadrant and half of the columns
-        
         pdl_wait();
         const int q = warp & 3, half = (warp - 4) >> 2;
         const uint32_t t_src = tmem + ((uint32_t)(q * 32) << 16);
         uint8_t* stg = outs + (warp - 4) * Cfg::OUT_BYTES;
         const uint32_t accF_a = tc::smem_u32(acc_full), accE_a = tc::smem_u32(acc_empty);
         const uint32_t accE_lead = CG == 1 ? accE_a : tc::dsmem_map(accE_a, leader);
-                int buf = 0;
+        int buf = 0;
         uint32_t bph = 0;
         for (int t = unit; t < total; t += units) {
             int mt, nt;
@@ -780,13 +780,14 @@ gemm_fp8_block_tile_kernel(const __grid_constant__ CUtensorMap tmA, const __grid
                     break;
                 }
                 tc::tc_fence_after_sync();
-                // 32 columns on their way from tensor memory while the 32 in front are added
                 float a, w_s;
                 asm volatile("ld.shared.f32 %0, [%1];" : "=f"(a) : "r"(scale_a + buf * SCALE_SLOT + (q * 32 + lane) * 4) : "memory");
                 asm volatile("ld.shared.f32 %0, [%1];" : "=f"(w_s) : "r"(scale_a + buf * SCALE_SLOT + 512 + half * 4) : "memory");
                 const float s = __fmul_rn(a, w_s);
                 const uint64_t s2 = f32x2(s, s);
                 const uint32_t src = t_src + buf * BN + half * W2;
+                // LW columns on their way from tensor memory while the LW in front are added: eight, where 128 sums leave registers for no more
+                // (16 spill: 138 us instead of 125 at 8191 x 4096 x 4096)
                 uint32_t v[2][LW];
                 tmem_ld<LW>(src, v[0]);
 #pragma unroll

@@ -2,8 +2,8 @@
 //
 // Stand behind the products that make logits and in front of the paged cache's lengths; no counterpart in the reference.
 //
-// Both read rows of a vocabulary once: a row belongs to a cluster of 1 to 8 CTAs that hold it (softmax: in registers) and exchange a few
-// numbers through distributed shared memory.  Rows start anywhere (odd vocabularies): 16-byte vectors lie where memory has them, and the
+// Both read rows of a vocabulary once: a row belongs to a cluster of 1 to 8 CTAs that hold it (softmax: in registers) and send one another a
+// few numbers.  Rows start anywhere (odd vocabularies): 16-byte vectors lie where memory has them, and the
 // first and last of a row are taken value by value.
 #include "common.cuh"
 #include "tc05.cuh"
@@ -679,7 +679,7 @@ extern "C" int frt_b200_softmax_rows(const void* in, long long in_stride, float*
     if (rows > 1 << 27 || vocab > 1 << 30) return FRT_ERR_UNSUPPORTED;
     if (rows == 0 || vocab == 0) return FRT_OK;
     const bool f32 = flags & 2;
-    if (!in || !out || misaligned(in, f32 ? 4 : 2) || misaligned(out, 4) || misaligned(temperature, 4)) return FRT_ERR_INVALID;
+    if (!in || !out || in == out || misaligned(in, f32 ? 4 : 2) || misaligned(out, 4) || misaligned(temperature, 4)) return FRT_ERR_INVALID;
     smp::SoftmaxParams p = {in, out, temperature, in_stride, out_stride, rows, vocab, 1, smp::status_word()};
     if (!p.status) return FRT_ERR_UNSUPPORTED;
     const cudaStream_t st = static_cast<cudaStream_t>(stream);

@@ -25,7 +25,7 @@ def product(**kw):
 
 
 def softmax(**kw):
-    return status("frt_b200_softmax_rows", dict(x=A, istride=100, out=A, ostride=100, t=None, rows=4, vocab=100, flags=0, stream=None), kw)
+    return status("frt_b200_softmax_rows", dict(x=A, istride=100, out=A + 64, ostride=100, t=None, rows=4, vocab=100, flags=0, stream=None), kw)
 
 
 def verify(**kw):
@@ -63,7 +63,7 @@ def test_product():
 def test_softmax():
     assert softmax(rows=0) == 0 and softmax(vocab=0) == 0
     for kw in (dict(rows=-1), dict(vocab=-1), dict(istride=99), dict(ostride=99), dict(x=None), dict(out=None), dict(x=A + 1), dict(x=A + 2, flags=2),
-               dict(out=A + 2), dict(t=A + 2)):
+               dict(out=A + 2), dict(out=A), dict(t=A + 2)):
         assert softmax(**kw) == -1, kw
     assert softmax(vocab=(1 << 30) + 1, istride=1 << 31, ostride=1 << 31) == -2 and softmax(rows=(1 << 27) + 1) == -2
 
