@@ -924,7 +924,8 @@ static int launch_tile(const void* A, const void* W, Params p, int K, cudaStream
     int rc = make_tmap_2d_u8(&tmA, A, (uint64_t)p.M, (uint64_t)K, (uint64_t)K, 128);
     if (!rc) rc = make_tmap_2d_u8(&tmW, W, (uint64_t)p.N, (uint64_t)K, (uint64_t)K, BN / CG);
     const uint64_t out_row = (uint64_t)p.N * (p.f32 ? 4 : 2);
-    p.tma = p.N % 8 == 0 && (reinterpret_cast<uintptr_t>(p.bias) & 15) == 0;
+    // rows at 16 bytes, bias read so, and a byte's place in a row is a 32-bit coordinate
+    p.tma = p.N % 8 == 0 && (reinterpret_cast<uintptr_t>(p.bias) & 15) == 0 && out_row <= 1u << 31;
     if (!rc && p.tma) rc = make_tmap_2d_u8(&tmD, p.out, (uint64_t)p.M, out_row, out_row, 32);
     if (!p.tma) tmD = tmA;
     if (rc) return rc;

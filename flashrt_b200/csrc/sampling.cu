@@ -695,9 +695,8 @@ extern "C" int frt_b200_verify_drafts(const float* target_probs, long long p_str
     if (n_tokens < 0 || batch < 0 || vocab < 1 || p_stride < vocab || (draft_probs && q_stride < vocab)) return FRT_ERR_INVALID;
     if (batch > 1 << 27 || vocab > 1 << 30) return FRT_ERR_UNSUPPORTED;
     if (batch == 0) return FRT_OK;
-    if (!target_probs || !tokens || !cu_seqlens || !u_accept || !u_sample || !out_tokens || !accepted || (kept_lens && !seq_lens) ||
-        out_tokens == tokens)
-        return FRT_ERR_INVALID;
+    if (!cu_seqlens || !u_sample || !accepted || (kept_lens && !seq_lens)) return FRT_ERR_INVALID;
+    if (n_tokens && (!target_probs || !tokens || !u_accept || !out_tokens || out_tokens == tokens)) return FRT_ERR_INVALID;
     if (misaligned(target_probs, 4) || misaligned(draft_probs, 4) || misaligned(tokens, 4) || misaligned(cu_seqlens, 4) || misaligned(seq_lens, 4) ||
         misaligned(u_accept, 4) || misaligned(u_sample, 4) || misaligned(out_tokens, 4) || misaligned(accepted, 4) || misaligned(kept_lens, 4))
         return FRT_ERR_INVALID;

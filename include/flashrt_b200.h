@@ -595,7 +595,8 @@ int frt_b200_gemm_fp8_block_nt(const void* A, const void* W, void* D, int M, int
  * Softmax of rows (no counterpart in the reference): out = exp((x - max) / T) / sum, fp32.  in (rows, vocab) bf16, with flags bit 1 fp32, rows
  *   in_stride elements apart; out (rows, vocab) fp32, rows out_stride elements apart; temperature (rows) fp32 or NULL: 1.  A temperature
  *   that is not above zero (0, negative, NaN): one at the first of the row's largest, zero elsewhere.  NaN counts as -infinity; a row of
- *   nothing else is zero; infinite entries share the whole.  Not in place.  vocab <= 2^30. */
+ *   nothing else is zero; infinite entries share the whole.  Not in place.  vocab <= 2^30.  A wait that gave up shows in
+ *   frt_b200_gemm_status. */
 int frt_b200_softmax_rows(const void* in, long long in_stride, float* out, long long out_stride, const float* temperature, int rows,
                           int vocab, int flags, void* stream);
 /* Drafted tokens against the target's probabilities, from given random numbers (no counterpart in the reference).  Sequence b has the rows
@@ -609,7 +610,7 @@ int frt_b200_softmax_rows(const void* in, long long in_stride, float* out, long 
  *   out_tokens (n_tokens), not `tokens` itself: the tokens that stand, the new one, then -1 up to the sequence's end; rows behind the last
  *   sequence are left as they were.  accepted (batch): drafted tokens that stand.  kept_lens (batch) or NULL: seq_lens less the drafted
  *   tokens that do not; may be seq_lens itself.  A sequence without rows, or whose rows leave [0, n_tokens): accepted 0, kept_lens =
- *   seq_lens, nothing else. */
+ *   seq_lens, nothing else.  A wait that gave up shows in frt_b200_gemm_status. */
 int frt_b200_verify_drafts(const float* target_probs, long long p_stride, const float* draft_probs, long long q_stride,
                            const int* tokens, const int* cu_seqlens, const int* seq_lens, const float* u_accept,
                            const float* u_sample, int* out_tokens, int* accepted, int* kept_lens, int n_tokens, int batch,

@@ -170,6 +170,45 @@ def test_rows_do_not_depend_on_their_neighbours():
         assert torch.equal(got[rows][:, cols], clean[rows][:, cols])
 
 
+def test_bias_and_output_at_odd_places():
+    """A bias that starts two bytes behind a boundary, an output 16 bytes behind one of 32."""
+    from flashrt_b200 import flash_rt_kernels as fvk
+    for m, n, k in ((5, 640, 512), (70, 640, 512), (300, 640, 512), (128, 1024, 4096)):
+        a, w, sa, sw, _ = (t.cuda() for t in operands(m, n, k, m + 1))
+        wide = torch.randn(n + 1, device="cuda").to(BF16)
+        for f32 in (False, True):
+            out = torch.full((m * n + 64,), -7.0, dtype=F32 if f32 else BF16, device="cuda")
+            at = 4 if f32 else 8
+            fvk.GemmRunner().fp8_block_nt(a.data_ptr(), w.data_ptr(), out.data_ptr() + 16, m, n, k, sa.data_ptr(), sw.data_ptr(), _stream(),
+                                          bias=wide.data_ptr() + 2, d_f32=f32)
+            torch.cuda.synchronize()
+            assert (out[:at] == -7).all() and (out[at + m * n:] == -7).all()
+            want, size = R.block_product(a.to(F64), w.to(F64), sa, sw)
+            close(out[at:at + m * n].view(m, n).cpu(), want.cpu(), size.cpu(), k // 128, wide[1:].cpu(), f32)
+
+
+def test_two_calls_at_once():
+    """Products, large and small, on two streams at the same time: nothing is shared."""
+    sides = [torch.cuda.Stream() for _ in range(2)]
+    jobs = [operands(m, n, k, m) for m, n, k in ((3000, 1024, 2048), (40, 8192, 1024), (100, 4096, 4096), (1, 2560, 2048))]
+    jobs = [tuple(t.cuda() for t in j) for j in jobs]
+    want = [product(*j[:4], j[4]) for j in jobs]
+    from flashrt_b200 import flash_rt_kernels as fvk
+    outs = [[torch.zeros_like(w) for w in want] for _ in sides]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for s, mine in zip(sides, outs):
+            with torch.cuda.stream(s):
+                for (a, w, sa, sw, b), o in zip(jobs, mine):
+                    fvk.GemmRunner().fp8_block_nt(a.data_ptr(), w.data_ptr(), o.data_ptr(), *o.shape, a.shape[1], sa.data_ptr(), sw.data_ptr(),
+                                                  _stream(), bias=b.data_ptr())
+    torch.cuda.synchronize()
+    for mine in outs:
+        for o, w in zip(mine, want):
+            assert torch.equal(o, w)
+    assert fvk.tensor_core_status() == 0
+
+
 def test_streams_and_graph():
     from flashrt_b200 import flash_rt_kernels as fvk
     m, n, k = 70, 1500, 2048

@@ -98,6 +98,23 @@ def test_softmax_ties_and_strides():
     close(softmax(wide, t, in_stride=1009, out_stride=1024, rows=7, vocab=1001), wide[:, :1001], t)
 
 
+def test_softmax_rows_that_start_anywhere():
+    """Inputs one value, outputs one or three values behind a boundary."""
+    from flashrt_b200 import flash_rt_kernels as fvk
+    g = torch.Generator().manual_seed(8)
+    for dtype in (BF16, F32):
+        for vocab, rows in ((5000, 3), (40000, 2), (70, 9), (131072, 40)):
+            for i, j in ((1, 0), (0, 1), (3, 3), (1, 3), (7, 2)):
+                x = (torch.randn(rows * vocab + 8, generator=g) * 3).to(dtype).cuda()
+                p = torch.full((rows * vocab + 8,), -3.0, device="cuda")
+                es = 2 if dtype == BF16 else 4
+                t = torch.full((rows,), 0.9).cuda()
+                fvk.softmax_rows(x.data_ptr() + i * es, p.data_ptr() + 4 * j, rows, vocab, _stream(), temperature=t.data_ptr(), in_f32=dtype == F32)
+                torch.cuda.synchronize()
+                assert (p[:j] == -3).all() and (p[j + rows * vocab:] == -3).all()
+                close(p[j:j + rows * vocab].view(rows, vocab).cpu(), x[i:i + rows * vocab].view(rows, vocab), t)
+
+
 # ------------------------------------------------------------------------------------------------ verification
 def rows_of(rng, n, vocab, zeros=0.0):
     p = rng.exponential(size=(n, vocab)) ** 3
@@ -184,6 +201,36 @@ def test_verify_borders():
     assert run(ok, None, [0, 40, 3, 4], [0, 4], [9], [0.0] * 4, [0.5])[1] == [0]
     for cu in ([0, 5], [-1, 2], [2, 1], [3, 3]):
         assert run(ok, None, [0, 1, 2, 3], cu, [9], [0.0] * 4, [0.5]) == ([-77] * 9, [0], [9]), cu
+
+
+def test_verify_without_rows_and_two_calls_at_once():
+    from flashrt_b200 import flash_rt_kernels as fvk
+    z = torch.zeros(4, dtype=I32, device="cuda")
+    f = torch.zeros(4, device="cuda")
+    acc, kept = torch.full((3,), 9, dtype=I32, device="cuda"), torch.full((3,), 9, dtype=I32, device="cuda")
+    lens = torch.tensor([5, 6, 7], dtype=I32, device="cuda")
+    fvk.verify_drafts(0, 0, 0, z.data_ptr(), lens.data_ptr(), 0, f.data_ptr(), 0, acc.data_ptr(), kept.data_ptr(), 0, 3, 100, _stream())
+    torch.cuda.synchronize()
+    assert acc.tolist() == [0, 0, 0] and kept.tolist() == [5, 6, 7]
+    rng = np.random.default_rng(3)
+    n, vocab = 64, 20000
+    p, q = torch.tensor(rows_of(rng, n, vocab)).cuda(), torch.tensor(rows_of(rng, n, vocab)).cuda()
+    tokens = q.argmax(1).roll(1).to(I32)
+    cu = torch.arange(0, n + 1, 4, dtype=I32, device="cuda")
+    u, v = torch.rand(n, device="cuda"), torch.rand(16, device="cuda")
+    lens = torch.full((16,), 50, dtype=I32, device="cuda")
+    want = R.verify(p.cpu().numpy(), q.cpu().numpy(), tokens.tolist(), cu.tolist(), lens.tolist(), u.cpu().numpy(), v.cpu().numpy())
+    sides = [torch.cuda.Stream() for _ in range(3)]
+    outs = [[torch.zeros(k, dtype=I32, device="cuda") for k in (n, 16, 16)] for _ in sides]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for s, o in zip(sides, outs):
+            with torch.cuda.stream(s):
+                fvk.verify_drafts(p.data_ptr(), q.data_ptr(), tokens.data_ptr(), cu.data_ptr(), lens.data_ptr(), u.data_ptr(), v.data_ptr(),
+                                  o[0].data_ptr(), o[1].data_ptr(), o[2].data_ptr(), n, 16, vocab, _stream())
+    torch.cuda.synchronize()
+    for o in outs:
+        assert tuple(x.tolist() for x in o) == want
 
 
 def test_greedy_rows_are_the_argmax():
