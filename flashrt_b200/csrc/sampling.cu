@@ -64,7 +64,7 @@ softmax_rows_kernel(SoftmaxParams p) {
     __shared__ int part3[2][WARPS];                          // first of its largest
     __shared__ uint4 box[2][8];                              // the same of each CTA of the cluster
     __shared__ uint64_t mail[2], there;
-    pdl_launch_dependents();
+    if (!STAGED) pdl_launch_dependents();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int ctas = p.ctas, rank = (int)(blockIdx.x % (unsigned)ctas), step = (int)(gridDim.x / (unsigned)ctas);
     const uint64_t deadline = tc::global_timer_ns() + FRT_KERNEL_DEADLINE_NS;
@@ -239,6 +239,7 @@ softmax_rows_kernel(SoftmaxParams p) {
         }
         __syncthreads();
         if (STAGED && tid == 0) fetch(row + step);           // everyone has taken this row's part
+        if (STAGED && row + step >= p.rows) pdl_launch_dependents();        // earlier, the next kernel's CTAs would be in the way of clusters
         // lane w of every warp has warp w's, later CTA w's
         auto join = [&](float& m, float& s, int& f) {
             const float its = m;
@@ -609,11 +610,12 @@ static int launch(void (*kernel)(P), const P& p, unsigned ctas, unsigned rows, u
 }
 
 // Form 2.  Clusters that the device holds at once: asked once per device and cluster size.
-template <int NV, bool F32>
+template <int THREADS, int NV, bool F32>
 static int launch_staying(SoftmaxParams p, int rows, cudaStream_t st) {
-    constexpr int THREADS = 512, SMEM = THREADS * NV * 16;
+    constexpr int SMEM = THREADS * NV * 16;
     static int known[64][4] = {};
-    const int c = p.ctas == 8 ? 3 : p.ctas / 2;
+    int c = 0;
+    while (1 << c < p.ctas) ++c;
     auto kernel = softmax_rows_kernel<THREADS, NV, F32, STAY>;
     cudaLaunchConfig_t cfg = {};
     cfg.blockDim = dim3(THREADS);
@@ -660,10 +662,14 @@ static int launch_softmax(SoftmaxParams p, int rows, cudaStream_t st) {
     if (each <= 2 * N16 * 256) return launch(softmax_rows_kernel<256, 2 * N16, F32, ONE_ROW>, p, ctas, rows, 256, st);
     if (each <= 2 * N16 * 512) {
         if (few || ctas == 1) return launch(softmax_rows_kernel<512, 2 * N16, F32, ONE_ROW>, p, ctas, rows, 512, st);
-        return launch_staying<2 * N16, F32>(p, rows, st);
+        // twice as many CTAs of half the threads where a cluster may be so large: 300 rows of 50257 28.5 -> 25.9 us (with 16 CTAs instead of 8,
+        // which needs leave, 384 rows of 131072 78 -> 90)
+        if (ctas == 8) return launch_staying<512, 2 * N16, F32>(p, rows, st);
+        p.ctas = 2 * ctas;
+        return launch_staying<256, 2 * N16, F32>(p, rows, st);
     }
     // a little more (a row that starts inside a vector has one more of them) is read twice rather than held by half as many CTAs
-    if (each > 2 * N16 * 640 && each <= 4 * N16 * 512) return launch_staying<4 * N16, F32>(p, rows, st);
+    if (each > 2 * N16 * 640 && each <= 4 * N16 * 512) return launch_staying<512, 4 * N16, F32>(p, rows, st);
     return launch(softmax_rows_kernel<512, 2 * N16, F32, READ_TWICE>, p, ctas, rows, 512, st);
 }
 
