@@ -39,7 +39,9 @@ __device__ __forceinline__ float warp_max(float x) {
 // Weights are exponentials against the warp's own maximum; the (maximum, sum) of warps meet in shared memory, those of the cluster's CTAs
 // by st.async (a cluster barrier waits for every store in front of it: 384 rows of 131072 in fp32 103 us with two a row), and a factor
 // takes a warp's weights to the row's probabilities.  NV vectors a thread.  FORM 0: a row a cluster; 1: what is behind NV vectors is read
-// twice; 2: clusters stay and go from row to row, the next row's part is copied to shared memory meanwhile.
+// twice; 2: clusters stay and go from row to row, the next row's part is copied to shared memory meanwhile (384 rows of 131072 78 us in fp32,
+// 5.2 TB/s, 73 in bf16; without the copy 124).  Clusters that stay let the next kernel in with their last row: at the start its CTAs take
+// places beside them (88).
 struct SoftmaxParams {
     const void* x;
     float* p;
