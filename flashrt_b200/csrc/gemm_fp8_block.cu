@@ -646,18 +646,37 @@ gemm_fp8_block_tile_kernel(const __grid_constant__ CUtensorMap tmA, const __grid
     pdl_launch_dependents();
 
     if (warp == 0) {
-        // ---------------- producer of this CTA's rows, bytes counted at the leader
+        // ---------------- producer of this CTA's rows, bytes counted at the leader; settled weights: the first ring of them before the wait
         const uint32_t ring = tc::smem_u32(smem), empty_a = tc::smem_u32(empty), full_a = tc::smem_u32(full);
         const uint32_t lead_full = CG == 1 ? full_a : tc::dsmem_map(full_a, leader);
-        pdl_wait();
+        const int ahead = p.early && unit < total ? min(STAGES, kb1 - kb0) : 0;
         int s = 0;
-        uint32_t ph = 1;
-        bool ready = true;
+        if (ahead) {
+            int mt, nt;
+            tile_at(unit, p.gm, m_tiles, n_tiles, mt, nt);
+            if (tc::elect_one())
+                for (int i = 0; i < ahead; ++i) {
+                    if (rank == 0) tc::mbar_arrive_expect_tx(full_a + 8 * i, CG * Cfg::STAGE_BYTES);
+                    load<CG>(ring + i * Cfg::STAGE_BYTES + Cfg::A_BYTES, &tmW, lead_full + 8 * i, (kb0 + i) * 128, nt * BN + (int)rank * (BN / CG));
+                }
+            __syncwarp();
+            pdl_wait();
+            if (tc::elect_one())
+                for (int i = 0; i < ahead; ++i)
+                    load<CG>(ring + i * Cfg::STAGE_BYTES, &tmA, lead_full + 8 * i, (kb0 + i) * 128, (mt * CG + (int)rank) * 128);
+            __syncwarp();
+            s = ahead % STAGES;
+        } else {
+            pdl_wait();
+        }
+        int skip = ahead;
+        uint32_t ph = ahead < STAGES;
+        bool ready = false;                                  // the first wait looks for itself
         for (int t = unit; t < total; t += units) {
             int mt, nt;
             tile_at(t, p.gm, m_tiles, n_tiles, mt, nt);
             const int m0 = (mt * CG + (int)rank) * 128, n0 = nt * BN + (int)rank * (BN / CG);
-            for (int kb = kb0; kb < kb1; ++kb) {
+            for (int kb = kb0 + skip; kb < kb1; ++kb) {
                 if (!tc::warp_wait(empty_a + 8 * s, ph, ready, deadline, abort_flag)) {
                     if (lane == 0) gave_up(p.status, abort_flag, ERR_PRODUCER);
                     t = total;
@@ -672,6 +691,7 @@ gemm_fp8_block_tile_kernel(const __grid_constant__ CUtensorMap tmA, const __grid
                     load<CG>(dst + Cfg::A_BYTES, &tmW, bar, kb * 128, n0);
                 }
             }
+            skip = 0;
         }
         // the last stages' returns arrive in this CTA's shared memory too: not after it has gone to another
         for (int i = 0; i < STAGES; ++i) {
