@@ -194,13 +194,6 @@ __device__ __forceinline__ float4 lds_v4(uint32_t a) {
     asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(a) : "memory");
     return v;
 }
-// four bytes from global to shared memory without a register between: nothing waits for them but cp.async.wait_group; absent ones are zero
-__device__ __forceinline__ void copy_4(uint32_t dst, const float* src, bool in) {
-    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(in ? 4 : 0) : "memory");
-}
-__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 // 8 columns of this thread's TMEM lane
 __device__ __forceinline__ void tmem_ld8(uint32_t taddr, uint32_t* v) {
     asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
@@ -217,27 +210,26 @@ __device__ __forceinline__ void store_one(const Params& p, size_t at, float v) {
 }
 
 // ---------------------------------------------------------------- up to 64 rows: weights on the lanes, tokens on the columns
-constexpr int LANE_SCALES = 4;
 template <int BN>
 struct LaneCfg {
     static constexpr int A_BYTES = 128 * 128, B_BYTES = BN * 128, STAGE_BYTES = A_BYTES + B_BYTES;
     static constexpr int STAGES = BN <= 32 ? 5 : 4;                          // about 100 KB: two CTAs per SM
     static constexpr int BUFS = BN == 64 ? 4 : 8;                            // accumulators: k-blocks under way
+    static constexpr int TMEM_COLS = BUFS * BN;
     static constexpr int RED_BYTES = 128 * BN * 4;                           // a rank's partial, where the ring was
     static_assert(RED_BYTES <= STAGES * STAGE_BYTES, "partials in the ring");
-    static constexpr int SLOT_BYTES = BN * 4 + 16;                            // a k-block's scales: tokens, weights
-    static constexpr int SCALE_BYTES = 4 * LANE_SCALES * SLOT_BYTES;         // of each epilogue warp
-    static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + 1024 + 256 + SCALE_BYTES;
-    static constexpr int TMEM_COLS = BUFS * BN;
+    static constexpr int HALVES = BN >= 64 ? 2 : 1, W = BN / HALVES;         // four warps of the epilogue for each half of the columns
+    static constexpr int THREADS = 32 * (3 + 4 * HALVES);                    // producer, issuer, scales
+    static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + 1024 + 256 + BUFS * BN * 4;
 };
 
 // S = 1: grid of as many CTAs as there is room for, each walks over n tiles.  S > 1: grid (n tiles, S), cluster (1, S), rank r takes the
 // k-blocks [kb r / S, kb (r + 1) / S); the ranks then lay their partials into shared memory and each finishes every S-th four tokens.
 template <int BN>
-__global__ void __launch_bounds__(192, 2)
+__global__ void __launch_bounds__(LaneCfg<BN>::THREADS, 2)
 gemm_fp8_block_lane_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmW, Params p) {
     using Cfg = LaneCfg<BN>;
-    constexpr int STAGES = Cfg::STAGES, BUFS = Cfg::BUFS;
+    constexpr int STAGES = Cfg::STAGES, BUFS = Cfg::BUFS, W = Cfg::W, LW = (BN == 64 ? 8 : 16);
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
     uint64_t* full = reinterpret_cast<uint64_t*>(smem + STAGES * Cfg::STAGE_BYTES);
@@ -247,7 +239,7 @@ gemm_fp8_block_lane_kernel(const __grid_constant__ CUtensorMap tmA, const __grid
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + BUFS);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
     static_assert((2 * STAGES + 2 * BUFS) * 8 + 8 <= 256, "barriers");
-    uint8_t* scales = smem + STAGES * Cfg::STAGE_BYTES + 256;
+    const uint32_t scale_a = tc::smem_u32(smem + STAGES * Cfg::STAGE_BYTES + 256);
     const uint64_t deadline = tc::global_timer_ns() + FRT_KERNEL_DEADLINE_NS;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int S = (int)gridDim.y, rank = (int)blockIdx.y, tiles = (p.N + 127) / 128;
@@ -259,8 +251,8 @@ gemm_fp8_block_lane_kernel(const __grid_constant__ CUtensorMap tmA, const __grid
             tc::mbar_init(&empty[s], 1);
         }
         for (int i = 0; i < BUFS; ++i) {
-            tc::mbar_init(&acc_full[i], 1);
-            tc::mbar_init(&acc_empty[i], 4);
+            tc::mbar_init(&acc_full[i], 2);                  // the products, the scales
+            tc::mbar_init(&acc_empty[i], 4 * Cfg::HALVES);
         }
         *abort_flag = 0;
         tc::mbar_fence_init();
@@ -343,63 +335,85 @@ gemm_fp8_block_lane_kernel(const __grid_constant__ CUtensorMap tmA, const __grid
                 if (++s == STAGES) { s = 0; ph ^= 1; }
                 if (++buf == BUFS) { buf = 0; bph ^= 1; }
             }
-    } else {
-        // ---------------- epilogue: warps 2..5, lane quadrant = warp % 4; a thread's lane is one output channel
+    } else if (warp == 2) {
+        // ---------------- scales of a k-block, a buffer's beside it: of its tokens times the weights', a lane has every 32nd.  Four blocks'
+        // loads are under way.  Tokens behind the last have its scale: what they make of it is not stored.
         pdl_wait();
-        const int q = warp & 3;
-        const uint32_t t_src = tmem + ((uint32_t)(q * 32) << 16);
-        const uint32_t sc = tc::smem_u32(scales) + (warp - 2) * (LANE_SCALES * Cfg::SLOT_BYTES);
-        constexpr int PER = (BN + 31) / 32;                    // scales of a lane
+        constexpr int PER = (BN + 31) / 32;
+        struct Scales { float a[PER], w; };
+        int row[PER], buf = 0;
+        uint32_t bph = 1;
+#pragma unroll
+        for (int i = 0; i < PER; ++i) row[i] = min(lane + 32 * i, p.M - 1);
+        for (int t = (int)blockIdx.x; t < tiles; t += (int)gridDim.x) {
+            const float* ws = p.w_scale + (size_t)t * p.kb + kb0;
+            const float* as = p.a_scale + kb0 * p.a_stride;
+            auto ask = [&](int kb, Scales& r) {              // block after block
+                if (kb >= kb1) return;
+                r.w = *ws++;
+#pragma unroll
+                for (int i = 0; i < PER; ++i) r.a[i] = as[row[i]];
+                as += p.a_stride;
+            };
+            auto give = [&](const Scales& r) {
+                if (!tc::mbar_wait_until(tc::smem_u32(&acc_empty[buf]), bph, deadline, abort_flag)) gave_up(p.status, abort_flag, ERR_EPILOGUE);
+                const uint32_t to = scale_a + buf * (BN * 4) + lane * 4;
+#pragma unroll
+                for (int i = 0; i < PER; ++i)
+                    if (BN >= 32 || lane < BN) asm volatile("st.shared.f32 [%0], %1;" ::"r"(to + 128 * i), "f"(__fmul_rn(r.a[i], r.w)) : "memory");
+                __syncwarp();
+                if (lane == 0) tc::mbar_arrive(&acc_full[buf]);
+                if (++buf == BUFS) { buf = 0; bph ^= 1; }
+            };
+            Scales r[4] = {};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) ask(kb0 + i, r[i]);
+            for (int kb = kb0; kb < kb1; kb += 4)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (kb + i < kb1) {
+                        give(r[i]);
+                        ask(kb + i + 4, r[i]);
+                    }
+            if (__any_sync(0xffffffffu, *abort_flag != 0)) break;
+        }
+    } else {
+        // ---------------- epilogue: lane quadrant = warp % 4, a thread's lane is one output channel; a half of the tokens
+        pdl_wait();
+        const int q = warp & 3, half = (warp - 3) >> 2;
+        const uint32_t t_src = tmem + ((uint32_t)(q * 32) << 16) + half * W;
         int buf = 0;
         uint32_t bph = 0;
         bool ok = true;
         for (int t = (int)blockIdx.x; t < tiles && ok; t += (int)gridDim.x) {
             const int n = t * 128 + q * 32 + lane;
-            const bool in = n < p.N;
-            float acc[BN];
+            float acc[W];
 #pragma unroll
-            for (int j = 0; j < BN; ++j) acc[j] = 0.0f;
-            // scales of a k-block come LANE_SCALES - 1 blocks ahead into the warp's own shared memory, token by token, the weights' behind them
-            auto ask = [&](int kb) {
-                if (kb < kb1) {
-                    const uint32_t to = sc + (kb % LANE_SCALES) * Cfg::SLOT_BYTES;
-#pragma unroll
-                    for (int i = 0; i < PER; ++i) {
-                        const int m = lane + 32 * i;
-                        if (BN >= 32 || lane < BN) copy_4(to + m * 4, p.a_scale + (m < p.M ? kb * p.a_stride + m : 0), m < p.M);
-                    }
-                    if (lane == 0) copy_4(to + BN * 4, p.w_scale + (size_t)t * p.kb + kb, true);
-                }
-                copy_commit();
-            };
-            for (int i = 0; i < LANE_SCALES - 1; ++i) ask(kb0 + i);
+            for (int j = 0; j < W; ++j) acc[j] = 0.0f;
             for (int kb = kb0; kb < kb1; ++kb) {
-                const uint32_t slot = sc + (kb % LANE_SCALES) * Cfg::SLOT_BYTES;
-                ask(kb + LANE_SCALES - 1);
-                copy_wait<LANE_SCALES - 1>();
-                __syncwarp();
-                float w_s;
-                asm volatile("ld.shared.f32 %0, [%1];" : "=f"(w_s) : "r"(slot + BN * 4) : "memory");
                 ok = tc::warp_wait(tc::smem_u32(&acc_full[buf]), bph, false, deadline, abort_flag);
                 if (!ok) {
                     if (lane == 0) gave_up(p.status, abort_flag, ERR_EPILOGUE);
                     break;
                 }
                 tc::tc_fence_after_sync();
+                const uint32_t src = t_src + buf * BN, slot = scale_a + buf * (BN * 4) + half * (W * 4);
 #pragma unroll
-                for (int c = 0; c < BN; c += 16) {
-                    if (c >= p.M) break;
-                    uint32_t v[16];
-                    __syncwarp();
-                    tc::tmem_ld16(t_src + buf * BN + c, v);
+                for (int c = 0; c < W; c += LW) {
+                    if (half * W + c >= p.M) break;
+                    uint32_t v[LW];
+                    float4 f[LW / 4];
+                    tmem_ld<LW>(src + c, v);
+#pragma unroll
+                    for (int j = 0; j < LW / 4; ++j) f[j] = lds_v4(slot + c * 4 + j * 16);
                     tc::tmem_ld_wait();
 #pragma unroll
-                    for (int j = 0; j < 16; j += 4) {
-                        const float4 f = lds_v4(slot + (c + j) * 4);
-                        acc[c + j] = __fmaf_rn(__uint_as_float(v[j]), __fmul_rn(f.x, w_s), acc[c + j]);
-                        acc[c + j + 1] = __fmaf_rn(__uint_as_float(v[j + 1]), __fmul_rn(f.y, w_s), acc[c + j + 1]);
-                        acc[c + j + 2] = __fmaf_rn(__uint_as_float(v[j + 2]), __fmul_rn(f.z, w_s), acc[c + j + 2]);
-                        acc[c + j + 3] = __fmaf_rn(__uint_as_float(v[j + 3]), __fmul_rn(f.w, w_s), acc[c + j + 3]);
+                    for (int j = 0; j < LW; j += 4) {
+                        const float4 s = f[j / 4];
+                        const uint64_t r0 = fma_f32x2(f32x2(__uint_as_float(v[j]), __uint_as_float(v[j + 1])), f32x2(s.x, s.y), f32x2(acc[c + j], acc[c + j + 1]));
+                        const uint64_t r1 = fma_f32x2(f32x2(__uint_as_float(v[j + 2]), __uint_as_float(v[j + 3])), f32x2(s.z, s.w), f32x2(acc[c + j + 2], acc[c + j + 3]));
+                        f32x2_parts(r0, acc[c + j], acc[c + j + 1]);
+                        f32x2_parts(r1, acc[c + j + 2], acc[c + j + 3]);
                     }
                 }
                 tc::tc_fence_before_sync();
@@ -407,31 +421,30 @@ gemm_fp8_block_lane_kernel(const __grid_constant__ CUtensorMap tmA, const __grid
                 if (lane == 0) tc::mbar_arrive(&acc_empty[buf]);
                 if (++buf == BUFS) { buf = 0; bph ^= 1; }
             }
-            copy_wait<0>();
-            __syncwarp();                                      // the next tile's scales go to the same place
             if (!ok) break;
             if (S > 1) {                                       // [four tokens][channel]: a warp's store is 512 contiguous bytes
-                const uint32_t red = tc::smem_u32(smem) + (uint32_t)(q * 32 + lane) * 16;
+                const uint32_t red = tc::smem_u32(smem) + (uint32_t)(half * (W / 4) * 128 + q * 32 + lane) * 16;
 #pragma unroll
-                for (int j = 0; j < BN; j += 4)
-                    if (j < p.M) sts_v4(red + j * 512, acc[j], acc[j + 1], acc[j + 2], acc[j + 3]);
-            } else if (in) {
+                for (int j = 0; j < W; j += 4)
+                    if (half * W + j < p.M) sts_v4(red + j * 512, acc[j], acc[j + 1], acc[j + 2], acc[j + 3]);
+            } else if (n < p.N) {
                 const float bias = p.bias ? __bfloat162float(p.bias[n]) : 0.0f;
+                const size_t at = (size_t)(half * W) * p.N + n;
 #pragma unroll
-                for (int j = 0; j < BN; ++j)
-                    if (j < p.M) store_one(p, (size_t)j * p.N + n, p.bias ? __fadd_rn(acc[j], bias) : acc[j]);
+                for (int j = 0; j < W; ++j)
+                    if (half * W + j < p.M) store_one(p, at + (size_t)j * p.N, p.bias ? __fadd_rn(acc[j], bias) : acc[j]);
             }
         }
     }
     if (S > 1) {
         __syncwarp();
         tc::cluster_sync_all();                              // all partials are there
-        if (warp >= 2 && !*abort_flag) {
-            const int q = warp & 3, n = (int)blockIdx.x * 128 + q * 32 + lane;
+        if (warp >= 3 && !*abort_flag) {
+            const int q = warp & 3, half = (warp - 3) >> 2, n = (int)blockIdx.x * 128 + q * 32 + lane;
             const bool in = n < p.N;
             const float bias = in && p.bias ? __bfloat162float(p.bias[n]) : 0.0f;
             const uint32_t red = tc::smem_u32(smem) + (uint32_t)(q * 32 + lane) * 16;
-            for (int g = rank; 4 * g < p.M; g += S) {        // four tokens; the ranks' partials are all on their way before the first is added
+            for (int g = rank + S * half; 4 * g < p.M; g += S * Cfg::HALVES) {   // four tokens; the ranks' partials are all on their way before the first is added
                 float4 w[8];
 #pragma unroll
                 for (int r = 0; r < 8; ++r)
@@ -923,7 +936,7 @@ static int launch_lane(const void* A, const void* W, Params p, int K, int splits
     cudaLaunchConfig_t cfg = {};
     cudaLaunchAttribute attr[2];
     cfg.gridDim = dim3(splits > 1 || tiles < room ? tiles : room, splits);
-    cfg.blockDim = dim3(192);
+    cfg.blockDim = dim3(Cfg::THREADS);
     cfg.dynamicSmemBytes = Cfg::SMEM_BYTES;
     set_attrs(cfg, attr, 1, (unsigned)splits, stream);
     const cudaError_t e = cudaLaunchKernelEx(&cfg, gemm_fp8_block_lane_kernel<BN>, tmA, tmW, p);
@@ -1062,8 +1075,7 @@ extern "C" int frt_b200_gemm_fp8_block_nt(const void* A, const void* W, void* D,
     p.f32 = flags & 2;
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
     const int sms = device_sm_count(), n128 = (N + 127) / 128, n256 = (N + 255) / 256;
-    // 33 to 64 rows of wide weights: as rows of tiles the tokens are staged half as often (64 x 32768 x 2048 16.6 us against 18.1)
-    if (M <= 32 || (M <= 64 && 4 * n256 < 3 * sms)) {
+    if (M <= 64) {
         // K splits (a cluster) while the tiles alone leave SMs idle and every rank keeps two k-blocks
         int splits = 1;
         while (splits < 8 && n128 * splits * 2 <= 2 * sms && p.kb / (splits * 2) >= 2) splits *= 2;
