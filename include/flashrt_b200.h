@@ -584,7 +584,8 @@ int frt_b200_quantize_fp8_groups(const void* in_bf16, long long in_stride, void*
                                  int rows, int dim, int flags, void* stream);
 /* D(M,N) = sum_j a_scale[j][m] * w_scale[n / 128][j] * (sum_{k in block j} A[m][k] W[n][k]) + bias[n], blocks j of 128 along K
  *   (no counterpart in the reference): A (M, K) and W (N, K) E4M3, K contiguous, 16-byte aligned; a_scale (ceil(K / 128), a_scale_stride >= M)
- *   as the quantiser leaves it, w_scale (ceil(N / 128), ceil(K / 128)) fp32; bias (N) bf16 or NULL; D bf16, with flags bit 1 fp32 (logits).
+ *   as the quantiser leaves it, w_scale (ceil(N / 128), ceil(K / 128)) fp32; bias (N) bf16 or NULL; D 16-byte aligned, bf16, with flags bit 1
+ *   fp32 (logits).
  *   Sums are fp32, over a block of 128 in the tensor core, then block by block, each scaled; the order of the blocks is that of K, where K
  *   is split over CTAs (few rows, few tiles) that of the parts.  K % 16 == 0, K <= 2^20; any M and N up to 2^30.  flags bit 0: the weights
  *   are settled and may be read before the kernel in front has ended.  A wait that gave up shows in frt_b200_gemm_status. */
@@ -631,8 +632,8 @@ int frt_b200_paged_plan(const int* kept_lens, const int* new_lens, int* block_ta
                         const int* free_in, int* free_out, int* cu_seqlens, int* seq_lens, int* positions, long long* slots,
                         int* refused, int tokens, int batch, int num_blocks, int block_size, int flags, void* stream);
 /* Tokens are dropped (no counterpart in the reference): drafted ones that do not stand (kept_lens of frt_b200_verify_drafts), or a whole
- *   sequence (0).  The table's entries of blocks behind ceil(kept_lens / block_size), up to ceil(seq_lens / block_size), become -1; those
- *   that are blocks of the pool go on the list, a sequence's last one and the last sequence's first, so that a plan that takes as many finds
+ *   sequence (0).  Of the table's entries of blocks behind ceil(kept_lens / block_size), up to ceil(seq_lens / block_size), those that are
+ *   blocks of the pool become -1 and go on the list, a sequence's last one and the last sequence's first, so that a plan that takes as many finds
  *   them in their old places.  *free_out = *free_in + their number, at most num_blocks; not free_in itself.  Blocks carry no count of
  *   their users: one that two rows share is put on the list by each that drops it. */
 int frt_b200_paged_release(const int* kept_lens, const int* seq_lens, int* block_table, int table_stride, int* free_list,

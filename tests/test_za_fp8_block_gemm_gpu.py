@@ -239,3 +239,30 @@ def test_streams_and_graph():
         torch.cuda.synchronize()
         assert torch.equal(got, out) and got.abs().max() > 0
     assert fvk.tensor_core_status() == 0
+
+
+@pytest.mark.parametrize("m,n,k", [(5, 700, 4096), (48, 1001, 1024), (96, 4096, 512), (130, 4096, 4096), (817, 2048, 4096), (2100, 1800, 640)])
+def test_settled_weights_behind_the_quantiser(m, n, k):
+    """Weights read early, activations not: quantiser and product in turn over one pair of buffers give the bits of products that wait for all."""
+    from flashrt_b200 import flash_rt_kernels as fvk
+    _, w, _, sw, _ = (t.cuda() for t in operands(2, n, k, m))
+    xs = [torch.randn(m, k, generator=torch.Generator().manual_seed(i)).to(BF16).cuda() for i in range(8)]
+    q, s = torch.empty(m, k, dtype=E4M3, device="cuda"), torch.empty((k + 127) // 128, m, device="cuda")
+    outs = {pdl: [torch.zeros(m, n, dtype=BF16, device="cuda") for _ in xs] for pdl in (False, True)}
+
+    def chain(pdl):
+        for x, out in zip(xs, outs[pdl]):
+            fvk.quantize_fp8_groups(x.data_ptr(), q.data_ptr(), s.data_ptr(), m, k, _stream())
+            fvk.GemmRunner().fp8_block_nt(q.data_ptr(), w.data_ptr(), out.data_ptr(), m, n, k, s.data_ptr(), sw.data_ptr(), _stream(), pdl=pdl)
+    chain(False)
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        chain(True)
+    for _ in range(3):
+        graph.replay()
+    torch.cuda.synchronize()
+    for plain, early in zip(outs[False], outs[True]):
+        assert torch.equal(plain, early) and plain.abs().max() > 0
+    assert fvk.tensor_core_status() == 0
