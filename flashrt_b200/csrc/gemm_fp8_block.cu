@@ -52,35 +52,31 @@ struct Quotient {
     }
 };
 
-template <int U>
-__global__ void __launch_bounds__(256)
+template <int U, bool DOWN>
+__global__ void __launch_bounds__(256, U == 2 ? 6 : 1)
 quantize_groups_kernel(const __nv_bfloat16* x, long long x_stride, uint8_t* out, float* scale, long long scale_stride, int rows, int dim,
-                       int groups, unsigned items, int down) {
+                       int groups) {
     pdl_launch_dependents();
     pdl_wait();
     const int me = threadIdx.x & 7;
-    const unsigned slot = threadIdx.x >> 3, first = blockIdx.x * (32u * U) + slot;
-    // down: a block has 32 rows of U neighbouring groups, so that its scales fill lines; otherwise (row, group) in one row, group fastest
-    const unsigned across = (unsigned)(groups + U - 1) / U, row0 = down ? blockIdx.x / across * 32u + slot : 0, grp0 = down ? blockIdx.x % across * U : 0;
+    const unsigned slot = threadIdx.x >> 3, across = (unsigned)(groups + U - 1) / U;
+    const unsigned block_row = DOWN ? blockIdx.x / across : 0, item = DOWN ? 0 : blockIdx.x * 32u + slot;
+    const int row = DOWN ? (int)(block_row * 32u + slot) : (int)(item / (unsigned)groups);
+    const int grp = DOWN ? (int)((blockIdx.x - block_row * across) * U) : (int)(item - (unsigned)row * (unsigned)groups);
     const bool wide = ((reinterpret_cast<uintptr_t>(x) | (uintptr_t)(x_stride * 2)) & 31) == 0;
+    auto there = [&](int i) { return row < rows && grp + i < groups; };
+    auto in = [&](int i) { return there(i) && (grp + i) * 128 + me * 16 < dim; };
     uint32_t v[U][8];
-    int row[U], grp[U];
-    bool in[U], there[U];
 #pragma unroll
     for (int i = 0; i < U; ++i) {
-        const unsigned item = first + 32u * i;
-        row[i] = down ? (int)row0 : (int)(item / (unsigned)groups);
-        grp[i] = down ? (int)(grp0 + i) : (int)(item - (unsigned)row[i] * (unsigned)groups);
-        there[i] = row[i] < rows && grp[i] < groups;
-        in[i] = there[i] && grp[i] * 128 + me * 16 < dim;
-        const __nv_bfloat16* src = x + (in[i] ? row[i] * x_stride + grp[i] * 128 + me * 16 : 0);
+        const __nv_bfloat16* src = x + (in(i) ? row * x_stride + (grp + i) * 128 + me * 16 : 0);
         ld_stream_32(src, wide, true, v[i]);
     }
 #pragma unroll
     for (int i = 0; i < U; ++i) {
         float f[16], top = 0.0f;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) unpack_bf16x2(in[i] ? v[i][j] : 0u, f[2 * j], f[2 * j + 1]);
+        for (int j = 0; j < 8; ++j) unpack_bf16x2(in(i) ? v[i][j] : 0u, f[2 * j], f[2 * j + 1]);
 #pragma unroll
         for (int j = 0; j < 16; ++j) top = fmaxf(top, fabsf(f[j]));
 #pragma unroll
@@ -100,14 +96,14 @@ quantize_groups_kernel(const __nv_bfloat16* x, long long x_stride, uint8_t* out,
         }
         top = fmaxf(top, 448e-12f);
         const Quotient q(top);
-        if (in[i]) {
+        if (in(i)) {
             uint4 o;
             uint32_t* w = &o.x;
 #pragma unroll
             for (int j = 0; j < 4; ++j) w[j] = q(f + 4 * j);
-            st_global_v4(out + (size_t)row[i] * dim + grp[i] * 128 + me * 16, o);
+            st_global_v4(out + (size_t)row * dim + (grp + i) * 128 + me * 16, o);
         }
-        if (me == 0 && there[i]) scale[grp[i] * scale_stride + row[i]] = __fdiv_rn(top, 448.0f);
+        if (me == 0 && there(i)) scale[(grp + i) * scale_stride + row] = __fdiv_rn(top, 448.0f);
         __syncwarp();
     }
 }
@@ -1011,13 +1007,11 @@ static long long tile_clusters() {
     return known[dev] - 1;
 }
 
-template <int U>
+template <int U, bool DOWN>
 static int launch_quantize(const void* x, long long stride, void* out, float* scale, long long scale_stride, int rows, int dim, cudaStream_t stream) {
     const int groups = (dim + 127) / 128;
-    const unsigned items = (unsigned)((long long)rows * groups);
     cudaLaunchConfig_t cfg = {};
-    const int down = rows >= 32 * U;
-    cfg.gridDim = dim3(down ? (unsigned)((rows + 31) / 32) * (unsigned)((groups + U - 1) / U) : (items + 32 * U - 1) / (32 * U));
+    cfg.gridDim = dim3(DOWN ? (unsigned)((rows + 31) / 32) * (unsigned)((groups + U - 1) / U) : ((unsigned)rows * (unsigned)groups + 31u) / 32u);
     cfg.blockDim = dim3(256);
     cfg.stream = stream;
     cudaLaunchAttribute attr[1];
@@ -1025,8 +1019,8 @@ static int launch_quantize(const void* x, long long stride, void* out, float* sc
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, quantize_groups_kernel<U>, static_cast<const __nv_bfloat16*>(x), stride,
-                                             static_cast<uint8_t*>(out), scale, scale_stride, rows, dim, groups, items, down);
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, quantize_groups_kernel<U, DOWN>, static_cast<const __nv_bfloat16*>(x), stride,
+                                             static_cast<uint8_t*>(out), scale, scale_stride, rows, dim, groups);
     return e == cudaSuccess ? FRT_OK : FRT_CUDA_ERR(e);
 }
 
@@ -1045,9 +1039,10 @@ extern "C" int frt_b200_quantize_fp8_groups(const void* in_bf16, long long in_st
     if (!in_bf16 || !out8 || !group_scale) return FRT_ERR_INVALID;
     if (misaligned(in_bf16, 16) || misaligned(out8, 16) || misaligned(group_scale, 4)) return FRT_ERR_INVALID;
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (rows < 32) return f8b::launch_quantize<1, false>(in_bf16, in_stride, out8, group_scale, scale_stride, rows, dim, st);
     const bool few = (long long)rows * ((dim + 127) / 128) < 256ll * device_sm_count();
-    if (few) return f8b::launch_quantize<1>(in_bf16, in_stride, out8, group_scale, scale_stride, rows, dim, st);
-    return f8b::launch_quantize<4>(in_bf16, in_stride, out8, group_scale, scale_stride, rows, dim, st);
+    if (few) return f8b::launch_quantize<1, true>(in_bf16, in_stride, out8, group_scale, scale_stride, rows, dim, st);
+    return f8b::launch_quantize<2, true>(in_bf16, in_stride, out8, group_scale, scale_stride, rows, dim, st);
 }
 
 extern "C" int frt_b200_gemm_fp8_block_nt(const void* A, const void* W, void* D, int M, int N, int K, const float* a_scale,
