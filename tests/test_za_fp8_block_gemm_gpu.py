@@ -43,6 +43,12 @@ def test_quantize_groups(rows, dim):
     check_codes(x, *quantize(x.cuda()))
 
 
+@pytest.mark.parametrize("rows,dim", [(31, 4112), (32, 4112), (33, 160), (63, 80000), (64, 80000), (9001, 528)])
+def test_quantize_blocks_of_rows(rows, dim):
+    """Rows on both sides of a block of 32, an odd number of groups, more rows than whole blocks have."""
+    test_quantize_groups(rows, dim)
+
+
 def test_quantize_every_significand():
     """Every pair of bf16 significands (value, largest) at four exponents: all quotients that the definition can meet."""
     sig = (1.0 + torch.arange(128) / 128).to(F64)
