@@ -39,9 +39,9 @@ __device__ __forceinline__ float warp_max(float x) {
 // Weights are exponentials against the warp's own maximum; the (maximum, sum) of warps meet in shared memory, those of the cluster's CTAs
 // by st.async (a cluster barrier waits for every store in front of it: 384 rows of 131072 in fp32 103 us with two a row), and a factor
 // takes a warp's weights to the row's probabilities.  NV vectors a thread.  FORM 0: a row a cluster; 1: what is behind NV vectors is read
-// twice; 2: clusters stay and go from row to row, the next row's part is copied to shared memory meanwhile (384 rows of 131072 78 us in fp32,
-// 5.2 TB/s, 73 in bf16; without the copy 124).  Clusters that stay let the next kernel in with their last row: at the start its CTAs take
-// places beside them (88).
+// twice; 2: clusters stay and go from row to row, the next row's part is copied to shared memory meanwhile (384 rows of 131072 71 us in fp32,
+// 5.7 TB/s, 63 in bf16; without the copy 124).  Clusters that stay let the next kernel in with their last row: at the start its CTAs take
+// places beside them (88, when a row took 78).
 struct SoftmaxParams {
     const void* x;
     float* p;
@@ -57,7 +57,7 @@ struct Yes { static constexpr bool value = true; };
 struct No { static constexpr bool value = false; };
 
 template <int THREADS, int NV, bool F32, int FORM>
-__global__ void __launch_bounds__(THREADS, NV * (F32 ? 4 : 8) > 32 ? 1 : 1024 / THREADS)
+__global__ void __launch_bounds__(THREADS, (NV * (F32 ? 4 : 8) > 32 ? 512 : 1024) / THREADS)
 softmax_rows_kernel(SoftmaxParams p) {
     constexpr int VE = F32 ? 4 : 8, ES = F32 ? 4 : 2, WARPS = THREADS / 32;      // values of 16 bytes, bytes of a value
     constexpr bool HELD = FORM != READ_TWICE, STAGED = FORM == STAY;
@@ -664,11 +664,9 @@ static int launch_softmax(SoftmaxParams p, int rows, cudaStream_t st) {
     if (each <= 2 * N16 * 256) return launch(softmax_rows_kernel<256, 2 * N16, F32, ONE_ROW>, p, ctas, rows, 256, st);
     if (each <= 2 * N16 * 512) {
         if (few || ctas == 1) return launch(softmax_rows_kernel<512, 2 * N16, F32, ONE_ROW>, p, ctas, rows, 512, st);
-        // twice as many CTAs of half the threads where a cluster may be so large: 300 rows of 50257 28.5 -> 25.9 us (with 16 CTAs instead of 8,
-        // which needs leave, 384 rows of 131072 78 -> 90)
-        if (ctas == 8) return launch_staying<512, 2 * N16, F32>(p, rows, st);
-        p.ctas = 2 * ctas;
-        return launch_staying<256, 2 * N16, F32>(p, rows, st);
+        // 64 values a thread: with 32, twice the threads and as many rows under way, 384 rows of 131072 79 us instead of 71 (bf16 73 instead
+        // of 63), 300 of 50257 27.2 instead of 25.2; on 16 CTAs a row, which needs leave, 90
+        return launch_staying<256, 4 * N16, F32>(p, rows, st);
     }
     // a little more (a row that starts inside a vector has one more of them) is read twice rather than held by half as many CTAs
     if (each > 2 * N16 * 640 && each <= 4 * N16 * 512) return launch_staying<512, 4 * N16, F32>(p, rows, st);

@@ -86,6 +86,26 @@ def test_softmax_masks_and_special_values():
                 assert torch.allclose(p[r], (hit / hit.sum()).float().cpu(), rtol=1e-6, atol=0)
 
 
+@pytest.mark.parametrize("rows,vocab", [(700, 20001), (320, 50257), (170, 131071), (160, 131072), (80, 230001)])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_softmax_clusters_that_go_from_row_to_row(rows, vocab, dtype):
+    """More rows than clusters find room, of every kind, one behind the other."""
+    x = (torch.randn(rows, vocab, device="cuda", generator=torch.Generator("cuda").manual_seed(vocab)) * 4).to(dtype)
+    x[3::17] = -INF
+    x[5::17, 1:] = -INF
+    x[7::17, ::3] = NAN
+    x[8::17, vocab // 2] = INF
+    x[11::17, :vocab - 1] = torch.finfo(dtype).min
+    t = torch.full((rows,), 0.7)
+    t[2::5], t[4::7] = 0.0, 3.0
+    t = t.cuda()
+    p = softmax(x, t)
+    assert not p.isnan().any()
+    for r in range(0, rows, 64):
+        close(p[r:r + 64], x[r:r + 64], t[r:r + 64])
+    assert torch.equal(p, softmax(x, t))
+
+
 def test_softmax_ties_and_strides():
     x = torch.zeros(6, 30000)
     x[1, 29999], x[2, 777], x[2, 20000], x[3, :] = 1, 2, 2, -5
