@@ -207,24 +207,25 @@ __device__ __forceinline__ void store_one(const Params& p, size_t at, float v) {
     else static_cast<__nv_bfloat16*>(p.out)[at] = __float2bfloat16_rn(v);
 }
 
-// ---------------------------------------------------------------- up to 64 rows: weights on the lanes, tokens on the columns
+// ---------------------------------------------------------------- up to 64 rows (128 of narrow weights): weights on the lanes, tokens on the columns
 template <int BN>
 struct LaneCfg {
     static constexpr int A_BYTES = 128 * 128, B_BYTES = BN * 128, STAGE_BYTES = A_BYTES + B_BYTES;
-    static constexpr int STAGES = BN <= 32 ? 5 : 4;                          // about 100 KB: two CTAs per SM
-    static constexpr int BUFS = BN == 64 ? 4 : 8;                            // accumulators: k-blocks under way
-    static constexpr int TMEM_COLS = BUFS * BN;
+    static constexpr int PER_SM = BN <= 64 ? 2 : 1;                          // CTAs: of about 100 KB, or of all there is
+    static constexpr int STAGES = BN <= 32 ? 5 : BN == 64 ? 4 : BN == 96 ? 7 : 6;
+    static constexpr int BUFS = BN <= 32 ? 8 : 4, BUF_COLS = BN == 96 ? 128 : BN, TMEM_COLS = BUFS * BUF_COLS;      // accumulators: k-blocks under way
     static constexpr int RED_BYTES = 128 * BN * 4;                           // a rank's partial, where the ring was
     static_assert(RED_BYTES <= STAGES * STAGE_BYTES, "partials in the ring");
     static constexpr int HALVES = BN >= 64 ? 2 : 1, W = BN / HALVES;         // four warps of the epilogue for each half of the columns
     static constexpr int THREADS = 32 * (3 + 4 * HALVES);                    // producer, issuer, scales
     static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + 1024 + 256 + BUFS * BN * 4;
+    static_assert(PER_SM * TMEM_COLS <= 512 && PER_SM * (SMEM_BYTES + 1024) <= 228 * 1024, "CTAs of an SM");
 };
 
 // S = 1: grid of as many CTAs as there is room for, each walks over n tiles.  S > 1: grid (n tiles, S), cluster (1, S), rank r takes the
 // k-blocks [kb r / S, kb (r + 1) / S); the ranks then lay their partials into shared memory and each finishes every S-th four tokens.
 template <int BN>
-__global__ void __launch_bounds__(LaneCfg<BN>::THREADS, 2)
+__global__ void __launch_bounds__(LaneCfg<BN>::THREADS, LaneCfg<BN>::PER_SM)
 gemm_fp8_block_lane_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmW, Params p) {
     using Cfg = LaneCfg<BN>;
     constexpr int STAGES = Cfg::STAGES, BUFS = Cfg::BUFS, W = Cfg::W, LW = (BN == 64 ? 8 : 16);
@@ -325,7 +326,7 @@ gemm_fp8_block_lane_kernel(const __grid_constant__ CUtensorMap tmA, const __grid
                 if (tc::elect_one()) {
                     const uint64_t so = (uint64_t)(s * (Cfg::STAGE_BYTES >> 4));
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) tc::mma_f8(tmem + buf * BN, dA0 + so + 2 * k, dB0 + so + 2 * k, idesc, k > 0 ? 1u : 0u);
+                    for (int k = 0; k < 4; ++k) tc::mma_f8(tmem + buf * Cfg::BUF_COLS, dA0 + so + 2 * k, dB0 + so + 2 * k, idesc, k > 0 ? 1u : 0u);
                     tc::mma_commit(empty_a + 8 * s);
                     tc::mma_commit(accF_a + 8 * buf);
                 }
@@ -395,7 +396,7 @@ gemm_fp8_block_lane_kernel(const __grid_constant__ CUtensorMap tmA, const __grid
                     break;
                 }
                 tc::tc_fence_after_sync();
-                const uint32_t src = t_src + buf * BN, slot = scale_a + buf * (BN * 4) + half * (W * 4);
+                const uint32_t src = t_src + buf * Cfg::BUF_COLS, slot = scale_a + buf * (BN * 4) + half * (W * 4);
 #pragma unroll
                 for (int c = 0; c < W; c += LW) {
                     if (half * W + c >= p.M) break;
@@ -930,7 +931,7 @@ static int launch_lane(const void* A, const void* W, Params p, int K, int splits
     int rc = make_tmap_2d_u8(&tmA, A, (uint64_t)p.M, (uint64_t)K, (uint64_t)K, BN);
     if (!rc) rc = make_tmap_2d_u8(&tmW, W, (uint64_t)p.N, (uint64_t)K, (uint64_t)K, 128);
     if (rc) return rc;
-    const int tiles = (p.N + 127) / 128, room = 2 * device_sm_count();
+    const int tiles = (p.N + 127) / 128, room = Cfg::PER_SM * device_sm_count();
     cudaLaunchConfig_t cfg = {};
     cudaLaunchAttribute attr[2];
     cfg.gridDim = dim3(splits > 1 || tiles < room ? tiles : room, splits);
@@ -979,27 +980,25 @@ static int launch_tile(const void* A, const void* W, Params p, int K, cudaStream
 }
 
 // Clusters of a sharing form that the device holds at once (a cluster lies in one GPC, whose SMs its size need not divide): asked once.
-template <int CG, int BN, int S>
-static long long tile_clusters() {
-    using Cfg = TileCfg<CG, BN>;
-    static int known[64] = {0};
+template <int SMEM, typename K>
+static long long clusters_held(int (&known)[64], K kernel, dim3 cluster, int threads) {
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 0;
     if (!known[dev]) {
         cudaLaunchConfig_t cfg = {};
-        cfg.gridDim = dim3(CG * S);
-        cfg.blockDim = dim3(TILE_THREADS);
-        cfg.dynamicSmemBytes = Cfg::SMEM_BYTES;
+        cfg.gridDim = cluster;
+        cfg.blockDim = dim3(threads);
+        cfg.dynamicSmemBytes = SMEM;
         cudaLaunchAttribute attr[1];
         attr[0].id = cudaLaunchAttributeClusterDimension;
-        attr[0].val.clusterDim.x = CG * S;
-        attr[0].val.clusterDim.y = 1;
+        attr[0].val.clusterDim.x = cluster.x;
+        attr[0].val.clusterDim.y = cluster.y;
         attr[0].val.clusterDim.z = 1;
         cfg.attrs = attr;
         cfg.numAttrs = 1;
         int n = 0;
-        cudaError_t e = cudaFuncSetAttribute(gemm_fp8_block_tile_kernel<CG, BN, S>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::SMEM_BYTES);
-        if (e == cudaSuccess) e = cudaOccupancyMaxActiveClusters(&n, gemm_fp8_block_tile_kernel<CG, BN, S>, &cfg);
+        cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
+        if (e == cudaSuccess) e = cudaOccupancyMaxActiveClusters(&n, kernel, &cfg);
         if (e != cudaSuccess) {
             cudaGetLastError();                              // not this launch's error: the form is not offered
             n = 0;
@@ -1007,6 +1006,16 @@ static long long tile_clusters() {
         known[dev] = n + 1;
     }
     return known[dev] - 1;
+}
+template <int CG, int BN, int S>
+static long long tile_clusters() {
+    static int known[64] = {0};
+    return clusters_held<TileCfg<CG, BN>::SMEM_BYTES>(known, gemm_fp8_block_tile_kernel<CG, BN, S>, dim3(CG * S), TILE_THREADS);
+}
+template <int BN, int S>
+static long long lane_clusters() {
+    static int known[64] = {0};
+    return clusters_held<LaneCfg<BN>::SMEM_BYTES>(known, gemm_fp8_block_lane_kernel<BN>, dim3(1, S), LaneCfg<BN>::THREADS);
 }
 
 template <int U, bool DOWN>
@@ -1100,7 +1109,15 @@ extern "C" int frt_b200_gemm_fp8_block_nt(const void* A, const void* W, void* D,
     offer(5, m256 * n128, 2, 2, 0.30, 3.8, f8b::tile_clusters<2, 128, 2>);
     offer(6, m128 * n256, 1, 2, 0.50, 5.0, f8b::tile_clusters<1, 256, 2>);
     offer(7, m128 * n256, 1, 4, 0.50, 7.0, f8b::tile_clusters<1, 256, 4>);
+    if (M <= 128) {
+        // K shared by four or eight with the weights on the lanes: 96 x 4096 x 4096 8.4 us against 9.5, 96 x 4096 x 14336 20 against 28; by two, or
+        // by none, no gain (96 x 6144 x 4096 11.9 against 11.2), and where the clusters do not all fit a loss (96 x 2048 x 2048 by eight 11)
+        offer(8, n128, 1, 4, 0.34, 2.7, M <= 96 ? f8b::lane_clusters<96, 4> : f8b::lane_clusters<128, 4>);
+        offer(9, n128, 1, 8, 0.34, 2.7, M <= 96 ? f8b::lane_clusters<96, 8> : f8b::lane_clusters<128, 8>);
+    }
     switch (form) {
+        case 8: return M <= 96 ? f8b::launch_lane<96>(A, W, p, K, 4, st) : f8b::launch_lane<128>(A, W, p, K, 4, st);
+        case 9: return M <= 96 ? f8b::launch_lane<96>(A, W, p, K, 8, st) : f8b::launch_lane<128>(A, W, p, K, 8, st);
         case 1: return f8b::launch_tile<1, 256, 1>(A, W, p, K, st);
         case 2: return f8b::launch_tile<2, 128, 1>(A, W, p, K, st);
         case 3: return f8b::launch_tile<1, 128, 1>(A, W, p, K, st);
