@@ -13,8 +13,9 @@
 // products, which go there for their sums too; with the signals between the warps a k-block takes 0.47 us, 2.2 PFLOP/s, where the products
 // with one scale per tensor, taken out once a tile, reach 2.9.
 //
-// More than 64 rows: the tokens are the rows of a tile (a thread of the epilogue owns a row, its scale is one register), on CTA pairs or
-// single CTAs; up to 64 rows: the weights are the 128 lanes and the tokens the columns, because nothing is left but streaming the weights.
+// Up to 64 rows the weights are the 128 lanes and the tokens the columns, because nothing is left but streaming the weights; so are tiles of 96
+// or 128 tokens where there are so few that four or eight CTAs can share K.  Otherwise the tokens are the rows of a tile (a thread of the
+// epilogue owns a row, its scale is one register), on CTA pairs or single CTAs.
 #include "common.cuh"
 #include "tc05.cuh"
 #include "flashrt_b200.h"
@@ -207,7 +208,7 @@ __device__ __forceinline__ void store_one(const Params& p, size_t at, float v) {
     else static_cast<__nv_bfloat16*>(p.out)[at] = __float2bfloat16_rn(v);
 }
 
-// ---------------------------------------------------------------- up to 64 rows (128 of narrow weights): weights on the lanes, tokens on the columns
+// ---------------------------------------------------------------- few rows (up to 64, or few tiles): weights on the lanes, tokens on the columns
 template <int BN>
 struct LaneCfg {
     static constexpr int A_BYTES = 128 * 128, B_BYTES = BN * 128, STAGE_BYTES = A_BYTES + B_BYTES;
@@ -222,7 +223,7 @@ struct LaneCfg {
     static_assert(PER_SM * TMEM_COLS <= 512 && PER_SM * (SMEM_BYTES + 1024) <= 228 * 1024, "CTAs of an SM");
 };
 
-// S = 1: grid of as many CTAs as there is room for, each walks over n tiles.  S > 1: grid (n tiles, S), cluster (1, S), rank r takes the
+// S = 1: grid of as many CTAs as there is room for, each walks over n tiles.  S > 1: grid (n tiles, S, tiles of tokens), cluster (1, S), rank r takes the
 // k-blocks [kb r / S, kb (r + 1) / S); the ranks then lay their partials into shared memory and each finishes every S-th four tokens.
 template <int BN>
 __global__ void __launch_bounds__(LaneCfg<BN>::THREADS, LaneCfg<BN>::PER_SM)
@@ -242,6 +243,7 @@ gemm_fp8_block_lane_kernel(const __grid_constant__ CUtensorMap tmA, const __grid
     const uint64_t deadline = tc::global_timer_ns() + FRT_KERNEL_DEADLINE_NS;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int S = (int)gridDim.y, rank = (int)blockIdx.y, tiles = (p.N + 127) / 128;
+    const int m0 = (int)blockIdx.z * BN, M = min(p.M - m0, BN);          // the tokens of this CTA
     const int kb0 = (int)((long long)p.kb * rank / S), kb1 = (int)((long long)p.kb * (rank + 1) / S);
 
     if (threadIdx.x == 0) {
@@ -278,7 +280,7 @@ gemm_fp8_block_lane_kernel(const __grid_constant__ CUtensorMap tmA, const __grid
         pdl_wait();
         if (tc::elect_one())
             for (int s = 0; s < ahead; ++s)
-                tc::tma_load_2d(ring + s * Cfg::STAGE_BYTES + Cfg::A_BYTES, &tmA, full_a + 8 * s, (kb0 + s) * 128, 0);
+                tc::tma_load_2d(ring + s * Cfg::STAGE_BYTES + Cfg::A_BYTES, &tmA, full_a + 8 * s, (kb0 + s) * 128, m0);
         __syncwarp();
         int s = ahead % STAGES, skip = ahead;
         uint32_t ph = ahead < STAGES;
@@ -293,7 +295,7 @@ gemm_fp8_block_lane_kernel(const __grid_constant__ CUtensorMap tmA, const __grid
                     const uint32_t dst = ring + s * Cfg::STAGE_BYTES, bar = full_a + 8 * s;
                     tc::mbar_arrive_expect_tx(bar, Cfg::STAGE_BYTES);
                     tc::tma_load_2d(dst, &tmW, bar, kb * 128, t * 128);
-                    tc::tma_load_2d(dst + Cfg::A_BYTES, &tmA, bar, kb * 128, 0);
+                    tc::tma_load_2d(dst + Cfg::A_BYTES, &tmA, bar, kb * 128, m0);
                 }
                 __syncwarp();
                 if (++s == STAGES) { s = 0; ph ^= 1; }
@@ -343,7 +345,7 @@ gemm_fp8_block_lane_kernel(const __grid_constant__ CUtensorMap tmA, const __grid
         int row[PER], buf = 0;
         uint32_t bph = 1;
 #pragma unroll
-        for (int i = 0; i < PER; ++i) row[i] = min(lane + 32 * i, p.M - 1);
+        for (int i = 0; i < PER; ++i) row[i] = m0 + min(lane + 32 * i, M - 1);
         for (int t = (int)blockIdx.x; t < tiles; t += (int)gridDim.x) {
             const float* ws = p.w_scale + (size_t)t * p.kb + kb0;
             const float* as = p.a_scale + kb0 * p.a_stride;
@@ -399,7 +401,7 @@ gemm_fp8_block_lane_kernel(const __grid_constant__ CUtensorMap tmA, const __grid
                 const uint32_t src = t_src + buf * Cfg::BUF_COLS, slot = scale_a + buf * (BN * 4) + half * (W * 4);
 #pragma unroll
                 for (int c = 0; c < W; c += LW) {
-                    if (half * W + c >= p.M) break;
+                    if (half * W + c >= M) break;
                     uint32_t v[LW];
                     float4 f[LW / 4];
                     tmem_ld<LW>(src + c, v);
@@ -425,13 +427,13 @@ gemm_fp8_block_lane_kernel(const __grid_constant__ CUtensorMap tmA, const __grid
                 const uint32_t red = tc::smem_u32(smem) + (uint32_t)(half * (W / 4) * 128 + q * 32 + lane) * 16;
 #pragma unroll
                 for (int j = 0; j < W; j += 4)
-                    if (half * W + j < p.M) sts_v4(red + j * 512, acc[j], acc[j + 1], acc[j + 2], acc[j + 3]);
+                    if (half * W + j < M) sts_v4(red + j * 512, acc[j], acc[j + 1], acc[j + 2], acc[j + 3]);
             } else if (n < p.N) {
                 const float bias = p.bias ? __bfloat162float(p.bias[n]) : 0.0f;
-                const size_t at = (size_t)(half * W) * p.N + n;
+                const size_t at = (size_t)(m0 + half * W) * p.N + n;
 #pragma unroll
                 for (int j = 0; j < W; ++j)
-                    if (half * W + j < p.M) store_one(p, at + (size_t)j * p.N, p.bias ? __fadd_rn(acc[j], bias) : acc[j]);
+                    if (half * W + j < M) store_one(p, at + (size_t)j * p.N, p.bias ? __fadd_rn(acc[j], bias) : acc[j]);
             }
         }
     }
@@ -443,7 +445,7 @@ gemm_fp8_block_lane_kernel(const __grid_constant__ CUtensorMap tmA, const __grid
             const bool in = n < p.N;
             const float bias = in && p.bias ? __bfloat162float(p.bias[n]) : 0.0f;
             const uint32_t red = tc::smem_u32(smem) + (uint32_t)(q * 32 + lane) * 16;
-            for (int g = rank + S * half; 4 * g < p.M; g += S * Cfg::HALVES) {   // four tokens; the ranks' partials are all on their way before the first is added
+            for (int g = rank + S * half; 4 * g < M; g += S * Cfg::HALVES) {   // four tokens; the ranks' partials are all on their way before the first is added
                 float4 w[8];
 #pragma unroll
                 for (int r = 0; r < 8; ++r)
@@ -460,7 +462,7 @@ gemm_fp8_block_lane_kernel(const __grid_constant__ CUtensorMap tmA, const __grid
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const int m = 4 * g + e;
-                    if (in && m < p.M) store_one(p, (size_t)m * p.N + n, p.bias ? __fadd_rn(sum[e], bias) : sum[e]);
+                    if (in && m < M) store_one(p, (size_t)(m0 + m) * p.N + n, p.bias ? __fadd_rn(sum[e], bias) : sum[e]);
                 }
             }
         }
@@ -934,7 +936,7 @@ static int launch_lane(const void* A, const void* W, Params p, int K, int splits
     const int tiles = (p.N + 127) / 128, room = Cfg::PER_SM * device_sm_count();
     cudaLaunchConfig_t cfg = {};
     cudaLaunchAttribute attr[2];
-    cfg.gridDim = dim3(splits > 1 || tiles < room ? tiles : room, splits);
+    cfg.gridDim = dim3(splits > 1 || tiles < room ? tiles : room, splits, (unsigned)((p.M + BN - 1) / BN));       // S = 1: one tile of tokens
     cfg.blockDim = dim3(Cfg::THREADS);
     cfg.dynamicSmemBytes = Cfg::SMEM_BYTES;
     set_attrs(cfg, attr, 1, (unsigned)splits, stream);
@@ -1103,21 +1105,21 @@ extern "C" int frt_b200_gemm_fp8_block_nt(const void* A, const void* W, void* D,
     };
     offer(0, m256 * n256, 2, 1, 0.47, 0.0, nullptr);
     offer(1, m128 * n256, 1, 1, 0.50, 0.0, nullptr);
-    offer(2, m256 * n128, 2, 1, 0.30, 0.0, nullptr);
+    offer(2, m256 * n128, 2, 1, 0.30, 0.8, nullptr);         // the pair's signals: 512 x 2048 x 2048 7.8 against 7.4 on single CTAs
     offer(3, m128 * n128, 1, 1, 0.345, 0.0, nullptr);
     offer(4, m128 * n128, 1, 2, 0.345, 2.5, f8b::tile_clusters<1, 128, 2>);
     offer(5, m256 * n128, 2, 2, 0.30, 3.8, f8b::tile_clusters<2, 128, 2>);
     offer(6, m128 * n256, 1, 2, 0.50, 5.0, f8b::tile_clusters<1, 256, 2>);
     offer(7, m128 * n256, 1, 4, 0.50, 7.0, f8b::tile_clusters<1, 256, 4>);
-    if (M <= 128) {
-        // K shared by four or eight with the weights on the lanes: 96 x 4096 x 4096 8.4 us against 9.5, 96 x 4096 x 14336 20 against 28; by two, or
-        // by none, no gain (96 x 6144 x 4096 11.9 against 11.2), and where the clusters do not all fit a loss (96 x 2048 x 2048 by eight 11)
-        offer(8, n128, 1, 4, 0.34, 2.7, M <= 96 ? f8b::lane_clusters<96, 4> : f8b::lane_clusters<128, 4>);
-        offer(9, n128, 1, 8, 0.34, 2.7, M <= 96 ? f8b::lane_clusters<96, 8> : f8b::lane_clusters<128, 8>);
-    }
+    // K shared by four or eight with the weights on the lanes, tiles of 96 or 128 tokens: 96 x 4096 x 4096 8.4 us against 9.5, 96 x 4096 x 14336 20
+    // against 28, 129 x 2048 x 16384 18 against 30; by two, or by none, no gain (96 x 6144 x 4096 11.9 against
+    // 11.2), and where the clusters do not all fit a loss (96 x 2048 x 2048 by eight 11, by four 6)
+    const bool of96 = (M + 95) / 96 == m128;
+    offer(8, m128 * n128, 1, 4, of96 ? 0.34 : 0.40, 2.7, of96 ? f8b::lane_clusters<96, 4> : f8b::lane_clusters<128, 4>);
+    offer(9, m128 * n128, 1, 8, of96 ? 0.34 : 0.40, 2.7, of96 ? f8b::lane_clusters<96, 8> : f8b::lane_clusters<128, 8>);
     switch (form) {
-        case 8: return M <= 96 ? f8b::launch_lane<96>(A, W, p, K, 4, st) : f8b::launch_lane<128>(A, W, p, K, 4, st);
-        case 9: return M <= 96 ? f8b::launch_lane<96>(A, W, p, K, 8, st) : f8b::launch_lane<128>(A, W, p, K, 8, st);
+        case 8: return of96 ? f8b::launch_lane<96>(A, W, p, K, 4, st) : f8b::launch_lane<128>(A, W, p, K, 4, st);
+        case 9: return of96 ? f8b::launch_lane<96>(A, W, p, K, 8, st) : f8b::launch_lane<128>(A, W, p, K, 8, st);
         case 1: return f8b::launch_tile<1, 256, 1>(A, W, p, K, st);
         case 2: return f8b::launch_tile<2, 128, 1>(A, W, p, K, st);
         case 3: return f8b::launch_tile<1, 128, 1>(A, W, p, K, st);

@@ -132,6 +132,14 @@ def test_shapes(m, n, k):
     check(m, n, k, bias=False, f32=True, pdl=True)
 
 
+@pytest.mark.parametrize("m,n,k", [(65, 2048, 2048), (96, 130, 7168), (97, 4096, 2064), (128, 1000, 4096), (129, 2048, 2048), (192, 500, 8192),
+                                   (193, 1030, 4112), (300, 512, 7168), (257, 1000, 4100 // 16 * 16), (385, 7, 4096), (512, 130, 2048)])
+def test_tiles_of_tokens_that_share_k(m, n, k):
+    """Few tiles and a long K: four or eight CTAs share it, the last tile of tokens may have one row."""
+    check(m, n, k)
+    check(m, n, k, bias=False, f32=True, pdl=True)
+
+
 def test_scales_far_apart():
     """Blocks whose scales lie ten orders of magnitude apart, and scales of zero."""
     for m in (9, 90, 300):
