@@ -240,7 +240,6 @@ gemm_fp8_block_lane_kernel(const __grid_constant__ CUtensorMap tmA, const __grid
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
     static_assert((2 * STAGES + 2 * BUFS) * 8 + 8 <= 256, "barriers");
     const uint32_t scale_a = tc::smem_u32(smem + STAGES * Cfg::STAGE_BYTES + 256);
-    const uint64_t deadline = tc::global_timer_ns() + FRT_KERNEL_DEADLINE_NS;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int S = (int)gridDim.y, rank = (int)blockIdx.y, tiles = (p.N + 127) / 128;
     const int m0 = (int)blockIdx.z * BN, M = min(p.M - m0, BN);          // the tokens of this CTA
@@ -286,7 +285,7 @@ gemm_fp8_block_lane_kernel(const __grid_constant__ CUtensorMap tmA, const __grid
         uint32_t ph = ahead < STAGES;
         for (int t = (int)blockIdx.x; t < tiles; t += (int)gridDim.x) {
             for (int kb = kb0 + skip; kb < kb1; ++kb) {
-                if (!tc::warp_wait(empty_a + 8 * s, ph, false, deadline, abort_flag)) {
+                if (!tc::warp_wait_limited(empty_a + 8 * s, ph, false, abort_flag)) {
                     if (lane == 0) gave_up(p.status, abort_flag, ERR_PRODUCER);
                     t = tiles;
                     break;
@@ -304,7 +303,7 @@ gemm_fp8_block_lane_kernel(const __grid_constant__ CUtensorMap tmA, const __grid
         }
         // the last stages' returns arrive in this CTA's shared memory too: not after it has gone to another
         for (int i = 0; i < STAGES; ++i) {
-            if (!tc::warp_wait(empty_a + 8 * s, ph, false, deadline, abort_flag)) break;
+            if (!tc::warp_wait_limited(empty_a + 8 * s, ph, false, abort_flag)) break;
             if (++s == STAGES) { s = 0; ph ^= 1; }
         }
     } else if (warp == 1) {
@@ -316,10 +315,11 @@ gemm_fp8_block_lane_kernel(const __grid_constant__ CUtensorMap tmA, const __grid
         const uint64_t dB0 = tc::make_desc_kmajor_sw128(tc::smem_u32(smem + Cfg::A_BYTES));
         int s = 0, buf = 0;
         uint32_t ph = 0, bph = 1;                              // the first round of the buffers is empty
+        if (!tc::mbar_try_wait(full_a, 0)) pdl_wait();         // the first stage's limit counts from behind the kernel in front
         for (int t = (int)blockIdx.x; t < tiles; t += (int)gridDim.x)
             for (int kb = kb0; kb < kb1; ++kb) {
-                if (!tc::warp_wait(accE_a + 8 * buf, bph, false, deadline, abort_flag) ||
-                    !tc::warp_wait(full_a + 8 * s, ph, false, deadline, abort_flag)) {
+                if (!tc::warp_wait_limited(accE_a + 8 * buf, bph, false, abort_flag) ||
+                    !tc::warp_wait_limited(full_a + 8 * s, ph, false, abort_flag)) {
                     if (lane == 0) gave_up(p.status, abort_flag, ERR_MMA);
                     t = tiles;
                     break;
@@ -357,7 +357,7 @@ gemm_fp8_block_lane_kernel(const __grid_constant__ CUtensorMap tmA, const __grid
                 as += p.a_stride;
             };
             auto give = [&](const Scales& r) {
-                if (!tc::mbar_wait_until(tc::smem_u32(&acc_empty[buf]), bph, deadline, abort_flag)) gave_up(p.status, abort_flag, ERR_EPILOGUE);
+                if (!tc::mbar_wait_limited(tc::smem_u32(&acc_empty[buf]), bph, abort_flag)) gave_up(p.status, abort_flag, ERR_EPILOGUE);
                 const uint32_t to = scale_a + buf * (BN * 4) + lane * 4;
 #pragma unroll
                 for (int i = 0; i < PER; ++i)
@@ -392,7 +392,7 @@ gemm_fp8_block_lane_kernel(const __grid_constant__ CUtensorMap tmA, const __grid
 #pragma unroll
             for (int j = 0; j < W; ++j) acc[j] = 0.0f;
             for (int kb = kb0; kb < kb1; ++kb) {
-                ok = tc::warp_wait(tc::smem_u32(&acc_full[buf]), bph, false, deadline, abort_flag);
+                ok = tc::warp_wait_limited(tc::smem_u32(&acc_full[buf]), bph, false, abort_flag);
                 if (!ok) {
                     if (lane == 0) gave_up(p.status, abort_flag, ERR_EPILOGUE);
                     break;
@@ -628,7 +628,6 @@ gemm_fp8_block_tile_kernel(const __grid_constant__ CUtensorMap tmA, const __grid
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
     static_assert((2 * STAGES + 3 * BUFS) * 8 + 8 <= 256, "barriers");
     const uint32_t scale_a = tc::smem_u32(outs + 8 * Cfg::OUT_BYTES + 256);
-    const uint64_t deadline = tc::global_timer_ns() + FRT_KERNEL_DEADLINE_NS;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t cluster_rank = CG * S > 1 ? tc::cluster_ctarank() : 0u, rank = cluster_rank % CG, leader = cluster_rank - rank;
     const int split = (int)cluster_rank / CG;
@@ -691,7 +690,7 @@ gemm_fp8_block_tile_kernel(const __grid_constant__ CUtensorMap tmA, const __grid
             tile_at(t, p.gm, m_tiles, n_tiles, mt, nt);
             const int m0 = (mt * CG + (int)rank) * 128, n0 = nt * BN + (int)rank * (BN / CG);
             for (int kb = kb0 + skip; kb < kb1; ++kb) {
-                if (!tc::warp_wait(empty_a + 8 * s, ph, ready, deadline, abort_flag)) {
+                if (!tc::warp_wait_limited(empty_a + 8 * s, ph, ready, abort_flag)) {
                     if (lane == 0) gave_up(p.status, abort_flag, ERR_PRODUCER);
                     t = total;
                     break;
@@ -709,7 +708,7 @@ gemm_fp8_block_tile_kernel(const __grid_constant__ CUtensorMap tmA, const __grid
         }
         // the last stages' returns arrive in this CTA's shared memory too: not after it has gone to another
         for (int i = 0; i < STAGES; ++i) {
-            if (!tc::warp_wait(empty_a + 8 * s, ph, false, deadline, abort_flag)) break;
+            if (!tc::warp_wait_limited(empty_a + 8 * s, ph, false, abort_flag)) break;
             if (++s == STAGES) { s = 0; ph ^= 1; }
         }
     } else if ((warp & 1) && warp < 2 * ISSUERS && rank == 0) {
@@ -722,10 +721,11 @@ gemm_fp8_block_tile_kernel(const __grid_constant__ CUtensorMap tmA, const __grid
         const int mine = unit < total ? ((total - 1 - unit) / units + 1) * (kb1 - kb0) : 0;       // k-blocks of this unit's tiles
         int s = warp >> 1, buf = warp >> 1;
         uint32_t ph = 0, bph = 1;                            // the first round of the buffers is empty
-        bool ready = false;
+        bool ready = tc::mbar_test(full_a + 8 * s, 0);
+        if (!ready) pdl_wait();                              // the first stage's limit counts from behind the kernel in front
         for (int i = warp >> 1; i < mine; i += ISSUERS) {
-            if (!tc::warp_wait(full_a + 8 * s, ph, ready, deadline, abort_flag) ||
-                !tc::warp_wait(accE_a + 8 * buf, bph, false, deadline, abort_flag)) {
+            if (!tc::warp_wait_limited(full_a + 8 * s, ph, ready, abort_flag) ||
+                !tc::warp_wait_limited(accE_a + 8 * buf, bph, false, abort_flag)) {
                 if (lane == 0) gave_up(p.status, abort_flag, ERR_MMA);
                 break;
             }
@@ -769,7 +769,7 @@ gemm_fp8_block_tile_kernel(const __grid_constant__ CUtensorMap tmA, const __grid
                 as += p.a_stride;
             };
             auto give = [&](const Scales& r) {
-                if (!tc::mbar_wait_until(tc::smem_u32(&scale_empty[buf]), bph, deadline, abort_flag)) gave_up(p.status, abort_flag, ERR_EPILOGUE);
+                if (!tc::mbar_wait_limited(tc::smem_u32(&scale_empty[buf]), bph, abort_flag)) gave_up(p.status, abort_flag, ERR_EPILOGUE);
                 const uint32_t to = scale_a + buf * SCALE_SLOT;
                 sts_v4(to + lane * 16, r.a[0], r.a[1], r.a[2], r.a[3]);
                 if (lane < 2) asm volatile("st.shared.f32 [%0], %1;" ::"r"(to + 512 + lane * 4), "f"(r.w) : "memory");
@@ -808,7 +808,7 @@ gemm_fp8_block_tile_kernel(const __grid_constant__ CUtensorMap tmA, const __grid
             for (int j = 0; j < W2; ++j) acc[j] = 0.0f;
             bool ok = true;
             for (int kb = kb0; kb < kb1; ++kb) {
-                ok = tc::warp_wait(accF_a + 8 * buf, bph, false, deadline, abort_flag);
+                ok = tc::warp_wait_limited(accF_a + 8 * buf, bph, false, abort_flag);
                 if (!ok) {
                     if (lane == 0) gave_up(p.status, abort_flag, ERR_EPILOGUE);
                     break;

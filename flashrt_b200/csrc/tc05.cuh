@@ -59,8 +59,8 @@ __device__ __forceinline__ uint64_t global_timer_ns() {
     asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
     return t;
 }
-// Every wait of a kernel shares one wall-clock deadline taken at kernel start, so a protocol error
-// ends the whole kernel after FRT_KERNEL_DEADLINE_NS instead of spinning.
+// Every wait ends after FRT_KERNEL_DEADLINE_NS, so a protocol error ends the whole kernel instead of spinning: mbar_wait_until's callers
+// share one wall-clock deadline taken at kernel start, mbar_wait_limited's have that long for each wait.
 #ifndef FRT_KERNEL_DEADLINE_NS
 #define FRT_KERNEL_DEADLINE_NS 2000000000ull
 #endif
@@ -91,18 +91,21 @@ __device__ __forceinline__ bool mbar_test(uint32_t bar, uint32_t parity) {
         : "memory");
     return ok != 0;
 }
+__device__ __forceinline__ bool mbar_try_wait(uint32_t bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred P;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 P, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, P;\n\t}"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity)
+        : "memory");
+    return ok != 0;
+}
 __device__ __forceinline__ bool mbar_wait_until(uint32_t bar, uint32_t parity, uint64_t deadline_ns,
                                                 volatile int* abort_flag) {
     for (uint32_t i = 0;; ++i) {
-        uint32_t ok;
-        asm volatile(
-            "{\n\t.reg .pred P;\n\t"
-            "mbarrier.try_wait.parity.shared::cta.b64 P, [%1], %2;\n\t"
-            "selp.u32 %0, 1, 0, P;\n\t}"
-            : "=r"(ok)
-            : "r"(bar), "r"(parity)
-            : "memory");
-        if (ok) return true;
+        if (mbar_try_wait(bar, parity)) return true;
         if (*abort_flag) return false;
         if ((i & 3) == 3 && global_timer_ns() > deadline_ns) return false;
     }
@@ -114,6 +117,15 @@ __device__ __forceinline__ bool mbar_wait_until(uint32_t bar, uint32_t parity, u
 __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, bool ready, uint64_t deadline_ns,
                                           volatile int* abort_flag) {
     const bool ok = ready || mbar_wait_until(bar, parity, deadline_ns, abort_flag);
+    return __all_sync(0xffffffffu, ok) != 0;
+}
+// The same with a limit of its own for each wait, from its first look that failed: a kernel may then take longer than one limit, since
+// its work or the kernel in front does; a wait that can begin before that one has ended stands behind pdl_wait all the same.
+__device__ __forceinline__ bool mbar_wait_limited(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
+    return mbar_try_wait(bar, parity) || mbar_wait_until(bar, parity, global_timer_ns() + FRT_KERNEL_DEADLINE_NS, abort_flag);
+}
+__device__ __forceinline__ bool warp_wait_limited(uint32_t bar, uint32_t parity, bool ready, volatile int* abort_flag) {
+    const bool ok = ready || mbar_wait_limited(bar, parity, abort_flag);
     return __all_sync(0xffffffffu, ok) != 0;
 }
 __device__ __forceinline__ void mbar_arrive_expect_tx(uint32_t bar, uint32_t bytes) {

@@ -1,0 +1,47 @@
+"""Bounded waits of kernels that start while the one in front still runs, read from the sources: how long a launch stays resident before
+its turn, and how long its own work takes, is not its waits' affair."""
+import os
+import re
+
+import pytest
+
+CSRC = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "flashrt_b200", "csrc")
+WAIT = r"tc::(?:mbar|warp)_wait\w*\("
+
+
+def source(name):
+    text = open(os.path.join(CSRC, name)).read()
+    return re.sub(r"//[^\n]*|/\*.*?\*/", "", text, flags=re.S)
+
+
+def block(text, at):
+    """The braces that open behind `at`, with what is between them."""
+    start = i = text.index("{", at)
+    depth = 0
+    while True:
+        depth += {"{": 1, "}": -1}.get(text[i], 0)
+        i += 1
+        if depth == 0:
+            return text[start:i]
+
+
+@pytest.mark.parametrize("name", ["gemm_fp8_block.cu"])
+def test_every_wait_has_a_limit_of_its_own(name):
+    text = source(name)
+    assert "DEADLINE" not in text and "wait_until" not in text and "deadline" not in text
+    waits = re.findall(WAIT, text)
+    assert waits and all("_limited(" in w for w in waits)
+
+
+def test_roles_of_the_block_scaled_products_wait_behind_the_kernel_in_front():
+    text = source("gemm_fp8_block.cu")
+    roles = 0
+    for kernel in ("gemm_fp8_block_lane_kernel", "gemm_fp8_block_tile_kernel"):
+        body = block(text, text.index(kernel))
+        for m in re.finditer(r"if \([^{;]*warp[^{;]*\) \{|else \{", body):
+            role = block(body, m.start())
+            first = re.search(WAIT, role)
+            if first:
+                assert 0 <= role.find("pdl_wait();") < first.start(), (kernel, m.group())
+                roles += 1
+    assert roles == 8                                      # two kernels: producer, issuer, scales, epilogue
