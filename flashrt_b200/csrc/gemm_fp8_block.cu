@@ -308,6 +308,7 @@ gemm_fp8_block_lane_kernel(const __grid_constant__ CUtensorMap tmA, const __grid
         }
     } else if (warp == 1) {
         // ---------------- MMA issuer (whole warp): a k-block, a buffer
+        pdl_wait();                                          // the first stage's limit counts from here
         constexpr uint32_t idesc = tc::make_idesc(0, 0, 0, 0, 128, BN);
         const uint32_t full_a = tc::smem_u32(full), empty_a = tc::smem_u32(empty);
         const uint32_t accF_a = tc::smem_u32(acc_full), accE_a = tc::smem_u32(acc_empty);
@@ -315,7 +316,6 @@ gemm_fp8_block_lane_kernel(const __grid_constant__ CUtensorMap tmA, const __grid
         const uint64_t dB0 = tc::make_desc_kmajor_sw128(tc::smem_u32(smem + Cfg::A_BYTES));
         int s = 0, buf = 0;
         uint32_t ph = 0, bph = 1;                              // the first round of the buffers is empty
-        if (!tc::mbar_try_wait(full_a, 0)) pdl_wait();         // the first stage's limit counts from behind the kernel in front
         for (int t = (int)blockIdx.x; t < tiles; t += (int)gridDim.x)
             for (int kb = kb0; kb < kb1; ++kb) {
                 if (!tc::warp_wait_limited(accE_a + 8 * buf, bph, false, abort_flag) ||
@@ -713,6 +713,7 @@ gemm_fp8_block_tile_kernel(const __grid_constant__ CUtensorMap tmA, const __grid
         }
     } else if ((warp & 1) && warp < 2 * ISSUERS && rank == 0) {
         // ---------------- MMA issuers for the tiles, warps 1 and (two issuers) 3: a k-block, a buffer
+        pdl_wait();                                          // the first stage's limit counts from here
         constexpr uint32_t idesc = tc::make_idesc(0, 0, 0, 0, 128 * CG, BN);
         const uint64_t dA0 = tc::make_desc_kmajor_sw128(tc::smem_u32(smem));
         const uint64_t dB0 = tc::make_desc_kmajor_sw128(tc::smem_u32(smem + Cfg::A_BYTES));
@@ -721,8 +722,7 @@ gemm_fp8_block_tile_kernel(const __grid_constant__ CUtensorMap tmA, const __grid
         const int mine = unit < total ? ((total - 1 - unit) / units + 1) * (kb1 - kb0) : 0;       // k-blocks of this unit's tiles
         int s = warp >> 1, buf = warp >> 1;
         uint32_t ph = 0, bph = 1;                            // the first round of the buffers is empty
-        bool ready = tc::mbar_test(full_a + 8 * s, 0);
-        if (!ready) pdl_wait();                              // the first stage's limit counts from behind the kernel in front
+        bool ready = false;
         for (int i = warp >> 1; i < mine; i += ISSUERS) {
             if (!tc::warp_wait_limited(full_a + 8 * s, ph, ready, abort_flag) ||
                 !tc::warp_wait_limited(accE_a + 8 * buf, bph, false, abort_flag)) {

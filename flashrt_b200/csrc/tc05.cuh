@@ -119,10 +119,19 @@ __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, bool re
     const bool ok = ready || mbar_wait_until(bar, parity, deadline_ns, abort_flag);
     return __all_sync(0xffffffffu, ok) != 0;
 }
-// The same with a limit of its own for each wait, from its first look that failed: a kernel may then take longer than one limit, since
+// The same with a limit of its own for each wait, from its fourth look that failed: a kernel may then take longer than one limit, since
 // its work or the kernel in front does; a wait that can begin before that one has ended stands behind pdl_wait all the same.
 __device__ __forceinline__ bool mbar_wait_limited(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
-    return mbar_try_wait(bar, parity) || mbar_wait_until(bar, parity, global_timer_ns() + FRT_KERNEL_DEADLINE_NS, abort_flag);
+    uint64_t start = 0;
+    for (uint32_t i = 0;; ++i) {
+        if (mbar_try_wait(bar, parity)) return true;
+        if (*abort_flag) return false;
+        if ((i & 3) == 3) {
+            const uint64_t now = global_timer_ns();
+            if (start == 0) start = now;
+            if (now - start > FRT_KERNEL_DEADLINE_NS) return false;
+        }
+    }
 }
 __device__ __forceinline__ bool warp_wait_limited(uint32_t bar, uint32_t parity, bool ready, volatile int* abort_flag) {
     const bool ok = ready || mbar_wait_limited(bar, parity, abort_flag);
