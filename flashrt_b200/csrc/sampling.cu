@@ -69,7 +69,6 @@ softmax_rows_kernel(SoftmaxParams p) {
     if (!STAGED) pdl_launch_dependents();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int ctas = p.ctas, rank = (int)(blockIdx.x % (unsigned)ctas), step = (int)(gridDim.x / (unsigned)ctas);
-    const uint64_t deadline = tc::global_timer_ns() + FRT_KERNEL_DEADLINE_NS;
     int no_flag = 0;
     if (tid == 0 && (STAGED || ctas > 1)) {
         tc::mbar_init(&mail[0], 1);
@@ -140,7 +139,7 @@ softmax_rows_kernel(SoftmaxParams p) {
         };
         // NaN: fmaxf leaves it out, here and in a weight's argument, which it puts at the lower end
         float v[NV * VE], top = -INFINITY;
-        if (STAGED && !tc::mbar_wait_until(&there, (uint32_t)odd, deadline, &no_flag) && tid == 0) atomicCAS(p.status, 0, ERR_ROW);
+        if (STAGED && !tc::mbar_wait_limited(tc::smem_u32(&there), (uint32_t)odd, &no_flag) && tid == 0) atomicCAS(p.status, 0, ERR_ROW);
         {
             uint4 w[NV];
 #pragma unroll
@@ -260,7 +259,7 @@ softmax_rows_kernel(SoftmaxParams p) {
                 tc::st_async_v4(tc::dsmem_map(tc::smem_u32(&box[odd][rank]), (uint32_t)lane), tc::dsmem_map(tc::smem_u32(&mail[odd]), (uint32_t)lane),
                                 __float_as_uint(m), __float_as_uint(total), (uint32_t)f, 0u);
             // a box is written again two rows on, when every CTA has sent the row between, and so has read this one
-            if (!tc::mbar_wait_until(&mail[odd], (uint32_t)(turn >> 1) & 1u, deadline, &no_flag) && tid == 0) atomicCAS(p.status, 0, ERR_MAIL);
+            if (!tc::mbar_wait_limited(tc::smem_u32(&mail[odd]), (uint32_t)(turn >> 1) & 1u, &no_flag) && tid == 0) atomicCAS(p.status, 0, ERR_MAIL);
             const uint4 its = lane < ctas ? box[odd][lane] : make_uint4(0xff800000u, 0u, 0x7fffffffu, 0u);
             m = __uint_as_float(its.x);
             total = __uint_as_float(its.y);
@@ -345,7 +344,6 @@ verify_drafts_kernel(VerifyParams a) {
     __shared__ uint64_t mail[2];
     pdl_launch_dependents();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const uint64_t deadline = tc::global_timer_ns() + FRT_KERNEL_DEADLINE_NS;
     int no_flag = 0;
     if (a.ctas > 1) {
         if (tid == 0) {
@@ -500,7 +498,7 @@ verify_drafts_kernel(VerifyParams a) {
                 tc::st_async_v4(tc::dsmem_map(tc::smem_u32(&box[turn][rank]), (uint32_t)lane), tc::dsmem_map(tc::smem_u32(&mail[turn]), (uint32_t)lane),
                                 (uint32_t)bits, (uint32_t)(bits >> 32), 0u, 0u);
             }
-            if (!tc::mbar_wait_until(&mail[turn], 0, deadline, &no_flag) && tid == 0) atomicCAS(a.status, 0, ERR_MAIL);
+            if (!tc::mbar_wait_limited(tc::smem_u32(&mail[turn]), 0, &no_flag) && tid == 0) atomicCAS(a.status, 0, ERR_MAIL);
             __syncwarp();
 #pragma unroll
             for (int r = 0; r < 8; ++r)

@@ -25,7 +25,7 @@ def block(text, at):
             return text[start:i]
 
 
-@pytest.mark.parametrize("name", ["gemm_fp8_block.cu"])
+@pytest.mark.parametrize("name", ["gemm_fp8_block.cu", "sampling.cu"])
 def test_every_wait_has_a_limit_of_its_own(name):
     text = source(name)
     assert "DEADLINE" not in text and "wait_until" not in text and "deadline" not in text
@@ -45,3 +45,10 @@ def test_roles_of_the_block_scaled_products_wait_behind_the_kernel_in_front():
                 assert 0 <= role.find("pdl_wait();") < first.start(), (kernel, m.group())
                 roles += 1
     assert roles == 8                                      # two kernels: producer, issuer, scales, epilogue
+
+
+@pytest.mark.parametrize("kernel", ["softmax_rows_kernel", "verify_drafts_kernel"])
+def test_probabilities_and_verification_wait_behind_the_kernel_in_front(kernel):
+    text = source("sampling.cu")
+    body = block(text, text.index(kernel + "("))
+    assert 0 <= body.find("pdl_wait();") < re.search(WAIT, body).start()

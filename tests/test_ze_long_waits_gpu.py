@@ -97,3 +97,34 @@ def test_a_product_of_more_than_two_seconds():
     bound = size * (128 * 2.0 ** -23 + (k // 128 + 2) * 2.0 ** -24)
     bound = bound * (1 + 2.0 ** -8) + want.abs() * 2.0 ** -8
     assert ((out[rows][:, cols].to(F64) - want).abs() <= bound).all()
+
+
+def _logits(rows, vocab, dtype):
+    x = torch.randn(rows, vocab, generator=torch.Generator("cuda").manual_seed(rows), device="cuda") * 3
+    return x.to(dtype)
+
+
+@pytest.mark.parametrize("rows,vocab,dtype", [(1, 50257, BF16), (300, 50257, F32), (40, 131072, F32), (20, 150001, BF16)])
+def test_probabilities_and_verification_behind_a_long_kernel(rows, vocab, dtype, long_kernel):
+    """Clusters of a row, clusters that stay, rows that are not held; a sequence of all rows, whose last tokens are the likeliest."""
+    from flashrt_b200 import flash_rt_kernels as fvk
+    x = _logits(rows, vocab, dtype)
+    p, q = (torch.full((rows, vocab), float("nan"), device="cuda") for _ in range(2))
+    cu, lens = torch.tensor([0, rows], dtype=I32, device="cuda"), torch.tensor([rows + 7], dtype=I32, device="cuda")
+    tokens = torch.cat([torch.zeros(1, dtype=I32, device="cuda"), x.float().argmax(1)[:-1].to(I32)])
+    u, v = torch.full((rows,), 0.001, device="cuda"), torch.full((1,), 0.6, device="cuda")
+    outs = [torch.full((rows + 2,), -9, dtype=I32, device="cuda") for _ in range(2)]
+
+    def step(probs, out):
+        fvk.softmax_rows(x.data_ptr(), probs.data_ptr(), rows, vocab, _stream(), in_f32=dtype == F32)
+        fvk.verify_drafts(probs.data_ptr(), 0, tokens.data_ptr(), cu.data_ptr(), lens.data_ptr(), u.data_ptr(), v.data_ptr(), out.data_ptr(),
+                          out.data_ptr() + 4 * rows, out.data_ptr() + 4 * rows + 4, rows, 1, vocab, _stream())
+    step(p, outs[0])
+    torch.cuda.synchronize()
+    long_kernel()
+    step(q, outs[1])
+    torch.cuda.synchronize()
+    assert fvk._lib.call_status("frt_b200_gemm_status", 1) == 0
+    assert torch.equal(p, q) and p.isfinite().all() and torch.equal(*outs) and (outs[0][:1] >= 0).all()
+    want, accepted, kept = R.verify(p.cpu().numpy(), None, tokens.tolist(), [0, rows], [rows + 7], u.tolist(), v.tolist())
+    assert outs[0].tolist() == want + accepted + kept
