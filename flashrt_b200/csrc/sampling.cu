@@ -34,6 +34,15 @@ __device__ __forceinline__ float warp_max(float x) {
     return y;
 }
 
+// A wait of this warp gave up: the warp asks for nothing and sends nothing any more, gives copies and messages on their way a bounded time (the
+// CTA's shared memory is another's once its last warp has left), and leaves.  The CTA's barriers wait for threads that have not left,
+// so its other warps go on until a wait of their own gives up, which it does where it needed this one.
+__device__ __forceinline__ void gave_up(int* status, int code) {
+    if ((threadIdx.x & 31) == 0) atomicCAS(status, 0, code);
+    const uint64_t until = tc::global_timer_ns() + 1000000ull;
+    while (tc::global_timer_ns() < until) {}
+}
+
 // ------------------------------------------------------------------------------------------------ softmax
 //   p = exp((x - max) / T) / sum;  T not above zero: one on the first of the largest;  nothing but -infinity and NaN: zeros.
 // Weights are exponentials against the warp's own maximum; the (maximum, sum) of warps meet in shared memory, those of the cluster's CTAs
@@ -139,7 +148,7 @@ softmax_rows_kernel(SoftmaxParams p) {
         };
         // NaN: fmaxf leaves it out, here and in a weight's argument, which it puts at the lower end
         float v[NV * VE], top = -INFINITY;
-        if (STAGED && !tc::mbar_wait_limited(tc::smem_u32(&there), (uint32_t)odd, &no_flag) && tid == 0) atomicCAS(p.status, 0, ERR_ROW);
+        if (STAGED && !tc::warp_wait_limited(tc::smem_u32(&there), (uint32_t)odd, false, &no_flag)) return gave_up(p.status, ERR_ROW);
         {
             uint4 w[NV];
 #pragma unroll
@@ -259,7 +268,7 @@ softmax_rows_kernel(SoftmaxParams p) {
                 tc::st_async_v4(tc::dsmem_map(tc::smem_u32(&box[odd][rank]), (uint32_t)lane), tc::dsmem_map(tc::smem_u32(&mail[odd]), (uint32_t)lane),
                                 __float_as_uint(m), __float_as_uint(total), (uint32_t)f, 0u);
             // a box is written again two rows on, when every CTA has sent the row between, and so has read this one
-            if (!tc::mbar_wait_limited(tc::smem_u32(&mail[odd]), (uint32_t)(turn >> 1) & 1u, &no_flag) && tid == 0) atomicCAS(p.status, 0, ERR_MAIL);
+            if (!tc::warp_wait_limited(tc::smem_u32(&mail[odd]), (uint32_t)(turn >> 1) & 1u, false, &no_flag)) return gave_up(p.status, ERR_MAIL);
             const uint4 its = lane < ctas ? box[odd][lane] : make_uint4(0xff800000u, 0u, 0x7fffffffu, 0u);
             m = __uint_as_float(its.x);
             total = __uint_as_float(its.y);
@@ -498,8 +507,7 @@ verify_drafts_kernel(VerifyParams a) {
                 tc::st_async_v4(tc::dsmem_map(tc::smem_u32(&box[turn][rank]), (uint32_t)lane), tc::dsmem_map(tc::smem_u32(&mail[turn]), (uint32_t)lane),
                                 (uint32_t)bits, (uint32_t)(bits >> 32), 0u, 0u);
             }
-            if (!tc::mbar_wait_limited(tc::smem_u32(&mail[turn]), 0, &no_flag) && tid == 0) atomicCAS(a.status, 0, ERR_MAIL);
-            __syncwarp();
+            if (!tc::warp_wait_limited(tc::smem_u32(&mail[turn]), 0, false, &no_flag)) return gave_up(a.status, ERR_MAIL);
 #pragma unroll
             for (int r = 0; r < 8; ++r)
                 if (r < ctas) {

@@ -52,3 +52,16 @@ def test_probabilities_and_verification_wait_behind_the_kernel_in_front(kernel):
     text = source("sampling.cu")
     body = block(text, text.index(kernel + "("))
     assert 0 <= body.find("pdl_wait();") < re.search(WAIT, body).start()
+
+
+def test_a_wait_that_gave_up_ends_its_warp_in_probabilities_and_verification():
+    """Nothing is asked for or sent behind a wait that gave up: its warp writes the status word, stays for a bounded time, in which what is
+    on its way lands before the shared memory is another's, and leaves; looked at by whole warps, since collectives follow."""
+    text = source("sampling.cu")
+    end = block(text, text.index("void gave_up("))
+    assert re.search(r"atomicCAS\(status, 0, code\);.*until = tc::global_timer_ns\(\) \+ \d+ull;\s*while \(tc::global_timer_ns\(\) < until\) \{\}", end, re.S)
+    for kernel, n in (("softmax_rows_kernel", 2), ("verify_drafts_kernel", 1)):
+        body = block(text, text.index(kernel + "("))
+        waits = re.findall(r"!tc::warp_wait_limited\([^;]*\)\) return gave_up\(\w+\.status, ERR_\w+\);", body)
+        assert len(waits) == len(re.findall(WAIT, body)) == n
+        assert not re.search(r"if \([^;]*(?:tid|lane|warp) [=<][^;]*" + WAIT, body)      # by every warp, not behind a choice of some
