@@ -34,6 +34,14 @@ __device__ __forceinline__ float warp_max(float x) {
     return y;
 }
 
+// exp((x - m) / T), c = log2(e) / T, x not above m.  By halves, since logits of both signs can lie further apart than the largest number while a large T
+// brings them near; equal ones weigh one by comparison, since 0 times infinity (both infinite, or a T next to nothing) would stand there.  NaN
+// (a masked one at infinite T) weighs nothing.
+__device__ __forceinline__ float weight_of(float x, float m, float c) {
+    const float half = __fmul_rn(__fmaf_rn(0.5f, x, __fmul_rn(-0.5f, m)), c);
+    return x == m ? 1.0f : exp2_approx(fmaxf(__fadd_rn(half, half), -3.0e38f));
+}
+
 // A wait of this warp gave up: the warp asks for nothing and sends nothing any more, gives copies and messages on their way a bounded time (the
 // CTA's shared memory is another's once its last warp has left), and leaves.  The CTA's barriers wait for threads that have not left,
 // so its other warps go on until a wait of their own gives up, which it does where it needed this one.
@@ -181,9 +189,10 @@ softmax_rows_kernel(SoftmaxParams p) {
             for (int k = 0; k < VE; ++k) top = fmaxf(top, w[k]);
         });
         top = warp_max(top);
-        // weights two at a time; where the maximum is infinite (the infinite ones share the mass), or the temperature so small that its
-        // reciprocal is, the largest are one by comparison, since 0 times infinity would stand there
-        const bool plain = fabsf(top) < INFINITY && c < INFINITY;
+        // weights two at a time; one by one where the maximum is infinite (the infinite ones share the mass) or so large that differences could be,
+        // or where the temperature is so small that its reciprocal is
+        const bool nothing = top == -INFINITY;               // this warp's entries are all masked: zeros
+        const bool plain = !nothing && top < 0x1p102f && c < INFINITY;
         const uint64_t minus_top = f32x2(-top, -top), c2 = f32x2(c, c);
         auto weigh = [&](float* w, auto slow) {
             if (!decltype(slow)::value) {
@@ -196,10 +205,9 @@ softmax_rows_kernel(SoftmaxParams p) {
                 }
             } else {
 #pragma unroll
-                for (int k = 0; k < VE; ++k) w[k] = w[k] == top ? 1.0f : exp2_approx(fmaxf(__fmul_rn(__fsub_rn(w[k], top), c), -3.0e38f));
+                for (int k = 0; k < VE; ++k) w[k] = weight_of(w[k], top, c);
             }
         };
-        const bool nothing = top == -INFINITY;               // this warp's entries are all masked: zeros
         uint64_t sum2 = 0;
         int first = 0x7fffffff;
         auto look = [&](int j, float* w) {
@@ -254,8 +262,7 @@ softmax_rows_kernel(SoftmaxParams p) {
         auto join = [&](float& m, float& s, int& f) {
             const float its = m;
             m = warp_max(its);
-            const float w = its == m ? 1.0f : exp2_approx(fmaxf(__fmul_rn(__fsub_rn(its, m), c), -3.0e38f));
-            s = warp_sum_butterfly(__fmul_rn(s, w));
+            s = warp_sum_butterfly(__fmul_rn(s, weight_of(its, m, c)));
             f = __reduce_min_sync(0xffffffffu, its == m ? f : 0x7fffffff);
         };
         float m = lane < WARPS ? part[odd][lane] : -INFINITY, total = lane < WARPS ? part2[odd][lane] : 0.0f;
@@ -276,7 +283,7 @@ softmax_rows_kernel(SoftmaxParams p) {
             join(m, total, f);
         }
         if (m == -INFINITY) f = -1;
-        const float factor = __fdiv_rn(top == m ? 1.0f : exp2_approx(fmaxf(__fmul_rn(__fsub_rn(top, m), c), -3.0e38f)), total);
+        const float factor = __fdiv_rn(weight_of(top, m, c), total);
         const uint64_t factor2 = f32x2(factor, factor);
         auto store = [&](int j, float* w) {
             const int e = j * VE - at.skew;
