@@ -323,7 +323,8 @@ extern "C" int frt_b200_paged_plan(const int* kept_lens, const int* new_lens, in
     if (blk::too_large(tokens, batch, num_blocks, table_stride, block_size)) return FRT_ERR_UNSUPPORTED;
     if (!free_in || !free_out || !cu_seqlens || (!free_list && num_blocks)) return FRT_ERR_INVALID;
     if (batch && (!kept_lens || !new_lens || !seq_lens || (!block_table && table_stride))) return FRT_ERR_INVALID;
-    if (free_in == free_out || (batch && (kept_lens == seq_lens || new_lens == seq_lens))) return FRT_ERR_INVALID;      // read while they are written
+    auto meet = [&](const int* a) { return a < seq_lens + batch && seq_lens < a + batch; };
+    if (free_in == free_out || (batch && (meet(kept_lens) || meet(new_lens)))) return FRT_ERR_INVALID;      // read while they are written
     if (misaligned(kept_lens, 4) || misaligned(new_lens, 4) || misaligned(block_table, 4) || misaligned(free_list, 4) || misaligned(free_in, 4) ||
         misaligned(free_out, 4) || misaligned(cu_seqlens, 4) || misaligned(seq_lens, 4) || misaligned(positions, 4) || misaligned(slots, 8) ||
         misaligned(refused, 4))

@@ -690,6 +690,18 @@ static int launch_softmax(SoftmaxParams p, int rows, cudaStream_t st) {
 }  // namespace frt
 
 static bool misaligned(const void* a, uintptr_t n) { return (reinterpret_cast<uintptr_t>(a) & (n - 1)) != 0; }
+// a and b share bytes: rows of a_bytes every a_step (rows of one buffer may lie between those of another)
+static bool rows_meet(const void* a, long long a_bytes, long long a_step, const void* b, long long b_bytes, long long b_step, int rows) {
+    const uintptr_t a0 = reinterpret_cast<uintptr_t>(a), b0 = reinterpret_cast<uintptr_t>(b);
+    if (a0 >= b0 + (uintptr_t)(rows - 1) * b_step + b_bytes || b0 >= a0 + (uintptr_t)(rows - 1) * a_step + a_bytes) return false;
+    for (long long i = 0, j = 0; i < rows && j < rows;) {
+        const uintptr_t x = a0 + (uintptr_t)i * a_step, y = b0 + (uintptr_t)j * b_step;
+        if (x < y + b_bytes && y < x + a_bytes) return true;
+        if (x < y) ++i;
+        else ++j;
+    }
+    return false;
+}
 
 extern "C" int frt_b200_softmax_rows(const void* in, long long in_stride, float* out, long long out_stride, const float* temperature, int rows,
                                      int vocab, int flags, void* stream) {
@@ -698,7 +710,9 @@ extern "C" int frt_b200_softmax_rows(const void* in, long long in_stride, float*
     if (rows > 1 << 27 || vocab > 1 << 30) return FRT_ERR_UNSUPPORTED;
     if (rows == 0 || vocab == 0) return FRT_OK;
     const bool f32 = flags & 2;
-    if (!in || !out || in == out || misaligned(in, f32 ? 4 : 2) || misaligned(out, 4) || misaligned(temperature, 4)) return FRT_ERR_INVALID;
+    if (!in || !out || misaligned(in, f32 ? 4 : 2) || misaligned(out, 4) || misaligned(temperature, 4)) return FRT_ERR_INVALID;
+    const long long es = f32 ? 4 : 2;                        // rows are read while others are written
+    if (rows_meet(in, vocab * es, in_stride * es, out, vocab * 4ll, out_stride * 4, rows)) return FRT_ERR_INVALID;
     smp::SoftmaxParams p = {in, out, temperature, in_stride, out_stride, rows, vocab, 1, smp::status_word()};
     if (!p.status) return FRT_ERR_UNSUPPORTED;
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
@@ -715,7 +729,8 @@ extern "C" int frt_b200_verify_drafts(const float* target_probs, long long p_str
     if (batch > 1 << 27 || vocab > 1 << 30) return FRT_ERR_UNSUPPORTED;
     if (batch == 0) return FRT_OK;
     if (!cu_seqlens || !u_sample || !accepted || (kept_lens && !seq_lens)) return FRT_ERR_INVALID;
-    if (n_tokens && (!target_probs || !tokens || !u_accept || !out_tokens || out_tokens == tokens)) return FRT_ERR_INVALID;
+    if (n_tokens && (!target_probs || !tokens || !u_accept || !out_tokens)) return FRT_ERR_INVALID;
+    if (n_tokens && rows_meet(tokens, 4ll * n_tokens, 0, out_tokens, 4ll * n_tokens, 0, 1)) return FRT_ERR_INVALID;     // read while they are written
     if (misaligned(target_probs, 4) || misaligned(draft_probs, 4) || misaligned(tokens, 4) || misaligned(cu_seqlens, 4) || misaligned(seq_lens, 4) ||
         misaligned(u_accept, 4) || misaligned(u_sample, 4) || misaligned(out_tokens, 4) || misaligned(accepted, 4) || misaligned(kept_lens, 4))
         return FRT_ERR_INVALID;

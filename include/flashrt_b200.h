@@ -596,7 +596,7 @@ int frt_b200_gemm_fp8_block_nt(const void* A, const void* W, void* D, int M, int
  * Softmax of rows (no counterpart in the reference): out = exp((x - max) / T) / sum, fp32.  in (rows, vocab) bf16, with flags bit 1 fp32, rows
  *   in_stride elements apart; out (rows, vocab) fp32, rows out_stride elements apart; temperature (rows) fp32 or NULL: 1.  A temperature
  *   that is not above zero (0, negative, NaN): one at the first of the row's largest, zero elsewhere.  NaN counts as -infinity; a row of
- *   nothing else is zero; infinite entries share the whole.  Not in place.  vocab <= 2^30.  A wait that gave up shows in
+ *   nothing else is zero; infinite entries share the whole.  No row of out lies over one of in.  vocab <= 2^30.  A wait that gave up shows in
  *   frt_b200_gemm_status. */
 int frt_b200_softmax_rows(const void* in, long long in_stride, float* out, long long out_stride, const float* temperature, int rows,
                           int vocab, int flags, void* stream);
@@ -608,7 +608,7 @@ int frt_b200_softmax_rows(const void* in, long long in_stride, float* out, long 
  *   does not.  Behind the last that stands comes a token from max(p - q, 0) of the first row whose token does not (without draft_probs: p
  *   without that token; where nothing is left: p), or from p of the sequence's last row: the first entry whose running sum is above
  *   u_sample[b] * sum, in 64 bits (u_sample is taken into [0, 1); -1 if all is zero).
- *   out_tokens (n_tokens), not `tokens` itself: the tokens that stand, the new one, then -1 up to the sequence's end; rows behind the last
+ *   out_tokens (n_tokens), which shares no entry with `tokens`: the tokens that stand, the new one, then -1 up to the sequence's end; rows behind the last
  *   sequence are left as they were.  accepted (batch): drafted tokens that stand.  kept_lens (batch) or NULL: seq_lens less the drafted
  *   tokens that do not; may be seq_lens itself.  A sequence without rows, or whose rows leave [0, n_tokens): accepted 0, kept_lens =
  *   seq_lens, nothing else.  A wait that gave up shows in frt_b200_gemm_status. */
@@ -627,7 +627,7 @@ int frt_b200_verify_drafts(const float* target_probs, long long p_stride, const 
  *   offset, -1 for rows behind the last sequence and for pages that are no block of the pool (either may be NULL); *refused (or NULL).
  *   A sequence with a negative length, or with more blocks than its row has entries, brings nothing (its seq_lens is max(kept, 0)); from the
  *   first one on for which the list or `tokens` rows do not suffice, none brings anything.  *refused counts them all.
- *   Other entries of the table stay as they were.  free_out is not free_in, seq_lens neither kept_lens nor new_lens. */
+ *   Other entries of the table stay as they were.  free_out is not free_in, seq_lens shares no entry with kept_lens or new_lens. */
 int frt_b200_paged_plan(const int* kept_lens, const int* new_lens, int* block_table, int table_stride, const int* free_list,
                         const int* free_in, int* free_out, int* cu_seqlens, int* seq_lens, int* positions, long long* slots,
                         int* refused, int tokens, int batch, int num_blocks, int block_size, int flags, void* stream);

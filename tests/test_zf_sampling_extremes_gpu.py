@@ -51,3 +51,26 @@ def test_logits_further_apart_than_the_largest_number(rows, vocab, dtype):
     assert (off <= want * rel + 2.0 ** -120).all(), (off / (want * rel + 2.0 ** -120)).max()
     spread = [r for r in range(rows) if r % 5 < 2 and float(t[r]) >= 1e38]
     assert all(len(p[r].unique()) >= 2 or t[r] == INF for r in spread) and spread       # far ones count there, they are not all or nothing
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_probabilities_between_the_rows_of_their_logits(dtype):
+    """Rows of one buffer: logits, probabilities right behind them, a gap.  Only what shares bytes is refused."""
+    from flashrt_b200 import flash_rt_kernels as fvk
+    rows, vocab = 9, 1000
+    es = 2 if dtype == BF16 else 4
+    step = vocab * (es + 4) + 16
+    buffer = torch.full((rows * step,), 0x5a, dtype=torch.uint8, device="cuda")
+    rows_of = buffer.view(rows, step)
+    x = (torch.randn(rows, vocab, generator=torch.Generator().manual_seed(1)) * 3).to(dtype).cuda()
+    rows_of[:, :vocab * es] = x.view(torch.uint8)
+    t = torch.full((rows,), 0.8, device="cuda")
+    args = dict(temperature=t.data_ptr(), in_f32=dtype == F32, in_stride=step // es, out_stride=step // 4)
+    stream = torch.cuda.current_stream().cuda_stream
+    with pytest.raises(fvk.KernelError):
+        fvk.softmax_rows(buffer.data_ptr(), buffer.data_ptr() + vocab * es - 4, rows, vocab, stream, **args)
+    fvk.softmax_rows(buffer.data_ptr(), buffer.data_ptr() + vocab * es, rows, vocab, stream, **args)
+    torch.cuda.synchronize()
+    assert torch.equal(rows_of[:, vocab * es:-16].contiguous().view(F32).cpu(), softmax(x, t))
+    assert torch.equal(rows_of[:, :vocab * es].contiguous().view(dtype), x) and (rows_of[:, -16:] == 0x5a).all()
+    assert fvk._lib.call_status("frt_b200_gemm_status", 1) == 0
