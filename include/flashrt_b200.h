@@ -596,16 +596,17 @@ int frt_b200_gemm_fp8_block_nt(const void* A, const void* W, void* D, int M, int
  * Softmax of rows (no counterpart in the reference): out = exp((x - max) / T) / sum, fp32.  in (rows, vocab) bf16, with flags bit 1 fp32, rows
  *   in_stride elements apart; out (rows, vocab) fp32, rows out_stride elements apart; temperature (rows) fp32 or NULL: 1.  A temperature
  *   that is not above zero (0, negative, NaN): one at the first of the row's largest, zero elsewhere.  NaN counts as -infinity; a row of
- *   nothing else is zero; infinite entries share the whole.  No row of out lies over one of in.  vocab <= 2^30.  A wait that gave up shows in
- *   frt_b200_gemm_status. */
+ *   nothing else is zero; infinite entries share the whole; weights below 2^-126 of the largest may become zero.  No row of out lies over one
+ *   of in.  vocab <= 2^30.  A wait that gave up shows in frt_b200_gemm_status. */
 int frt_b200_softmax_rows(const void* in, long long in_stride, float* out, long long out_stride, const float* temperature, int rows,
                           int vocab, int flags, void* stream);
 /* Drafted tokens against the target's probabilities, from given random numbers (no counterpart in the reference).  Sequence b has the rows
  *   cu_seqlens[b] .. cu_seqlens[b + 1] - 1 of this step: a token that stands already and the drafted ones behind it; row t answers with
  *   token t + 1.  tokens (n_tokens) int32; target_probs, draft_probs (n_tokens, vocab) fp32, not negative, finite, rows p_stride / q_stride
- *   elements apart (a sequence's last row of draft_probs is not read; NULL: all of the draft's probability lay on its token).
+ *   elements apart (a sequence's last row of draft_probs is not read; NULL: all of the draft's probability lay on its token; rows that lie
+ *   otherwise to 16 bytes than the target's, as with another stride, are read value by value).
  *   Drafted token d of row t stands if those in front do and u_accept[t] * q[t][d] < p[t][d], in 64 bits; a token outside the vocabulary
- *   does not.  Behind the last that stands comes a token from max(p - q, 0) of the first row whose token does not (without draft_probs: p
+ *   does not.  So u_accept -1 lets a token stand whatever p says, if its q is above zero or draft_probs NULL: the rows of a prompt.  Behind the last that stands comes a token from max(p - q, 0) of the first row whose token does not (without draft_probs: p
  *   without that token; where nothing is left: p), or from p of the sequence's last row: the first entry whose running sum is above
  *   u_sample[b] * sum, in 64 bits (u_sample is taken into [0, 1); -1 if all is zero).
  *   out_tokens (n_tokens), which shares no entry with `tokens`: the tokens that stand, the new one, then -1 up to the sequence's end; rows behind the last
@@ -635,7 +636,8 @@ int frt_b200_paged_plan(const int* kept_lens, const int* new_lens, int* block_ta
  *   sequence (0).  Of the table's entries of blocks behind ceil(kept_lens / block_size), up to ceil(seq_lens / block_size), those that are
  *   blocks of the pool become -1 and go on the list, a sequence's last one and the last sequence's first, so that a plan that takes as many finds
  *   them in their old places.  *free_out = *free_in + their number, at most num_blocks; not free_in itself.  Blocks carry no count of
- *   their users: one that two rows share is put on the list by each that drops it. */
+ *   their users: one that two rows share is put on the list by each that drops it, also while the other still reads it, so that a plan hands it
+ *   out twice or too early.  Rows with shared blocks do not go through this call while another row holds them. */
 int frt_b200_paged_release(const int* kept_lens, const int* seq_lens, int* block_table, int table_stride, int* free_list,
                            const int* free_in, int* free_out, int batch, int num_blocks, int block_size, int flags, void* stream);
 
