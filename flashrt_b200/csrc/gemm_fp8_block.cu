@@ -10,12 +10,13 @@
 // scales and add it to the tile's sums, which they keep in registers (fp32: the block's scales differ, so tensor memory cannot hold them).
 // The buffers go round, so that the next block's products run meanwhile.  That taking out is what bounds many rows: 256 x 256 x 128 on a CTA
 // pair are 512 cycles of products, and a warp's 128 columns come out of tensor memory in 370 cycles when it is idle but in 850 beside the
-// products, which go there for their sums too; with the signals between the warps a k-block takes 0.47 us, 2.2 PFLOP/s, where the products
-// with one scale per tensor, taken out once a tile, reach 2.9.
+// products, which go there for their sums too.  With the signals between the warps a k-block takes 0.53 us, 2.3 PFLOP/s on all pairs, where the
+// products with one scale per tensor, taken out once a tile, take 0.41 (3.0; both from K 1024 to 8192 of 8192 x 9472, sixteen whole waves).  A
+// tile's fill and store add 1.4 us: 8191 x 4096 x 4096, seven waves of which the last is not full, 120 to 128 us by the data, 2.1 to 2.3 PFLOP/s.
 //
 // Up to 64 rows the weights are the 128 lanes and the tokens the columns, because nothing is left but streaming the weights; so are tiles of 96
-// or 128 tokens where there are so few that four or eight CTAs can share K.  Otherwise the tokens are the rows of a tile (a thread of the
-// epilogue owns a row, its scale is one register), on CTA pairs or single CTAs.
+// or 128 tokens where four or eight CTAs share K and all their clusters fit on the device (few tiles).  Otherwise the tokens are the rows of a
+// tile (a thread of the epilogue owns a row, its scale is one register), on CTA pairs or single CTAs.
 #include "common.cuh"
 #include "tc05.cuh"
 #include "flashrt_b200.h"
@@ -34,7 +35,7 @@ namespace f8b {
 // Eight lanes have a group, 16 values each; U groups a lane, whose loads are all under way at once.  What a row of groups costs beside its
 // bytes is the scale, one of four bytes in a line of its own; DOWN: a block has 32 rows of U neighbouring groups, so that scales fill lines.
 // Issue is busy for 76 % of the time and memory waits for it: blocks of two groups a lane, six an SM (40 registers), overlap their ends better
-// than four of four groups (817 x 16384 9.1 us against 10.1, 8191 x 4096 19.7 against 19.9) or of one (11.0, 24.0).
+// than four of four groups (817 x 16384 9.1 us against 10.1, 8191 x 4096 19.7 against 19.9) or of one (11.0, 24.0); eight bytes a thread spill for it.
 struct Quotient {
     uint64_t t, r;                                           // -t / 1024 and its reciprocal, twice: normal numbers for every bf16 t
     __device__ __forceinline__ explicit Quotient(float top) {
@@ -208,7 +209,7 @@ __device__ __forceinline__ void store_one(const Params& p, size_t at, float v) {
     else static_cast<__nv_bfloat16*>(p.out)[at] = __float2bfloat16_rn(v);
 }
 
-// ---------------------------------------------------------------- few rows (up to 64, or few tiles): weights on the lanes, tokens on the columns
+// ------------------------------- weights on the lanes, tokens on the columns: up to 64 rows, or tiles of 96 or 128 whose K four or eight CTAs share
 template <int BN>
 struct LaneCfg {
     static constexpr int A_BYTES = 128 * 128, B_BYTES = BN * 128, STAGE_BYTES = A_BYTES + B_BYTES;
@@ -958,7 +959,8 @@ static int launch_tile(const void* A, const void* W, Params p, int K, cudaStream
     int rc = make_tmap_2d_u8(&tmA, A, (uint64_t)p.M, (uint64_t)K, (uint64_t)K, 128);
     if (!rc) rc = make_tmap_2d_u8(&tmW, W, (uint64_t)p.N, (uint64_t)K, (uint64_t)K, BN / CG);
     const uint64_t out_row = (uint64_t)p.N * (p.f32 ? 4 : 2);
-    // rows at 16 bytes, bias read so, and a byte's place in a row is a 32-bit coordinate
+    // Rows at 16 bytes, bias read so, and a byte's place in a row is a 32-bit coordinate.  Otherwise values are stored one by one and nothing is
+    // summed meanwhile: 80 x 50257 x 2048 40 us (50256: 28, fp32 30.5), 384 rows 70 (46, 52), 2000 325 (215, 224), 8191 x 50257 x 512 831 (313, 404).
     p.tma = p.N % 8 == 0 && (reinterpret_cast<uintptr_t>(p.bias) & 15) == 0 && out_row <= 1u << 31;
     if (!rc && p.tma) rc = make_tmap_2d_u8(&tmD, p.out, (uint64_t)p.M, out_row, out_row, 32);
     if (!p.tma) tmD = tmA;
@@ -1084,7 +1086,9 @@ extern "C" int frt_b200_gemm_fp8_block_nt(const void* A, const void* W, void* D,
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
     const int sms = device_sm_count(), n128 = (N + 127) / 128, n256 = (N + 255) / 256;
     if (M <= 64) {
-        // K splits (a cluster) while the tiles alone leave SMs idle and every rank keeps two k-blocks
+        // K splits (a cluster) while the tiles alone leave SMs idle and every rank keeps two k-blocks.  A cluster lies in one GPC, so 33 of eight and
+        // 69 to 71 of four fit at two CTAs an SM: where this asks for a few more (34 to 37 tiles, 72 to 74), the last run behind the first (one
+        // row, K 3584: 4224 columns 6.8 us, 4352 to 4736 10.6 to 10.9, 4864 7.1; 8832 8.9, 9216 to 9472 13.3, 9600 9.5).
         int splits = 1;
         while (splits < 8 && n128 * splits * 2 <= 2 * sms && p.kb / (splits * 2) >= 2) splits *= 2;
         if (M <= 16) return f8b::launch_lane<16>(A, W, p, K, splits, st);
@@ -1095,6 +1099,8 @@ extern "C" int frt_b200_gemm_fp8_block_nt(const void* A, const void* W, void* D,
     // shared, the exchange, and only if the device holds all clusters at once.  Measured at 128 x 4096 x 4096 (12 us in 128-column tiles, 10 with
     // K shared by two, 18 in 256-column ones), 256 x 2048 x 8192 (20 on pairs of 128 columns, 13 with K shared by two), 817 x 2048 x 16384 (66 in
     // 256-column tiles, 40 with K shared by two), 8191 x 4096 x 4096 (125 on pairs of 256 columns, 129 on single CTAs, 162 on pairs of 128).
+    // A k-block's time is that of products; where memory is slower (96 x 32768 x 2048: 0.7 us a k-block, 128 CTAs at 32 KB, 0.64 at the copy rate)
+    // all forms read the same weights, and whole waves decide.
     const long long m128 = (M + 127) / 128, m256 = (M + 255) / 256;
     double best = 1e30;
     int form = 0;

@@ -2,7 +2,7 @@
 //
 // Stand behind the products that make logits and in front of the paged cache's lengths; no counterpart in the reference.
 //
-// Both read rows of a vocabulary once: a row belongs to a cluster of 1 to 8 CTAs that hold it (softmax: in registers) and send one another a
+// Both read rows of a vocabulary once, where a cluster of 1 to 8 CTAs holds one (softmax: in registers); its CTAs send one another a
 // few numbers.  Rows start anywhere (odd vocabularies): 16-byte vectors lie where memory has them, and the
 // first and last of a row are taken value by value.
 #include "common.cuh"
@@ -55,8 +55,8 @@ __device__ __forceinline__ void gave_up(int* status, int code) {
 //   p = exp((x - max) / T) / sum;  T not above zero: one on the first of the largest;  nothing but -infinity and NaN: zeros.
 // Weights are exponentials against the warp's own maximum; the (maximum, sum) of warps meet in shared memory, those of the cluster's CTAs
 // by st.async (a cluster barrier waits for every store in front of it: 384 rows of 131072 in fp32 103 us with two a row), and a factor
-// takes a warp's weights to the row's probabilities.  NV vectors a thread.  FORM 0: a row a cluster; 1: what is behind NV vectors is read
-// twice; 2: clusters stay and go from row to row, the next row's part is copied to shared memory meanwhile (384 rows of 131072 71 us in fp32,
+// takes a warp's weights to the row's probabilities.  NV vectors a thread.  FORM 0: a row a cluster; 1: the same, and what is behind NV vectors is
+// read three times (maximum, sum, output; the last two find it in L2); 2: clusters stay and go from row to row, the next row's part is copied to shared memory meanwhile (384 rows of 131072 71 us in fp32,
 // 5.7 TB/s, 63 in bf16; without the copy 124).  Clusters that stay let the next kernel in with their last row: at the start its CTAs take
 // places beside them (88, when a row took 78).
 struct SoftmaxParams {
@@ -67,7 +67,7 @@ struct SoftmaxParams {
     int rows, vocab, ctas;       // ctas: of a row
     int* status;
 };
-constexpr int ONE_ROW = 0, READ_TWICE = 1, STAY = 2;
+constexpr int ONE_ROW = 0, READ_AGAIN = 1, STAY = 2;
 enum { ERR_MAIL = 1, ERR_ROW = 2 };
 
 struct Yes { static constexpr bool value = true; };
@@ -77,7 +77,7 @@ template <int THREADS, int NV, bool F32, int FORM>
 __global__ void __launch_bounds__(THREADS, (NV * (F32 ? 4 : 8) > 32 ? 512 : 1024) / THREADS)
 softmax_rows_kernel(SoftmaxParams p) {
     constexpr int VE = F32 ? 4 : 8, ES = F32 ? 4 : 2, WARPS = THREADS / 32;      // values of 16 bytes, bytes of a value
-    constexpr bool HELD = FORM != READ_TWICE, STAGED = FORM == STAY;
+    constexpr bool HELD = FORM != READ_AGAIN, STAGED = FORM == STAY;
     extern __shared__ uint4 stage[];                         // STAY: the next row's part
     __shared__ float part[2][WARPS], part2[2][WARPS];        // of each warp: maximum, sum
     __shared__ int part3[2][WARPS];                          // first of its largest
@@ -325,6 +325,8 @@ softmax_rows_kernel(SoftmaxParams p) {
 //   the last row.  The token is the first whose running sum is above v times the sum of all, in 64 bits.
 // A warp has a run of neighbouring entries in SLOTS stretches; the sums of stretches stay in registers, those of runs go through shared
 // memory, those of CTAs through the cluster, and from there the search goes back down: CTA, warp, stretch, lane, and the lane's four.
+// Two CTAs an SM leave 64 registers a thread, and 176 bytes of each spill (to L1, outside the loop over a run).  Rows of q that lie otherwise to
+// 16 bytes than p's (another stride) are read value by value: 64 sequences of 131072 19.9 us instead of 14.8.
 constexpr int VERIFY_THREADS = 512, VERIFY_WARPS = VERIFY_THREADS / 32, SLOTS = 8;
 
 struct VerifyParams {
@@ -681,9 +683,12 @@ static int launch_softmax(SoftmaxParams p, int rows, cudaStream_t st) {
         // of 63), 300 of 50257 27.2 instead of 25.2; on 16 CTAs a row, which needs leave, 90
         return launch_staying<256, 4 * N16, F32>(p, rows, st);
     }
-    // a little more (a row that starts inside a vector has one more of them) is read twice rather than held by half as many CTAs
+    // A little more (a row that starts inside a vector has one more of them) is read again rather than held by clusters of twice the threads, of
+    // which an SM has one: 384 rows of 131071 90 us against 150 (bf16 91 against 130), of 140000 113 against 139 (108 against 124), of 151936
+    // 140 against 139.5 (113 against 124), 16 rows of them 8.5 against 11.5.  From five quarters on they are held: 384 of 163848 144 against
+    // 147 (bf16 129 against 120), of 180000 148 against 171 (130 against 141), of 262136 169 against 301 (149 against 211).
     if (each > 2 * N16 * 640 && each <= 4 * N16 * 512) return launch_staying<512, 4 * N16, F32>(p, rows, st);
-    return launch(softmax_rows_kernel<512, 2 * N16, F32, READ_TWICE>, p, ctas, rows, 512, st);
+    return launch(softmax_rows_kernel<512, 2 * N16, F32, READ_AGAIN>, p, ctas, rows, 512, st);
 }
 
 }  // namespace smp

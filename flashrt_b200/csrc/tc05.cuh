@@ -398,7 +398,7 @@ __device__ __forceinline__ void cluster_sync_all() {
     __syncwarp();                                           // the form is aligned: lanes may come from code that parted them
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
-// The barrier in two halves, for work of a CTA's own between its last access to a peer's shared memory and the end.
+// The barrier in two halves, for work of a CTA's own between them: its start, before its first access to a peer's shared memory.
 __device__ __forceinline__ void cluster_arrive() {
     __syncwarp();
     asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
