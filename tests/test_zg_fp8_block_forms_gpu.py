@@ -1,5 +1,6 @@
 """Every form of the block-scaled product against 64 bits, the form read from the launch: whole and part tiles, outputs by TMA (N % 8 == 0), in
 vectors and value by value, K that ends inside a block, more tiles than places."""
+import ctypes
 import re
 
 import pytest
@@ -51,14 +52,40 @@ def product(a, w, sa, sw, bias, f32, pdl):
     return out[:m * n].view(m, n)
 
 
+class KernelNode(ctypes.Structure):
+    """CUDA_KERNEL_NODE_PARAMS_v2 of the driver's interface."""
+    _fields_ = [("func", ctypes.c_void_p), ("grid", ctypes.c_uint * 3), ("block", ctypes.c_uint * 3), ("shared", ctypes.c_uint),
+                ("params", ctypes.c_void_p), ("extra", ctypes.c_void_p), ("kern", ctypes.c_void_p), ("ctx", ctypes.c_void_p)]
+
+
+def form_of(a, w, sa, sw):
+    """The kernel of a product's launch, read from a graph that holds nothing else."""
+    from flashrt_b200 import flash_rt_kernels as fvk
+    m, n, k = a.shape[0], w.shape[0], a.shape[1]
+    out = torch.empty(m, n, device="cuda")
+    graph, side = torch.cuda.CUDAGraph(keep_graph=True), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=side):
+        fvk.GemmRunner().fp8_block_nt(a.data_ptr(), w.data_ptr(), out.data_ptr(), m, n, k, sa.data_ptr(), sw.data_ptr(), side.cuda_stream, d_f32=True)
+    cuda = ctypes.CDLL("libcuda.so.1")
+    handle, count = ctypes.c_void_p(graph.raw_cuda_graph()), ctypes.c_size_t(0)
+    assert cuda.cuGraphGetNodes(handle, None, ctypes.byref(count)) == 0 and count.value == 1
+    nodes, node, name = (ctypes.c_void_p * 1)(), KernelNode(), ctypes.c_char_p()
+    assert cuda.cuGraphGetNodes(handle, nodes, ctypes.byref(count)) == 0
+    assert cuda.cuGraphKernelNodeGetParams_v2(ctypes.c_void_p(nodes[0]), ctypes.byref(node)) == 0
+    if node.func:
+        assert cuda.cuFuncGetName(ctypes.byref(name), ctypes.c_void_p(node.func)) == 0
+    else:
+        assert cuda.cuKernelGetName(ctypes.byref(name), ctypes.c_void_p(node.kern)) == 0
+    kind, numbers = re.search(r"gemm_fp8_block_(\w+?_kernel)I((?:Li\d+E)+)E", name.value.decode()).groups()
+    return f"{kind}<{', '.join(re.findall(r'[0-9]+', numbers))}>"
+
+
 @pytest.mark.parametrize("form,m,n,k", [(f, *s) for f, shapes in FORMS for s in shapes])
 def test_form(form, m, n, k):
-    from torch.profiler import ProfilerActivity, profile
     a, w, sa, sw, bias = operands(m, n, k, m + n)
-    with profile(activities=[ProfilerActivity.CUDA]) as prof:
-        plain = product(a, w, sa, sw, None, True, False)
-    names = {re.sub(r".*gemm_fp8_block_(\w+<[^>]*>).*", r"\1", e.key) for e in prof.key_averages() if "gemm_fp8_block" in e.key}
-    assert names == {form}
+    assert form_of(a, w, sa, sw) == form
+    plain = product(a, w, sa, sw, None, True, False)
     want, size = R.block_product(a, w, sa, sw)
     # a block's 128 additions in the tensor core (2^-23 of its magnitudes each); two roundings of the scale, one of each block's fma, eight of
     # parts of K, one of the bias (2^-24 each); bf16: half a step
