@@ -56,9 +56,10 @@ __device__ __forceinline__ void gave_up(int* status, int code) {
 // Weights are exponentials against the warp's own maximum; the (maximum, sum) of warps meet in shared memory, those of the cluster's CTAs
 // by st.async (a cluster barrier waits for every store in front of it: 384 rows of 131072 in fp32 103 us with two a row), and a factor
 // takes a warp's weights to the row's probabilities.  NV vectors a thread.  FORM 0: a row a cluster; 1: the same, and what is behind NV vectors is
-// read three times (maximum, sum, output; the last two find it in L2); 2: clusters stay and go from row to row, the next row's part is copied to shared memory meanwhile (384 rows of 131072 71 us in fp32,
-// 5.7 TB/s, 63 in bf16; without the copy 124).  Clusters that stay let the next kernel in with their last row: at the start its CTAs take
-// places beside them (88, when a row took 78).
+// read three times (maximum, sum, output; the last two find it in L2; bf16 spills 84 bytes of stores and 152 of loads a thread at 64 registers);
+// 2: clusters stay and go from row to row, the next row's part is copied to shared memory meanwhile (384 rows of 131072 71 us in fp32, 5.7 TB/s,
+// 63 in bf16; without the copy 124).  Clusters that stay let the next kernel in with their last row: at the start its CTAs take places beside
+// them (88, when a row took 78).
 struct SoftmaxParams {
     const void* x;
     float* p;
@@ -325,8 +326,8 @@ softmax_rows_kernel(SoftmaxParams p) {
 //   the last row.  The token is the first whose running sum is above v times the sum of all, in 64 bits.
 // A warp has a run of neighbouring entries in SLOTS stretches; the sums of stretches stay in registers, those of runs go through shared
 // memory, those of CTAs through the cluster, and from there the search goes back down: CTA, warp, stretch, lane, and the lane's four.
-// Two CTAs an SM leave 64 registers a thread, and 176 bytes of each spill (to L1, outside the loop over a run).  Rows of q that lie otherwise to
-// 16 bytes than p's (another stride) are read value by value: 64 sequences of 131072 19.9 us instead of 14.8.
+// Two CTAs an SM leave 64 registers a thread; 176 bytes of stores and 200 of loads spill.  Rows of q that lie otherwise to 16 bytes than p's
+// (another stride) are read value by value: 64 sequences of 131072 19.9 us instead of 14.8.
 constexpr int VERIFY_THREADS = 512, VERIFY_WARPS = VERIFY_THREADS / 32, SLOTS = 8;
 
 struct VerifyParams {
