@@ -439,8 +439,19 @@ gemm_fp8_block_lane_kernel(const __grid_constant__ CUtensorMap tmA, const __grid
         }
     }
     if (S > 1) {
+        // Tensor memory goes back before this CTA waits for its peers: one of them may wait for columns that a cluster of another stream's kernel
+        // holds, whose CTA beside this one waits for these.  Between the issuer's arrival and its wait, so that nobody waits for it.
         __syncwarp();
-        tc::cluster_sync_all();                              // all partials are there
+        tc::tc_fence_before_sync();
+        if (warp >= 3) asm volatile("barrier.cta.arrive 1, %0;" ::"n"(32 * (1 + 4 * Cfg::HALVES)) : "memory");
+        tc::cluster_arrive();
+        if (warp == 1) {
+            asm volatile("barrier.cta.sync 1, %0;" ::"n"(32 * (1 + 4 * Cfg::HALVES)) : "memory");
+            tc::tc_fence_after_sync();
+            if (*abort_flag) let_copies_land();
+            tmem_give<1>(tmem, Cfg::TMEM_COLS);
+        }
+        tc::cluster_wait();                                  // all partials are there
         if (warp >= 3 && !*abort_flag) {
             const int q = warp & 3, half = (warp - 3) >> 2, n = (int)blockIdx.x * 128 + q * 32 + lane;
             const bool in = n < p.N;
@@ -471,6 +482,7 @@ gemm_fp8_block_lane_kernel(const __grid_constant__ CUtensorMap tmA, const __grid
         tc::cluster_sync_all();                              // nobody leaves while its partial is read
     }
     if (*abort_flag && threadIdx.x == 0) let_copies_land();
+    if (S > 1) return;
     tc::tc_fence_before_sync();
     __syncthreads();
     tc::tc_fence_after_sync();

@@ -65,3 +65,20 @@ def test_a_wait_that_gave_up_ends_its_warp_in_probabilities_and_verification():
         waits = re.findall(r"!tc::warp_wait_limited\([^;]*\)\) return gave_up\(\w+\.status, ERR_\w+\);", body)
         assert len(waits) == len(re.findall(WAIT, body)) == n
         assert not re.search(r"if \([^;]*(?:tid|lane|warp) [=<][^;]*" + WAIT, body)      # by every warp, not behind a choice of some
+
+
+@pytest.mark.parametrize("name,kernel", [("gemm_fp8_block.cu", "gemm_fp8_block_lane_kernel")])
+def test_tensor_memory_goes_back_before_a_cta_waits_for_its_peers(name, kernel):
+    """Two CTAs an SM: a cluster whose one CTA waits for columns that another kernel's cluster holds, while its other CTA holds columns which that
+    cluster's other CTA waits for, would never end, since neither the allocation nor the cluster's barrier has a limit."""
+    text = source(name)
+    body = block(text, text.index(kernel + "("))
+    shared = block(body, body.rindex("if (S > 1) {"))
+    # the warps that read it say so and arrive; the issuer arrives, waits for them, frees it, and waits for the peers only then
+    order = [r"if \(warp >= \d\) asm volatile\(\"barrier\.cta\.arrive 1,", r"cluster_arrive\(\);", r"if \(warp == 1\) \{\s*asm volatile\(\"barrier\.cta\.sync 1,",
+             r"if \(\*abort_flag\) let_copies_land\(\);\s*(?:tmem_give<1>|tc::tmem_dealloc)\(", r"cluster_wait\(\);", r"cluster_sync_all\(\);"]
+    places = [re.search(o, shared).start() for o in order]
+    assert places == sorted(places) and shared.count("cluster_sync_all();") == shared.count("cluster_wait();") == 1
+    assert re.search(r"if \(S > 1\) return;.*__syncthreads\(\);.*if \(warp == 1\) (?:tmem_give<1>|tc::tmem_dealloc)\(", body, re.S)
+    counts = re.findall(r'barrier\.cta\.(?:arrive|sync) 1, %0;" ::"n"\((.*?)\) : "memory"', shared)
+    assert len(counts) == 2 and len(set(counts)) == 1
