@@ -309,7 +309,19 @@ gemm_int8_lane_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
         }
     }
     if (S > 1) {
-        tc::cluster_sync_all();                              // all partials are there
+        // Tensor memory goes back before this CTA waits for its peers: one of them may wait for columns that a cluster of another stream's kernel
+        // holds, whose CTA beside this one waits for these.  Between the issuer's arrival and its wait, so that nobody waits for it.
+        __syncwarp();
+        tc::tc_fence_before_sync();
+        if (warp >= 2) asm volatile("barrier.cta.arrive 1, %0;" ::"n"(5 * 32) : "memory");
+        tc::cluster_arrive();
+        if (warp == 1) {
+            asm volatile("barrier.cta.sync 1, %0;" ::"n"(5 * 32) : "memory");
+            tc::tc_fence_after_sync();
+            if (*abort_flag) let_copies_land();
+            tc::tmem_dealloc(tmem, Cfg::TMEM_COLS);
+        }
+        tc::cluster_wait();                                  // all partials are there
         if (warp >= 2 && !*abort_flag) {
             const int q = warp & 3, n = n0 + q * 32 + lane;
             const bool in = n < p.N;
@@ -340,6 +352,7 @@ gemm_int8_lane_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
         tc::cluster_sync_all();                              // nobody leaves while its partial is read
     }
     if (*abort_flag && threadIdx.x == 0) let_copies_land();
+    if (S > 1) return;
     tc::tc_fence_before_sync();
     __syncthreads();
     tc::tc_fence_after_sync();

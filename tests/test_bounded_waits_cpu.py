@@ -67,7 +67,7 @@ def test_a_wait_that_gave_up_ends_its_warp_in_probabilities_and_verification():
         assert not re.search(r"if \([^;]*(?:tid|lane|warp) [=<][^;]*" + WAIT, body)      # by every warp, not behind a choice of some
 
 
-@pytest.mark.parametrize("name,kernel", [("gemm_fp8_block.cu", "gemm_fp8_block_lane_kernel")])
+@pytest.mark.parametrize("name,kernel", [("gemm_fp8_block.cu", "gemm_fp8_block_lane_kernel"), ("gemm_int8.cu", "gemm_int8_lane_kernel")])
 def test_tensor_memory_goes_back_before_a_cta_waits_for_its_peers(name, kernel):
     """Two CTAs an SM: a cluster whose one CTA waits for columns that another kernel's cluster holds, while its other CTA holds columns which that
     cluster's other CTA waits for, would never end, since neither the allocation nor the cluster's barrier has a limit."""
