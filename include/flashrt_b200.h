@@ -606,7 +606,8 @@ int frt_b200_softmax_rows(const void* in, long long in_stride, float* out, long 
  *   elements apart (a sequence's last row of draft_probs is not read; NULL: all of the draft's probability lay on its token; rows that lie
  *   otherwise to 16 bytes than the target's, as with another stride, are read value by value).
  *   Drafted token d of row t stands if those in front do and u_accept[t] * q[t][d] < p[t][d], in 64 bits; a token outside the vocabulary
- *   does not.  So u_accept -1 lets a token stand whatever p says, if its q is above zero or draft_probs NULL: the rows of a prompt.  Behind the last that stands comes a token from max(p - q, 0) of the first row whose token does not (without draft_probs: p
+ *   does not.  So u_accept -1 lets a token stand whatever p says, if its q is above zero or draft_probs NULL: the rows of a prompt.
+ *   Behind the last that stands comes a token from max(p - q, 0) of the first row whose token does not (without draft_probs: p
  *   without that token; where nothing is left: p), or from p of the sequence's last row: the first entry whose running sum is above
  *   u_sample[b] * sum, in 64 bits (u_sample is taken into [0, 1); -1 if all is zero).
  *   out_tokens (n_tokens), which shares no entry with `tokens`: the tokens that stand, the new one, then -1 up to the sequence's end; rows behind the last
